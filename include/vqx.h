@@ -659,6 +659,114 @@ int vqx_gptq_block(const float* work, int64_t rows, int64_t ld, int64_t col0, in
 int vqx_chol_inverse_block(const float* a, int64_t lda, int32_t n, float* li, int64_t ldl, int32_t* info,
                            vqx_stream_t stream);
 
+/*
+ * A serving cache of keys and values in 4 bits (this library's own; the
+ * reference has none): fp4_e2m1 codes with one E8M0 scale for each 32 elements
+ * of a head, the format vqx_mx_quantize packs.
+ * codes: uint8 [2, pages, kv_heads, page_size, dim / 2], keys then values,
+ * element 2 i in the low nibble, 16-byte aligned; scales: uint8 [2, pages,
+ * kv_heads, page_size, dim / 32], 255 standing for NaN.  With a table (int32
+ * [seqs, pages_per_seq]) token t of sequence b is in slot t % page_size of
+ * page table[b][t / page_size]; without one, page b is sequence b.  A table
+ * entry outside [0, pages) is no page: what is on it is neither written nor
+ * attended to, and reads as zeros.  lengths (int32 [seqs]) counts the tokens of
+ * each sequence, those of the current call included: the i-th last new token
+ * of sequence b stands at lengths[b] - i.  dim: 64, 128 or 256; fewer than
+ * 2^32 rows of one plane.
+ */
+typedef struct vqx_kv4_cache {
+  uint8_t* codes;
+  uint8_t* scales;
+  const int32_t* table; /* or NULL */
+  int32_t* lengths;     /* written by vqx_kv4_evict for the cache it fills */
+  int64_t pages;
+  int64_t pages_per_seq; /* with a table */
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t dim;
+  int32_t seqs;
+} vqx_kv4_cache;
+
+/*
+ * Queries of the new tokens: q [n, heads, dim] of dtype F32, BF16 or F16, with
+ * strides in elements (rows contiguous, starting on 16 bytes).  The new tokens
+ * of sequence b are cu[b] .. cu[b + 1] - 1 (int32 [seqs + 1], from 0 to n), or n
+ * / seqs each where cu is NULL; most (with cu): no sequence has more of them
+ * (0: n), and those that one has beyond it get NaN.  Query head x reads kv
+ * head x / (heads / kv_heads).  A token at position p sees tokens t <= p, and
+ * with a window only those with t > p - window.  Its score of t is
+ *   s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);
+ *   slopes (fp32 [heads], or NULL): s -= slopes[x] (p - t).
+ */
+typedef struct vqx_kv4_query {
+  const void* q;
+  const int32_t* cu;
+  const float* slopes;
+  int64_t n;
+  int64_t stride_n;
+  int64_t stride_h;
+  int32_t dtype;
+  int32_t heads;
+  int32_t most;
+  int32_t window;
+  float scale;
+  float softcap;
+} vqx_kv4_query;
+
+/*
+ * Writes keys and values [n, kv_heads, dim] of the new tokens into the cache,
+ * quantized: a block's scale is 2^(floor(log2(its largest magnitude)) - 2)
+ * within E8M0's 2^-127 .. 2^127, the log rounded to the dtype as
+ * vqx_mx_quantize has it (fp16: in fp32), and a value's quotient goes, as bf16,
+ * to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code.  (The
+ * fp4_e2m1 of vqx_mx_quantize rounds a quotient of 255 / 1024 up, as the
+ * reference does, and takes scales that E8M0 does not have.)  A block with an
+ * infinity or a NaN becomes NaN.  Tokens before position 0 or past the
+ * sequence's room are not written.
+ */
+int vqx_kv4_append(const vqx_kv4_cache* cache, const void* key, const void* value, int32_t dtype, int64_t n,
+                   int64_t key_stride_n, int64_t key_stride_h, int64_t value_stride_n, int64_t value_stride_h,
+                   const int32_t* cu, vqx_stream_t stream);
+
+/* The new tokens' keys and values as the cache holds them, contiguous
+ * [n, kv_heads, dim]; zeros where it holds none. */
+int vqx_kv4_read(const vqx_kv4_cache* cache, void* key, void* value, int32_t dtype, int64_t n, const int32_t* cu,
+                 vqx_stream_t stream);
+
+/*
+ * out [n, heads, dim] (the query's dtype) = softmax(scores) . values and lse
+ * [n, heads] = the log of the scores' exponentials' sum, fp32.  A row that sees
+ * nothing has out 0 and lse -inf.  An output element is NaN where the row sees
+ * a NaN key, or a NaN block of values with that element.  workspace:
+ * vqx_kv4_attention_workspace_size bytes for the same cache and query (it does
+ * not read the tensors), 16-byte aligned, or NULL where that is 0.
+ */
+int vqx_kv4_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes);
+int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, vqx_stream_t stream);
+
+/*
+ * weights[b][x][t] += the sum over sequence b's new tokens and kv head x's
+ * query heads of exp(score - lse), for the tokens t < weights_len that they
+ * see; weights: fp32 [seqs, kv_heads, weights_len], lse as vqx_kv4_attention
+ * gives it.  Sums have one order: the same call gives the same bits.
+ */
+int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, const float* lse, float* weights,
+                       int64_t weights_len, vqx_stream_t stream);
+
+/*
+ * Keeps min(budget, length) tokens of each sequence for each kv head: the
+ * latest `recent` and, of those before them, the heaviest by weights (fp32
+ * [seqs, kv_heads, weights_len]; lengths past weights_len count as that; equal
+ * weights by the lower place, NaN above all), in their order, moved to the
+ * front of `out`, another cache with as many sequences and kv heads and room
+ * for budget tokens each.  index: int32 [seqs, kv_heads, budget], where each
+ * kept token was, -1 past the end; out->lengths: their number; out_weights:
+ * fp32 [seqs, kv_heads, budget], their weights, 0 past the end.
+ */
+int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weights_len, int32_t budget, int32_t recent,
+                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, vqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

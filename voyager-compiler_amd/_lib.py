@@ -67,10 +67,44 @@ class VqxMxOperand(ctypes.Structure):
     ]
 
 
+class VqxKv4Cache(ctypes.Structure):
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_int64),
+        ("pages_per_seq", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("seqs", ctypes.c_int32),
+    ]
+
+
+class VqxKv4Query(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("cu", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("stride_n", ctypes.c_int64),
+        ("stride_h", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("most", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
+_KC = ctypes.POINTER(VqxKv4Cache)
+_KQ = ctypes.POINTER(VqxKv4Query)
 
 _SIGNATURES = {
     "vqx_version": ([], ctypes.c_char_p),
@@ -132,6 +166,12 @@ _SIGNATURES = {
     "vqx_gptq_block": ([_P, _I64, _I64, _I64, _I32, _P, ctypes.c_float, _P, _P, _I64, _P, _P, _P, _I64, _P],
                        ctypes.c_int),
     "vqx_chol_inverse_block": ([_P, _I64, _I32, _P, _I64, _P, _P], ctypes.c_int),
+    "vqx_kv4_append": ([_KC, _P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P], ctypes.c_int),
+    "vqx_kv4_read": ([_KC, _P, _P, _I32, _I64, _P, _P], ctypes.c_int),
+    "vqx_kv4_attention_workspace_size": ([_KC, _KQ, ctypes.POINTER(_I64)], ctypes.c_int),
+    "vqx_kv4_attention": ([_KC, _KQ, _P, _P, _P, _I64, _P], ctypes.c_int),
+    "vqx_kv4_accumulate": ([_KC, _KQ, _P, _P, _I64, _P], ctypes.c_int),
+    "vqx_kv4_evict": ([_KC, _P, _I64, _I32, _I32, _KC, _P, _P, _P], ctypes.c_int),
 }
 
 _lib = None

@@ -5,6 +5,7 @@
 
 #include "../../include/vqx.h"
 #include "vqx_kernels.h"
+#include "vqx_kv4.h"
 
 namespace vqx {
 
@@ -104,6 +105,100 @@ using namespace vqx;
     int _rc = (expr);          \
     if (_rc != kOk) return _rc; \
   } while (0)
+
+// A cache as the kernels see it; the sizes that its indexes assume are checked.
+static int to_view(const vqx_kv4_cache* c, const char* what, Kv4View* v) {
+  if (!c) return set_error(kErrInvalid, "%s: cache is NULL", what);
+  // a token without a page is loaded from row 0 and masked, so there is one
+  if (c->seqs != 0 && (!c->codes || !c->scales || !c->lengths || c->pages == 0))
+    return set_error(kErrInvalid, "%s: null cache tensor, or no pages", what);
+  if (c->dim != 64 && c->dim != 128 && c->dim != 256)
+    return set_error(kErrInvalid, "%s: heads of 64, 128 or 256 elements, not %d", what, c->dim);
+  if (c->seqs < 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->pages < 0 || c->pages_per_seq < 0)
+    return set_error(kErrInvalid, "%s: negative or empty sizes", what);
+  if (!aligned(c->codes, 16) || !aligned(c->scales, (unsigned)c->dim / 32))
+    return set_error(kErrInvalid, "%s: codes must be 16-byte aligned, scales to a row", what);
+  if (!c->table && c->pages < c->seqs)
+    return set_error(kErrInvalid, "%s: %lld pages for %d sequences without a table", what, (long long)c->pages, c->seqs);
+  // 2^31 pages, heads and tokens each: their product is checked in two steps
+  const int64_t limit = 1ll << 32;
+  if (c->pages >= 1ll << 31 || c->pages * c->kv_heads >= limit ||
+      c->pages * c->kv_heads * c->page_size >= limit)
+    return set_error(kErrUnsupported, "%s: a cache of 2^32 rows or more", what);
+  const int64_t per_seq = c->table ? c->pages_per_seq : 1;
+  if (per_seq >= 1ll << 31 || per_seq * c->page_size >= (1ll << 31) - 4096)
+    return set_error(kErrUnsupported, "%s: room for 2^31 tokens or more in a sequence", what);
+  if ((int64_t)c->seqs * c->kv_heads >= 1ll << 24)
+    return set_error(kErrUnsupported, "%s: 2^24 heads of sequences or more", what);
+  v->codes = c->codes;
+  v->scales = c->scales;
+  v->table = c->table;
+  v->lengths = c->lengths;
+  v->plane_rows = (uint64_t)(c->pages * c->kv_heads * c->page_size);
+  v->pages = (uint32_t)c->pages;
+  v->per_seq = (uint32_t)per_seq;
+  v->kv = (uint32_t)c->kv_heads;
+  v->size = (uint32_t)c->page_size;
+  v->cap = (uint32_t)(per_seq * c->page_size);
+  v->shift = (c->page_size & (c->page_size - 1)) == 0 ? 31 - clz32((uint32_t)c->page_size) : -1;
+  v->seqs = (uint32_t)c->seqs;
+  return kOk;
+}
+
+static int to_tokens(const Kv4View& c, const int32_t* cu, int64_t n, const char* what, Kv4Tokens* t) {
+  if (n < 0 || n >= 1ll << 31) return set_error(kErrInvalid, "%s: %lld new tokens", what, (long long)n);
+  if (!cu && (c.seqs == 0 ? n != 0 : n % c.seqs != 0))
+    return set_error(kErrInvalid, "%s: %lld new tokens for %u sequences without offsets", what, (long long)n, c.seqs);
+  if (c.seqs == 0 && n != 0) return set_error(kErrInvalid, "%s: new tokens of no sequence", what);
+  t->cu = cu;
+  t->n = (int32_t)n;
+  t->each = cu || c.seqs == 0 ? 0 : (int32_t)(n / c.seqs);
+  return kOk;
+}
+
+static int kv4_float(int32_t dtype, const char* what) {
+  if (dtype != kF32 && dtype != kBF16 && dtype != kF16)
+    return set_error(kErrInvalid, "%s: float32, bfloat16 or float16 tensors, not dtype %d", what, dtype);
+  return kOk;
+}
+
+// Rows of a strided [n, heads, dim] tensor are read 16 bytes at a time.
+static int kv4_strided(const void* p, int32_t dtype, int64_t sn, int64_t sh, const char* what) {
+  const int64_t per = dtype == kF32 ? 4 : 8;
+  if (!aligned(p, 16) || sn % per != 0 || sh % per != 0)
+    return set_error(kErrInvalid, "%s: rows must start on 16 bytes", what);
+  return kOk;
+}
+
+static int to_query(const Kv4View& c, int dim, const vqx_kv4_query* q, const char* what, Kv4Query* v) {
+  if (!q) return set_error(kErrInvalid, "%s: query is NULL", what);
+  int rc = kv4_float(q->dtype, what);
+  if (rc == kOk) rc = to_tokens(c, q->cu, q->n, what, &v->tokens);
+  if (rc != kOk) return rc;
+  if (q->heads <= 0 || q->heads % (int32_t)c.kv != 0)
+    return set_error(kErrInvalid, "%s: %d query heads for %u kv heads", what, q->heads, c.kv);
+  if (q->n > 0 && !q->q) return set_error(kErrInvalid, "%s: null tensor", what);
+  rc = kv4_strided(q->q, q->dtype, q->stride_n, q->stride_h, what);
+  if (rc != kOk) return rc;
+  if (!(q->softcap >= 0.0f) || q->softcap > 3.0e38f)
+    return set_error(kErrInvalid, "%s: a softcap is positive, or 0 for none", what);
+  if (q->window < 0) return set_error(kErrInvalid, "%s: a window is positive, or 0 for none", what);
+  if (q->most < 0) return set_error(kErrInvalid, "%s: most is negative", what);
+  v->q = q->q;
+  v->sn = q->stride_n;
+  v->sh = q->stride_h;
+  v->heads = q->heads;
+  v->group = q->heads / (int32_t)c.kv;
+  v->most = q->cu ? (q->most == 0 || q->most > q->n ? (int32_t)q->n : q->most) : v->tokens.each;
+  if ((int64_t)v->most * v->group >= 1ll << 30)
+    return set_error(kErrUnsupported, "%s: 2^30 query rows or more for a kv head", what);
+  v->window = q->window;
+  v->scale = q->scale;
+  v->softcap = q->softcap;
+  v->slopes = q->slopes;
+  (void)dim;
+  return kOk;
+}
 
 extern "C" {
 
@@ -528,6 +623,105 @@ int vqx_chol_inverse_block(const float* a, int64_t lda, int32_t n, float* li, in
                            vqx_stream_t stream) {
   g_err[0] = 0;
   return chol_inverse_block(a, lda, n, li, ldl, info, (hipStream_t)stream);
+}
+
+int vqx_kv4_append(const vqx_kv4_cache* cache, const void* key, const void* value, int32_t dtype, int64_t n,
+                   int64_t key_stride_n, int64_t key_stride_h, int64_t value_stride_n, int64_t value_stride_h,
+                   const int32_t* cu, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Tokens t;
+  int rc = to_view(cache, "kv4_append", &c);
+  if (rc == kOk) rc = kv4_float(dtype, "kv4_append");
+  if (rc == kOk) rc = to_tokens(c, cu, n, "kv4_append", &t);
+  if (rc != kOk || n == 0) return rc;
+  if (!key || !value) return set_error(kErrInvalid, "kv4_append: null tensor");
+  rc = kv4_strided(key, dtype, key_stride_n, key_stride_h, "kv4_append");
+  if (rc == kOk) rc = kv4_strided(value, dtype, value_stride_n, value_stride_h, "kv4_append");
+  if (rc != kOk) return rc;
+  return kv4_append(c, cache->dim, t, key, value, dtype, key_stride_n, key_stride_h, value_stride_n, value_stride_h,
+                    (hipStream_t)stream);
+}
+
+int vqx_kv4_read(const vqx_kv4_cache* cache, void* key, void* value, int32_t dtype, int64_t n, const int32_t* cu,
+                 vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Tokens t;
+  int rc = to_view(cache, "kv4_read", &c);
+  if (rc == kOk) rc = kv4_float(dtype, "kv4_read");
+  if (rc == kOk) rc = to_tokens(c, cu, n, "kv4_read", &t);
+  if (rc != kOk || n == 0) return rc;
+  if (!key || !value) return set_error(kErrInvalid, "kv4_read: null tensor");
+  if (!aligned(key, 16) || !aligned(value, 16))
+    return set_error(kErrInvalid, "kv4_read: outputs must be 16-byte aligned");
+  return kv4_read(c, cache->dim, t, key, value, dtype, (hipStream_t)stream);
+}
+
+int vqx_kv4_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return set_error(kErrInvalid, "kv4_attention_workspace_size: bytes is NULL");
+  Kv4View c;
+  Kv4Query q;
+  int rc = to_view(cache, "kv4_attention", &c);
+  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_attention", &q);
+  if (rc != kOk) return rc;
+  *bytes = kv4_workspace(c, cache->dim, q, query->dtype);
+  return kOk;
+}
+
+int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Query q;
+  int rc = to_view(cache, "kv4_attention", &c);
+  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_attention", &q);
+  if (rc != kOk || query->n == 0) return rc;
+  if (!out || !lse) return set_error(kErrInvalid, "kv4_attention: null tensor");
+  if (!aligned(out, 16)) return set_error(kErrInvalid, "kv4_attention: out must be 16-byte aligned");
+  const int64_t need = kv4_workspace(c, cache->dim, q, query->dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(kErrInvalid, "kv4_attention: needs a 16-byte aligned workspace of %lld bytes, not %lld",
+                     (long long)need, (long long)workspace_bytes);
+  return kv4_attention(c, cache->dim, q, query->dtype, out, lse, (float*)workspace, (hipStream_t)stream);
+}
+
+int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, const float* lse, float* weights,
+                       int64_t weights_len, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Query q;
+  int rc = to_view(cache, "kv4_accumulate", &c);
+  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_accumulate", &q);
+  if (rc != kOk || query->n == 0) return rc;
+  if (!lse || !weights) return set_error(kErrInvalid, "kv4_accumulate: null tensor");
+  if (weights_len < 0) return set_error(kErrInvalid, "kv4_accumulate: weights of %lld tokens", (long long)weights_len);
+  return kv4_accumulate(c, cache->dim, q, query->dtype, lse, weights, weights_len, (hipStream_t)stream);
+}
+
+int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weights_len, int32_t budget, int32_t recent,
+                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c, o;
+  int rc = to_view(cache, "kv4_evict", &c);
+  if (rc == kOk) rc = to_view(out, "kv4_evict (kept)", &o);
+  if (rc != kOk) return rc;
+  if (out->dim != cache->dim || o.kv != c.kv || o.seqs != c.seqs)
+    return set_error(kErrInvalid, "kv4_evict: the caches differ in sequences, kv heads or head size");
+  if (budget < 1 || (int64_t)budget > (int64_t)o.cap)
+    return set_error(kErrInvalid, "kv4_evict: a budget of %d tokens, room for %u", budget, o.cap);
+  if (recent < 0 || recent > budget)
+    return set_error(kErrInvalid, "kv4_evict: %d latest tokens of a budget of %d", recent, budget);
+  if (weights_len < 0) return set_error(kErrInvalid, "kv4_evict: weights of %lld tokens", (long long)weights_len);
+  if (c.seqs > 0 && (!weights || !index || !out_weights)) return set_error(kErrInvalid, "kv4_evict: null tensor");
+  const uint64_t in_bytes = 2 * c.plane_rows * (uint64_t)(cache->dim / 2),
+                 out_bytes = 2 * o.plane_rows * (uint64_t)(cache->dim / 2);
+  const uint64_t a = (uint64_t)(uintptr_t)c.codes, z = (uint64_t)(uintptr_t)o.codes;
+  if (a < z + out_bytes && z < a + in_bytes)
+    return set_error(kErrInvalid, "kv4_evict: the kept tokens go to another cache, not onto this one");
+  return kv4_evict(c, cache->dim, weights, weights_len, budget, recent, o, index, out->lengths, out_weights,
+                   (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,858 @@
+// Attention over a 4-bit cache of keys and values.
+//
+// The scores of 16 query rows are formed transposed, S^T = K Q^T, so that a
+// lane of the accumulator has one row's scores of several tokens, and the
+// output likewise, O^T = V^T P^T: a row's running maximum and sum are then
+// values of its lanes, and the weights P leave the first product in the very
+// layout the second one takes them in.
+//
+// Keys go into the matrix instruction as they are stored: the scaled fp4 form
+// takes 32 codes a lane and one E8M0 byte for them.  Its other operand holds a
+// query as a sum of e4m3 terms with one power of two for each row: a term has
+// 4 significant bits, so 2 of them are a bf16 query, 3 a fp16 one and 6 a fp32
+// one, exactly where a value is within 2^-14 of its row's largest and to 2^-22
+// of that one below.  Values are turned into bf16, which holds every code times
+// its scale exactly, and meet the weights as 2 bf16 terms, 3 for fp32 outputs:
+// a weight is off by 2^-16 or 2^-24 of itself, well below the half step of its
+// output (2^-8 and 2^-11, 2^-24).  Everything else (scores, maxima, sums,
+// outputs until their one rounding) is fp32.
+#include "vqx_kv4.h"
+
+namespace vqx {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+struct Bf16 {};
+struct F16 {};
+template <typename T>
+struct Terms;
+template <>
+struct Terms<Bf16> {
+  static constexpr int kQ = 2, kP = 2;
+};
+template <>
+struct Terms<F16> {
+  static constexpr int kQ = 3, kP = 2;
+};
+template <>
+struct Terms<float> {
+  static constexpr int kQ = 6, kP = 3;
+};
+
+constexpr int kRows = 16;       // query rows of a tile
+constexpr int kStep = 32;       // tokens of a wave's step
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+constexpr float kLowest = -3.0e38f;  // below every finite score, and finite: no inf - inf
+// A row's reference stays until a score passes it by this (in powers of two):
+// the weights then stay below 2^8, and the sums are rescaled a few times only.
+constexpr float kSlack = 8.0f;
+
+// 16 values from p as fp32.
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[4 * k + i] = a[i];
+  }
+}
+__device__ __forceinline__ void load16(const Bf16* p, float (&x)[16]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u32x4 a = reinterpret_cast<const u32x4*>(p)[k];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[8 * k + 2 * i] = u2f(a[i] << 16), x[8 * k + 2 * i + 1] = u2f(a[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void load16(const F16* p, float (&x)[16]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u32x4 a = reinterpret_cast<const u32x4*>(p)[k];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[8 * k + 2 * i] = h2f_exact(a[i] & 0xFFFFu), x[8 * k + 2 * i + 1] = h2f_exact(a[i] >> 16);
+  }
+}
+__device__ __forceinline__ const float* element(const void* p, int64_t i, float) {
+  return static_cast<const float*>(p) + i;
+}
+template <typename T>
+__device__ __forceinline__ const T* element(const void* p, int64_t i, T) {
+  return reinterpret_cast<const T*>(static_cast<const uint16_t*>(p) + i);
+}
+
+// The e4m3 terms of one row of a tile, as the scaled product's B operand: lane
+// (row, g) has elements 16 g .. 16 g + 15 of each half of 64 of a group of 128.
+template <int D, typename T>
+struct QueryTerms {
+  static constexpr int kGroups = (D + 127) / 128;
+  static constexpr int kTerms = Terms<T>::kQ;
+  i32x8 v[kTerms][kGroups];
+  int scale;  // the first term's E8M0 byte; each further one is 4 less
+
+  // p: the row's first element, or NULL for a row of zeros
+  __device__ __forceinline__ void load(const void* p, int64_t at, bool live, int g) {
+    constexpr int kHalves = D / 64;
+    float x[kHalves][16];
+#pragma unroll
+    for (int k = 0; k < kHalves; ++k) {
+      if (live) {
+        load16(element(p, at + 64 * k + 16 * g, T()), x[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[k][i] = 0.0f;
+      }
+    }
+    uint32_t amax = 0;
+#pragma unroll
+    for (int k = 0; k < kHalves; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) amax = umax32(amax, f2u(x[k][i]) & 0x7FFFFFFFu);
+    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 16));
+    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 32));
+    // the largest in [2^7, 2^8), below e4m3's 448; a row below 2^-90 keeps that
+    // scale, one with an infinity or a NaN becomes NaN (past 464 there is no value)
+    int e = amax < 0x7F800000u ? (int)(amax >> 23) - 127 : 0;
+    if (e < -90) e = -90;
+    const float r = exp2i(7 - e);
+    scale = e - 7 + 127;
+#pragma unroll
+    for (int k = 0; k < kHalves; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[k][i] *= r;
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t) {
+#pragma unroll
+      for (int k = 0; k < 2 * kGroups; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int w = 0;
+          if (k < kHalves) {
+            float* y = &x[k < kHalves ? k : 0][4 * i];
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+            if (t + 1 < kTerms) {
+              const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+              y[0] = (y[0] - a.x) * 16.0f, y[1] = (y[1] - a.y) * 16.0f;
+              y[2] = (y[2] - b.x) * 16.0f, y[3] = (y[3] - b.y) * 16.0f;
+            }
+          }
+          v[t][k / 2][4 * (k & 1) + i] = w;
+        }
+      }
+    }
+  }
+};
+
+// How a call is cut up.  A tile is 16 query rows of one kv head (row r is new
+// token r / group, head r % group); each split of a tile's tokens leaves its
+// sums in the workspace: 16 * D outputs, 16 references and 16 sums.
+struct Kv4Plan {
+  int32_t tiles, chunk, splits;
+};
+
+// Where the rows of one tile stand.
+struct TileRows {
+  int first, count;  // the sequence's first new token and their number
+  int base;          // position of new token 0
+  int rows;          // count * group
+  int lo, hi;        // tokens that any row of the tile sees: [lo, hi), lo a multiple of kStep
+  int pos_min, pos_max;
+};
+
+__device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile, int tile_size) {
+  TileRows r;
+  kv4_span(q.tokens, b, r.first, r.count);
+  const int length = c.lengths[b];
+  r.base = length - r.count;
+  const int n = r.count < q.most ? r.count : q.most;
+  r.rows = n * q.group;
+  const int r0 = tile * tile_size, r1 = r0 + tile_size < r.rows ? r0 + tile_size : r.rows;
+  r.pos_min = r.base + r0 / q.group;
+  r.pos_max = r1 > r0 ? r.base + (r1 - 1) / q.group : -1;
+  r.hi = r.pos_max + 1 < 0 ? 0 : ((uint32_t)(r.pos_max + 1) > c.cap ? (int)c.cap : r.pos_max + 1);
+  r.lo = 0;
+  if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(kStep - 1);
+  if (r.lo > r.hi) r.lo = r.hi & ~(kStep - 1);
+  return r;
+}
+
+// What a score becomes, in powers of two: capped by a tanh, less its slope for
+// each token of distance.
+struct Curve {
+  float scale;          // of a plain score
+  float inner, outer;   // capped: outer * tanh(score * inner)
+  float slope;
+  bool capped;
+};
+
+// tanh to a few units of fp32: near 0 by its series (the next term is below
+// 2^-26 of the sum), beyond by the exponential.
+__device__ __forceinline__ float tanh32(float x) {
+  const float a = __builtin_fabsf(x), z = x * x;
+  const float s = x + x * z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * 0.0218694885f)));
+  const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * (2.0f * kLog2e)));
+  return a < 0.25f ? s : __builtin_copysignf(t, x);
+}
+
+__device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
+  Curve k;
+  k.scale = q.scale * kLog2e;
+  k.capped = q.softcap != 0.0f;
+  k.inner = k.capped ? q.scale / q.softcap : 0.0f;
+  k.outer = q.softcap * kLog2e;
+  k.slope = q.slopes ? q.slopes[head] * kLog2e : 0.0f;
+  return k;
+}
+
+template <bool kExtra>
+__device__ __forceinline__ float curved(const Curve& k, float s, int away) {
+  if (!kExtra) return s * k.scale;
+  const float x = k.capped ? k.outer * tanh32(s * k.inner) : s * k.scale;
+  return x - k.slope * (float)away;
+}
+
+// The keys and values of one step of 32 tokens as a wave's loads leave them.
+// Keys: lane (token & 15, g) has block g of its token, twice.  Values: lane
+// (m, g) has the D / 16 elements from m D / 16 of tokens 4 g .. 4 g + 3 and
+// 16 + 4 g .. 16 + 4 g + 3, and all scale bytes of those tokens.
+template <int D>
+struct Loaded {
+  static constexpr int kGroups = (D + 127) / 128;
+  static constexpr int kWords = D == 256 ? 2 : 1;     // of a token's values
+  static constexpr int kScaleWords = D / 32;          // of four tokens' scales
+  u32x4 k[2][kGroups];
+  uint32_t ks[2][kGroups];
+  uint32_t v[8][kWords];
+  uint32_t vs[2][kScaleWords];
+  uint32_t valid;  // bit t: token t of the step is there
+  int t0;
+};
+
+template <int D>
+__device__ __forceinline__ void load_values(const uint8_t* p, uint32_t (&w)[Loaded<D>::kWords]) {
+  if constexpr (D == 64) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else if constexpr (D == 128) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(p);
+    w[0] = a[0], w[1] = a[1];
+  }
+}
+
+struct __attribute__((packed, aligned(1))) Raw16 {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(1))) Raw8 {
+  u32x2 v;
+};
+
+template <int D, bool kKeys, bool kValues>
+__device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t page, bool aligned_pages, int t0,
+                                          int hi, int lane, Loaded<D>& s) {
+  constexpr int kRow = D / 2, kScales = D / 32, kGroups = Loaded<D>::kGroups;
+  const int m = lane & 15, g = lane >> 4;
+  s.t0 = t0;
+  if (aligned_pages && t0 + kStep <= hi) {
+    // the whole step lies on one page: one base, and offsets that are constants
+    const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane((int)page);
+    const uint32_t row = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_row(c, pg, h, (uint32_t)t0));
+    s.valid = pg < c.pages ? 0xFFFFFFFFu : 0u;
+    if constexpr (kKeys) {
+      const uint8_t* kc = c.codes + (uint64_t)row * kRow;
+      const uint8_t* ks = c.scales + (uint64_t)row * kScales;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int a = 0; a < kGroups; ++a) {
+          const uint32_t block = D == 64 ? (g & 1) : 4 * a + g;
+          s.k[i][a] = *reinterpret_cast<const u32x4*>(kc + (uint32_t)(i * 16 * kRow) + m * kRow + block * 16);
+          s.ks[i][a] = ks[(uint32_t)(i * 16 * kScales) + m * kScales + block];
+        }
+    }
+    if constexpr (kValues) {
+      const uint64_t vrow = c.plane_rows + row;
+      const uint8_t* vc = c.codes + vrow * kRow;
+      const uint8_t* vs = c.scales + vrow * kScales;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        load_values<D>(vc + (uint32_t)(4 * g * kRow + m * (kRow / 16)) + ((j >> 2) * 16 + (j & 3)) * kRow, s.v[j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // four tokens' scales are next to each other, not always on 16 bytes
+        const uint8_t* p = vs + (uint32_t)(4 * g * kScales) + i * 16 * kScales;
+        if constexpr (D == 64) {
+          const u32x2 a = reinterpret_cast<const Raw8*>(p)->v;
+          s.vs[i][0] = a[0], s.vs[i][1] = a[1];
+        } else {
+#pragma unroll
+          for (int k = 0; k < kScales / 4; ++k) {
+            const u32x4 a = reinterpret_cast<const Raw16*>(p)[k].v;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s.vs[i][4 * k + x] = a[x];
+          }
+        }
+      }
+    }
+    return;
+  }
+  // lane l (and l + 32) finds the row of token l; past the end it is the last
+  // token's, which nothing reads beyond and no row counts
+  const int t = t0 + (lane & 31), tc = t < hi ? t : hi - 1;
+  const uint32_t mine = kv4_row(c, page, h, (uint32_t)tc);
+  s.valid = (uint32_t)__ballot(t < hi && page < c.pages);
+  if constexpr (kKeys) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint64_t row = (uint32_t)__shfl((int)mine, 16 * i + m);
+#pragma unroll
+      for (int a = 0; a < kGroups; ++a) {
+        const uint32_t block = D == 64 ? (g & 1) : 4 * a + g;
+        s.k[i][a] = *reinterpret_cast<const u32x4*>(c.codes + row * kRow + block * 16);
+        s.ks[i][a] = c.scales[row * kScales + block];
+      }
+    }
+  }
+  if constexpr (kValues) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t row = c.plane_rows + (uint32_t)__shfl((int)mine, (j >> 2) * 16 + 4 * g + (j & 3));
+      load_values<D>(c.codes + row * kRow + m * (kRow / 16), s.v[j]);
+      const uint8_t* p = c.scales + row * kScales;
+      if constexpr (D == 64) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(p);
+        s.vs[j >> 2][(j & 3) >> 1] = (j & 1) ? s.vs[j >> 2][(j & 3) >> 1] | w << 16 : w;
+      } else if constexpr (D == 128) {
+        s.vs[j >> 2][j & 3] = *reinterpret_cast<const uint32_t*>(p);
+      } else {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(p);
+        s.vs[j >> 2][2 * (j & 3)] = a[0], s.vs[j >> 2][2 * (j & 3) + 1] = a[1];
+      }
+    }
+  }
+}
+
+// Scores of the step's tokens 16 i + 4 g + r in x[4 i + r], lane (row, g).
+template <int D, typename T>
+__device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loaded<D>& s, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int a = 0; a < Loaded<D>::kGroups; ++a) {
+      const i32x8 k = {(int)s.k[i][a][0], (int)s.k[i][a][1], (int)s.k[i][a][2], (int)s.k[i][a][3], 0, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < Terms<T>::kQ; ++t)
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.v[t][a], acc, 4, 0, 0, (int)s.ks[i][a], 0,
+                                                               q.scale - 4 * t);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[4 * i + r] = acc[r];
+  }
+}
+
+// The row's curve and mask on those scores; seen: bit 4 i + r.
+template <bool kExtra>
+__device__ __forceinline__ void finish_scores(const Curve& k, float (&x)[8], uint32_t valid, int t0, int g, int pos,
+                                              int window, bool masked, uint32_t& seen) {
+  seen = 0xFFu;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int t = t0 + (j >> 2) * 16 + 4 * g + (j & 3);
+    x[j] = curved<kExtra>(k, x[j], pos - t);
+  }
+  if (masked) {
+    seen = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = t0 + u;
+      const bool in = (valid >> u & 1u) && t <= pos && (window == 0 || t > pos - window);
+      x[j] = in ? x[j] : -__builtin_huge_valf();
+      seen |= (uint32_t)in << j;
+    }
+  }
+}
+
+__device__ __forceinline__ bool needs_mask(const TileRows& r, uint32_t valid, int t0, int window) {
+  return valid != 0xFFFFFFFFu || t0 + kStep - 1 > r.pos_min || (window && t0 <= r.pos_max - window);
+}
+
+// bf16x2 words of two values whose codes' byte is b of w
+template <int kByte>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte));
+}
+
+// Few rows, many tokens: the cache is read once for each tile of 16 rows, and
+// that reading is the bound.  A workgroup has one tile, one kv head and one
+// run of tokens; its four waves take steps of 32 tokens in turn, each straight
+// from memory into the operands' registers, one step ahead, and are joined at
+// the end.
+template <int D, typename T, bool kExtra>
+__global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
+                                                       float* ws) {
+  constexpr int kTiles = D / 16;      // of 16 output elements
+  constexpr int kPer = D / 4;         // output elements of a lane
+  constexpr int kPad = D + 4;
+  __shared__ __align__(16) float part[2][kRows][kPad];
+  __shared__ float part_m[2][kRows], part_l[2][kRows];
+  __shared__ uint32_t part_bad[2][kRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const uint32_t split = blockIdx.x % (uint32_t)plan.splits, slot = blockIdx.x / (uint32_t)plan.splits;
+  const int tile = (int)(slot % (uint32_t)plan.tiles);
+  const uint32_t b = slot / (uint32_t)plan.tiles / c.kv, h = slot / (uint32_t)plan.tiles % c.kv;
+  const TileRows rows = tile_rows(c, q, b, tile, kRows);
+  const int r = tile * kRows + n;
+  const bool live = r < rows.rows;
+  const int token = r / q.group, head = (int)h * q.group + r % q.group;
+  const int64_t at_row = (int64_t)(rows.first + token) * q.heads + head;
+  if (rows.count > q.most && tile == 0 && split == 0) {
+    // more new tokens than the call was told of: these rows have no result
+    const int64_t extra = (int64_t)(rows.count - q.most) * q.group;
+    for (int64_t e = tid; e < extra; e += 256) {
+      const int64_t row = (int64_t)(rows.first + q.most + e / q.group) * q.heads + (int64_t)h * q.group + e % q.group;
+      lse[row] = __builtin_nanf("");
+      for (int d = 0; d < D; ++d) {
+        if constexpr (sizeof(T) == 4)
+          static_cast<float*>(out)[row * D + d] = __builtin_nanf("");
+        else
+          static_cast<uint16_t*>(out)[row * D + d] = 0x7FFFu;
+      }
+    }
+  }
+  if (tile * kRows >= rows.rows) return;
+  const int begin = rows.lo + (int)split * plan.chunk;
+  int end = begin + plan.chunk;
+  if (end > rows.hi) end = rows.hi;
+  if (begin >= end && split > 0) return;
+  const int steps = begin < end ? (end - begin + kStep - 1) / kStep : 0;
+  const int pos = live ? rows.base + token : -1;
+  const Curve curve = curve_of(q, live ? head : (int)h * q.group);
+  const bool aligned_pages = !c.table || c.size % kStep == 0;
+
+  float m = kLowest, l = 0.0f;
+  uint32_t bad = 0;  // blocks of values that are NaN in a token the row sees
+  f32x4 acc[kTiles];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0, 0, 0, 0};
+
+  if (wave < steps) {
+    QueryTerms<D, T> terms;
+    terms.load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
+
+    // the page of this lane's token in the wave's s-th step
+    auto page_of = [&](int s) -> uint32_t {
+      if (!c.table) return b;
+      int t = begin + s * kStep + (lane & 31);
+      return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
+    };
+    auto work = [&](const Loaded<D>& s) {
+      float x[8];
+      step_scores<D, T>(terms, s, x);
+      const bool masked = needs_mask(rows, s.valid, s.t0, q.window);
+      uint32_t seen;
+      finish_scores<kExtra>(curve, x, s.valid, s.t0, g, pos, q.window, masked, seen);
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, x[j]);
+      if (__ballot(top > m + kSlack)) {
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float next = __builtin_fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) acc[j] *= f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - m), l += x[j];
+      // the weights' bf16 terms, two tokens a word
+      u32x4 p[Terms<T>::kP];
+#pragma unroll
+      for (int t = 0; t < Terms<T>::kP; ++t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+          p[t][j] = w;
+          if (t + 1 < Terms<T>::kP) x[2 * j] -= u2f(w << 16), x[2 * j + 1] -= u2f(w & 0xFFFF0000u);
+        }
+      }
+      // this lane's block of each token's scales
+      float vs[8];
+      const uint32_t block = (uint32_t)n * (D / 16) / 32;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t w;
+        if constexpr (D == 64)
+          w = s.vs[j >> 2][(j & 3) >> 1] >> (16 * (j & 1));
+        else if constexpr (D == 128)
+          w = s.vs[j >> 2][j & 3];
+        else
+          w = block >= 4 ? s.vs[j >> 2][2 * (j & 3) + 1] : s.vs[j >> 2][2 * (j & 3)];
+        vs[j] = u2f((w >> (8 * (block & 3)) & 0xFFu) << 23);
+      }
+      float most = vs[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) most = __builtin_fmaxf(most, vs[j]);
+      if (__ballot(most == __builtin_huge_valf())) {
+        // byte 255: a weight of 0 must not meet a NaN.  The value is taken as
+        // tiny, and the rows that see the token note its blocks.
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t nan = 0;
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            const int byte = (j & 3) * (D / 32) + k;
+            nan |= (uint32_t)((s.vs[j >> 2][byte >> 2] >> (8 * (byte & 3)) & 0xFFu) == 255u) << k;
+          }
+          if (seen >> j & 1u) bad |= nan;
+          if (vs[j] == __builtin_huge_valf()) vs[j] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < Loaded<D>::kWords; ++w) {
+        // byte by byte: two elements of two tokens in one word each, then the
+        // halves exchanged so that a word has two tokens of one element
+        auto product = [&](auto which) {
+          constexpr int kByte = decltype(which)::value;
+          u32x4 even, odd;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t x0 = fp4_pair<kByte>(s.v[2 * j][w], vs[2 * j]),
+                           x1 = fp4_pair<kByte>(s.v[2 * j + 1][w], vs[2 * j + 1]);
+            even[j] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+            odd[j] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+          }
+          constexpr int kTile = 2 * kByte;
+#pragma unroll
+          for (int t = 0; t < Terms<T>::kP; ++t) {
+            const bf16x8 pt = __builtin_bit_cast(bf16x8, p[t]);
+            acc[8 * w + kTile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pt,
+                                                                         acc[8 * w + kTile], 0, 0, 0);
+            acc[8 * w + kTile + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pt,
+                                                                             acc[8 * w + kTile + 1], 0, 0, 0);
+          }
+        };
+        product(std::integral_constant<int, 0>());
+        product(std::integral_constant<int, 1>());
+        if constexpr (D > 64) {
+          product(std::integral_constant<int, 2>());
+          product(std::integral_constant<int, 3>());
+        }
+      }
+    };
+
+    Loaded<D> one, two;
+    uint32_t page = page_of(wave);
+    load_step<D, true, true>(c, h, page, aligned_pages, begin + wave * kStep, end, lane, one);
+    page = page_of(wave + kWaves);
+    int s = wave;
+    while (true) {
+      if (s + kWaves < steps)
+        load_step<D, true, true>(c, h, page, aligned_pages, begin + (s + kWaves) * kStep, end, lane, two);
+      page = page_of(s + 2 * kWaves);
+      work(one);
+      s += kWaves;
+      if (s >= steps) break;
+      if (s + kWaves < steps)
+        load_step<D, true, true>(c, h, page, aligned_pages, begin + (s + kWaves) * kStep, end, lane, one);
+      page = page_of(s + 2 * kWaves);
+      work(two);
+      s += kWaves;
+      if (s >= steps) break;
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    bad |= (uint32_t)__shfl_xor((int)bad, 16);
+    bad |= (uint32_t)__shfl_xor((int)bad, 32);
+  }
+
+  // join the waves: 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+  for (int half = 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+      const int z = wave - half;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 4)
+          *reinterpret_cast<f32x4*>(&part[z][n][g * kPer + i * kTiles + j]) =
+              f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+      if (g == 0) part_m[z][n] = m, part_l[z][n] = l, part_bad[z][n] = bad;
+    }
+    __syncthreads();
+    if (wave < half) {
+      const float m1 = part_m[wave][n], top = __builtin_fmaxf(m, m1);
+      const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+      m = top;
+      l = l * f0 + part_l[wave][n] * f1;
+      bad |= part_bad[wave][n];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 4) {
+          const f32x4 o = *reinterpret_cast<const f32x4*>(&part[wave][n][g * kPer + i * kTiles + j]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[j + x][i] = acc[j + x][i] * f0 + o[x] * f1;
+        }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  const float inv = plan.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      const uint32_t block = (uint32_t)(g * kPer + i * kTiles + j) / 32;
+      acc[j][i] = bad >> block & 1u ? __builtin_nanf("") : acc[j][i] * inv;
+    }
+  if (plan.splits > 1) {
+    float* o = ws + (int64_t)blockIdx.x * (kRows * D + 2 * kRows);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < kTiles; j += 4)
+        *reinterpret_cast<f32x4*>(o + n * D + g * kPer + i * kTiles + j) =
+            f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    if (g == 0) o[kRows * D + n] = m, o[kRows * D + kRows + n] = l;
+    return;
+  }
+  if (!live) return;
+  if (g == 0) lse[at_row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t d = at_row * D + g * kPer + i * kTiles;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < kTiles; j += 4)
+        *reinterpret_cast<f32x4*>(static_cast<float*>(out) + d + j) =
+            f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < kTiles; j += 2) {
+        uint32_t w;
+        if constexpr (std::is_same<T, Bf16>::value)
+          w = pack_bf16x2(acc[j][i], acc[j + 1][i]);
+        else
+          w = f2h_exact(acc[j][i]) | f2h_exact(acc[j + 1][i]) << 16;
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + d + j) = w;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void put(void* out, int64_t i, float v, float) { static_cast<float*>(out)[i] = v; }
+__device__ __forceinline__ void put(void* out, int64_t i, float v, Bf16) {
+  static_cast<uint16_t*>(out)[i] = (uint16_t)f2bf(v);
+}
+__device__ __forceinline__ void put(void* out, int64_t i, float v, F16) {
+  static_cast<uint16_t*>(out)[i] = (uint16_t)f2h_exact(v);
+}
+
+// The splits of one row joined, in their order: a workgroup a row, its waves
+// taking splits in turn.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
+                                                       const float* ws) {
+  constexpr int kPer = D / 64;
+  __shared__ float sum[kWaves][D], sum_l[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t slot = blockIdx.x / kRows, b = slot / (uint32_t)plan.tiles / c.kv,
+                 h = slot / (uint32_t)plan.tiles % c.kv;
+  const int tile = (int)(slot % (uint32_t)plan.tiles), n = blockIdx.x % kRows, r = tile * kRows + n;
+  const TileRows rows = tile_rows(c, q, b, tile, kRows);
+  if (r >= rows.rows) return;
+  const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
+  const float* first = ws + (int64_t)slot * plan.splits * (kRows * D + 2 * kRows);
+  constexpr int64_t kSlot = kRows * D + 2 * kRows;
+  float m = kLowest;
+  for (int s = lane; s < splits; s += 64) m = __builtin_fmaxf(m, first[s * kSlot + kRows * D + n]);
+  for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+  float l = 0.0f, o[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
+#pragma unroll 4
+  for (int s = wave; s < splits; s += kWaves) {
+    const float* p = first + s * kSlot;
+    const float f = __builtin_amdgcn_exp2f(p[kRows * D + n] - m);
+    l += p[kRows * D + kRows + n] * f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] += p[n * D + lane + 64 * k] * f;
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) sum[wave][lane + 64 * k] = o[k];
+  if (lane == 0) sum_l[wave] = l;
+  __syncthreads();
+  l = (sum_l[0] + sum_l[1]) + (sum_l[2] + sum_l[3]);
+  const int64_t row = (int64_t)(rows.first + r / q.group) * q.heads + (int)h * q.group + r % q.group;
+  if (threadIdx.x == 0) lse[row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  for (int d = threadIdx.x; d < D; d += 256)
+    put(out, row * D + d, ((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])) * inv, T());
+}
+
+// The attention weights of every row added to its kv head's tokens.  A wave
+// owns its tokens and walks over all rows, so that a token's sum has one order
+// and one writer; the rows' statistics are known (lse), so the values are not
+// read.
+template <int D, typename T, bool kExtra>
+__global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int chunk, int chunks, const float* lse,
+                                                        float* weights, int64_t weights_len) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const uint32_t slot = blockIdx.x / (uint32_t)chunks, b = slot / c.kv, h = slot % c.kv;
+  TileRows all = tile_rows(c, q, b, 0, 0x40000000);
+  int hi = all.hi < weights_len ? all.hi : (int)weights_len;
+  const int begin = all.lo + (int)(blockIdx.x % (uint32_t)chunks) * chunk;
+  int end = begin + chunk;
+  if (end > hi) end = hi;
+  const bool aligned_pages = !c.table || c.size % kStep == 0;
+  const int tiles = (all.rows + kRows - 1) / kRows;
+  float* w = weights + (int64_t)slot * weights_len;
+  for (int t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
+    const int t = t0 + (lane & 31);
+    const uint32_t page = kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
+    Loaded<D> s;
+    load_step<D, true, false>(c, h, page, aligned_pages, t0, end, lane, s);
+    float add[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add[j] = 0.0f;
+    for (int tile = 0; tile < tiles; ++tile) {
+      const TileRows rows = tile_rows(c, q, b, tile, kRows);
+      if (t0 >= rows.hi || t0 + kStep <= rows.lo) continue;
+      const int r = tile * kRows + n;
+      const bool live = r < rows.rows;
+      const int token = r / q.group, head = (int)h * q.group + r % q.group;
+      QueryTerms<D, T> terms;
+      terms.load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
+      const float base = live ? lse[(int64_t)(rows.first + token) * q.heads + head] * kLog2e : 0.0f;
+      float x[8];
+      step_scores<D, T>(terms, s, x);
+      uint32_t seen;
+      finish_scores<kExtra>(curve_of(q, live ? head : (int)h * q.group), x, s.valid, t0, g,
+                            live ? rows.base + token : -1, q.window,
+                            needs_mask(rows, s.valid, t0, q.window) || (tile + 1) * kRows > rows.rows, seen);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) add[j] += seen >> j & 1u ? __builtin_amdgcn_exp2f(x[j] - base) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      for (int d = 1; d < 16; d *= 2) add[j] += __shfl_xor(add[j], d);
+    }
+    // lane (j, g) writes token j of its group
+    float mine = add[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mine = n == j ? add[j] : mine;
+    const int u = (n >> 2) * 16 + 4 * g + (n & 3);
+    if (n < 8 && t0 + u < end && (s.valid >> u & 1u)) w[t0 + u] += mine;
+  }
+}
+
+Kv4Plan kv4_plan(const Kv4View& c, const Kv4Query& q) {
+  Kv4Plan p;
+  p.tiles = (int32_t)(((int64_t)q.most * q.group + kRows - 1) / kRows);
+  // the most tokens a tile can see
+  int64_t span = c.cap;
+  if (q.window) {
+    const int64_t seen = (int64_t)q.window + kRows / q.group + 2 + kStep;
+    if (seen < span) span = seen;
+  }
+  const int64_t heads = (int64_t)c.seqs * c.kv * p.tiles;
+  // enough workgroups for every compute unit to have some to wait with, none
+  // with fewer than two steps for each wave
+  const int64_t want = (4ll * num_cus() + heads - 1) / (heads > 0 ? heads : 1);
+  int64_t chunk = (span + want - 1) / want;
+  if (chunk < 2 * kWaves * kStep) chunk = 2 * kWaves * kStep;
+  chunk = (chunk + kWaves * kStep - 1) / (kWaves * kStep) * (kWaves * kStep);
+  p.chunk = (int32_t)chunk;
+  p.splits = (int32_t)((span + chunk - 1) / chunk);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+}  // namespace
+
+int64_t kv4_workspace(const Kv4View& c, int dim, const Kv4Query& q, int) {
+  if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return 0;
+  const Kv4Plan p = kv4_plan(c, q);
+  return p.splits > 1 ? (int64_t)c.seqs * c.kv * p.tiles * p.splits * (kRows * dim + 2 * kRows) * 4 : 0;
+}
+
+#define VQX_KV4_DIMS(CALL, T)  \
+  if (dim == 64)               \
+    CALL(64, T);               \
+  else if (dim == 128)         \
+    CALL(128, T);              \
+  else                         \
+    CALL(256, T)
+#define VQX_KV4_TYPES(CALL)    \
+  if (dtype == kBF16) {        \
+    VQX_KV4_DIMS(CALL, Bf16);  \
+  } else if (dtype == kF16) {  \
+    VQX_KV4_DIMS(CALL, F16);   \
+  } else {                     \
+    VQX_KV4_DIMS(CALL, float); \
+  }
+
+int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void* out, float* lse, float* ws,
+                  hipStream_t st) {
+  if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
+  const Kv4Plan p = kv4_plan(c, q);
+  const bool extra = q.softcap != 0.0f || q.slopes;
+  const int64_t slots = (int64_t)p.tiles * c.seqs * c.kv;
+  if (slots * (p.splits > kRows ? p.splits : kRows) >= 1ll << 31)
+    return set_error(kErrUnsupported, "kv4_attention: %lld tiles of %d splits do not fit a launch", (long long)slots,
+                     p.splits);
+  const dim3 grid((unsigned)(slots * p.splits));
+#define VQX_KV4_ROWS(D, T)                                                                                       \
+  do {                                                                                                           \
+    if (extra)                                                                                                   \
+      hipLaunchKernelGGL((kv4_rows_kernel<D, T, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);          \
+    else                                                                                                         \
+      hipLaunchKernelGGL((kv4_rows_kernel<D, T, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);         \
+    if (p.splits > 1)                                                                                            \
+      hipLaunchKernelGGL((kv4_join_kernel<D, T>), dim3((unsigned)(slots * kRows)), dim3(256), 0,  \
+                         st, c, q, p, out, lse, ws);                                                             \
+  } while (0)
+  VQX_KV4_TYPES(VQX_KV4_ROWS)
+#undef VQX_KV4_ROWS
+  return check_launch("kv4_attention");
+}
+
+int kv4_accumulate(const Kv4View& c, int dim, const Kv4Query& q, int dtype, const float* lse, float* weights,
+                   int64_t weights_len, hipStream_t st) {
+  if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
+  int64_t span = c.cap;
+  if (q.window && (int64_t)q.window + q.most + kStep < span) span = (int64_t)q.window + q.most + kStep;
+  const int64_t heads = (int64_t)c.seqs * c.kv;
+  const int64_t want = (8ll * num_cus() + heads - 1) / heads;
+  int64_t chunk = (span + want - 1) / want;
+  chunk = (chunk + kWaves * kStep - 1) / (kWaves * kStep) * (kWaves * kStep);
+  if (chunk < kWaves * kStep) chunk = kWaves * kStep;
+  const bool extra = q.softcap != 0.0f || q.slopes;
+  const int64_t chunks = (span + chunk - 1) / chunk;
+  if (chunks * heads >= 1ll << 31)
+    return set_error(kErrUnsupported, "kv4_accumulate: %lld runs of tokens do not fit a launch", (long long)(chunks * heads));
+  const dim3 grid((unsigned)(chunks * heads));
+#define VQX_KV4_WEIGH(D, T)                                                                                       \
+  do {                                                                                                            \
+    if (extra)                                                                                                    \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, true>), grid, dim3(256), 0, st, c, q, (int)chunk, (int)chunks, lse, weights,  \
+                         weights_len);                                                                            \
+    else                                                                                                          \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, false>), grid, dim3(256), 0, st, c, q, (int)chunk, (int)chunks, lse, weights, \
+                         weights_len);                                                                            \
+  } while (0)
+  VQX_KV4_TYPES(VQX_KV4_WEIGH)
+#undef VQX_KV4_WEIGH
+  return check_launch("kv4_accumulate");
+}
+
+}  // namespace vqx

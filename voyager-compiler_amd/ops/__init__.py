@@ -1,4 +1,4 @@
-"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``)."""
+"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``, ``kv4.py``)."""
 
 from .quantized import (  # noqa: F401
     calculate_mx_qparam,
@@ -12,3 +12,4 @@ from .quantized import (  # noqa: F401
     register_table,
     vmap,
 )
+from .kv4 import kv4_accumulate, kv4_append, kv4_attention, kv4_evict, kv4_read  # noqa: F401

@@ -1,0 +1,304 @@
+"""A serving cache of keys and values in 4 bits, and the attention that reads it.
+
+``torch.ops.quantized_ops.kv4_*``, this build's own: the reference has no cache.
+The cache holds keys and values in the packed form of ``quantize_mx_packed(x,
+"fp4_e2m1", -1, 32)``, page by page:
+
+* ``codes``  uint8 [2, pages, kv heads, page size, D / 2], keys then values,
+  element 2 i in the low nibble; D is 64, 128 or 256;
+* ``scales`` uint8 [2, pages, kv heads, page size, D / 32], E8M0, 255 for NaN;
+* ``table``  int32 [sequences, pages per sequence], or None: page b is
+  sequence b.  An entry outside [0, pages) is no page: what is on it is neither
+  written nor attended to;
+* ``lengths`` int32 [sequences]: the tokens of each, new ones included.
+
+New tokens come one sequence after another, those of sequence b at
+``cu[b]:cu[b + 1]`` (int32), or as many for each where ``cu`` is None, and stand
+at the end of their sequence.  ``most`` (with ``cu``): no sequence has more of
+them; without it the launch is as large as one sequence with all of them needs.
+
+A step of a server: ``kv4_append`` the new keys and values, ``kv4_attention``
+(and, where tokens are to be weighed, ``kv4_accumulate``), and where a cache
+has grown over its budget ``kv4_evict`` into another one.  All of it is
+enqueued on the current stream without a look at the device's data, so a decode
+step can be captured into a graph and replayed as ``lengths`` grows.
+"""
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib
+from .quantized import quantized_ops_lib
+
+_SCHEMAS = {
+    "kv4_append": (
+        "kv4_append(Tensor key, Tensor value, Tensor(a!) codes, Tensor(b!) scales, Tensor lengths, "
+        "Tensor? cu=None, Tensor? table=None) -> ()"),
+    "kv4_read": (
+        "kv4_read(Tensor codes, Tensor scales, Tensor lengths, SymInt n, Tensor? cu=None, Tensor? table=None, "
+        "ScalarType dtype=bfloat16) -> (Tensor, Tensor)"),
+    "kv4_attention": (
+        "kv4_attention(Tensor query, Tensor codes, Tensor scales, Tensor lengths, Tensor? cu=None, int? most=None, "
+        "Tensor? table=None, *, float? scale=None, float softcap=0.0, int window=0, Tensor? slopes=None) "
+        "-> (Tensor, Tensor)"),
+    "kv4_accumulate": (
+        "kv4_accumulate(Tensor query, Tensor lse, Tensor codes, Tensor scales, Tensor lengths, Tensor(a!) weights, "
+        "Tensor? cu=None, int? most=None, Tensor? table=None, *, float? scale=None, float softcap=0.0, "
+        "int window=0, Tensor? slopes=None) -> ()"),
+    "kv4_evict": (
+        "kv4_evict(Tensor codes, Tensor scales, Tensor weights, Tensor lengths, int budget, int recent, "
+        "Tensor(a!) out_codes, Tensor(b!) out_scales, Tensor(c!) out_weights, Tensor? table=None, "
+        "Tensor? out_table=None) -> (Tensor, Tensor)"),
+}
+for _s in _SCHEMAS.values():
+    quantized_ops_lib.define(_s)
+
+
+def _impl(name):
+    return torch.library.impl(quantized_ops_lib, name, "CUDA")
+
+
+_FLOATS = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _refuse(what, message):
+    raise ValueError(f"vqx: {what}: {message}")
+
+
+def _int32(t, shape, name, what, device):
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        _refuse(what, f"{name} must be a contiguous int32 tensor of shape {list(shape)}, "
+                      f"not {t.dtype} {list(t.shape)}")
+    if t.device != device:
+        _refuse(what, f"{name} is on {t.device}, the cache on {device}")
+    return t.data_ptr()
+
+
+def _cache(codes, scales, lengths, table, what):
+    """The cache as the library takes it.  Tensors that a kernel writes or
+    whose layout its indexes assume are checked, never copied."""
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        _refuse(what, f"codes and scales must be uint8, not {codes.dtype} and {scales.dtype}")
+    shape = codes.shape
+    if len(shape) != 5 or shape[0] != 2 or shape[4] not in (32, 64, 128):
+        _refuse(what, "codes must be [2, pages, kv heads, page size, D / 2] with D 64, 128 or 256, "
+                      f"not {list(shape)}")
+    if scales.shape[:4] != shape[:4] or scales.ndim != 5 or scales.shape[4] * 16 != shape[4]:
+        _refuse(what, f"scales must be [2, pages, kv heads, page size, D / 32], not {list(scales.shape)} "
+                      f"for codes {list(shape)}")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        _refuse(what, "codes and scales must be contiguous")
+    device = codes.device
+    if scales.device != device:
+        _refuse(what, f"scales are on {scales.device}, codes on {device}")
+    if lengths.ndim != 1:
+        _refuse(what, f"lengths must be [sequences], not {list(lengths.shape)}")
+    seqs = lengths.shape[0]
+    at, tab, per = _int32(lengths, (seqs,), "lengths", what, device), None, 0
+    if table is not None:
+        if table.ndim != 2:
+            _refuse(what, f"table must be [sequences, pages], not {list(table.shape)}")
+        per = table.shape[1]
+        tab = _int32(table, (seqs, per), "table", what, device)
+        if per == 0:
+            _refuse(what, "table has no pages for a sequence")
+    return _lib.VqxKv4Cache(codes.data_ptr(), scales.data_ptr(), tab, at, shape[1], per, shape[2], shape[3],
+                            2 * shape[4], seqs)
+
+
+def _offsets(cu, n, seqs, what, device):
+    if cu is not None:
+        return _int32(cu, (seqs + 1,), "cu", what, device)
+    if n % seqs if seqs else n:
+        _refuse(what, f"{n} new tokens for {seqs} sequences need cu")
+    return None
+
+
+def _rows(t, heads, dim, name, what, device):
+    """t [n, heads, dim] with rows that start on 16 bytes, copied if they do not."""
+    if t.ndim != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        _refuse(what, f"{name} must be [new tokens, {'heads' if heads is None else heads}, {dim}], "
+                      f"not {list(t.shape)}")
+    if t.dtype not in _FLOATS:
+        _refuse(what, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    if t.device != device:
+        _refuse(what, f"{name} is on {t.device}, the cache on {device}")
+    sn, sh, sd = t.stride()
+    size = t.element_size()
+    if sd != 1 or (sn * size) % 16 or (sh * size) % 16 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _query(query, cache, codes, cu, most, scale, softcap, window, slopes, what):
+    """(the queries as the library takes them, the tensor that holds them)."""
+    dim, kv, device = cache.dim, cache.kv_heads, codes.device
+    q = _rows(query, None, dim, "query", what, device)
+    n, heads = q.shape[0], q.shape[1]
+    if heads == 0 or heads % kv:
+        _refuse(what, f"{heads} query heads for {kv} kv heads")
+    offsets = _offsets(cu, n, cache.seqs, what, device)
+    if most is not None and most < (1 if n else 0):
+        _refuse(what, f"most is {most}")
+    if window < 0 or window > 0x7FFFFFFF:
+        _refuse(what, f"a window is positive, or 0 for none, not {window}")
+    if not 0.0 <= softcap < math.inf:
+        _refuse(what, f"a softcap is positive, or 0 for none, not {softcap}")
+    bias = None
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous():
+            _refuse(what, f"slopes must be a contiguous float32 tensor of {heads}, not {slopes.dtype} "
+                          f"{list(slopes.shape)}")
+        if slopes.device != device:
+            _refuse(what, f"slopes are on {slopes.device}, the cache on {device}")
+        bias = slopes.data_ptr()
+    sn, sh, _ = q.stride()
+    return _lib.VqxKv4Query(q.data_ptr(), offsets, bias, n, sn, sh, _FLOATS[q.dtype], heads,
+                            0 if most is None else min(most, n), window, dim ** -0.5 if scale is None else scale,
+                            softcap), q
+
+
+def _weights(weights, seqs, kv, name, what, device):
+    if weights.dtype != torch.float32 or weights.ndim != 3 or weights.shape[:2] != (seqs, kv) \
+            or not weights.is_contiguous():
+        _refuse(what, f"{name} must be a contiguous float32 tensor [{seqs}, {kv}, tokens], not {weights.dtype} "
+                      f"{list(weights.shape)}")
+    if weights.device != device:
+        _refuse(what, f"{name} are on {weights.device}, the cache on {device}")
+    return weights.data_ptr()
+
+
+@_impl("kv4_append")
+def kv4_append(key, value, codes, scales, lengths, cu=None, table=None):
+    """Quantize the new tokens' keys and values [n, kv heads, D] into their
+    places in the cache."""
+    what = "kv4_append"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    k = _rows(key, c.kv_heads, c.dim, "key", what, codes.device)
+    v = _rows(value, c.kv_heads, c.dim, "value", what, codes.device)
+    n = k.shape[0]
+    if v.shape[0] != n or v.dtype != k.dtype:
+        _refuse(what, f"key and value differ: {key.dtype} {list(key.shape)}, {value.dtype} {list(value.shape)}")
+    offsets = _offsets(cu, n, c.seqs, what, codes.device)
+    ks, vs = k.stride(), v.stride()
+    _lib.call("vqx_kv4_append", c, k.data_ptr(), v.data_ptr(), _FLOATS[k.dtype], n, ks[0], ks[1], vs[0], vs[1],
+              offsets, _lib.stream_of(codes))
+
+
+@_impl("kv4_read")
+def kv4_read(codes, scales, lengths, n, cu=None, table=None, dtype=torch.bfloat16):
+    """The keys and values [n, kv heads, D] of the n new tokens as the cache
+    holds them."""
+    what = "kv4_read"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    if dtype not in _FLOATS:
+        _refuse(what, f"float32, bfloat16 or float16 values, not {dtype}")
+    if n < 0:
+        _refuse(what, f"{n} new tokens")
+    offsets = _offsets(cu, n, c.seqs, what, codes.device)
+    k = torch.empty((n, c.kv_heads, c.dim), dtype=dtype, device=codes.device)
+    v = torch.empty_like(k)
+    _lib.call("vqx_kv4_read", c, k.data_ptr(), v.data_ptr(), _FLOATS[dtype], n, offsets, _lib.stream_of(codes))
+    return k, v
+
+
+@_impl("kv4_attention")
+def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None, *, scale=None, softcap=0.0,
+                  window=0, slopes=None):
+    """(out, lse) of the new tokens' queries [n, heads, D] over their
+    sequences: each sees what is at or before its place, the last `window`
+    tokens of it if that is not 0.  Scores are scale q.k (1 / sqrt(D)), capped to
+    softcap tanh(s / softcap) if that is not 0, less slopes[head] for each
+    token of distance.  out has the queries' dtype; lse [n, heads] is fp32.
+    A query that sees nothing has out 0 and lse -inf."""
+    what = "kv4_attention"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    qs, q = _query(query, c, codes, cu, most, scale, softcap, window, slopes, what)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    need = ctypes.c_int64(0)
+    _lib.call("vqx_kv4_attention_workspace_size", c, qs, need)
+    need = need.value
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else None
+    _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), ws, need, _lib.stream_of(codes))
+    return out, lse
+
+
+@_impl("kv4_accumulate")
+def kv4_accumulate(query, lse, codes, scales, lengths, weights, cu=None, most=None, table=None, *, scale=None,
+                   softcap=0.0, window=0, slopes=None):
+    """Add to weights (fp32 [sequences, kv heads, tokens]) what the attention of
+    these queries gives each cached token, over the new tokens and the query
+    heads of a kv head; lse as kv4_attention gives it."""
+    what = "kv4_accumulate"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    qs, q = _query(query, c, codes, cu, most, scale, softcap, window, slopes, what)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.device != q.device:
+        _refuse(what, f"lse must be a contiguous float32 tensor {list(q.shape[:2])}, not {lse.dtype} "
+                      f"{list(lse.shape)}")
+    w = _weights(weights, c.seqs, c.kv_heads, "weights", what, codes.device)
+    _lib.call("vqx_kv4_accumulate", c, qs, lse.data_ptr(), w, weights.shape[2], _lib.stream_of(codes))
+
+
+@_impl("kv4_evict")
+def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_scales, out_weights, table=None,
+              out_table=None):
+    """Keep min(budget, length) tokens of each sequence for each kv head, the
+    latest `recent` and the heaviest before them, in their order at the front of
+    the other cache; equal weights go by the lower place.  Returns (index int32
+    [sequences, kv heads, budget]: where each kept token was, -1 past the end;
+    the new lengths); out_weights gets their weights, 0 past the end."""
+    what = "kv4_evict"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    device = codes.device
+    kept = torch.empty_like(lengths)
+    o = _cache(out_codes, out_scales, kept, out_table, what)
+    if out_codes.device != device:
+        _refuse(what, f"the caches are on {device} and {out_codes.device}")
+    if not 1 <= budget < 2 ** 31 or not 0 <= recent <= budget:
+        _refuse(what, f"a budget of {budget} tokens, {recent} of them the latest")
+    w = _weights(weights, c.seqs, c.kv_heads, "weights", what, device)
+    ow = _weights(out_weights, c.seqs, c.kv_heads, "out_weights", what, device)
+    if out_weights.shape[2] != budget:
+        _refuse(what, f"out_weights are for {out_weights.shape[2]} tokens, the budget is {budget}")
+    index = torch.empty((c.seqs, c.kv_heads, budget), dtype=torch.int32, device=device)
+    _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow,
+              _lib.stream_of(codes))
+    return index, kept
+
+
+# ---------------------------------------------------------------------------
+# fake (meta) implementations for tracing
+# ---------------------------------------------------------------------------
+@torch.library.register_fake("quantized_ops::kv4_append")
+def _(key, value, codes, scales, lengths, cu=None, table=None):
+    return None
+
+
+@torch.library.register_fake("quantized_ops::kv4_read")
+def _(codes, scales, lengths, n, cu=None, table=None, dtype=torch.bfloat16):
+    shape = (n, codes.shape[2], 2 * codes.shape[4])
+    return codes.new_empty(shape, dtype=dtype), codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.register_fake("quantized_ops::kv4_attention")
+def _(query, codes, scales, lengths, cu=None, most=None, table=None, **kwargs):
+    return query.new_empty(query.shape), query.new_empty(query.shape[:2], dtype=torch.float32)
+
+
+@torch.library.register_fake("quantized_ops::kv4_accumulate")
+def _(query, lse, codes, scales, lengths, weights, cu=None, most=None, table=None, **kwargs):
+    return None
+
+
+@torch.library.register_fake("quantized_ops::kv4_evict")
+def _(codes, scales, weights, lengths, budget, recent, out_codes, out_scales, out_weights, table=None,
+      out_table=None):
+    return (lengths.new_empty((lengths.shape[0], codes.shape[2], budget)), torch.empty_like(lengths))
