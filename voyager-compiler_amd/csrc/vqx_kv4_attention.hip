@@ -6,24 +6,22 @@
 // values of its lanes, and the weights P leave the first product in the very
 // layout the second one takes them in.
 //
-// Keys go into the matrix instruction as they are stored: the scaled fp4 form
-// takes 32 codes a lane and one E8M0 byte for them.  Its other operand holds a
-// query as a sum of e4m3 terms with one power of two for each row: a term has
-// 4 significant bits, so 2 of them are a bf16 query, 3 a fp16 one and 6 a fp32
-// one, exactly where a value is within 2^-14 of its row's largest and to 2^-22
-// of that one below.  Values are turned into bf16, which holds every code times
-// its scale exactly, and meet the weights as 2 bf16 terms, 3 for fp32 outputs:
-// a weight is off by 2^-16 or 2^-24 of itself, well below the half step of its
-// output (2^-8 and 2^-11, 2^-24).  Everything else (scores, maxima, sums,
-// outputs until their one rounding) is fp32.
+// Both products are bf16 matrix products with fp32 sums.  Keys and values are
+// turned into bf16, which holds every code times its scale exactly.  A query is
+// 1, 2 or 3 bf16 terms (bf16, fp16, fp32), which hold it exactly; the weights
+// are 2, 3 for fp32 outputs, off by 2^-16 or 2^-24 of themselves: well below
+// the half step of their output (2^-8 and 2^-11, 2^-24).  Everything else
+// (scores, maxima, sums, outputs until their one rounding) is fp32.
+// The scaled product that takes fp4 as it is stored would save the keys'
+// conversion (32 of some 250 vector instructions a step), but its other operand
+// holds 4 bits, and what is 2^7 and more below the largest product of an
+// instruction is cut off: with a query as two e4m3 terms the scores were off by
+// 2^-17 of their sums' magnitude in the mean, against 2^-25 here.
 #include "vqx_kv4.h"
 
 namespace vqx {
 namespace {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 struct Bf16 {};
@@ -32,15 +30,15 @@ template <typename T>
 struct Terms;
 template <>
 struct Terms<Bf16> {
-  static constexpr int kQ = 2, kP = 2;
+  static constexpr int kQ = 1, kP = 2;
 };
 template <>
 struct Terms<F16> {
-  static constexpr int kQ = 3, kP = 2;
+  static constexpr int kQ = 2, kP = 2;
 };
 template <>
 struct Terms<float> {
-  static constexpr int kQ = 6, kP = 3;
+  static constexpr int kQ = 3, kP = 3;
 };
 
 constexpr int kRows = 16;       // query rows of a tile
@@ -53,98 +51,57 @@ constexpr float kLowest = -3.0e38f;  // below every finite score, and finite: no
 // the weights then stay below 2^8, and the sums are rescaled a few times only.
 constexpr float kSlack = 8.0f;
 
-// 16 values from p as fp32.
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * k);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[4 * k + i] = a[i];
-  }
+// 8 values from element i of p as bf16 terms, their sum the value.
+__device__ __forceinline__ void load_terms(const void* p, int64_t i, Bf16, u32x4 (&t)[1]) {
+  t[0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
 }
-__device__ __forceinline__ void load16(const Bf16* p, float (&x)[16]) {
+template <int kTerms>
+__device__ __forceinline__ void split_terms(float (&x)[8], u32x4 (&t)[kTerms]) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const u32x4 a = reinterpret_cast<const u32x4*>(p)[k];
+  for (int k = 0; k < kTerms; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[8 * k + 2 * i] = u2f(a[i] << 16), x[8 * k + 2 * i + 1] = u2f(a[i] & 0xFFFF0000u);
-  }
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+      t[k][j] = w;
+      if (k + 1 < kTerms) x[2 * j] -= u2f(w << 16), x[2 * j + 1] -= u2f(w & 0xFFFF0000u);
+    }
 }
-__device__ __forceinline__ void load16(const F16* p, float (&x)[16]) {
+__device__ __forceinline__ void load_terms(const void* p, int64_t i, F16, u32x4 (&t)[2]) {
+  const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
+  float x[8];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const u32x4 a = reinterpret_cast<const u32x4*>(p)[k];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[8 * k + 2 * i] = h2f_exact(a[i] & 0xFFFFu), x[8 * k + 2 * i + 1] = h2f_exact(a[i] >> 16);
-  }
+  for (int j = 0; j < 4; ++j) x[2 * j] = h2f_exact(a[j] & 0xFFFFu), x[2 * j + 1] = h2f_exact(a[j] >> 16);
+  split_terms(x, t);
 }
-__device__ __forceinline__ const float* element(const void* p, int64_t i, float) {
-  return static_cast<const float*>(p) + i;
-}
-template <typename T>
-__device__ __forceinline__ const T* element(const void* p, int64_t i, T) {
-  return reinterpret_cast<const T*>(static_cast<const uint16_t*>(p) + i);
+__device__ __forceinline__ void load_terms(const void* p, int64_t i, float, u32x4 (&t)[3]) {
+  const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+  const f32x4 a = q[0], b = q[1];
+  float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  split_terms(x, t);
 }
 
-// The e4m3 terms of one row of a tile, as the scaled product's B operand: lane
-// (row, g) has elements 16 g .. 16 g + 15 of each half of 64 of a group of 128.
+// The order of a row's elements in the first product.  Lane (token or row, g)
+// of product i has the 8 elements from key_element(i, g): those of a lane are
+// 16 bytes of codes for each 128 elements of a head (8 bytes of 64).
+template <int D>
+__device__ __forceinline__ int key_element(int i, int g) {
+  return D == 64 ? 16 * g + 8 * i : 128 * (i / 4) + 32 * g + 8 * (i % 4);
+}
+
+// One row's query as that product's B operand.
 template <int D, typename T>
 struct QueryTerms {
-  static constexpr int kGroups = (D + 127) / 128;
   static constexpr int kTerms = Terms<T>::kQ;
-  i32x8 v[kTerms][kGroups];
-  int scale;  // the first term's E8M0 byte; each further one is 4 less
+  u32x4 v[D / 32][kTerms];
 
-  // p: the row's first element, or NULL for a row of zeros
   __device__ __forceinline__ void load(const void* p, int64_t at, bool live, int g) {
-    constexpr int kHalves = D / 64;
-    float x[kHalves][16];
 #pragma unroll
-    for (int k = 0; k < kHalves; ++k) {
+    for (int i = 0; i < D / 32; ++i) {
       if (live) {
-        load16(element(p, at + 64 * k + 16 * g, T()), x[k]);
+        load_terms(p, at + key_element<D>(i, g), T(), v[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[k][i] = 0.0f;
-      }
-    }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int k = 0; k < kHalves; ++k)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) amax = umax32(amax, f2u(x[k][i]) & 0x7FFFFFFFu);
-    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 16));
-    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 32));
-    // the largest in [2^7, 2^8), below e4m3's 448; a row below 2^-90 keeps that
-    // scale, one with an infinity or a NaN becomes NaN (past 464 there is no value)
-    int e = amax < 0x7F800000u ? (int)(amax >> 23) - 127 : 0;
-    if (e < -90) e = -90;
-    const float r = exp2i(7 - e);
-    scale = e - 7 + 127;
-#pragma unroll
-    for (int k = 0; k < kHalves; ++k)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[k][i] *= r;
-#pragma unroll
-    for (int t = 0; t < kTerms; ++t) {
-#pragma unroll
-      for (int k = 0; k < 2 * kGroups; ++k) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int w = 0;
-          if (k < kHalves) {
-            float* y = &x[k < kHalves ? k : 0][4 * i];
-            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
-            if (t + 1 < kTerms) {
-              const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-              y[0] = (y[0] - a.x) * 16.0f, y[1] = (y[1] - a.y) * 16.0f;
-              y[2] = (y[2] - b.x) * 16.0f, y[3] = (y[3] - b.y) * 16.0f;
-            }
-          }
-          v[t][k / 2][4 * (k & 1) + i] = w;
-        }
+        for (int t = 0; t < kTerms; ++t) v[i][t] = u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -219,7 +176,8 @@ __device__ __forceinline__ float curved(const Curve& k, float s, int away) {
 }
 
 // The keys and values of one step of 32 tokens as a wave's loads leave them.
-// Keys: lane (token & 15, g) has block g of its token, twice.  Values: lane
+// Keys: lane (token & 15, g) has key_element's codes of its token, twice, and
+// the scales they need.  Values: lane
 // (m, g) has the D / 16 elements from m D / 16 of tokens 4 g .. 4 g + 3 and
 // 16 + 4 g .. 16 + 4 g + 3, and all scale bytes of those tokens.
 template <int D>
@@ -227,13 +185,31 @@ struct Loaded {
   static constexpr int kGroups = (D + 127) / 128;
   static constexpr int kWords = D == 256 ? 2 : 1;     // of a token's values
   static constexpr int kScaleWords = D / 32;          // of four tokens' scales
-  u32x4 k[2][kGroups];
+  uint32_t k[2][D / 32];
   uint32_t ks[2][kGroups];
   uint32_t v[8][kWords];
   uint32_t vs[2][kScaleWords];
   uint32_t valid;  // bit t: token t of the step is there
   int t0;
 };
+
+template <int D>
+__device__ __forceinline__ void load_keys(const uint8_t* codes, const uint8_t* scales, int g,
+                                          uint32_t (&k)[D / 32], uint32_t (&s)[Loaded<D>::kGroups]) {
+  if constexpr (D == 64) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(codes + 8 * g);
+    k[0] = a[0], k[1] = a[1];
+    s[0] = scales[g >> 1];
+  } else {
+#pragma unroll
+    for (int a = 0; a < D / 128; ++a) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(codes + 64 * a + 16 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[4 * a + i] = w[i];
+      s[a] = scales[4 * a + g];
+    }
+  }
+}
 
 template <int D>
 __device__ __forceinline__ void load_values(const uint8_t* p, uint32_t (&w)[Loaded<D>::kWords]) {
@@ -257,7 +233,7 @@ struct __attribute__((packed, aligned(1))) Raw8 {
 template <int D, bool kKeys, bool kValues>
 __device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t page, bool aligned_pages, int t0,
                                           int hi, int lane, Loaded<D>& s) {
-  constexpr int kRow = D / 2, kScales = D / 32, kGroups = Loaded<D>::kGroups;
+  constexpr int kRow = D / 2, kScales = D / 32;
   const int m = lane & 15, g = lane >> 4;
   s.t0 = t0;
   if (aligned_pages && t0 + kStep <= hi) {
@@ -270,12 +246,7 @@ __device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t
       const uint8_t* ks = c.scales + (uint64_t)row * kScales;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int a = 0; a < kGroups; ++a) {
-          const uint32_t block = D == 64 ? (g & 1) : 4 * a + g;
-          s.k[i][a] = *reinterpret_cast<const u32x4*>(kc + (uint32_t)(i * 16 * kRow) + m * kRow + block * 16);
-          s.ks[i][a] = ks[(uint32_t)(i * 16 * kScales) + m * kScales + block];
-        }
+        load_keys<D>(kc + (uint32_t)((i * 16 + m) * kRow), ks + (uint32_t)((i * 16 + m) * kScales), g, s.k[i], s.ks[i]);
     }
     if constexpr (kValues) {
       const uint64_t vrow = c.plane_rows + row;
@@ -312,12 +283,7 @@ __device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint64_t row = (uint32_t)__shfl((int)mine, 16 * i + m);
-#pragma unroll
-      for (int a = 0; a < kGroups; ++a) {
-        const uint32_t block = D == 64 ? (g & 1) : 4 * a + g;
-        s.k[i][a] = *reinterpret_cast<const u32x4*>(c.codes + row * kRow + block * 16);
-        s.ks[i][a] = c.scales[row * kScales + block];
-      }
+      load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, g, s.k[i], s.ks[i]);
     }
   }
   if constexpr (kValues) {
@@ -339,6 +305,13 @@ __device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t
   }
 }
 
+// bf16x2 words of the two values whose codes are byte kByte of w.  The scale's
+// exponent counts: 0 is 2^-127, that of an infinity makes a NaN.
+template <int kByte>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte));
+}
+
 // Scores of the step's tokens 16 i + 4 g + r in x[4 i + r], lane (row, g).
 template <int D, typename T>
 __device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loaded<D>& s, float (&x)[8]) {
@@ -346,12 +319,14 @@ __device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loa
   for (int i = 0; i < 2; ++i) {
     f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-    for (int a = 0; a < Loaded<D>::kGroups; ++a) {
-      const i32x8 k = {(int)s.k[i][a][0], (int)s.k[i][a][1], (int)s.k[i][a][2], (int)s.k[i][a][3], 0, 0, 0, 0};
+    for (int a = 0; a < D / 32; ++a) {
+      const float scale = u2f(s.ks[i][a / 4] << 23);
+      const uint32_t w = s.k[i][a];
+      const u32x4 k = {fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)};
 #pragma unroll
       for (int t = 0; t < Terms<T>::kQ; ++t)
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.v[t][a], acc, 4, 0, 0, (int)s.ks[i][a], 0,
-                                                               q.scale - 4 * t);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q.v[a][t]),
+                                                      acc, 0, 0, 0);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[4 * i + r] = acc[r];
@@ -382,12 +357,6 @@ __device__ __forceinline__ void finish_scores(const Curve& k, float (&x)[8], uin
 
 __device__ __forceinline__ bool needs_mask(const TileRows& r, uint32_t valid, int t0, int window) {
   return valid != 0xFFFFFFFFu || t0 + kStep - 1 > r.pos_min || (window && t0 <= r.pos_max - window);
-}
-
-// bf16x2 words of two values whose codes' byte is b of w
-template <int kByte>
-__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte));
 }
 
 // Few rows, many tokens: the cache is read once for each tile of 16 rows, and
@@ -473,17 +442,8 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - m), l += x[j];
-      // the weights' bf16 terms, two tokens a word
       u32x4 p[Terms<T>::kP];
-#pragma unroll
-      for (int t = 0; t < Terms<T>::kP; ++t) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = pack_bf16x2(x[2 * j], x[2 * j + 1]);
-          p[t][j] = w;
-          if (t + 1 < Terms<T>::kP) x[2 * j] -= u2f(w << 16), x[2 * j + 1] -= u2f(w & 0xFFFF0000u);
-        }
-      }
+      split_terms(x, p);
       // this lane's block of each token's scales
       float vs[8];
       const uint32_t block = (uint32_t)n * (D / 16) / 32;
