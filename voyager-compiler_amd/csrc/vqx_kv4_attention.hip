@@ -19,6 +19,7 @@
 // 2^-17 of their sums' magnitude in the mean, against 2^-25 here.
 #include "vqx_kv4.h"
 
+#define VQX_RB (D == 64 ? 3 : (D == 128 ? 2 : 1))
 namespace vqx {
 namespace {
 
@@ -30,15 +31,15 @@ template <typename T>
 struct Terms;
 template <>
 struct Terms<Bf16> {
-  static constexpr int kQ = 1, kP = 2;
+  static constexpr int kQ = 1, kP = 2, kBlockP = 1;
 };
 template <>
 struct Terms<F16> {
-  static constexpr int kQ = 2, kP = 2;
+  static constexpr int kQ = 2, kP = 2, kBlockP = 2;
 };
 template <>
 struct Terms<float> {
-  static constexpr int kQ = 3, kP = 3;
+  static constexpr int kQ = 3, kP = 3, kBlockP = 3;
 };
 
 constexpr int kRows = 16;       // query rows of a tile
@@ -94,11 +95,14 @@ struct QueryTerms {
   static constexpr int kTerms = Terms<T>::kQ;
   u32x4 v[D / 32][kTerms];
 
-  __device__ __forceinline__ void load(const void* p, int64_t at, bool live, int g) {
+  // flip: 0, or the bf16 sign bits of a negative scale
+  __device__ __forceinline__ void load(const void* p, int64_t at, bool live, int g, uint32_t flip) {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
       if (live) {
         load_terms(p, at + key_element<D>(i, g), T(), v[i]);
+#pragma unroll
+        for (int t = 0; t < kTerms; ++t) v[i][t] ^= flip;
       } else {
 #pragma unroll
         for (int t = 0; t < kTerms; ++t) v[i][t] = u32x4{0, 0, 0, 0};
@@ -107,11 +111,11 @@ struct QueryTerms {
   }
 };
 
-// How a call is cut up.  A tile is 16 query rows of one kv head (row r is new
-// token r / group, head r % group); each split of a tile's tokens leaves its
-// sums in the workspace: 16 * D outputs, 16 references and 16 sums.
+// How a call is cut up.  A tile is `rows` query rows of one kv head (row r is
+// new token r / group, head r % group); each split of a tile's tokens leaves
+// its sums in the workspace: rows * D outputs, rows references and rows sums.
 struct Kv4Plan {
-  int32_t tiles, chunk, splits;
+  int32_t rows, tiles, chunk, splits;
 };
 
 // Where the rows of one tile stand.
@@ -143,7 +147,7 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
 // What a score becomes, in powers of two: capped by a tanh, less its slope for
 // each token of distance.
 struct Curve {
-  float scale;          // of a plain score
+  float scale;          // of a plain score, >= 0: the queries carry its sign
   float inner, outer;   // capped: outer * tanh(score * inner)
   float slope;
   bool capped;
@@ -160,9 +164,9 @@ __device__ __forceinline__ float tanh32(float x) {
 
 __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   Curve k;
-  k.scale = q.scale * kLog2e;
+  k.scale = __builtin_fabsf(q.scale) * kLog2e;
   k.capped = q.softcap != 0.0f;
-  k.inner = k.capped ? q.scale / q.softcap : 0.0f;
+  k.inner = k.capped ? __builtin_fabsf(q.scale) / q.softcap : 0.0f;
   k.outer = q.softcap * kLog2e;
   k.slope = q.slopes ? q.slopes[head] * kLog2e : 0.0f;
   return k;
@@ -312,12 +316,15 @@ __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte));
 }
 
-// Scores of the step's tokens 16 i + 4 g + r in x[4 i + r], lane (row, g).
-template <int D, typename T>
-__device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loaded<D>& s, float (&x)[8]) {
+// Scores of the step's tokens 16 i + 4 g + r in x[y][4 i + r], lane (row, g) of
+// each of kSub tiles of 16 rows.
+template <int D, typename T, int kSub>
+__device__ __forceinline__ void step_scores(const QueryTerms<D, T> (&q)[kSub], const Loaded<D>& s, float (&x)[kSub][8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    f32x4 acc = {0, 0, 0, 0};
+    f32x4 acc[kSub];
+#pragma unroll
+    for (int y = 0; y < kSub; ++y) acc[y] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int a = 0; a < D / 32; ++a) {
       const float scale = u2f(s.ks[i][a / 4] << 23);
@@ -325,11 +332,15 @@ __device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loa
       const u32x4 k = {fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)};
 #pragma unroll
       for (int t = 0; t < Terms<T>::kQ; ++t)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q.v[a][t]),
-                                                      acc, 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < kSub; ++y)
+          acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
+                                                           __builtin_bit_cast(bf16x8, q[y].v[a][t]), acc[y], 0, 0, 0);
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[4 * i + r] = acc[r];
+    for (int y = 0; y < kSub; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[y][4 * i + r] = acc[y][r];
   }
 }
 
@@ -359,13 +370,45 @@ __device__ __forceinline__ bool needs_mask(const TileRows& r, uint32_t valid, in
   return valid != 0xFFFFFFFFu || t0 + kStep - 1 > r.pos_min || (window && t0 <= r.pos_max - window);
 }
 
+__device__ __forceinline__ void put(void* out, int64_t i, float v, float) { static_cast<float*>(out)[i] = v; }
+__device__ __forceinline__ void put(void* out, int64_t i, float v, Bf16) {
+  static_cast<uint16_t*>(out)[i] = (uint16_t)f2bf(v);
+}
+__device__ __forceinline__ void put(void* out, int64_t i, float v, F16) {
+  static_cast<uint16_t*>(out)[i] = (uint16_t)f2h_exact(v);
+}
+// 4 consecutive elements, i a multiple of 4
+__device__ __forceinline__ void put4(void* out, int64_t i, f32x4 v, float) {
+  *reinterpret_cast<f32x4*>(static_cast<float*>(out) + i) = v;
+}
+__device__ __forceinline__ void put4(void* out, int64_t i, f32x4 v, Bf16) {
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + i) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+}
+__device__ __forceinline__ void put4(void* out, int64_t i, f32x4 v, F16) {
+  *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + i) =
+      u32x2{f2h_exact(v[0]) | f2h_exact(v[1]) << 16, f2h_exact(v[2]) | f2h_exact(v[3]) << 16};
+}
+
+// A sequence with more new tokens than the call was told of: their rows have
+// no result.
+template <int D, typename T>
+__device__ __forceinline__ void fill_beyond(const Kv4Query& q, const TileRows& rows, uint32_t h, void* out,
+                                            float* lse) {
+  const int64_t extra = (int64_t)(rows.count - q.most) * q.group;
+  for (int64_t e = threadIdx.x; e < extra; e += 256) {
+    const int64_t row = (int64_t)(rows.first + q.most + e / q.group) * q.heads + (int64_t)h * q.group + e % q.group;
+    lse[row] = __builtin_nanf("");
+    for (int d = 0; d < D; ++d) put(out, row * D + d, __builtin_nanf(""), T());
+  }
+}
+
 // Few rows, many tokens: the cache is read once for each tile of 16 rows, and
 // that reading is the bound.  A workgroup has one tile, one kv head and one
 // run of tokens; its four waves take steps of 32 tokens in turn, each straight
 // from memory into the operands' registers, one step ahead, and are joined at
 // the end.
 template <int D, typename T, bool kExtra>
-__global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
+__global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                        float* ws) {
   constexpr int kTiles = D / 16;      // of 16 output elements
   constexpr int kPer = D / 4;         // output elements of a lane
@@ -382,20 +425,7 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv
   const bool live = r < rows.rows;
   const int token = r / q.group, head = (int)h * q.group + r % q.group;
   const int64_t at_row = (int64_t)(rows.first + token) * q.heads + head;
-  if (rows.count > q.most && tile == 0 && split == 0) {
-    // more new tokens than the call was told of: these rows have no result
-    const int64_t extra = (int64_t)(rows.count - q.most) * q.group;
-    for (int64_t e = tid; e < extra; e += 256) {
-      const int64_t row = (int64_t)(rows.first + q.most + e / q.group) * q.heads + (int64_t)h * q.group + e % q.group;
-      lse[row] = __builtin_nanf("");
-      for (int d = 0; d < D; ++d) {
-        if constexpr (sizeof(T) == 4)
-          static_cast<float*>(out)[row * D + d] = __builtin_nanf("");
-        else
-          static_cast<uint16_t*>(out)[row * D + d] = 0x7FFFu;
-      }
-    }
-  }
+  if (rows.count > q.most && tile == 0 && split == 0) fill_beyond<D, T>(q, rows, h, out, lse);
   if (tile * kRows >= rows.rows) return;
   const int begin = rows.lo + (int)split * plan.chunk;
   int end = begin + plan.chunk;
@@ -413,8 +443,9 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv
   for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0, 0, 0, 0};
 
   if (wave < steps) {
-    QueryTerms<D, T> terms;
-    terms.load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
+    QueryTerms<D, T> terms[1];
+    terms[0].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
+                  q.scale < 0.0f ? 0x80008000u : 0u);
 
     // the page of this lane's token in the wave's s-th step
     auto page_of = [&](int s) -> uint32_t {
@@ -423,8 +454,9 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv
       return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
     };
     auto work = [&](const Loaded<D>& s) {
-      float x[8];
-      step_scores<D, T>(terms, s, x);
+      float scores[1][8];
+      step_scores<D, T, 1>(terms, s, scores);
+      float(&x)[8] = scores[0];
       const bool masked = needs_mask(rows, s.valid, s.t0, q.window);
       uint32_t seen;
       finish_scores<kExtra>(curve, x, s.valid, s.t0, g, pos, q.window, masked, seen);
@@ -588,33 +620,257 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv
   if (!live) return;
   if (g == 0) lse[at_row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t d = at_row * D + g * kPer + i * kTiles;
-    if constexpr (sizeof(T) == 4) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < kTiles; j += 4)
-        *reinterpret_cast<f32x4*>(static_cast<float*>(out) + d + j) =
-            f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
-    } else {
-#pragma unroll
-      for (int j = 0; j < kTiles; j += 2) {
-        uint32_t w;
-        if constexpr (std::is_same<T, Bf16>::value)
-          w = pack_bf16x2(acc[j][i], acc[j + 1][i]);
-        else
-          w = f2h_exact(acc[j][i]) | f2h_exact(acc[j + 1][i]) << 16;
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + d + j) = w;
-      }
-    }
-  }
+    for (int j = 0; j < kTiles; j += 4)
+      put4(out, at_row * D + g * kPer + i * kTiles + j, f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]},
+           T());
 }
 
-__device__ __forceinline__ void put(void* out, int64_t i, float v, float) { static_cast<float*>(out)[i] = v; }
-__device__ __forceinline__ void put(void* out, int64_t i, float v, Bf16) {
-  static_cast<uint16_t*>(out)[i] = (uint16_t)f2bf(v);
-}
-__device__ __forceinline__ void put(void* out, int64_t i, float v, F16) {
-  static_cast<uint16_t*>(out)[i] = (uint16_t)f2h_exact(v);
+// Rows of a kv head from which on the kernel for many rows is taken.
+constexpr int kManyRows = 32;
+
+// Many rows: a workgroup has 128 rows of one kv head, 32 of them a wave (64 and
+// 16 where a wave has one tile), and
+// walks over the tokens by 64.  The values of a step are turned into bf16 once,
+// transposed into LDS (two buffers, one barrier a step), and read by all four
+// waves; each wave turns the keys itself, since two of its tiles share them
+// and reading them from LDS as bf16 would take all of its bandwidth.  Bound by
+// the vector instructions of the softmax beside the matrix ones.
+// Tiles of 16 rows of a wave: 2, and 1 where the registers do not hold the
+// queries' terms and the outputs of 2.
+constexpr int block_sub(int dim, int q_terms) { return dim == 256 && q_terms > 1 ? 1 : 2; }
+constexpr int kBlockStep = 64;
+constexpr int kVRow = kBlockStep + 8;  // bf16 of one element's tokens in LDS: rows 16 bytes off each other's banks
+
+template <int D, typename T, bool kExtra>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
+                                                        float* ws) {
+  constexpr int kTiles = D / 16;
+  constexpr int kWords = Loaded<D>::kWords, kScales = D / 32;
+  constexpr int kP = Terms<T>::kBlockP;
+  constexpr int kSub = block_sub(D, Terms<T>::kQ), kBlockRows = 64 * kSub;
+  __shared__ __align__(16) uint16_t vt[2][D][kVRow];
+  __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  // heads first, so that with 8 of them each XCD's L2 has the cache of one;
+  // then the tiles from the last, which sees the most
+  const uint32_t heads = c.seqs * c.kv, slot = blockIdx.x % heads, rest = blockIdx.x / heads;
+  const uint32_t b = slot / c.kv, h = slot % c.kv;
+  const uint32_t split = rest % (uint32_t)plan.splits;
+  const int tile = plan.tiles - 1 - (int)(rest / (uint32_t)plan.splits);
+  const TileRows rows = tile_rows(c, q, b, tile, kBlockRows);
+  if (rows.count > q.most && tile == 0 && split == 0) fill_beyond<D, T>(q, rows, h, out, lse);
+  if (tile * kBlockRows >= rows.rows) return;
+  const int begin = rows.lo + (int)split * plan.chunk;
+  int end = begin + plan.chunk;
+  if (end > rows.hi) end = rows.hi;
+  if (begin >= end && split > 0) return;
+  const int steps = begin < end ? (end - begin + kBlockStep - 1) / kBlockStep : 0;
+  const bool aligned_pages = !c.table || c.size % kStep == 0;
+  const bool aligned_quads = !c.table || c.size % 4 == 0;
+
+  // the wave's own rows
+  const int r0 = tile * kBlockRows + wave * kSub * 16;
+  const TileRows mine = tile_rows(c, q, b, tile * kWaves + wave, 16 * kSub);
+  int row[kSub], pos[kSub];
+  Curve curve[kSub];
+  QueryTerms<D, T> terms[kSub];
+#pragma unroll
+  for (int y = 0; y < kSub; ++y) {
+    row[y] = r0 + 16 * y + n;
+    const bool live = row[y] < rows.rows;
+    const int token = row[y] / q.group, head = (int)h * q.group + row[y] % q.group;
+    pos[y] = live ? rows.base + token : -1;
+    curve[y] = curve_of(q, live ? head : (int)h * q.group);
+    terms[y].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
+                  q.scale < 0.0f ? 0x80008000u : 0u);
+  }
+  float m[kSub], l[kSub];
+  uint32_t bad[kSub];
+  f32x4 acc[kSub][kTiles];
+#pragma unroll
+  for (int y = 0; y < kSub; ++y) {
+    m[y] = kLowest, l[y] = 0.0f, bad[y] = 0;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) acc[y][j] = f32x4{0, 0, 0, 0};
+  }
+  if (tid < 2) nan_step[tid] = -1;
+
+  // Values: thread (quad, part) has D / 16 elements of four tokens.
+  const int quad = tid & 15, element = (tid >> 4) * (D / 16);
+  uint32_t v[4][kWords], vs[4];
+  auto load_v = [&](int step) {
+    const int t = begin + step * kBlockStep + 4 * quad;
+    const int t_q = t < end ? t : end - 1;
+    const uint32_t page = kv4_page(c, b, (uint32_t)t_q);
+    const uint32_t base = kv4_row(c, page, h, (uint32_t)t_q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t_i = t + i < end ? t + i : end - 1;
+      uint32_t r = base + (page < c.pages ? (uint32_t)(t_i - t_q) : 0u);
+      if (!aligned_quads) r = kv4_row(c, kv4_page(c, b, (uint32_t)t_i), h, (uint32_t)t_i);
+      const uint64_t at = c.plane_rows + r;
+      load_values<D>(c.codes + at * (D / 2) + element / 2, v[i]);
+      vs[i] = c.scales[at * kScales + element / 32];
+    }
+  };
+  // A step's place in LDS: a lane of the second product takes tokens
+  // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
+  auto store_v = [&](int step) {
+    uint16_t* to = &vt[step & 1][element][32 * (quad >> 3) + 8 * (quad & 3) + 4 * (quad >> 2 & 1)];
+    const bool nan = vs[0] == 255 || vs[1] == 255 || vs[2] == 255 || vs[3] == 255;
+    if (nan) nan_step[step & 1] = step;
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = vs[i] == 255 ? 0.0f : u2f(vs[i] << 23);
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      auto pair = [&](auto which) {
+        constexpr int kByte = decltype(which)::value;
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fp4_pair<kByte>(v[i][w], f[i]);
+        const u32x2 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
+        const u32x2 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte) * kVRow) = even;
+        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte + 1) * kVRow) = odd;
+      };
+      pair(std::integral_constant<int, 0>());
+      pair(std::integral_constant<int, 1>());
+      if constexpr (D > 64) {
+        pair(std::integral_constant<int, 2>());
+        pair(std::integral_constant<int, 3>());
+      }
+    }
+  };
+
+  // Keys: the wave's own, 32 tokens at a time.
+  auto page_of = [&](int s) -> uint32_t {
+    if (!c.table) return b;
+    const int t = begin + s * kStep + (lane & 31);
+    return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
+  };
+  auto work = [&](const Loaded<D>& s, int step, int half) {
+    if (s.t0 >= mine.hi || s.t0 + kStep <= mine.lo) return;
+    float x[kSub][8];
+    step_scores<D, T, kSub>(terms, s, x);
+    const bool masked = needs_mask(mine, s.valid, s.t0, q.window);
+    const bool nan = nan_step[step & 1] == step;
+    u32x4 p[kSub][kP];
+#pragma unroll
+    for (int y = 0; y < kSub; ++y) {
+      uint32_t seen = 0xFFu;
+      if (kExtra) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[y][j] = curved<true>(curve[y], x[y][j], pos[y] - (s.t0 + (j >> 2) * 16 + 4 * g + (j & 3)));
+      }
+      if (masked) {
+        seen = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = s.t0 + u;
+          const bool in = (s.valid >> u & 1u) && t <= pos[y] && (q.window == 0 || t > pos[y] - q.window);
+          x[y][j] = in ? x[y][j] : -__builtin_huge_valf();
+          seen |= (uint32_t)in << j;
+        }
+      }
+      const float scale = kExtra ? 1.0f : curve[y].scale;
+      float top = x[y][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, x[y][j]);
+      top *= scale;
+      if (__ballot(top > m[y] + kSlack)) {
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float next = __builtin_fmaxf(m[y], top), f = __builtin_amdgcn_exp2f(m[y] - next);
+        m[y] = next;
+        l[y] *= f;
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) acc[y][j] *= f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[y][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[y][j], scale, -m[y]));
+      if (masked) {
+        // a scale of 0 makes NaN of what is masked
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[y] += x[y][j];
+      split_terms(x[y], p[y]);
+      if (nan) {
+        // the blocks that were taken as tiny, for the rows that see them
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int u = (j >> 2) * 16 + 4 * g + (j & 3);
+          const int t = s.t0 + u < end ? s.t0 + u : end - 1;
+          if (seen >> j & 1u) {
+            const uint64_t at = c.plane_rows + kv4_row(c, kv4_page(c, b, (uint32_t)t), h, (uint32_t)t);
+            for (int k = 0; k < kScales; ++k) bad[y] |= (uint32_t)(c.scales[at * kScales + k] == 255) << k;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(&vt[step & 1][16 * j + n][32 * half + 8 * g]);
+#pragma unroll
+      for (int t = 0; t < kP; ++t)
+#pragma unroll
+        for (int y = 0; y < kSub; ++y)
+          acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, p[y][t]), acc[y][j], 0, 0, 0);
+    }
+  };
+
+  if (steps > 0) {
+    Loaded<D> one, two;
+    load_v(0);
+    uint32_t page = page_of(0);
+    load_step<D, true, false>(c, h, page, aligned_pages, begin, end, lane, one);
+    page = page_of(1);
+    __syncthreads();
+    store_v(0);
+    if (steps > 1) load_v(1);
+    for (int step = 0; step < steps; ++step) {
+      const int t0 = begin + step * kBlockStep;
+      __syncthreads();
+      if (step + 1 < steps) store_v(step + 1);
+      if (step + 2 < steps) load_v(step + 2);
+      const bool second = t0 + kStep < end;
+      if (second) load_step<D, true, false>(c, h, page, aligned_pages, t0 + kStep, end, lane, two);
+      page = page_of(2 * step + 2);
+      work(one, step, 0);
+      if (step + 1 < steps) load_step<D, true, false>(c, h, page, aligned_pages, t0 + kBlockStep, end, lane, one);
+      page = page_of(2 * step + 3);
+      if (second) work(two, step, 1);
+    }
+  }
+
+#pragma unroll
+  for (int y = 0; y < kSub; ++y) {
+    l[y] += __shfl_xor(l[y], 16);
+    l[y] += __shfl_xor(l[y], 32);
+    bad[y] |= (uint32_t)__shfl_xor((int)bad[y], 16);
+    bad[y] |= (uint32_t)__shfl_xor((int)bad[y], 32);
+    if (row[y] >= rows.rows) continue;
+    const float inv = plan.splits > 1 ? 1.0f : (l[y] == 0.0f ? 0.0f : 1.0f / l[y]);
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) acc[y][j] = bad[y] >> (j / 2) & 1u ? acc[y][j] * __builtin_nanf("") : acc[y][j] * inv;
+    if (plan.splits > 1) {
+      float* o = ws + (((int64_t)slot * plan.tiles + tile) * plan.splits + split) * (kBlockRows * D + 2 * kBlockRows);
+      const int k = row[y] - tile * kBlockRows;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4*>(o + k * D + 16 * j + 4 * g) = acc[y][j];
+      if (g == 0) o[kBlockRows * D + k] = m[y], o[kBlockRows * D + kBlockRows + k] = l[y];
+      continue;
+    }
+    const int64_t at = (int64_t)(rows.first + row[y] / q.group) * q.heads + (int64_t)h * q.group + row[y] % q.group;
+    if (g == 0) lse[at] = l[y] == 0.0f ? -__builtin_huge_valf() : (m[y] + __builtin_amdgcn_logf(l[y])) * kLn2;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) put4(out, at * D + 16 * j + 4 * g, acc[y][j], T());
+  }
 }
 
 // The splits of one row joined, in their order: a workgroup a row, its waves
@@ -625,27 +881,28 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   constexpr int kPer = D / 64;
   __shared__ float sum[kWaves][D], sum_l[kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t slot = blockIdx.x / kRows, b = slot / (uint32_t)plan.tiles / c.kv,
+  const uint32_t slot = blockIdx.x / (uint32_t)plan.rows, b = slot / (uint32_t)plan.tiles / c.kv,
                  h = slot / (uint32_t)plan.tiles % c.kv;
-  const int tile = (int)(slot % (uint32_t)plan.tiles), n = blockIdx.x % kRows, r = tile * kRows + n;
-  const TileRows rows = tile_rows(c, q, b, tile, kRows);
+  const int tile = (int)(slot % (uint32_t)plan.tiles), n = (int)(blockIdx.x % (uint32_t)plan.rows),
+            r = tile * plan.rows + n;
+  const TileRows rows = tile_rows(c, q, b, tile, plan.rows);
   if (r >= rows.rows) return;
   const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
-  const float* first = ws + (int64_t)slot * plan.splits * (kRows * D + 2 * kRows);
-  constexpr int64_t kSlot = kRows * D + 2 * kRows;
+  const int64_t size = (int64_t)plan.rows * (D + 2);
+  const float* o_n = ws + (int64_t)slot * plan.splits * size + (int64_t)n * D;
+  const float* m_n = ws + (int64_t)slot * plan.splits * size + (int64_t)plan.rows * D + n;
   float m = kLowest;
-  for (int s = lane; s < splits; s += 64) m = __builtin_fmaxf(m, first[s * kSlot + kRows * D + n]);
+  for (int s = lane; s < splits; s += 64) m = __builtin_fmaxf(m, m_n[s * size]);
   for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
   float l = 0.0f, o[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
 #pragma unroll 4
   for (int s = wave; s < splits; s += kWaves) {
-    const float* p = first + s * kSlot;
-    const float f = __builtin_amdgcn_exp2f(p[kRows * D + n] - m);
-    l += p[kRows * D + kRows + n] * f;
+    const float f = __builtin_amdgcn_exp2f(m_n[s * size] - m);
+    l += m_n[s * size + plan.rows] * f;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] += p[n * D + lane + 64 * k] * f;
+    for (int k = 0; k < kPer; ++k) o[k] += o_n[s * size + lane + 64 * k] * f;
   }
 #pragma unroll
   for (int k = 0; k < kPer; ++k) sum[wave][lane + 64 * k] = o[k];
@@ -690,11 +947,13 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
       const int r = tile * kRows + n;
       const bool live = r < rows.rows;
       const int token = r / q.group, head = (int)h * q.group + r % q.group;
-      QueryTerms<D, T> terms;
-      terms.load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
+      QueryTerms<D, T> terms[1];
+      terms[0].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
+                    q.scale < 0.0f ? 0x80008000u : 0u);
       const float base = live ? lse[(int64_t)(rows.first + token) * q.heads + head] * kLog2e : 0.0f;
-      float x[8];
-      step_scores<D, T>(terms, s, x);
+      float scores[1][8];
+      step_scores<D, T, 1>(terms, s, scores);
+      float(&x)[8] = scores[0];
       uint32_t seen;
       finish_scores<kExtra>(curve_of(q, live ? head : (int)h * q.group), x, s.valid, t0, g,
                             live ? rows.base + token : -1, q.window,
@@ -715,13 +974,15 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
   }
 }
 
-Kv4Plan kv4_plan(const Kv4View& c, const Kv4Query& q) {
+Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   Kv4Plan p;
-  p.tiles = (int32_t)(((int64_t)q.most * q.group + kRows - 1) / kRows);
+  const int64_t all = (int64_t)q.most * q.group;
+  p.rows = all > kManyRows ? 64 * block_sub(dim, dtype == kBF16 ? 1 : 2) : kRows;
+  p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   // the most tokens a tile can see
   int64_t span = c.cap;
   if (q.window) {
-    const int64_t seen = (int64_t)q.window + kRows / q.group + 2 + kStep;
+    const int64_t seen = (int64_t)q.window + p.rows / q.group + 2 + kStep;
     if (seen < span) span = seen;
   }
   const int64_t heads = (int64_t)c.seqs * c.kv * p.tiles;
@@ -739,10 +1000,10 @@ Kv4Plan kv4_plan(const Kv4View& c, const Kv4Query& q) {
 
 }  // namespace
 
-int64_t kv4_workspace(const Kv4View& c, int dim, const Kv4Query& q, int) {
+int64_t kv4_workspace(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return 0;
-  const Kv4Plan p = kv4_plan(c, q);
-  return p.splits > 1 ? (int64_t)c.seqs * c.kv * p.tiles * p.splits * (kRows * dim + 2 * kRows) * 4 : 0;
+  const Kv4Plan p = kv4_plan(c, dim, q, dtype);
+  return p.splits > 1 ? (int64_t)c.seqs * c.kv * p.tiles * p.splits * p.rows * (dim + 2) * 4 : 0;
 }
 
 #define VQX_KV4_DIMS(CALL, T)  \
@@ -764,25 +1025,33 @@ int64_t kv4_workspace(const Kv4View& c, int dim, const Kv4Query& q, int) {
 int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void* out, float* lse, float* ws,
                   hipStream_t st) {
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
-  const Kv4Plan p = kv4_plan(c, q);
+  const Kv4Plan p = kv4_plan(c, dim, q, dtype);
   const bool extra = q.softcap != 0.0f || q.slopes;
   const int64_t slots = (int64_t)p.tiles * c.seqs * c.kv;
-  if (slots * (p.splits > kRows ? p.splits : kRows) >= 1ll << 31)
+  if (slots * (p.splits > p.rows ? p.splits : p.rows) >= 1ll << 31)
     return set_error(kErrUnsupported, "kv4_attention: %lld tiles of %d splits do not fit a launch", (long long)slots,
                      p.splits);
   const dim3 grid((unsigned)(slots * p.splits));
-#define VQX_KV4_ROWS(D, T)                                                                                       \
-  do {                                                                                                           \
-    if (extra)                                                                                                   \
-      hipLaunchKernelGGL((kv4_rows_kernel<D, T, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);          \
-    else                                                                                                         \
-      hipLaunchKernelGGL((kv4_rows_kernel<D, T, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);         \
-    if (p.splits > 1)                                                                                            \
-      hipLaunchKernelGGL((kv4_join_kernel<D, T>), dim3((unsigned)(slots * kRows)), dim3(256), 0,  \
-                         st, c, q, p, out, lse, ws);                                                             \
+#define VQX_KV4_LAUNCH(NAME, D, T)                                                                                   \
+  do {                                                                                                             \
+    if (extra)                                                                                                     \
+      hipLaunchKernelGGL((NAME<D, T, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                       \
+    else                                                                                                           \
+      hipLaunchKernelGGL((NAME<D, T, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                      \
+  } while (0)
+#define VQX_KV4_ROWS(D, T)                                                                                         \
+  do {                                                                                                             \
+    if (p.rows == kRows)                                                                                           \
+      VQX_KV4_LAUNCH(kv4_rows_kernel, D, T);                                                                       \
+    else                                                                                                           \
+      VQX_KV4_LAUNCH(kv4_block_kernel, D, T);                                                                      \
+    if (p.splits > 1)                                                                                              \
+      hipLaunchKernelGGL((kv4_join_kernel<D, T>), dim3((unsigned)(slots * p.rows)), dim3(256), 0, st, c, q, p,     \
+                         out, lse, ws);                                                                            \
   } while (0)
   VQX_KV4_TYPES(VQX_KV4_ROWS)
 #undef VQX_KV4_ROWS
+#undef VQX_KV4_LAUNCH
   return check_launch("kv4_attention");
 }
 
