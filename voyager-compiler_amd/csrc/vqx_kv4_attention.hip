@@ -123,11 +123,12 @@ struct TileRows {
   int first, count;  // the sequence's first new token and their number
   int base;          // position of new token 0
   int rows;          // count * group
-  int lo, hi;        // tokens that any row of the tile sees: [lo, hi), lo a multiple of kStep
+  int lo, hi;        // tokens that any row of the tile sees: [lo, hi), lo a multiple of a step
   int pos_min, pos_max;
 };
 
-__device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile, int tile_size) {
+__device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile, int tile_size,
+                                              int step) {
   TileRows r;
   kv4_span(q.tokens, b, r.first, r.count);
   const int length = c.lengths[b];
@@ -139,15 +140,15 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
   r.pos_max = r1 > r0 ? r.base + (r1 - 1) / q.group : -1;
   r.hi = r.pos_max + 1 < 0 ? 0 : ((uint32_t)(r.pos_max + 1) > c.cap ? (int)c.cap : r.pos_max + 1);
   r.lo = 0;
-  if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(kStep - 1);
-  if (r.lo > r.hi) r.lo = r.hi & ~(kStep - 1);
+  if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(step - 1);
+  if (r.lo > r.hi) r.lo = r.hi & ~(step - 1);
   return r;
 }
 
 // What a score becomes, in powers of two: capped by a tanh, less its slope for
 // each token of distance.
 struct Curve {
-  float scale;          // of a plain score, >= 0: the queries carry its sign
+  float scale;          // of a plain score, positive: the queries carry its sign
   float inner, outer;   // capped: outer * tanh(score * inner)
   float slope;
   bool capped;
@@ -164,7 +165,8 @@ __device__ __forceinline__ float tanh32(float x) {
 
 __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   Curve k;
-  k.scale = __builtin_fabsf(q.scale) * kLog2e;
+  // not 0: a masked score, -inf, stays one
+  k.scale = __builtin_fmaxf(__builtin_fabsf(q.scale) * kLog2e, 1e-30f);
   k.capped = q.softcap != 0.0f;
   k.inner = k.capped ? __builtin_fabsf(q.scale) / q.softcap : 0.0f;
   k.outer = q.softcap * kLog2e;
@@ -197,20 +199,22 @@ struct Loaded {
   int t0;
 };
 
+// codes + at, scales + scale_at: a token's key; the offsets apart, so that a
+// common base stays in scalar registers.
 template <int D>
-__device__ __forceinline__ void load_keys(const uint8_t* codes, const uint8_t* scales, int g,
-                                          uint32_t (&k)[D / 32], uint32_t (&s)[Loaded<D>::kGroups]) {
+__device__ __forceinline__ void load_keys(const uint8_t* codes, const uint8_t* scales, uint32_t at, uint32_t scale_at,
+                                          int g, uint32_t (&k)[D / 32], uint32_t (&s)[Loaded<D>::kGroups]) {
   if constexpr (D == 64) {
-    const u32x2 a = *reinterpret_cast<const u32x2*>(codes + 8 * g);
+    const u32x2 a = *reinterpret_cast<const u32x2*>(codes + (at + 8 * g));
     k[0] = a[0], k[1] = a[1];
-    s[0] = scales[g >> 1];
+    s[0] = scales[scale_at + (g >> 1)];
   } else {
 #pragma unroll
     for (int a = 0; a < D / 128; ++a) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(codes + 64 * a + 16 * g);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(codes + (at + 16 * g) + 64 * a);
 #pragma unroll
       for (int i = 0; i < 4; ++i) k[4 * a + i] = w[i];
-      s[a] = scales[4 * a + g];
+      s[a] = scales[(scale_at + g) + 4 * a];
     }
   }
 }
@@ -234,61 +238,59 @@ struct __attribute__((packed, aligned(1))) Raw8 {
   u32x2 v;
 };
 
-template <int D, bool kKeys, bool kValues>
-__device__ __forceinline__ void load_step(const Kv4View& c, uint32_t h, uint32_t page, bool aligned_pages, int t0,
-                                          int hi, int lane, Loaded<D>& s) {
+// A whole step on one page: one base, and offsets that are constants.  `row` is
+// its first token's.
+template <int D>
+__device__ __forceinline__ void load_whole(const Kv4View& c, uint32_t page, uint32_t row, int t0, int lane,
+                                           Loaded<D>& s) {
   constexpr int kRow = D / 2, kScales = D / 32;
   const int m = lane & 15, g = lane >> 4;
   s.t0 = t0;
-  if (aligned_pages && t0 + kStep <= hi) {
-    // the whole step lies on one page: one base, and offsets that are constants
-    const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane((int)page);
-    const uint32_t row = (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_row(c, pg, h, (uint32_t)t0));
-    s.valid = pg < c.pages ? 0xFFFFFFFFu : 0u;
-    if constexpr (kKeys) {
-      const uint8_t* kc = c.codes + (uint64_t)row * kRow;
-      const uint8_t* ks = c.scales + (uint64_t)row * kScales;
+  s.valid = page < c.pages ? 0xFFFFFFFFu : 0u;
+  const uint8_t* kc = c.codes + (uint64_t)row * kRow;
+  const uint8_t* ks = c.scales + (uint64_t)row * kScales;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        load_keys<D>(kc + (uint32_t)((i * 16 + m) * kRow), ks + (uint32_t)((i * 16 + m) * kScales), g, s.k[i], s.ks[i]);
-    }
-    if constexpr (kValues) {
-      const uint64_t vrow = c.plane_rows + row;
-      const uint8_t* vc = c.codes + vrow * kRow;
-      const uint8_t* vs = c.scales + vrow * kScales;
+  for (int i = 0; i < 2; ++i)
+    load_keys<D>(kc, ks, (uint32_t)((i * 16 + m) * kRow), (uint32_t)((i * 16 + m) * kScales), g, s.k[i], s.ks[i]);
+  const uint64_t vrow = c.plane_rows + row;
+  const uint8_t* vc = c.codes + vrow * kRow;
+  const uint8_t* vs = c.scales + vrow * kScales;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        load_values<D>(vc + (uint32_t)(4 * g * kRow + m * (kRow / 16)) + ((j >> 2) * 16 + (j & 3)) * kRow, s.v[j]);
+  for (int j = 0; j < 8; ++j)
+    load_values<D>(vc + (uint32_t)(4 * g * kRow + m * (kRow / 16)) + ((j >> 2) * 16 + (j & 3)) * kRow, s.v[j]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // four tokens' scales are next to each other, not always on 16 bytes
-        const uint8_t* p = vs + (uint32_t)(4 * g * kScales) + i * 16 * kScales;
-        if constexpr (D == 64) {
-          const u32x2 a = reinterpret_cast<const Raw8*>(p)->v;
-          s.vs[i][0] = a[0], s.vs[i][1] = a[1];
-        } else {
+  for (int i = 0; i < 2; ++i) {
+    // four tokens' scales are next to each other, not always on 16 bytes
+    const uint8_t* p = vs + (uint32_t)(4 * g * kScales) + i * 16 * kScales;
+    if constexpr (D == 64) {
+      const u32x2 a = reinterpret_cast<const Raw8*>(p)->v;
+      s.vs[i][0] = a[0], s.vs[i][1] = a[1];
+    } else {
 #pragma unroll
-          for (int k = 0; k < kScales / 4; ++k) {
-            const u32x4 a = reinterpret_cast<const Raw16*>(p)[k].v;
+      for (int k = 0; k < kScales / 4; ++k) {
+        const u32x4 a = reinterpret_cast<const Raw16*>(p)[k].v;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s.vs[i][4 * k + x] = a[x];
-          }
-        }
+        for (int x = 0; x < 4; ++x) s.vs[i][4 * k + x] = a[x];
       }
     }
-    return;
   }
-  // lane l (and l + 32) finds the row of token l; past the end it is the last
-  // token's, which nothing reads beyond and no row counts
-  const int t = t0 + (lane & 31), tc = t < hi ? t : hi - 1;
-  const uint32_t mine = kv4_row(c, page, h, (uint32_t)tc);
-  s.valid = (uint32_t)__ballot(t < hi && page < c.pages);
-  if constexpr (kKeys) {
+}
+
+// Any step: lane l (and l + 32) has the page of token l and finds its row; past
+// the end that is the last token's, which no row counts.
+template <int D, bool kValues>
+__device__ __forceinline__ void load_any(const Kv4View& c, uint32_t h, uint32_t page, int t0, int end, int lane,
+                                         Loaded<D>& s) {
+  constexpr int kRow = D / 2, kScales = D / 32;
+  const int m = lane & 15, g = lane >> 4;
+  const int t = t0 + (lane & 31);
+  const uint32_t mine = kv4_row(c, page, h, (uint32_t)(t < end ? t : end - 1));
+  s.t0 = t0;
+  s.valid = (uint32_t)__ballot(t < end && page < c.pages);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint64_t row = (uint32_t)__shfl((int)mine, 16 * i + m);
-      load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, g, s.k[i], s.ks[i]);
-    }
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t row = (uint32_t)__shfl((int)mine, 16 * i + m);
+    load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, 0u, 0u, g, s.k[i], s.ks[i]);
   }
   if constexpr (kValues) {
 #pragma unroll
@@ -407,7 +409,7 @@ __device__ __forceinline__ void fill_beyond(const Kv4Query& q, const TileRows& r
 // run of tokens; its four waves take steps of 32 tokens in turn, each straight
 // from memory into the operands' registers, one step ahead, and are joined at
 // the end.
-template <int D, typename T, bool kExtra>
+template <int D, typename T, bool kExtra, bool kWhole>
 __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                        float* ws) {
   constexpr int kTiles = D / 16;      // of 16 output elements
@@ -416,11 +418,12 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
   __shared__ __align__(16) float part[2][kRows][kPad];
   __shared__ float part_m[2][kRows], part_l[2][kRows];
   __shared__ uint32_t part_bad[2][kRows];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t split = blockIdx.x % (uint32_t)plan.splits, slot = blockIdx.x / (uint32_t)plan.splits;
   const int tile = (int)(slot % (uint32_t)plan.tiles);
   const uint32_t b = slot / (uint32_t)plan.tiles / c.kv, h = slot / (uint32_t)plan.tiles % c.kv;
-  const TileRows rows = tile_rows(c, q, b, tile, kRows);
+  const TileRows rows = tile_rows(c, q, b, tile, kRows, kStep);
   const int r = tile * kRows + n;
   const bool live = r < rows.rows;
   const int token = r / q.group, head = (int)h * q.group + r % q.group;
@@ -434,7 +437,6 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
   const int steps = begin < end ? (end - begin + kStep - 1) / kStep : 0;
   const int pos = live ? rows.base + token : -1;
   const Curve curve = curve_of(q, live ? head : (int)h * q.group);
-  const bool aligned_pages = !c.table || c.size % kStep == 0;
 
   float m = kLowest, l = 0.0f;
   uint32_t bad = 0;  // blocks of values that are NaN in a token the row sees
@@ -447,10 +449,9 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
     terms[0].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
                   q.scale < 0.0f ? 0x80008000u : 0u);
 
-    // the page of this lane's token in the wave's s-th step
+    // the page of this lane's token in step s
     auto page_of = [&](int s) -> uint32_t {
-      if (!c.table) return b;
-      int t = begin + s * kStep + (lane & 31);
+      const int t = begin + s * kStep + (lane & 31);
       return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
     };
     auto work = [&](const Loaded<D>& s) {
@@ -541,24 +542,39 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
       }
     };
 
+    // steps that lie whole on a page go round this loop, two of them in flight
+    const int round = kWhole ? (end - begin) / kStep : steps;
     Loaded<D> one, two;
-    uint32_t page = page_of(wave);
-    load_step<D, true, true>(c, h, page, aligned_pages, begin + wave * kStep, end, lane, one);
-    page = page_of(wave + kWaves);
-    int s = wave;
-    while (true) {
-      if (s + kWaves < steps)
-        load_step<D, true, true>(c, h, page, aligned_pages, begin + (s + kWaves) * kStep, end, lane, two);
-      page = page_of(s + 2 * kWaves);
+    uint32_t page = 0;
+    auto load = [&](int s, Loaded<D>& to) {
+      const int t0 = begin + s * kStep;
+      if constexpr (kWhole) {
+        const uint32_t pg = (uint32_t)__builtin_amdgcn_readfirstlane((int)page);
+        load_whole<D>(c, pg, (uint32_t)__builtin_amdgcn_readfirstlane((int)kv4_row(c, pg, h, (uint32_t)t0)), t0, lane, to);
+      } else {
+        load_any<D, true>(c, h, page, t0, end, lane, to);
+      }
+      page = page_of(s + kWaves);
+    };
+    if (wave < round) {
+      page = page_of(wave);
+      load(wave, one);
+      int s = wave;
+      while (true) {
+        // the last round loads its own step again
+        load(s + kWaves < round ? s + kWaves : s, two);
+        work(one);
+        s += kWaves;
+        if (s >= round) break;
+        load(s + kWaves < round ? s + kWaves : s, one);
+        work(two);
+        s += kWaves;
+        if (s >= round) break;
+      }
+    }
+    if (kWhole && round < steps && wave == round % kWaves) {
+      load_any<D, true>(c, h, page_of(round), begin + round * kStep, end, lane, one);
       work(one);
-      s += kWaves;
-      if (s >= steps) break;
-      if (s + kWaves < steps)
-        load_step<D, true, true>(c, h, page, aligned_pages, begin + (s + kWaves) * kStep, end, lane, one);
-      page = page_of(s + 2 * kWaves);
-      work(two);
-      s += kWaves;
-      if (s >= steps) break;
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -639,11 +655,11 @@ constexpr int kManyRows = 32;
 // the vector instructions of the softmax beside the matrix ones.
 // Tiles of 16 rows of a wave: 2, and 1 where the registers do not hold the
 // queries' terms and the outputs of 2.
-constexpr int block_sub(int dim, int q_terms) { return dim == 256 && q_terms > 1 ? 1 : 2; }
+constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 : 2; }
 constexpr int kBlockStep = 64;
 constexpr int kVRow = kBlockStep + 8;  // bf16 of one element's tokens in LDS: rows 16 bytes off each other's banks
 
-template <int D, typename T, bool kExtra>
+template <int D, typename T, bool kExtra, bool kWhole>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                         float* ws) {
   constexpr int kTiles = D / 16;
@@ -652,14 +668,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   constexpr int kSub = block_sub(D, Terms<T>::kQ), kBlockRows = 64 * kSub;
   __shared__ __align__(16) uint16_t vt[2][D][kVRow];
   __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads first, so that with 8 of them each XCD's L2 has the cache of one;
   // then the tiles from the last, which sees the most
   const uint32_t heads = c.seqs * c.kv, slot = blockIdx.x % heads, rest = blockIdx.x / heads;
   const uint32_t b = slot / c.kv, h = slot % c.kv;
   const uint32_t split = rest % (uint32_t)plan.splits;
   const int tile = plan.tiles - 1 - (int)(rest / (uint32_t)plan.splits);
-  const TileRows rows = tile_rows(c, q, b, tile, kBlockRows);
+  const TileRows rows = tile_rows(c, q, b, tile, kBlockRows, kBlockStep);
   if (rows.count > q.most && tile == 0 && split == 0) fill_beyond<D, T>(q, rows, h, out, lse);
   if (tile * kBlockRows >= rows.rows) return;
   const int begin = rows.lo + (int)split * plan.chunk;
@@ -667,12 +684,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   if (end > rows.hi) end = rows.hi;
   if (begin >= end && split > 0) return;
   const int steps = begin < end ? (end - begin + kBlockStep - 1) / kBlockStep : 0;
-  const bool aligned_pages = !c.table || c.size % kStep == 0;
-  const bool aligned_quads = !c.table || c.size % 4 == 0;
 
   // the wave's own rows
   const int r0 = tile * kBlockRows + wave * kSub * 16;
-  const TileRows mine = tile_rows(c, q, b, tile * kWaves + wave, 16 * kSub);
+  const TileRows mine = tile_rows(c, q, b, tile * kWaves + wave, 16 * kSub, kStep);
   int row[kSub], pos[kSub];
   Curve curve[kSub];
   QueryTerms<D, T> terms[kSub];
@@ -697,33 +712,91 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   }
   if (tid < 2) nan_step[tid] = -1;
 
-  // Values: thread (quad, part) has D / 16 elements of four tokens.
+  // Loads go round without a branch, so that each wait is for its own: a token
+  // past the end is the last one, which no row counts.  Where pages hold whole
+  // steps (kWhole) a step has one base, its page looked up a step ahead;
+  // otherwise every lane looks its tokens' pages up, a step ahead too.
+  constexpr int kRow = D / 2;
   const int quad = tid & 15, element = (tid >> 4) * (D / 16);
-  uint32_t v[4][kWords], vs[4];
-  auto load_v = [&](int step) {
-    const int t = begin + step * kBlockStep + 4 * quad;
-    const int t_q = t < end ? t : end - 1;
-    const uint32_t page = kv4_page(c, b, (uint32_t)t_q);
-    const uint32_t base = kv4_row(c, page, h, (uint32_t)t_q);
+  struct Pages {
+    uint32_t k[4], v[4];  // kWhole: k[0] only
+  };
+  auto pages_of = [&](int step, Pages& p) {
+    const int t0 = begin + step * kBlockStep;
+    if constexpr (kWhole) {
+      p.k[0] = kv4_page(c, b, (uint32_t)(t0 < end ? t0 : end - 1));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t_i = t + i < end ? t + i : end - 1;
-      uint32_t r = base + (page < c.pages ? (uint32_t)(t_i - t_q) : 0u);
-      if (!aligned_quads) r = kv4_row(c, kv4_page(c, b, (uint32_t)t_i), h, (uint32_t)t_i);
-      const uint64_t at = c.plane_rows + r;
-      load_values<D>(c.codes + at * (D / 2) + element / 2, v[i]);
-      vs[i] = c.scales[at * kScales + element / 32];
+      for (int i = 0; i < 4; ++i) {
+        const int tk = t0 + 16 * i + n, tv = t0 + 4 * quad + i;
+        p.k[i] = kv4_page(c, b, (uint32_t)(tk < end ? tk : end - 1));
+        p.v[i] = kv4_page(c, b, (uint32_t)(tv < end ? tv : end - 1));
+      }
+    }
+  };
+  uint32_t v[4][kWords], vs[4];
+  auto load_v = [&](int step, const Pages& p) {
+    const int t0 = begin + step * kBlockStep;
+    if constexpr (kWhole) {
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)p.k[0]);
+      const int first = t0 < end ? t0 : end - 1, last = end - 1 - first;
+      const uint64_t row = c.plane_rows + kv4_row(c, page, h, (uint32_t)first);
+      const uint8_t* codes = c.codes + row * kRow;
+      const uint8_t* scales = c.scales + row * kScales;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = (uint32_t)(4 * quad + i < last ? 4 * quad + i : last);
+        load_values<D>(codes + (u * kRow + element / 2), v[i]);
+        vs[i] = scales[u * kScales + element / 32];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 4 * quad + i;
+        const uint64_t row = c.plane_rows + kv4_row(c, p.v[i], h, (uint32_t)(t < end ? t : end - 1));
+        load_values<D>(c.codes + row * kRow + element / 2, v[i]);
+        vs[i] = c.scales[row * kScales + element / 32];
+      }
+    }
+  };
+  auto load_k = [&](int step, int half, const Pages& p, Loaded<D>& s) {
+    const int t0 = begin + step * kBlockStep + half * kStep;
+    s.t0 = t0;
+    const int left = end - t0;  // tokens of the half that are there
+    s.valid = left >= kStep ? 0xFFFFFFFFu : (left > 0 ? (1u << left) - 1u : 0u);
+    if constexpr (kWhole) {
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)p.k[0]);
+      const int first = t0 < end ? t0 : end - 1, last = end - 1 - first;
+      const uint64_t row = kv4_row(c, page, h, (uint32_t)first);
+      if (page >= c.pages) s.valid = 0u;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t u = (uint32_t)(16 * i + n < last ? 16 * i + n : last);
+        load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, u * kRow, u * kScales, g, s.k[i], s.ks[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int t = t0 + 16 * i + n;
+        const uint32_t page = p.k[2 * half + i];
+        const uint64_t row = kv4_row(c, page, h, (uint32_t)(t < end ? t : end - 1));
+        s.valid &= ~((~(uint32_t)__ballot(page < c.pages) & 0xFFFFu) << (16 * i));
+        load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, 0u, 0u, g, s.k[i], s.ks[i]);
+      }
     }
   };
   // A step's place in LDS: a lane of the second product takes tokens
   // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
   auto store_v = [&](int step) {
     uint16_t* to = &vt[step & 1][element][32 * (quad >> 3) + 8 * (quad & 3) + 4 * (quad >> 2 & 1)];
-    const bool nan = vs[0] == 255 || vs[1] == 255 || vs[2] == 255 || vs[3] == 255;
-    if (nan) nan_step[step & 1] = step;
     float f[4];
+    if (umax32(umax32(vs[0], vs[1]), umax32(vs[2], vs[3])) == 255) {
+      nan_step[step & 1] = step;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = vs[i] == 255 ? 0.0f : u2f(vs[i] << 23);
+      for (int i = 0; i < 4; ++i) vs[i] = vs[i] == 255 ? 0u : vs[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = u2f(vs[i] << 23);
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
       auto pair = [&](auto which) {
@@ -745,73 +818,65 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     }
   };
 
-  // Keys: the wave's own, 32 tokens at a time.
-  auto page_of = [&](int s) -> uint32_t {
-    if (!c.table) return b;
-    const int t = begin + s * kStep + (lane & 31);
-    return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
+  // which of a step's scores the row sees, as bits
+  auto seen_of = [&](const Loaded<D>& s, int at) {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = s.t0 + u;
+      seen |= (uint32_t)((s.valid >> u & 1u) && t <= at && (q.window == 0 || t > at - q.window)) << j;
+    }
+    return seen;
   };
-  auto work = [&](const Loaded<D>& s, int step, int half) {
+  auto work = [&](const Loaded<D>& s, int step, int half, bool nan) {
     if (s.t0 >= mine.hi || s.t0 + kStep <= mine.lo) return;
     float x[kSub][8];
     step_scores<D, T, kSub>(terms, s, x);
-    const bool masked = needs_mask(mine, s.valid, s.t0, q.window);
-    const bool nan = nan_step[step & 1] == step;
-    u32x4 p[kSub][kP];
+    if (kExtra) {
 #pragma unroll
-    for (int y = 0; y < kSub; ++y) {
-      uint32_t seen = 0xFFu;
-      if (kExtra) {
+      for (int y = 0; y < kSub; ++y)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           x[y][j] = curved<true>(curve[y], x[y][j], pos[y] - (s.t0 + (j >> 2) * 16 + 4 * g + (j & 3)));
-      }
-      if (masked) {
-        seen = 0;
+    }
+    if (needs_mask(mine, s.valid, s.t0, q.window)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = s.t0 + u;
-          const bool in = (s.valid >> u & 1u) && t <= pos[y] && (q.window == 0 || t > pos[y] - q.window);
-          x[y][j] = in ? x[y][j] : -__builtin_huge_valf();
-          seen |= (uint32_t)in << j;
-        }
-      }
-      const float scale = kExtra ? 1.0f : curve[y].scale;
-      float top = x[y][0];
+      for (int y = 0; y < kSub; ++y) {
+        const uint32_t seen = seen_of(s, pos[y]);
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, x[y][j]);
-      top *= scale;
-      if (__ballot(top > m[y] + kSlack)) {
-        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-        const float next = __builtin_fmaxf(m[y], top), f = __builtin_amdgcn_exp2f(m[y] - next);
+        for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : -__builtin_huge_valf();
+      }
+    }
+    const float scale = kExtra ? 1.0f : curve[0].scale;
+    float top[kSub];
+    bool above = false;
+#pragma unroll
+    for (int y = 0; y < kSub; ++y) {
+      top[y] = x[y][0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top[y] = __builtin_fmaxf(top[y], x[y][j]);
+      top[y] *= scale;
+      above |= top[y] > m[y] + kSlack;
+    }
+    if (__ballot(above)) {
+#pragma unroll
+      for (int y = 0; y < kSub; ++y) {
+        float t = __builtin_fmaxf(top[y], __shfl_xor(top[y], 16));
+        t = __builtin_fmaxf(t, __shfl_xor(t, 32));
+        const float next = __builtin_fmaxf(m[y], t), f = __builtin_amdgcn_exp2f(m[y] - next);
         m[y] = next;
         l[y] *= f;
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) acc[y][j] *= f;
       }
+    }
+    u32x4 p[kSub][kP];
+#pragma unroll
+    for (int y = 0; y < kSub; ++y) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[y][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[y][j], scale, -m[y]));
-      if (masked) {
-        // a scale of 0 makes NaN of what is masked
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) l[y] += x[y][j];
+      l[y] += ((x[y][0] + x[y][1]) + (x[y][2] + x[y][3])) + ((x[y][4] + x[y][5]) + (x[y][6] + x[y][7]));
       split_terms(x[y], p[y]);
-      if (nan) {
-        // the blocks that were taken as tiny, for the rows that see them
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int u = (j >> 2) * 16 + 4 * g + (j & 3);
-          const int t = s.t0 + u < end ? s.t0 + u : end - 1;
-          if (seen >> j & 1u) {
-            const uint64_t at = c.plane_rows + kv4_row(c, kv4_page(c, b, (uint32_t)t), h, (uint32_t)t);
-            for (int k = 0; k < kScales; ++k) bad[y] |= (uint32_t)(c.scales[at * kScales + k] == 255) << k;
-          }
-        }
-      }
     }
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
@@ -822,29 +887,46 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         for (int y = 0; y < kSub; ++y)
           acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, p[y][t]), acc[y][j], 0, 0, 0);
     }
+    if (nan) {
+      // the blocks that were taken as tiny, for the rows that see them
+#pragma unroll
+      for (int y = 0; y < kSub; ++y) {
+        const uint32_t seen = seen_of(s, pos[y]);
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < 8; ++j) {
+          const int t = s.t0 + (j >> 2) * 16 + 4 * g + (j & 3);
+          if (seen >> j & 1u) {
+            const uint64_t at = c.plane_rows + kv4_row(c, kv4_page(c, b, (uint32_t)t), h, (uint32_t)t);
+#pragma clang loop unroll(disable)
+            for (int k = 0; k < kScales; ++k) bad[y] |= (uint32_t)(c.scales[at * kScales + k] == 255) << k;
+          }
+        }
+      }
+    }
   };
 
   if (steps > 0) {
     Loaded<D> one, two;
-    load_v(0);
-    uint32_t page = page_of(0);
-    load_step<D, true, false>(c, h, page, aligned_pages, begin, end, lane, one);
-    page = page_of(1);
+    Pages now, next, later;  // of this step, the next and the one after
+    pages_of(0, now);
+    pages_of(1, next);
+    pages_of(2, later);
+    load_v(0, now);
+    load_k(0, 0, now, one);
     __syncthreads();
     store_v(0);
-    if (steps > 1) load_v(1);
+    load_v(1, next);
     for (int step = 0; step < steps; ++step) {
-      const int t0 = begin + step * kBlockStep;
       __syncthreads();
-      if (step + 1 < steps) store_v(step + 1);
-      if (step + 2 < steps) load_v(step + 2);
-      const bool second = t0 + kStep < end;
-      if (second) load_step<D, true, false>(c, h, page, aligned_pages, t0 + kStep, end, lane, two);
-      page = page_of(2 * step + 2);
-      work(one, step, 0);
-      if (step + 1 < steps) load_step<D, true, false>(c, h, page, aligned_pages, t0 + kBlockStep, end, lane, one);
-      page = page_of(2 * step + 3);
-      if (second) work(two, step, 1);
+      const bool nan = nan_step[step & 1] == step;
+      store_v(step + 1);
+      load_v(step + 2, later);
+      load_k(step, 1, now, two);
+      work(one, step, 0, nan);
+      now = next, next = later;
+      load_k(step + 1, 0, now, one);
+      pages_of(step + 3, later);
+      work(two, step, 1, nan);
     }
   }
 
@@ -885,7 +967,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
                  h = slot / (uint32_t)plan.tiles % c.kv;
   const int tile = (int)(slot % (uint32_t)plan.tiles), n = (int)(blockIdx.x % (uint32_t)plan.rows),
             r = tile * plan.rows + n;
-  const TileRows rows = tile_rows(c, q, b, tile, plan.rows);
+  const TileRows rows = tile_rows(c, q, b, tile, plan.rows, plan.rows == kRows ? kStep : kBlockStep);
   if (r >= rows.rows) return;
   const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
   const int64_t size = (int64_t)plan.rows * (D + 2);
@@ -923,26 +1005,26 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
 template <int D, typename T, bool kExtra>
 __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int chunk, int chunks, const float* lse,
                                                         float* weights, int64_t weights_len) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slot = blockIdx.x / (uint32_t)chunks, b = slot / c.kv, h = slot % c.kv;
-  TileRows all = tile_rows(c, q, b, 0, 0x40000000);
+  TileRows all = tile_rows(c, q, b, 0, 0x40000000, kStep);
   int hi = all.hi < weights_len ? all.hi : (int)weights_len;
   const int begin = all.lo + (int)(blockIdx.x % (uint32_t)chunks) * chunk;
   int end = begin + chunk;
   if (end > hi) end = hi;
-  const bool aligned_pages = !c.table || c.size % kStep == 0;
   const int tiles = (all.rows + kRows - 1) / kRows;
   float* w = weights + (int64_t)slot * weights_len;
   for (int t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
     const int t = t0 + (lane & 31);
     const uint32_t page = kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
     Loaded<D> s;
-    load_step<D, true, false>(c, h, page, aligned_pages, t0, end, lane, s);
+    load_any<D, false>(c, h, page, t0, end, lane, s);
     float add[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) add[j] = 0.0f;
     for (int tile = 0; tile < tiles; ++tile) {
-      const TileRows rows = tile_rows(c, q, b, tile, kRows);
+      const TileRows rows = tile_rows(c, q, b, tile, kRows, kStep);
       if (t0 >= rows.hi || t0 + kStep <= rows.lo) continue;
       const int r = tile * kRows + n;
       const bool live = r < rows.rows;
@@ -977,12 +1059,12 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
 Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   Kv4Plan p;
   const int64_t all = (int64_t)q.most * q.group;
-  p.rows = all > kManyRows ? 64 * block_sub(dim, dtype == kBF16 ? 1 : 2) : kRows;
+  p.rows = all > kManyRows ? 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3)) : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   // the most tokens a tile can see
   int64_t span = c.cap;
   if (q.window) {
-    const int64_t seen = (int64_t)q.window + p.rows / q.group + 2 + kStep;
+    const int64_t seen = (int64_t)q.window + p.rows / q.group + 2 + kBlockStep;
     if (seen < span) span = seen;
   }
   const int64_t heads = (int64_t)c.seqs * c.kv * p.tiles;
@@ -1027,6 +1109,7 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
   const Kv4Plan p = kv4_plan(c, dim, q, dtype);
   const bool extra = q.softcap != 0.0f || q.slopes;
+  const bool whole = !c.table || c.size % (p.rows == kRows ? kStep : kBlockStep) == 0;
   const int64_t slots = (int64_t)p.tiles * c.seqs * c.kv;
   if (slots * (p.splits > p.rows ? p.splits : p.rows) >= 1ll << 31)
     return set_error(kErrUnsupported, "kv4_attention: %lld tiles of %d splits do not fit a launch", (long long)slots,
@@ -1034,10 +1117,14 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
   const dim3 grid((unsigned)(slots * p.splits));
 #define VQX_KV4_LAUNCH(NAME, D, T)                                                                                   \
   do {                                                                                                             \
-    if (extra)                                                                                                     \
-      hipLaunchKernelGGL((NAME<D, T, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                       \
+    if (extra && whole)                                                                                            \
+      hipLaunchKernelGGL((NAME<D, T, true, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                 \
+    else if (extra)                                                                                                \
+      hipLaunchKernelGGL((NAME<D, T, true, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                \
+    else if (whole)                                                                                                \
+      hipLaunchKernelGGL((NAME<D, T, false, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                \
     else                                                                                                           \
-      hipLaunchKernelGGL((NAME<D, T, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                      \
+      hipLaunchKernelGGL((NAME<D, T, false, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);               \
   } while (0)
 #define VQX_KV4_ROWS(D, T)                                                                                         \
   do {                                                                                                             \
