@@ -89,25 +89,29 @@ __device__ __forceinline__ int key_element(int i, int g) {
   return D == 64 ? 16 * g + 8 * i : 128 * (i / 4) + 32 * g + 8 * (i % 4);
 }
 
+// 8 elements of a row's query from element i as the B operand's terms, a
+// negative scale's sign included.
+template <typename T, int kTerms>
+__device__ __forceinline__ void load_query(const Kv4Query& q, int64_t i, bool live, T, u32x4 (&t)[kTerms]) {
+  const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u;
+  if (live) {
+    load_terms(q.q, i, T(), t);
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) t[k] ^= flip;
+  } else {
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) t[k] = u32x4{0, 0, 0, 0};
+  }
+}
+
 // One row's query as that product's B operand.
 template <int D, typename T>
 struct QueryTerms {
-  static constexpr int kTerms = Terms<T>::kQ;
-  u32x4 v[D / 32][kTerms];
+  u32x4 v[D / 32][Terms<T>::kQ];
 
-  // flip: 0, or the bf16 sign bits of a negative scale
-  __device__ __forceinline__ void load(const void* p, int64_t at, bool live, int g, uint32_t flip) {
+  __device__ __forceinline__ void load(const Kv4Query& q, int64_t at, bool live, int g) {
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      if (live) {
-        load_terms(p, at + key_element<D>(i, g), T(), v[i]);
-#pragma unroll
-        for (int t = 0; t < kTerms; ++t) v[i][t] ^= flip;
-      } else {
-#pragma unroll
-        for (int t = 0; t < kTerms; ++t) v[i][t] = u32x4{0, 0, 0, 0};
-      }
-    }
+    for (int i = 0; i < D / 32; ++i) load_query(q, at + key_element<D>(i, g), live, T(), v[i]);
   }
 };
 
@@ -318,15 +322,12 @@ __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, kByte));
 }
 
-// Scores of the step's tokens 16 i + 4 g + r in x[y][4 i + r], lane (row, g) of
-// each of kSub tiles of 16 rows.
-template <int D, typename T, int kSub>
-__device__ __forceinline__ void step_scores(const QueryTerms<D, T> (&q)[kSub], const Loaded<D>& s, float (&x)[kSub][8]) {
+// Scores of the step's tokens 16 i + 4 g + r in x[4 i + r], lane (row, g).
+template <int D, typename T>
+__device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loaded<D>& s, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    f32x4 acc[kSub];
-#pragma unroll
-    for (int y = 0; y < kSub; ++y) acc[y] = f32x4{0, 0, 0, 0};
+    f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
     for (int a = 0; a < D / 32; ++a) {
       const float scale = u2f(s.ks[i][a / 4] << 23);
@@ -334,15 +335,11 @@ __device__ __forceinline__ void step_scores(const QueryTerms<D, T> (&q)[kSub], c
       const u32x4 k = {fp4_pair<0>(w, scale), fp4_pair<1>(w, scale), fp4_pair<2>(w, scale), fp4_pair<3>(w, scale)};
 #pragma unroll
       for (int t = 0; t < Terms<T>::kQ; ++t)
-#pragma unroll
-        for (int y = 0; y < kSub; ++y)
-          acc[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
-                                                           __builtin_bit_cast(bf16x8, q[y].v[a][t]), acc[y], 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q.v[a][t]),
+                                                      acc, 0, 0, 0);
     }
 #pragma unroll
-    for (int y = 0; y < kSub; ++y)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[y][4 * i + r] = acc[y][r];
+    for (int r = 0; r < 4; ++r) x[4 * i + r] = acc[r];
   }
 }
 
@@ -445,9 +442,8 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
   for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0, 0, 0, 0};
 
   if (wave < steps) {
-    QueryTerms<D, T> terms[1];
-    terms[0].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
-                  q.scale < 0.0f ? 0x80008000u : 0u);
+    QueryTerms<D, T> terms;
+    terms.load(q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
 
     // the page of this lane's token in step s
     auto page_of = [&](int s) -> uint32_t {
@@ -455,9 +451,8 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
       return kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
     };
     auto work = [&](const Loaded<D>& s) {
-      float scores[1][8];
-      step_scores<D, T, 1>(terms, s, scores);
-      float(&x)[8] = scores[0];
+      float x[8];
+      step_scores<D, T>(terms, s, x);
       const bool masked = needs_mask(rows, s.valid, s.t0, q.window);
       uint32_t seen;
       finish_scores<kExtra>(curve, x, s.valid, s.t0, g, pos, q.window, masked, seen);
@@ -646,28 +641,28 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
 // Rows of a kv head from which on the kernel for many rows is taken.
 constexpr int kManyRows = 32;
 
-// Many rows: a workgroup has 128 rows of one kv head, 32 of them a wave (64 and
-// 16 where a wave has one tile), and
-// walks over the tokens by 64.  The values of a step are turned into bf16 once,
-// transposed into LDS (two buffers, one barrier a step), and read by all four
-// waves; each wave turns the keys itself, since two of its tiles share them
-// and reading them from LDS as bf16 would take all of its bandwidth.  Bound by
-// the vector instructions of the softmax beside the matrix ones.
+// Tokens of a step of the kernel for many rows.
+constexpr int kBlockStep = 64;
 // Tiles of 16 rows of a wave: 2, and 1 where the registers do not hold the
 // queries' terms and the outputs of 2.
 constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 : 2; }
-constexpr int kBlockStep = 64;
-constexpr int kVRow = kBlockStep + 8;  // bf16 of one element's tokens in LDS: rows 16 bytes off each other's banks
-
+// Many rows: a workgroup has 128 rows of one kv head, 32 of them a wave (64 and
+// 16 where a wave has one tile), and walks over the tokens by 64.  Keys and
+// values of a step are turned into bf16 once, the values transposed, into LDS
+// (two buffers, one barrier a step), and read by all four waves.  Bound by the
+// vector instructions of the softmax beside the matrix ones.
 template <int D, typename T, bool kExtra, bool kWhole>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
-                                                        float* ws) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out,
+                                                                         float* lse, float* ws) {
   constexpr int kTiles = D / 16;
-  constexpr int kWords = Loaded<D>::kWords, kScales = D / 32;
+  constexpr int kVWords = Loaded<D>::kWords, kKWords = D / 32, kRow = D / 2, kScales = D / 32;
+  constexpr int kKScales = D == 256 ? 2 : 1;  // of a thread's keys
   constexpr int kP = Terms<T>::kBlockP;
   constexpr int kSub = block_sub(D, Terms<T>::kQ), kBlockRows = 64 * kSub;
-  __shared__ __align__(16) uint16_t vt[2][D][kVRow];
-  __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block
+  // rows a 16-byte bank group off each other's
+  __shared__ __align__(16) uint16_t kt[2][kBlockStep][D + 8];
+  __shared__ __align__(16) uint16_t vt[2][D][kBlockStep + 8];
+  __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block of values
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads first, so that with 8 of them each XCD's L2 has the cache of one;
@@ -690,7 +685,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   const TileRows mine = tile_rows(c, q, b, tile * kWaves + wave, 16 * kSub, kStep);
   int row[kSub], pos[kSub];
   Curve curve[kSub];
-  QueryTerms<D, T> terms[kSub];
+  u32x4 terms[kSub][kKWords][Terms<T>::kQ];
 #pragma unroll
   for (int y = 0; y < kSub; ++y) {
     row[y] = r0 + 16 * y + n;
@@ -698,8 +693,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     const int token = row[y] / q.group, head = (int)h * q.group + row[y] % q.group;
     pos[y] = live ? rows.base + token : -1;
     curve[y] = curve_of(q, live ? head : (int)h * q.group);
-    terms[y].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
-                  q.scale < 0.0f ? 0x80008000u : 0u);
+    const int64_t at = (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh;
+#pragma unroll
+    for (int a = 0; a < kKWords; ++a) load_query(q, at + 32 * a + 8 * g, live, T(), terms[y][a]);
   }
   float m[kSub], l[kSub];
   uint32_t bad[kSub];
@@ -715,80 +711,86 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   // Loads go round without a branch, so that each wait is for its own: a token
   // past the end is the last one, which no row counts.  Where pages hold whole
   // steps (kWhole) a step has one base, its page looked up a step ahead;
-  // otherwise every lane looks its tokens' pages up, a step ahead too.
-  constexpr int kRow = D / 2;
+  // otherwise every thread looks its tokens' pages up, a step ahead too.
+  // Keys: thread (token, part) has D / 4 elements of a token; values: thread
+  // (quad, part) has D / 16 of four tokens.
+  const int k_token = tid >> 2, k_part = tid & 3;
   const int quad = tid & 15, element = (tid >> 4) * (D / 16);
   struct Pages {
-    uint32_t k[4], v[4];  // kWhole: k[0] only
+    uint32_t k, v[4], all;  // kWhole: k only
   };
+  auto clamped = [&](int t) { return (uint32_t)(t < end ? t : end - 1); };
   auto pages_of = [&](int step, Pages& p) {
     const int t0 = begin + step * kBlockStep;
     if constexpr (kWhole) {
-      p.k[0] = kv4_page(c, b, (uint32_t)(t0 < end ? t0 : end - 1));
+      p.k = kv4_page(c, b, clamped(t0));
+    } else {
+      p.k = kv4_page(c, b, clamped(t0 + k_token));
+      p.all = kv4_page(c, b, clamped(t0 + lane));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p.v[i] = kv4_page(c, b, clamped(t0 + 4 * quad + i));
+    }
+  };
+  uint32_t k[kKWords], ks[kKScales], v[4][kVWords], vs[4];
+  auto take_keys = [&](const uint8_t* codes, const uint8_t* scales, uint32_t at, uint32_t scale_at) {
+    if constexpr (D == 64) {
+      const u32x2 a = *reinterpret_cast<const u32x2*>(codes + (at + 8 * k_part));
+      k[0] = a[0], k[1] = a[1];
+      ks[0] = scales[scale_at + k_part / 2];
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tk = t0 + 16 * i + n, tv = t0 + 4 * quad + i;
-        p.k[i] = kv4_page(c, b, (uint32_t)(tk < end ? tk : end - 1));
-        p.v[i] = kv4_page(c, b, (uint32_t)(tv < end ? tv : end - 1));
+      for (int i = 0; i < kKScales; ++i) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(codes + (at + 16 * kKScales * k_part) + 16 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[4 * i + j] = a[j];
+        ks[i] = scales[(scale_at + kKScales * k_part) + i];
       }
     }
   };
-  uint32_t v[4][kWords], vs[4];
-  auto load_v = [&](int step, const Pages& p) {
+  // returns bit t: token t of the step is there
+  auto load = [&](int step, const Pages& p) -> uint64_t {
     const int t0 = begin + step * kBlockStep;
     if constexpr (kWhole) {
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)p.k[0]);
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)p.k);
       const int first = t0 < end ? t0 : end - 1, last = end - 1 - first;
-      const uint64_t row = c.plane_rows + kv4_row(c, page, h, (uint32_t)first);
-      const uint8_t* codes = c.codes + row * kRow;
-      const uint8_t* scales = c.scales + row * kScales;
+      const uint64_t at = kv4_row(c, page, h, (uint32_t)first), v_at = c.plane_rows + at;
+      const uint32_t u = (uint32_t)(k_token < last ? k_token : last);
+      take_keys(c.codes + at * kRow, c.scales + at * kScales, u * kRow, u * kScales);
+      const uint8_t* codes = c.codes + v_at * kRow;
+      const uint8_t* scales = c.scales + v_at * kScales;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t u = (uint32_t)(4 * quad + i < last ? 4 * quad + i : last);
-        load_values<D>(codes + (u * kRow + element / 2), v[i]);
-        vs[i] = scales[u * kScales + element / 32];
+        const uint32_t w = (uint32_t)(4 * quad + i < last ? 4 * quad + i : last);
+        load_values<D>(codes + (w * kRow + element / 2), v[i]);
+        vs[i] = scales[w * kScales + element / 32];
       }
+      const int left = end - t0;
+      const uint64_t there = left >= kBlockStep ? ~0ull : (left > 0 ? (1ull << left) - 1 : 0ull);
+      return page < c.pages ? there : 0ull;
     } else {
+      const uint64_t at = kv4_row(c, p.k, h, clamped(t0 + k_token));
+      take_keys(c.codes + at * kRow, c.scales + at * kScales, 0u, 0u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int t = t0 + 4 * quad + i;
-        const uint64_t row = c.plane_rows + kv4_row(c, p.v[i], h, (uint32_t)(t < end ? t : end - 1));
-        load_values<D>(c.codes + row * kRow + element / 2, v[i]);
-        vs[i] = c.scales[row * kScales + element / 32];
+        const uint64_t v_at = c.plane_rows + kv4_row(c, p.v[i], h, clamped(t0 + 4 * quad + i));
+        load_values<D>(c.codes + v_at * kRow + element / 2, v[i]);
+        vs[i] = c.scales[v_at * kScales + element / 32];
       }
-    }
-  };
-  auto load_k = [&](int step, int half, const Pages& p, Loaded<D>& s) {
-    const int t0 = begin + step * kBlockStep + half * kStep;
-    s.t0 = t0;
-    const int left = end - t0;  // tokens of the half that are there
-    s.valid = left >= kStep ? 0xFFFFFFFFu : (left > 0 ? (1u << left) - 1u : 0u);
-    if constexpr (kWhole) {
-      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)p.k[0]);
-      const int first = t0 < end ? t0 : end - 1, last = end - 1 - first;
-      const uint64_t row = kv4_row(c, page, h, (uint32_t)first);
-      if (page >= c.pages) s.valid = 0u;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t u = (uint32_t)(16 * i + n < last ? 16 * i + n : last);
-        load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, u * kRow, u * kScales, g, s.k[i], s.ks[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = t0 + 16 * i + n;
-        const uint32_t page = p.k[2 * half + i];
-        const uint64_t row = kv4_row(c, page, h, (uint32_t)(t < end ? t : end - 1));
-        s.valid &= ~((~(uint32_t)__ballot(page < c.pages) & 0xFFFFu) << (16 * i));
-        load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, 0u, 0u, g, s.k[i], s.ks[i]);
-      }
+      return __ballot(t0 + lane < end && p.all < c.pages);
     }
   };
   // A step's place in LDS: a lane of the second product takes tokens
   // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
-  auto store_v = [&](int step) {
+  auto store = [&](int step) {
+    uint16_t* kto = &kt[step & 1][k_token][k_part * (D / 4)];
+#pragma unroll
+    for (int i = 0; i < kKWords; ++i) {
+      const float f = u2f(ks[i / 4] << 23);
+      *reinterpret_cast<u32x4*>(kto + 8 * i) =
+          u32x4{fp4_pair<0>(k[i], f), fp4_pair<1>(k[i], f), fp4_pair<2>(k[i], f), fp4_pair<3>(k[i], f)};
+    }
     uint16_t* to = &vt[step & 1][element][32 * (quad >> 3) + 8 * (quad & 3) + 4 * (quad >> 2 & 1)];
+    constexpr int kNext = kBlockStep + 8;
     float f[4];
     if (umax32(umax32(vs[0], vs[1]), umax32(vs[2], vs[3])) == 255) {
       nan_step[step & 1] = step;
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = u2f(vs[i] << 23);
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) {
+    for (int w = 0; w < kVWords; ++w) {
       auto pair = [&](auto which) {
         constexpr int kByte = decltype(which)::value;
         uint32_t x[4];
@@ -806,8 +808,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         for (int i = 0; i < 4; ++i) x[i] = fp4_pair<kByte>(v[i][w], f[i]);
         const u32x2 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
         const u32x2 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
-        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte) * kVRow) = even;
-        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte + 1) * kVRow) = odd;
+        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte) * kNext) = even;
+        *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte + 1) * kNext) = odd;
       };
       pair(std::integral_constant<int, 0>());
       pair(std::integral_constant<int, 1>());
@@ -818,36 +820,56 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     }
   };
 
-  // which of a step's scores the row sees, as bits
-  auto seen_of = [&](const Loaded<D>& s, int at) {
+  // Scores of the half step's tokens 16 i + 4 g + r in x[y][4 i + r].
+  auto scores = [&](int step, int half, float (&x)[kSub][8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x4 s[kSub];
+#pragma unroll
+      for (int y = 0; y < kSub; ++y) s[y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int a = 0; a < kKWords; ++a) {
+        const bf16x8 key = *reinterpret_cast<const bf16x8*>(&kt[step & 1][32 * half + 16 * i + n][32 * a + 8 * g]);
+#pragma unroll
+        for (int t = 0; t < Terms<T>::kQ; ++t)
+#pragma unroll
+          for (int y = 0; y < kSub; ++y)
+            s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, __builtin_bit_cast(bf16x8, terms[y][a][t]), s[y], 0, 0, 0);
+      }
+#pragma unroll
+      for (int y = 0; y < kSub; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[y][4 * i + r] = s[y][r];
+    }
+  };
+  // which of a half step's scores the row sees, as bits
+  auto seen_of = [&](uint32_t valid, int t0, int at) {
     uint32_t seen = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = s.t0 + u;
-      seen |= (uint32_t)((s.valid >> u & 1u) && t <= at && (q.window == 0 || t > at - q.window)) << j;
+      const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = t0 + u;
+      seen |= (uint32_t)((valid >> u & 1u) && t <= at && (q.window == 0 || t > at - q.window)) << j;
     }
     return seen;
   };
-  auto work = [&](const Loaded<D>& s, int step, int half, bool nan) {
-    if (s.t0 >= mine.hi || s.t0 + kStep <= mine.lo) return;
-    float x[kSub][8];
-    step_scores<D, T, kSub>(terms, s, x);
+  const float scale = kExtra ? 1.0f : curve[0].scale;
+  // curve and mask, and the references moved where a score passes them
+  auto settle = [&](float (&x)[kSub][8], uint32_t valid, int t0) {
     if (kExtra) {
 #pragma unroll
       for (int y = 0; y < kSub; ++y)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          x[y][j] = curved<true>(curve[y], x[y][j], pos[y] - (s.t0 + (j >> 2) * 16 + 4 * g + (j & 3)));
+          x[y][j] = curved<true>(curve[y], x[y][j], pos[y] - (t0 + (j >> 2) * 16 + 4 * g + (j & 3)));
     }
-    if (needs_mask(mine, s.valid, s.t0, q.window)) {
+    if (needs_mask(mine, valid, t0, q.window)) {
 #pragma unroll
       for (int y = 0; y < kSub; ++y) {
-        const uint32_t seen = seen_of(s, pos[y]);
+        const uint32_t seen = seen_of(valid, t0, pos[y]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : -__builtin_huge_valf();
       }
     }
-    const float scale = kExtra ? 1.0f : curve[0].scale;
     float top[kSub];
     bool above = false;
 #pragma unroll
@@ -870,7 +892,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         for (int j = 0; j < kTiles; ++j) acc[y][j] *= f;
       }
     }
-    u32x4 p[kSub][kP];
+  };
+  auto weights = [&](float (&x)[kSub][8], u32x4 (&p)[kSub][kP]) {
 #pragma unroll
     for (int y = 0; y < kSub; ++y) {
 #pragma unroll
@@ -878,6 +901,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
       l[y] += ((x[y][0] + x[y][1]) + (x[y][2] + x[y][3])) + ((x[y][4] + x[y][5]) + (x[y][6] + x[y][7]));
       split_terms(x[y], p[y]);
     }
+  };
+  auto gather = [&](int step, int half, const u32x4 (&p)[kSub][kP]) {
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
       const bf16x8 a = *reinterpret_cast<const bf16x8*>(&vt[step & 1][16 * j + n][32 * half + 8 * g]);
@@ -887,18 +912,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         for (int y = 0; y < kSub; ++y)
           acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, p[y][t]), acc[y][j], 0, 0, 0);
     }
-    if (nan) {
-      // the blocks that were taken as tiny, for the rows that see them
+  };
+  // the blocks of values that were taken as tiny, for the rows that see them
+  auto note_nan = [&](uint64_t valid, int t0) {
+#pragma clang loop unroll(disable)
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int y = 0; y < kSub; ++y) {
-        const uint32_t seen = seen_of(s, pos[y]);
+        const uint32_t seen = seen_of((uint32_t)(valid >> (32 * half)), t0 + 32 * half, pos[y]);
 #pragma clang loop unroll(disable)
         for (int j = 0; j < 8; ++j) {
-          const int t = s.t0 + (j >> 2) * 16 + 4 * g + (j & 3);
+          const int t = t0 + 32 * half + (j >> 2) * 16 + 4 * g + (j & 3);
           if (seen >> j & 1u) {
             const uint64_t at = c.plane_rows + kv4_row(c, kv4_page(c, b, (uint32_t)t), h, (uint32_t)t);
 #pragma clang loop unroll(disable)
-            for (int k = 0; k < kScales; ++k) bad[y] |= (uint32_t)(c.scales[at * kScales + k] == 255) << k;
+            for (int x = 0; x < kScales; ++x) bad[y] |= (uint32_t)(c.scales[at * kScales + x] == 255) << x;
           }
         }
       }
@@ -906,27 +934,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   };
 
   if (steps > 0) {
-    Loaded<D> one, two;
-    Pages now, next, later;  // of this step, the next and the one after
-    pages_of(0, now);
-    pages_of(1, next);
-    pages_of(2, later);
-    load_v(0, now);
-    load_k(0, 0, now, one);
+    Pages next, later;  // of the step whose loads come next and of the one after
+    pages_of(0, next);
+    pages_of(1, later);
+    uint64_t valid = load(0, next), valid_next;
     __syncthreads();
-    store_v(0);
-    load_v(1, next);
+    store(0);
+    next = later;
+    valid_next = load(1, next);
+    pages_of(2, next);
     for (int step = 0; step < steps; ++step) {
+      const int t0 = begin + step * kBlockStep;
       __syncthreads();
       const bool nan = nan_step[step & 1] == step;
-      store_v(step + 1);
-      load_v(step + 2, later);
-      load_k(step, 1, now, two);
-      work(one, step, 0, nan);
-      now = next, next = later;
-      load_k(step + 1, 0, now, one);
-      pages_of(step + 3, later);
-      work(two, step, 1, nan);
+      store(step + 1);
+      const uint64_t valid_later = load(step + 2, next);
+      pages_of(step + 3, next);
+      if (t0 < mine.hi && t0 + kBlockStep > mine.lo) {
+        float x0[kSub][8], x1[kSub][8];
+        u32x4 p[kSub][kP];
+        scores(step, 0, x0);
+        settle(x0, (uint32_t)valid, t0);
+        scores(step, 1, x1);
+        weights(x0, p);
+        gather(step, 0, p);
+        settle(x1, (uint32_t)(valid >> 32), t0 + kStep);
+        weights(x1, p);
+        gather(step, 1, p);
+        if (nan) note_nan(valid, t0);
+      }
+      valid = valid_next, valid_next = valid_later;
     }
   }
 
@@ -942,10 +979,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     for (int j = 0; j < kTiles; ++j) acc[y][j] = bad[y] >> (j / 2) & 1u ? acc[y][j] * __builtin_nanf("") : acc[y][j] * inv;
     if (plan.splits > 1) {
       float* o = ws + (((int64_t)slot * plan.tiles + tile) * plan.splits + split) * (kBlockRows * D + 2 * kBlockRows);
-      const int k = row[y] - tile * kBlockRows;
+      const int r = row[y] - tile * kBlockRows;
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4*>(o + k * D + 16 * j + 4 * g) = acc[y][j];
-      if (g == 0) o[kBlockRows * D + k] = m[y], o[kBlockRows * D + kBlockRows + k] = l[y];
+      for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4*>(o + r * D + 16 * j + 4 * g) = acc[y][j];
+      if (g == 0) o[kBlockRows * D + r] = m[y], o[kBlockRows * D + kBlockRows + r] = l[y];
       continue;
     }
     const int64_t at = (int64_t)(rows.first + row[y] / q.group) * q.heads + (int64_t)h * q.group + row[y] % q.group;
@@ -1029,13 +1066,11 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
       const int r = tile * kRows + n;
       const bool live = r < rows.rows;
       const int token = r / q.group, head = (int)h * q.group + r % q.group;
-      QueryTerms<D, T> terms[1];
-      terms[0].load(q.q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g,
-                    q.scale < 0.0f ? 0x80008000u : 0u);
+      QueryTerms<D, T> terms;
+      terms.load(q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
       const float base = live ? lse[(int64_t)(rows.first + token) * q.heads + head] * kLog2e : 0.0f;
-      float scores[1][8];
-      step_scores<D, T, 1>(terms, s, scores);
-      float(&x)[8] = scores[0];
+      float x[8];
+      step_scores<D, T>(terms, s, x);
       uint32_t seen;
       finish_scores<kExtra>(curve_of(q, live ? head : (int)h * q.group), x, s.valid, t0, g,
                             live ? rows.base + token : -1, q.window,
