@@ -131,7 +131,7 @@ def workspace(L, cache, q):
     (dict(kv_heads=0), ValueError, "sizes"), (dict(page_size=0), ValueError, "sizes"), (dict(seqs=-1), ValueError, "sizes"),
     (dict(table=None, pages=1), ValueError, "without a table"),
     (dict(pages=1 << 31), RuntimeError, "2\\^32 rows"), (dict(pages=1 << 30, page_size=32), RuntimeError, "2\\^32 rows"),
-    (dict(pages_per_seq=1 << 30), RuntimeError, "2\\^31 tokens"), (dict(seqs=1 << 24), RuntimeError, "2\\^24 heads")])
+    (dict(pages_per_seq=1 << 26), RuntimeError, "2\\^30 tokens"), (dict(seqs=1 << 24), RuntimeError, "2\\^24 heads")])
 def test_library_cache_refusals(vqx, how, error, message):
     L = vqx._lib
     with pytest.raises(error, match=message):
@@ -142,7 +142,7 @@ def test_library_cache_refusals(vqx, how, error, message):
     (dict(dtype=3), "dtype 3"), (dict(n=3), "without offsets"), (dict(n=-2), "new tokens"), (dict(heads=3), "3 query heads"),
     (dict(heads=0), "0 query heads"), (dict(q=None), "null"), (dict(q=BASE + 4), "16 bytes"), (dict(stride_n=516), "16 bytes"),
     (dict(stride_h=4), "16 bytes"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
-    (dict(window=-1), "window"), (dict(most=-1), "most")])
+    (dict(window=-1), "window"), (dict(window=1 << 30), "window"), (dict(n=1 << 30), "new tokens"), (dict(most=-1), "most")])
 def test_library_query_refusals(vqx, how, message):
     L = vqx._lib
     with pytest.raises(ValueError, match=message):

@@ -126,8 +126,8 @@ static int to_view(const vqx_kv4_cache* c, const char* what, Kv4View* v) {
       c->pages * c->kv_heads * c->page_size >= limit)
     return set_error(kErrUnsupported, "%s: a cache of 2^32 rows or more", what);
   const int64_t per_seq = c->table ? c->pages_per_seq : 1;
-  if (per_seq >= 1ll << 31 || per_seq * c->page_size >= (1ll << 31) - 4096)
-    return set_error(kErrUnsupported, "%s: room for 2^31 tokens or more in a sequence", what);
+  if (per_seq >= 1ll << 31 || per_seq * c->page_size >= 1ll << 30)
+    return set_error(kErrUnsupported, "%s: room for 2^30 tokens or more in a sequence", what);
   if ((int64_t)c->seqs * c->kv_heads >= 1ll << 24)
     return set_error(kErrUnsupported, "%s: 2^24 heads of sequences or more", what);
   v->codes = c->codes;
@@ -146,7 +146,7 @@ static int to_view(const vqx_kv4_cache* c, const char* what, Kv4View* v) {
 }
 
 static int to_tokens(const Kv4View& c, const int32_t* cu, int64_t n, const char* what, Kv4Tokens* t) {
-  if (n < 0 || n >= 1ll << 31) return set_error(kErrInvalid, "%s: %lld new tokens", what, (long long)n);
+  if (n < 0 || n >= 1ll << 30) return set_error(kErrInvalid, "%s: %lld new tokens", what, (long long)n);
   if (!cu && (c.seqs == 0 ? n != 0 : n % c.seqs != 0))
     return set_error(kErrInvalid, "%s: %lld new tokens for %u sequences without offsets", what, (long long)n, c.seqs);
   if (c.seqs == 0 && n != 0) return set_error(kErrInvalid, "%s: new tokens of no sequence", what);
@@ -182,7 +182,8 @@ static int to_query(const Kv4View& c, int dim, const vqx_kv4_query* q, const cha
   if (rc != kOk) return rc;
   if (!(q->softcap >= 0.0f) || q->softcap > 3.0e38f)
     return set_error(kErrInvalid, "%s: a softcap is positive, or 0 for none", what);
-  if (q->window < 0) return set_error(kErrInvalid, "%s: a window is positive, or 0 for none", what);
+  if (q->window < 0 || q->window >= 1 << 30)
+    return set_error(kErrInvalid, "%s: a window is positive and below 2^30, or 0 for none", what);
   if (q->most < 0) return set_error(kErrInvalid, "%s: most is negative", what);
   v->q = q->q;
   v->sn = q->stride_n;

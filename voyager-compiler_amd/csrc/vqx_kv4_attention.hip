@@ -19,7 +19,6 @@
 // 2^-17 of their sums' magnitude in the mean, against 2^-25 here.
 #include "vqx_kv4.h"
 
-#define VQX_RB (D == 64 ? 3 : (D == 128 ? 2 : 1))
 namespace vqx {
 namespace {
 
@@ -135,7 +134,10 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
                                               int step) {
   TileRows r;
   kv4_span(q.tokens, b, r.first, r.count);
-  const int length = c.lengths[b];
+  // room, new tokens and windows are below 2^30 (checked by the host), a length
+  // is kept there, so that no place overflows
+  int length = c.lengths[b];
+  length = length < 0 ? 0 : (length > (1 << 30) ? 1 << 30 : length);
   r.base = length - r.count;
   const int n = r.count < q.most ? r.count : q.most;
   r.rows = n * q.group;
@@ -155,17 +157,8 @@ struct Curve {
   float scale;          // of a plain score, positive: the queries carry its sign
   float inner, outer;   // capped: outer * tanh(score * inner)
   float slope;
-  bool capped;
+  bool capped, sloped;
 };
-
-// tanh to a few units of fp32: near 0 by its series (the next term is below
-// 2^-26 of the sum), beyond by the exponential.
-__device__ __forceinline__ float tanh32(float x) {
-  const float a = __builtin_fabsf(x), z = x * x;
-  const float s = x + x * z * (-0.333333333f + z * (0.133333333f + z * (-0.0539682540f + z * 0.0218694885f)));
-  const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a * (2.0f * kLog2e)));
-  return a < 0.25f ? s : __builtin_copysignf(t, x);
-}
 
 __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   Curve k;
@@ -174,15 +167,50 @@ __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   k.capped = q.softcap != 0.0f;
   k.inner = k.capped ? __builtin_fabsf(q.scale) / q.softcap : 0.0f;
   k.outer = q.softcap * kLog2e;
+  k.sloped = q.slopes != nullptr;
   k.slope = q.slopes ? q.slopes[head] * kLog2e : 0.0f;
   return k;
 }
 
-template <bool kExtra>
-__device__ __forceinline__ float curved(const Curve& k, float s, int away) {
-  if (!kExtra) return s * k.scale;
-  const float x = k.capped ? k.outer * tanh32(s * k.inner) : s * k.scale;
-  return x - k.slope * (float)away;
+// Capped and sloped scores of a lane's 8 tokens, of which token j is t0 + (j / 4)
+// 16 + j % 4.  tanh to fp32's own error: up to 0.75 an odd polynomial (fitted to
+// 2^-25 of tanh), beyond by the exponential, which no wave computes whose
+// scores are all within the polynomial's range: a cap is mostly well above.
+__device__ __forceinline__ void curve_scores(const Curve& k, float (&x)[8], int pos, int t0) {
+  if (k.capped) {
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] *= k.inner;
+      most = __builtin_fmaxf(most, __builtin_fabsf(x[j]));
+    }
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float z = x[j] * x[j];
+      float p = __builtin_fmaf(z, -0.00476948991f, 0.0196649131f);
+      p = __builtin_fmaf(z, p, -0.0533902584f);
+      p = __builtin_fmaf(z, p, 0.133265212f);
+      p = __builtin_fmaf(z, p, -0.333330684f);
+      y[j] = __builtin_fmaf(x[j] * z, p, x[j]);
+    }
+    if (__ballot(!(most <= 0.75f))) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[j] * (2.0f * kLog2e)));
+        y[j] = __builtin_fabsf(x[j]) <= 0.75f ? y[j] : __builtin_fmaf(-2.0f, r, 1.0f);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = y[j] * k.outer;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= k.scale;
+  }
+  if (k.sloped) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] -= k.slope * (float)(pos - (t0 + (j >> 2) * 16 + (j & 3)));
+  }
 }
 
 // The keys and values of one step of 32 tokens as a wave's loads leave them.
@@ -348,10 +376,11 @@ template <bool kExtra>
 __device__ __forceinline__ void finish_scores(const Curve& k, float (&x)[8], uint32_t valid, int t0, int g, int pos,
                                               int window, bool masked, uint32_t& seen) {
   seen = 0xFFu;
+  if (kExtra) {
+    curve_scores(k, x, pos, t0 + 4 * g);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int t = t0 + (j >> 2) * 16 + 4 * g + (j & 3);
-    x[j] = curved<kExtra>(k, x[j], pos - t);
+    for (int j = 0; j < 8; ++j) x[j] *= k.scale;
   }
   if (masked) {
     seen = 0;
@@ -407,7 +436,7 @@ __device__ __forceinline__ void fill_beyond(const Kv4Query& q, const TileRows& r
 // from memory into the operands' registers, one step ahead, and are joined at
 // the end.
 template <int D, typename T, bool kExtra, bool kWhole>
-__global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
+__global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_rows_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                        float* ws) {
   constexpr int kTiles = D / 16;      // of 16 output elements
   constexpr int kPer = D / 4;         // output elements of a lane
@@ -638,8 +667,6 @@ __global__ __launch_bounds__(256, VQX_RB) void kv4_rows_kernel(Kv4View c, Kv4Que
            T());
 }
 
-// Rows of a kv head from which on the kernel for many rows is taken.
-constexpr int kManyRows = 32;
 
 // Tokens of a step of the kernel for many rows.
 constexpr int kBlockStep = 64;
@@ -857,10 +884,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   auto settle = [&](float (&x)[kSub][8], uint32_t valid, int t0) {
     if (kExtra) {
 #pragma unroll
-      for (int y = 0; y < kSub; ++y)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          x[y][j] = curved<true>(curve[y], x[y][j], pos[y] - (t0 + (j >> 2) * 16 + 4 * g + (j & 3)));
+      for (int y = 0; y < kSub; ++y) curve_scores(curve[y], x[y], pos[y], t0 + 4 * g);
     }
     if (needs_mask(mine, valid, t0, q.window)) {
 #pragma unroll
@@ -992,18 +1016,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   }
 }
 
-// The splits of one row joined, in their order: a workgroup a row, its waves
-// taking splits in turn.
-template <int D, typename T>
+// Splits of a row that one wave joins.
+constexpr int kFewSplits = 8;
+
+// The splits of one row joined, in their order: kShare waves of a workgroup a
+// row, which take its splits in turn.  One where there are few splits, as for
+// the many rows of a prompt: 20480 rows of 5 splits took 33 us with four.
+template <int D, typename T, int kShare>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                        const float* ws) {
   constexpr int kPer = D / 64;
   __shared__ float sum[kWaves][D], sum_l[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t slot = blockIdx.x / (uint32_t)plan.rows, b = slot / (uint32_t)plan.tiles / c.kv,
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t id = kShare == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
+  const uint32_t slot = id / (uint32_t)plan.rows, b = slot / (uint32_t)plan.tiles / c.kv,
                  h = slot / (uint32_t)plan.tiles % c.kv;
-  const int tile = (int)(slot % (uint32_t)plan.tiles), n = (int)(blockIdx.x % (uint32_t)plan.rows),
-            r = tile * plan.rows + n;
+  const int tile = (int)(slot % (uint32_t)plan.tiles), n = (int)(id % (uint32_t)plan.rows), r = tile * plan.rows + n;
+  if (b >= c.seqs) return;
   const TileRows rows = tile_rows(c, q, b, tile, plan.rows, plan.rows == kRows ? kStep : kBlockStep);
   if (r >= rows.rows) return;
   const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
@@ -1017,97 +1046,218 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
 #pragma unroll
   for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
 #pragma unroll 4
-  for (int s = wave; s < splits; s += kWaves) {
+  for (int s = kShare == 1 ? 0 : wave; s < splits; s += kShare) {
     const float f = __builtin_amdgcn_exp2f(m_n[s * size] - m);
     l += m_n[s * size + plan.rows] * f;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] += o_n[s * size + lane + 64 * k] * f;
+    for (int k = 0; k < kPer; ++k) o[k] += o_n[s * size + lane * kPer + k] * f;
   }
+  if constexpr (kShare > 1) {
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) sum[wave][lane + 64 * k] = o[k];
-  if (lane == 0) sum_l[wave] = l;
-  __syncthreads();
-  l = (sum_l[0] + sum_l[1]) + (sum_l[2] + sum_l[3]);
+    for (int k = 0; k < kPer; ++k) sum[wave][lane * kPer + k] = o[k];
+    if (lane == 0) sum_l[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    l = (sum_l[0] + sum_l[1]) + (sum_l[2] + sum_l[3]);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int d = lane * kPer + k;
+      o[k] = (sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]);
+    }
+  }
   const int64_t row = (int64_t)(rows.first + r / q.group) * q.heads + (int)h * q.group + r % q.group;
-  if (threadIdx.x == 0) lse[row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  if (lane == 0) lse[row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int d = threadIdx.x; d < D; d += 256)
-    put(out, row * D + d, ((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])) * inv, T());
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) put(out, row * D + lane * kPer + k, o[k] * inv, T());
 }
 
+// Tokens of a wave that weighs.
+constexpr int weigh_tokens(int dim) { return dim == 256 ? 32 : 64; }
+// Bytes of a tile's queries and statistics in LDS.
+constexpr int weigh_tile(int dim, int q_terms) { return kRows * (q_terms * (dim + 8) * 2 + 4); }
+
 // The attention weights of every row added to its kv head's tokens.  A wave
-// owns its tokens and walks over all rows, so that a token's sum has one order
-// and one writer; the rows' statistics are known (lse), so the values are not
-// read.
+// owns 64 tokens (32 of a head of 256), holds their keys as bf16 and walks over
+// all rows, so that a token's sum has one order and one writer; the rows'
+// statistics are known (lse), so the values are not read.  The rows' terms lie
+// in LDS, as many tiles at a time as fit, for the four waves (read tile by tile
+// from memory, 260 rows over 16385 tokens took 64 us).  One tile of rows is
+// bound by the reading of the keys, many by the exponentials.
 template <int D, typename T, bool kExtra>
-__global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int chunk, int chunks, const float* lse,
+__global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int chunks, int most_tiles, const float* lse,
                                                         float* weights, int64_t weights_len) {
+  constexpr int kRow = D / 2, kScales = D / 32, kWords = D / 32;
+  constexpr int kParts = weigh_tokens(D) / 16;
+  constexpr int kQ = Terms<T>::kQ;
+  struct Tile {  // rows a 16-byte bank group off each other's
+    uint16_t q[kRows][kQ][D + 8];
+    float lse[kRows];
+  };
+  extern __shared__ __align__(16) uint8_t shared[];
+  Tile* held = reinterpret_cast<Tile*>(shared);  // [most_tiles]
+  static_assert(sizeof(Tile) == weigh_tile(D, kQ), "");
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t slot = blockIdx.x / (uint32_t)chunks, b = slot / c.kv, h = slot % c.kv;
-  TileRows all = tile_rows(c, q, b, 0, 0x40000000, kStep);
-  int hi = all.hi < weights_len ? all.hi : (int)weights_len;
-  const int begin = all.lo + (int)(blockIdx.x % (uint32_t)chunks) * chunk;
-  int end = begin + chunk;
-  if (end > hi) end = hi;
-  const int tiles = (all.rows + kRows - 1) / kRows;
-  float* w = weights + (int64_t)slot * weights_len;
-  for (int t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
-    const int t = t0 + (lane & 31);
-    const uint32_t page = kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
-    Loaded<D> s;
-    load_any<D, false>(c, h, page, t0, end, lane, s);
-    float add[8];
+  const TileRows all = tile_rows(c, q, b, 0, 0x40000000, kStep);
+  const int end = all.hi < weights_len ? all.hi : (int)weights_len;
+  const int w0 = all.lo + (int)(blockIdx.x % (uint32_t)chunks) * kWaves * weigh_tokens(D);
+  if (w0 >= end) return;
+  const int t0 = w0 + wave * weigh_tokens(D);
+  u32x4 key[kParts][kWords];
+  uint64_t valid = 0;
+  {
+    uint32_t k[kParts][kWords], s[kParts][Loaded<D>::kGroups], page[kParts];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) add[j] = 0.0f;
-    for (int tile = 0; tile < tiles; ++tile) {
-      const TileRows rows = tile_rows(c, q, b, tile, kRows, kStep);
-      if (t0 >= rows.hi || t0 + kStep <= rows.lo) continue;
-      const int r = tile * kRows + n;
-      const bool live = r < rows.rows;
-      const int token = r / q.group, head = (int)h * q.group + r % q.group;
-      QueryTerms<D, T> terms;
-      terms.load(q, (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh, live, g);
-      const float base = live ? lse[(int64_t)(rows.first + token) * q.heads + head] * kLog2e : 0.0f;
-      float x[8];
-      step_scores<D, T>(terms, s, x);
-      uint32_t seen;
-      finish_scores<kExtra>(curve_of(q, live ? head : (int)h * q.group), x, s.valid, t0, g,
-                            live ? rows.base + token : -1, q.window,
-                            needs_mask(rows, s.valid, t0, q.window) || (tile + 1) * kRows > rows.rows, seen);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) add[j] += seen >> j & 1u ? __builtin_amdgcn_exp2f(x[j] - base) : 0.0f;
+    for (int i = 0; i < kParts; ++i) {
+      const int t = t0 + 16 * i + n;
+      page[i] = kv4_page(c, b, (uint32_t)(t < end ? t : end - 1));
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      for (int d = 1; d < 16; d *= 2) add[j] += __shfl_xor(add[j], d);
+    for (int i = 0; i < kParts; ++i) {
+      const int t = t0 + 16 * i + n;
+      const uint64_t row = kv4_row(c, page[i], h, (uint32_t)(t < end ? t : end - 1));
+      valid |= (__ballot(t < end && page[i] < c.pages) & 0xFFFFull) << (16 * i);
+      load_keys<D>(c.codes + row * kRow, c.scales + row * kScales, 0u, 0u, g, k[i], s[i]);
     }
-    // lane (j, g) writes token j of its group
-    float mine = add[0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) mine = n == j ? add[j] : mine;
-    const int u = (n >> 2) * 16 + 4 * g + (n & 3);
-    if (n < 8 && t0 + u < end && (s.valid >> u & 1u)) w[t0 + u] += mine;
+    for (int i = 0; i < kParts; ++i)
+#pragma unroll
+      for (int a = 0; a < kWords; ++a) {
+        const float f = u2f(s[i][a / 4] << 23);
+        key[i][a] = u32x4{fp4_pair<0>(k[i][a], f), fp4_pair<1>(k[i][a], f), fp4_pair<2>(k[i][a], f), fp4_pair<3>(k[i][a], f)};
+      }
   }
+  float add[4 * kParts];
+#pragma unroll
+  for (int j = 0; j < 4 * kParts; ++j) add[j] = 0.0f;
+  const int tokens = all.rows / q.group, tiles = (all.rows + kRows - 1) / kRows;
+  // tiles from the first whose rows are not all before the workgroup's tokens
+  const int skip = w0 > all.base ? (int)((uint32_t)(w0 - all.base) * (uint32_t)q.group / kRows) : 0;
+  const int step_token = kRows / q.group, step_which = kRows % q.group;
+  for (int first = skip; first < tiles; first += most_tiles) {
+    const int batch = tiles - first < most_tiles ? tiles - first : most_tiles;
+    if (first > skip) __syncthreads();
+    // the terms of these rows: 8 elements of a row a thread, four rows' loads in
+    // flight (one at a time, 260 rows over 16385 tokens took 61 us)
+    constexpr int kAhead = 4, kEach = 256 / (D / 8);  // rows of a round of the threads
+    const int e = tid % (D / 8) * 8;
+    for (int i0 = tid / (D / 8); i0 < batch * kRows; i0 += kAhead * kEach) {
+      u32x4 t[kAhead][kQ];
+      float statistic[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int r = first * kRows + i0 + a * kEach, rc = r < all.rows ? r : all.rows - 1;
+        const int64_t at = all.first + rc / q.group;
+        const int head = (int)h * q.group + rc % q.group;
+        load_query(q, at * q.sn + (int64_t)head * q.sh + e, true, T(), t[a]);
+        statistic[a] = lse[at * q.heads + head];
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a * kEach;
+        if (i >= batch * kRows) break;
+#pragma unroll
+        for (int k = 0; k < kQ; ++k) *reinterpret_cast<u32x4*>(&held[i / kRows].q[i % kRows][k][e]) = t[a][k];
+        if (e == 0) held[i / kRows].lse[i % kRows] = statistic[a] * kLog2e;
+      }
+    }
+    __syncthreads();
+    if (t0 >= end) continue;
+    // row n of a tile: its token and the head of its group, kept up by steps of
+    // 16 rows (a division is some 25 instructions)
+    int token = (first * kRows + n) / q.group, which = (first * kRows + n) % q.group;
+#pragma clang loop unroll(disable)
+    for (int tile = 0; tile < batch; ++tile) {
+      const float base = held[tile].lse[n];
+      const int pos = token < tokens ? all.base + token : -1;
+      const int pos_first = __builtin_amdgcn_readfirstlane(pos), pos_last = __builtin_amdgcn_readlane(pos, 15);
+      const Curve curve = curve_of(q, (int)h * q.group + which);
+      token += step_token, which += step_which;
+      if (which >= q.group) which -= q.group, ++token;
+      // a window that has passed these tokens, or rows that have not come to them
+      if (q.window && pos_first - q.window >= t0 + weigh_tokens(D) - 1) continue;
+      if (pos_last >= pos_first && pos_last < t0) continue;
+      const bool masked = valid != (kParts == 4 ? ~0ull : 0xFFFFFFFFull) || t0 + weigh_tokens(D) - 1 > pos_first ||
+                          (q.window && t0 <= pos_last - q.window) || pos_last < pos_first;
+      float x[4 * kParts];
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int a = 0; a < kWords; ++a)
+#pragma unroll
+          for (int t = 0; t < kQ; ++t)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8, key[i][a]),
+                *reinterpret_cast<const bf16x8*>(&held[tile].q[n][t][key_element<D>(a, g)]), acc, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = acc[j];
+      }
+      if (kExtra) {
+#pragma unroll
+        for (int i = 0; i < kParts / 2; ++i)
+          curve_scores(curve, *reinterpret_cast<float(*)[8]>(&x[8 * i]), pos, t0 + 32 * i + 4 * g);
+      }
+      const float scale = kExtra ? 1.0f : curve.scale;
+#pragma unroll
+      for (int j = 0; j < 4 * kParts; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], scale, -base));
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 4 * kParts; ++j) {
+          const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = t0 + u;
+          const bool seen = (valid >> u & 1u) && t <= pos && (q.window == 0 || t > pos - q.window);
+          x[j] = seen ? x[j] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4 * kParts; ++j) add[j] += x[j];
+    }
+  }
+  if (t0 >= end) return;
+  float* w = weights + (int64_t)slot * weights_len + t0;
+  // lane (n, g) of the 16 of a group keeps token (n / 4) 16 + 4 g + n % 4
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 4 * kParts; ++j) {
+    float a = add[j];
+    for (int d = 1; d < 16; d *= 2) a += __shfl_xor(a, d);
+    sum = n == j ? a : sum;
+  }
+  const int u = (n >> 2) * 16 + 4 * g + (n & 3);
+  if (n < 4 * kParts && (valid >> u & 1u)) w[u] += sum;
 }
+
+// Tiles of 16 rows by 32 tokens of a call from which on the kernel for many rows
+// is taken.  Its workgroups have 8 times the rows and a time of their own of
+// some 20 us with the join, so that below they do not fill the card: bf16, heads
+// of 128, with it and with the other, 512 new tokens of 4096 (131072 tiles) 75
+// and 91 us, 2048 of 2048 (262144) 77 and 123, 8 x 256 of 1000 (128000) 55 and
+// 108, 8 x 64 of 2000 (64000) 51 and 53, 1024 of 1024 (65536) 58 and 46, 256 of
+// 2000 (32000) 40 and 29.
+constexpr int64_t kManyTiles = 100000;
 
 Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   Kv4Plan p;
-  const int64_t all = (int64_t)q.most * q.group;
-  p.rows = all > kManyRows ? 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3)) : kRows;
+  const int64_t all = (int64_t)q.most * q.group, seqs = (int64_t)c.seqs * c.kv;
+  // the most tokens that rows of `tokens` new ones can see
+  auto span_of = [&](int64_t tokens) {
+    const int64_t seen = (int64_t)q.window + tokens + kBlockStep;
+    return q.window && seen < (int64_t)c.cap ? seen : (int64_t)c.cap;
+  };
+  const double tiles = (double)seqs * ((all + kRows - 1) / kRows) * (double)(span_of(q.most) / kStep);
+  p.rows = all > kRows && tiles >= kManyTiles ? 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3)) : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
-  // the most tokens a tile can see
-  int64_t span = c.cap;
-  if (q.window) {
-    const int64_t seen = (int64_t)q.window + p.rows / q.group + 2 + kBlockStep;
-    if (seen < span) span = seen;
-  }
-  const int64_t heads = (int64_t)c.seqs * c.kv * p.tiles;
-  // enough workgroups for every compute unit to have some to wait with, none
-  // with fewer than two steps for each wave
-  const int64_t want = (4ll * num_cus() + heads - 1) / (heads > 0 ? heads : 1);
+  const int64_t span = span_of(p.rows / q.group + 2);
+  // two workgroups for every compute unit, as many as are resident, and none
+  // with less than two steps a wave, eight of the kernel for many rows: one
+  // costs some 5 us beside its tokens (4 a unit instead of 2: 16 sequences of
+  // 4000 tokens 27 and 23 us, one of 131073 47 and 38)
+  const int64_t heads = seqs * p.tiles, want = (2ll * num_cus() + heads - 1) / (heads > 0 ? heads : 1);
+  const int64_t least = p.rows == kRows ? 2 * kWaves * kStep : 8 * kBlockStep;
   int64_t chunk = (span + want - 1) / want;
-  if (chunk < 2 * kWaves * kStep) chunk = 2 * kWaves * kStep;
+  if (chunk < least) chunk = least;
   chunk = (chunk + kWaves * kStep - 1) / (kWaves * kStep) * (kWaves * kStep);
   p.chunk = (int32_t)chunk;
   p.splits = (int32_t)((span + chunk - 1) / chunk);
@@ -1167,9 +1317,12 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
       VQX_KV4_LAUNCH(kv4_rows_kernel, D, T);                                                                       \
     else                                                                                                           \
       VQX_KV4_LAUNCH(kv4_block_kernel, D, T);                                                                      \
-    if (p.splits > 1)                                                                                              \
-      hipLaunchKernelGGL((kv4_join_kernel<D, T>), dim3((unsigned)(slots * p.rows)), dim3(256), 0, st, c, q, p,     \
-                         out, lse, ws);                                                                            \
+    if (p.splits > kFewSplits)                                                                                     \
+      hipLaunchKernelGGL((kv4_join_kernel<D, T, kWaves>), dim3((unsigned)(slots * p.rows)), dim3(256), 0, st, c,   \
+                         q, p, out, lse, ws);                                                                      \
+    else if (p.splits > 1)                                                                                         \
+      hipLaunchKernelGGL((kv4_join_kernel<D, T, 1>), dim3((unsigned)(slots * p.rows / kWaves)), dim3(256), 0, st,  \
+                         c, q, p, out, lse, ws);                                                                   \
   } while (0)
   VQX_KV4_TYPES(VQX_KV4_ROWS)
 #undef VQX_KV4_ROWS
@@ -1182,24 +1335,24 @@ int kv4_accumulate(const Kv4View& c, int dim, const Kv4Query& q, int dtype, cons
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
   int64_t span = c.cap;
   if (q.window && (int64_t)q.window + q.most + kStep < span) span = (int64_t)q.window + q.most + kStep;
-  const int64_t heads = (int64_t)c.seqs * c.kv;
-  const int64_t want = (8ll * num_cus() + heads - 1) / heads;
-  int64_t chunk = (span + want - 1) / want;
-  chunk = (chunk + kWaves * kStep - 1) / (kWaves * kStep) * (kWaves * kStep);
-  if (chunk < kWaves * kStep) chunk = kWaves * kStep;
+  const int64_t heads = (int64_t)c.seqs * c.kv, tokens = kWaves * weigh_tokens(dim);
   const bool extra = q.softcap != 0.0f || q.slopes;
-  const int64_t chunks = (span + chunk - 1) / chunk;
+  const int64_t chunks = (span + tokens - 1) / tokens;
   if (chunks * heads >= 1ll << 31)
     return set_error(kErrUnsupported, "kv4_accumulate: %lld runs of tokens do not fit a launch", (long long)(chunks * heads));
   const dim3 grid((unsigned)(chunks * heads));
-#define VQX_KV4_WEIGH(D, T)                                                                                       \
-  do {                                                                                                            \
-    if (extra)                                                                                                    \
-      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, true>), grid, dim3(256), 0, st, c, q, (int)chunk, (int)chunks, lse, weights,  \
-                         weights_len);                                                                            \
-    else                                                                                                          \
-      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, false>), grid, dim3(256), 0, st, c, q, (int)chunk, (int)chunks, lse, weights, \
-                         weights_len);                                                                            \
+  // LDS for the rows that there are, as many as leave room for two workgroups more
+  const int tile = weigh_tile(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3));
+  const int64_t tiles = ((int64_t)q.most * q.group + kRows - 1) / kRows;
+  const int most = (int)(tiles < 48 * 1024 / tile ? tiles : 48 * 1024 / tile);
+#define VQX_KV4_WEIGH(D, T)                                                                                          \
+  do {                                                                                                               \
+    if (extra)                                                                                                       \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, true>), grid, dim3(256), most * tile, st, c, q, (int)chunks, most,  \
+                         lse, weights, weights_len);                                                                 \
+    else                                                                                                             \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, false>), grid, dim3(256), most * tile, st, c, q, (int)chunks, most, \
+                         lse, weights, weights_len);                                                                 \
   } while (0)
   VQX_KV4_TYPES(VQX_KV4_WEIGH)
 #undef VQX_KV4_WEIGH

@@ -142,8 +142,8 @@ def _query(query, cache, codes, cu, most, scale, softcap, window, slopes, what):
     offsets = _offsets(cu, n, cache.seqs, what, device)
     if most is not None and most < (1 if n else 0):
         _refuse(what, f"most is {most}")
-    if window < 0 or window > 0x7FFFFFFF:
-        _refuse(what, f"a window is positive, or 0 for none, not {window}")
+    if not 0 <= window < 2 ** 30:
+        _refuse(what, f"a window is positive and below 2^30, or 0 for none, not {window}")
     if not 0.0 <= softcap < math.inf:
         _refuse(what, f"a softcap is positive, or 0 for none, not {softcap}")
     bias = None
