@@ -126,6 +126,95 @@ def test_attention(ops, i):
     check_attention(ops, kind, q, codes, scales, torch.tensor(lens, dtype=torch.int32), table=table, **how)
 
 
+def widened(codes, scales, table, tiles):
+    """The same cache with room for so many tokens that a call of `tiles` tiles
+    of 16 rows, over all sequences and kv heads, is one for many rows (100000
+    tiles of 16 rows by 32 tokens): a table of pages that are none, or longer
+    sequences."""
+    room = -(-100000 // tiles) * 32 + 64
+    if table is not None:
+        more = room // codes.shape[3] + 1 - table.shape[1]
+        return codes, scales, torch.nn.functional.pad(table, (0, max(0, more)), value=-1)
+    pad = (0, 0, 0, max(0, room - codes.shape[3]))
+    return torch.nn.functional.pad(codes, pad), torch.nn.functional.pad(scales, pad), None
+
+
+MANY = [i for i, c in enumerate(CASES) if c[3] * c[5] > 16] + [
+    ("bf16", 128, 2, 4, [500, 130, 64], 61, 64, {}), ("bf16", 128, 1, 2, [1000, 400], 150, 128, {}),
+    ("bf16", 64, 1, 5, [300, 63], 40, 256, dict(softcap=3.0)), ("f16", 128, 1, 4, [129, 190], 33, 64, dict(slopes=True)),
+    ("f32", 128, 2, 1, [200, 90], 80, 64, dict(window=50, softcap=9.0)), ("f32", 64, 1, 3, [333], 100, 0, {}),
+    ("bf16", 256, 1, 3, [140, 70], 50, 64, dict(window=64)), ("f16", 256, 1, 2, [200], 90, 16, dict(softcap=30.0)),
+    ("f32", 256, 1, 2, [150], 70, 64, dict(slopes=True)), ("bf16", 128, 1, 4, [70], 70, 0, dict(scale=-0.2)),
+    ("bf16", 128, 1, 40, [3, 33], 1, 64, {})]
+
+
+@pytest.mark.parametrize("i", range(len(MANY)))
+def test_attention_many_rows(ops, i):
+    """The kernel for many rows, at small sizes: what takes it is the room."""
+    kind, dim, kv, group, lens, new, page, how = CASES[MANY[i]] if isinstance(MANY[i], int) else MANY[i]
+    print("case", (kind, dim, kv, group, lens, new, page, how), flush=True)
+    g = torch.Generator().manual_seed(i)
+    heads, seqs = kv * group, len(lens)
+    codes, scales, table = make_cache(seqs, kv, dim, max(lens), page, i)
+    codes, scales, table = widened(codes, scales, table, seqs * kv * -(-new * group // 16))
+    q = torch.randn(seqs * new, heads, dim, generator=g).to(TYPES[kind])
+    how = dict(how)
+    if how.get("slopes"):
+        how["slopes"] = torch.exp2(-8.0 * torch.arange(1, heads + 1) / heads)
+    if how.get("window"):
+        # a window bounds what a tile can see: more sequences, that have nothing
+        more = -(-100000 * 32 // (kv * -(-new * group // 16) * (how["window"] + new)))
+        lens = lens + [0] * more
+        q = torch.nn.functional.pad(q, (0, 0, 0, 0, 0, new * more))
+        if table is not None:
+            table = torch.nn.functional.pad(table[:, :64], (0, 0, 0, more), value=-1)
+        else:
+            codes, scales = (torch.nn.functional.pad(x[..., :max(lens), :], (0, 0, 0, 0, 0, 0, 0, more)) for x in (codes, scales))
+    check_attention(ops, kind, q, codes, scales, torch.tensor(lens, dtype=torch.int32), table=table, weigh=False, **how)
+
+
+@pytest.mark.parametrize("page", [0, 48, 64])
+def test_attention_many_rows_and_heads(ops, page):
+    """As many tiles as need no splits: outputs straight from the kernel."""
+    g = torch.Generator().manual_seed(page)
+    seqs, kv, group, dim, new = 65, 8, 2, 64, 20
+    lens = torch.randint(1, 90, (seqs,), generator=g).int()
+    lens[0] = 90
+    codes, scales, table = widened(*make_cache(seqs, kv, dim, 90, page), seqs * kv * 3)
+    q = torch.randn(seqs * new, kv * group, dim, generator=g).bfloat16()
+    check_attention(ops, "bf16", q, codes, scales, lens, table=table, weigh=False)
+
+
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attention_many_rows_nan_and_bad_pages(ops, dim, page):
+    new = 20
+    codes, scales, table = make_cache(3, 1, dim, 128, page)
+    for t, plane, block in ((80, 1, 0), (88, 1, dim // 32 - 1), (95, 0, 0), (3, 1, 1)):
+        _, p, slot = ref.places(table, codes.shape[3], codes.shape[1], 0, [t])[0]
+        scales[plane, p, 0, slot, block] = 255
+    table[1, 0], table[2, 1] = -1, codes.shape[1]
+    codes, scales, table = widened(codes, scales, table, 3 * 3)
+    q = torch.randn(3 * new, 2, dim, generator=torch.Generator().manual_seed(1)).bfloat16()
+    lens = torch.tensor([96, 100, 128], dtype=torch.int32)
+    out, lse = check_attention(ops, "bf16", q, codes, scales, lens, table=table, weigh=False)
+    assert not lse[:19].isnan().any() and lse[19].isnan().all()
+    assert not out[:4].isnan()[..., 64:].any() and not out[new:].isnan().any()
+
+
+def test_attention_many_rows_ragged(ops):
+    new, most = [0, 1, 70, 9, 0, 130], 100
+    lens = torch.tensor([40, 300, 170, 4, 0, 140], dtype=torch.int32)
+    cu = torch.tensor([0] + new).cumsum(0).int()
+    codes, scales, table = widened(*make_cache(6, 2, 128, 300, 16), 6 * 2 * 19)
+    q = torch.randn(sum(new), 6, 128, generator=torch.Generator().manual_seed(3)).bfloat16()
+    out, lse = check_attention(ops, "bf16", q, codes, scales, lens, cu, None, table, weigh=False)
+    d = on(q, codes, scales, lens, cu, table)
+    short, short_lse = ops.kv4_attention(d[0], d[1], d[2], d[3], d[4], most, d[5])
+    assert short[80 + most:].isnan().all() and short_lse[80 + most:].isnan().all()
+    near(short[:80 + most], out[:80 + most].cpu().double(), 2.0 ** -7 * out[:80 + most].cpu().double().abs() + 2.0 ** -6, "most")
+
+
 @pytest.mark.parametrize("kind,dim", [("bf16", 128), ("f16", 64), ("f32", 256)])
 @pytest.mark.parametrize("most", [None, 70, 200])
 def test_attention_ragged(ops, kind, dim, most):

@@ -49,7 +49,7 @@ def test_cache_refusals(kv4, i, change, message):
 
 def query(kv4, q, cu=None, most=None, scale=None, softcap=0.0, window=0, slopes=None):
     args = cache_args()
-    return kv4._query(q, kv4._cache(*args, "x"), args[0], cu, most, scale, softcap, window, slopes, "x")
+    return kv4._query(q, kv4._cache(*args, "x"), args[0].device, cu, most, scale, softcap, window, slopes, "x")[:2]
 
 
 def test_a_sound_query(kv4):

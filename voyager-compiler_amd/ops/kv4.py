@@ -67,10 +67,10 @@ def _refuse(what, message):
     raise ValueError(f"vqx: {what}: {message}")
 
 
-def _int32(t, shape, name, what, device):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        _refuse(what, f"{name} must be a contiguous int32 tensor of shape {list(shape)}, "
-                      f"not {t.dtype} {list(t.shape)}")
+def _int32(t, n, name, what, device):
+    """The address of t, a contiguous int32 vector of n on the cache's device."""
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        _refuse(what, f"{name} must be a contiguous int32 tensor of shape [{n}], not {t.dtype} {list(t.shape)}")
     if t.device != device:
         _refuse(what, f"{name} is on {t.device}, the cache on {device}")
     return t.data_ptr()
@@ -85,7 +85,8 @@ def _cache(codes, scales, lengths, table, what):
     if len(shape) != 5 or shape[0] != 2 or shape[4] not in (32, 64, 128):
         _refuse(what, "codes must be [2, pages, kv heads, page size, D / 2] with D 64, 128 or 256, "
                       f"not {list(shape)}")
-    if scales.shape[:4] != shape[:4] or scales.ndim != 5 or scales.shape[4] * 16 != shape[4]:
+    _, pages, kv, size, half = shape
+    if scales.shape != (2, pages, kv, size, half // 16):
         _refuse(what, f"scales must be [2, pages, kv heads, page size, D / 32], not {list(scales.shape)} "
                       f"for codes {list(shape)}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
@@ -93,55 +94,65 @@ def _cache(codes, scales, lengths, table, what):
     device = codes.device
     if scales.device != device:
         _refuse(what, f"scales are on {scales.device}, codes on {device}")
-    if lengths.ndim != 1:
+    if lengths.dim() != 1:
         _refuse(what, f"lengths must be [sequences], not {list(lengths.shape)}")
     seqs = lengths.shape[0]
-    at, tab, per = _int32(lengths, (seqs,), "lengths", what, device), None, 0
+    at, tab, per = _int32(lengths, seqs, "lengths", what, device), None, 0
     if table is not None:
-        if table.ndim != 2:
-            _refuse(what, f"table must be [sequences, pages], not {list(table.shape)}")
-        per = table.shape[1]
-        tab = _int32(table, (seqs, per), "table", what, device)
+        if table.dim() != 2 or table.shape[0] != seqs or table.dtype != torch.int32 or not table.is_contiguous():
+            _refuse(what, f"table must be a contiguous int32 tensor [{seqs}, pages of a sequence], not {table.dtype} "
+                          f"{list(table.shape)}")
+        if table.device != device:
+            _refuse(what, f"table is on {table.device}, the cache on {device}")
+        per, tab = table.shape[1], table.data_ptr()
         if per == 0:
             _refuse(what, "table has no pages for a sequence")
-    return _lib.VqxKv4Cache(codes.data_ptr(), scales.data_ptr(), tab, at, shape[1], per, shape[2], shape[3],
-                            2 * shape[4], seqs)
+    return _lib.VqxKv4Cache(codes.data_ptr(), scales.data_ptr(), tab, at, pages, per, kv, size, 2 * half, seqs)
 
 
 def _offsets(cu, n, seqs, what, device):
     if cu is not None:
-        return _int32(cu, (seqs + 1,), "cu", what, device)
+        return _int32(cu, seqs + 1, "cu", what, device)
     if n % seqs if seqs else n:
         _refuse(what, f"{n} new tokens for {seqs} sequences need cu")
     return None
 
 
 def _rows(t, heads, dim, name, what, device):
-    """t [n, heads, dim] with rows that start on 16 bytes, copied if they do not."""
-    if t.ndim != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+    """t [n, heads, dim] with rows that start on 16 bytes, copied if they do
+    not, its strides and its dtype's tag."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         _refuse(what, f"{name} must be [new tokens, {'heads' if heads is None else heads}, {dim}], "
-                      f"not {list(t.shape)}")
-    if t.dtype not in _FLOATS:
+                      f"not {list(shape)}")
+    tag = _FLOATS.get(t.dtype)
+    if tag is None:
         _refuse(what, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if t.device != device:
         _refuse(what, f"{name} is on {t.device}, the cache on {device}")
     sn, sh, sd = t.stride()
-    size = t.element_size()
-    if sd != 1 or (sn * size) % 16 or (sh * size) % 16 or t.data_ptr() % 16:
+    per = 3 if tag == _lib.F32 else 7  # elements of 16 bytes, less 1
+    if sd != 1 or sn & per or sh & per or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        sn, sh, _ = t.stride()
+    return t, sn, sh, tag
 
 
-def _query(query, cache, codes, cu, most, scale, softcap, window, slopes, what):
-    """(the queries as the library takes them, the tensor that holds them)."""
-    dim, kv, device = cache.dim, cache.kv_heads, codes.device
-    q = _rows(query, None, dim, "query", what, device)
-    n, heads = q.shape[0], q.shape[1]
+def _query(query, cache, device, cu, most, scale, softcap, window, slopes, what):
+    """(the queries as the library takes them, the tensor that holds them, a
+    key of all that their workspace depends on beside the cache's sizes)."""
+    dim, kv, seqs = cache.dim, cache.kv_heads, cache.seqs
+    q, sn, sh, tag = _rows(query, None, dim, "query", what, device)
+    n, heads, _ = q.shape
     if heads == 0 or heads % kv:
         _refuse(what, f"{heads} query heads for {kv} kv heads")
-    offsets = _offsets(cu, n, cache.seqs, what, device)
-    if most is not None and most < (1 if n else 0):
+    offsets = _offsets(cu, n, seqs, what, device)
+    if most is None:
+        most = 0
+    elif most < (1 if n else 0):
         _refuse(what, f"most is {most}")
+    elif most > n:
+        most = n
     if not 0 <= window < 2 ** 30:
         _refuse(what, f"a window is positive and below 2^30, or 0 for none, not {window}")
     if not 0.0 <= softcap < math.inf:
@@ -154,10 +165,9 @@ def _query(query, cache, codes, cu, most, scale, softcap, window, slopes, what):
         if slopes.device != device:
             _refuse(what, f"slopes are on {slopes.device}, the cache on {device}")
         bias = slopes.data_ptr()
-    sn, sh, _ = q.stride()
-    return _lib.VqxKv4Query(q.data_ptr(), offsets, bias, n, sn, sh, _FLOATS[q.dtype], heads,
-                            0 if most is None else min(most, n), window, dim ** -0.5 if scale is None else scale,
-                            softcap), q
+    return (_lib.VqxKv4Query(q.data_ptr(), offsets, bias, n, sn, sh, tag, heads, most, window,
+                             dim ** -0.5 if scale is None else scale, softcap),
+            q, (n, heads, tag, most, window, cu is None))
 
 
 def _weights(weights, seqs, kv, name, what, device):
@@ -177,15 +187,15 @@ def kv4_append(key, value, codes, scales, lengths, cu=None, table=None):
     what = "kv4_append"
     _lib.require_device(codes, what)
     c = _cache(codes, scales, lengths, table, what)
-    k = _rows(key, c.kv_heads, c.dim, "key", what, codes.device)
-    v = _rows(value, c.kv_heads, c.dim, "value", what, codes.device)
+    device, kv, dim = codes.device, c.kv_heads, c.dim
+    k, kn, kh, tag = _rows(key, kv, dim, "key", what, device)
+    v, vn, vh, vtag = _rows(value, kv, dim, "value", what, device)
     n = k.shape[0]
-    if v.shape[0] != n or v.dtype != k.dtype:
+    if v.shape[0] != n or vtag != tag:
         _refuse(what, f"key and value differ: {key.dtype} {list(key.shape)}, {value.dtype} {list(value.shape)}")
-    offsets = _offsets(cu, n, c.seqs, what, codes.device)
-    ks, vs = k.stride(), v.stride()
-    _lib.call("vqx_kv4_append", c, k.data_ptr(), v.data_ptr(), _FLOATS[k.dtype], n, ks[0], ks[1], vs[0], vs[1],
-              offsets, _lib.stream_of(codes))
+    offsets = _offsets(cu, n, c.seqs, what, device)
+    _lib.call("vqx_kv4_append", c, k.data_ptr(), v.data_ptr(), tag, n, kn, kh, vn, vh, offsets,
+              _lib.stream_of(codes))
 
 
 @_impl("kv4_read")
@@ -206,6 +216,24 @@ def kv4_read(codes, scales, lengths, n, cu=None, table=None, dtype=torch.bfloat1
     return k, v
 
 
+_WS = {}
+
+
+def _workspace_bytes(c, qs, device, key):
+    """Workspace vqx_kv4_attention needs for these sizes on ``device`` (0: no
+    splits to join), cached per sizes."""
+    key = (c.pages_per_seq, c.page_size, c.kv_heads, c.dim, c.seqs, device.index, key)
+    n = _WS.get(key)
+    if n is None:
+        if len(_WS) >= 4096:
+            _WS.clear()
+        got = ctypes.c_int64(0)
+        with torch.cuda.device(device):
+            _lib.call("vqx_kv4_attention_workspace_size", c, qs, got)
+        n = _WS[key] = got.value
+    return n
+
+
 @_impl("kv4_attention")
 def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None, *, scale=None, softcap=0.0,
                   window=0, slopes=None):
@@ -218,13 +246,12 @@ def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None,
     what = "kv4_attention"
     _lib.require_device(codes, what)
     c = _cache(codes, scales, lengths, table, what)
-    qs, q = _query(query, c, codes, cu, most, scale, softcap, window, slopes, what)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    need = ctypes.c_int64(0)
-    _lib.call("vqx_kv4_attention_workspace_size", c, qs, need)
-    need = need.value
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else None
+    device = codes.device
+    qs, q, key = _query(query, c, device, cu, most, scale, softcap, window, slopes, what)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+    need = _workspace_bytes(c, qs, device, key)
+    ws = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
     _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), ws, need, _lib.stream_of(codes))
     return out, lse
 
@@ -238,7 +265,7 @@ def kv4_accumulate(query, lse, codes, scales, lengths, weights, cu=None, most=No
     what = "kv4_accumulate"
     _lib.require_device(codes, what)
     c = _cache(codes, scales, lengths, table, what)
-    qs, q = _query(query, c, codes, cu, most, scale, softcap, window, slopes, what)
+    qs, q, _ = _query(query, c, codes.device, cu, most, scale, softcap, window, slopes, what)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous() or lse.device != q.device:
         _refuse(what, f"lse must be a contiguous float32 tensor {list(q.shape[:2])}, not {lse.dtype} "
                       f"{list(lse.shape)}")
