@@ -762,10 +762,14 @@ int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, c
  * front of `out`, another cache with as many sequences and kv heads and room
  * for budget tokens each.  index: int32 [seqs, kv_heads, budget], where each
  * kept token was, -1 past the end; out->lengths: their number; out_weights:
- * fp32 [seqs, kv_heads, budget], their weights, 0 past the end.
+ * fp32 [seqs, kv_heads, budget], their weights, 0 past the end.  workspace:
+ * vqx_kv4_evict_workspace_size bytes for the same cache and weights_len, 16-byte
+ * aligned, or NULL where that is 0.
  */
+int vqx_kv4_evict_workspace_size(const vqx_kv4_cache* cache, int64_t weights_len, int64_t* bytes);
 int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weights_len, int32_t budget, int32_t recent,
-                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, vqx_stream_t stream);
+                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, void* workspace,
+                  int64_t workspace_bytes, vqx_stream_t stream);
 
 #ifdef __cplusplus
 }

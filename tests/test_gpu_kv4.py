@@ -433,6 +433,39 @@ def test_evict(ops, lens, budget, recent, page):
     same(dos, want_s, "scales")
 
 
+@pytest.mark.parametrize("room,budget,recent,kind", [
+    (8193, 8192, 0, "random"), (20000, 3000, 500, "random"), (20000, 3000, 500, "few"), (16385, 16000, 1, "equal"),
+    (70000, 100, 10, "random"), (150000, 40000, 64, "few"), (150000, 149999, 0, "random"), (30000, 29000, 29000, "few")])
+def test_evict_of_long_sequences(ops, room, budget, recent, kind):
+    """The selection by slices: the places alone, against a sort."""
+    g = torch.Generator().manual_seed(room + budget)
+    lens = torch.tensor([room, room - 77, 9000 if room > 9000 else room, min(budget, room), 1, 0], dtype=torch.int32)
+    seqs, kv = 6, 2
+    codes, scales, table = make_cache(seqs, kv, 64, 16, 0)
+    table = torch.zeros(seqs, -(-room // 16), dtype=torch.int32)  # all on one page
+    w = torch.randn(seqs, kv, room, generator=g)
+    if kind == "few":
+        w = (w * 2).round() / 2  # a handful of weights, -0 and 0 among them
+    if kind == "equal":
+        w.fill_(0.125)
+    oc, os_, ot = make_cache(seqs, kv, 64, 16, 0)
+    ot = torch.full((seqs, -(-budget // 16)), -1, dtype=torch.int32)
+    dc, ds, dt, dw, dl, doc, dos, dot = on(codes, scales, table, w, lens, oc, os_, ot)
+    ow = torch.full((seqs, kv, budget), 7.0, device=DEV)
+    index, kept = ops.kv4_evict(dc, ds, dw, dl, budget, recent, doc, dos, ow, dt, dot)
+    j = torch.arange(room)
+    n = lens.long()[:, None, None]
+    key = torch.where(j >= n - recent, math.inf, w)
+    key = torch.where(j >= n, -math.inf, key)
+    order = torch.sort(key, dim=-1, descending=True, stable=True).indices[..., :budget]
+    want = torch.sort(torch.where(order < n, order, room), dim=-1).values
+    live = want < n
+    same(index, torch.where(live, want, -1).int(), "index")
+    same(kept, lens.clamp(max=budget), "lengths")
+    same(ow, torch.where(live, w.gather(-1, want.clamp(max=room - 1)), 0.0), "weights")
+    same(doc, oc, "codes")
+
+
 def test_evict_of_a_token_without_a_page(ops):
     """It is kept as zeros; one that goes to no page is not written."""
     codes, scales, table = make_cache(1, 1, 64, 64, 16)

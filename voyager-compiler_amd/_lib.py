@@ -171,7 +171,8 @@ _SIGNATURES = {
     "vqx_kv4_attention_workspace_size": ([_KC, _KQ, ctypes.POINTER(_I64)], ctypes.c_int),
     "vqx_kv4_attention": ([_KC, _KQ, _P, _P, _P, _I64, _P], ctypes.c_int),
     "vqx_kv4_accumulate": ([_KC, _KQ, _P, _P, _I64, _P], ctypes.c_int),
-    "vqx_kv4_evict": ([_KC, _P, _I64, _I32, _I32, _KC, _P, _P, _P], ctypes.c_int),
+    "vqx_kv4_evict_workspace_size": ([_KC, _I64, ctypes.POINTER(_I64)], ctypes.c_int),
+    "vqx_kv4_evict": ([_KC, _P, _I64, _I32, _I32, _KC, _P, _P, _P, _I64, _P], ctypes.c_int),
 }
 
 _lib = None

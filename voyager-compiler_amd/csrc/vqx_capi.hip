@@ -701,8 +701,20 @@ int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, c
   return kv4_accumulate(c, cache->dim, q, query->dtype, lse, weights, weights_len, (hipStream_t)stream);
 }
 
+int vqx_kv4_evict_workspace_size(const vqx_kv4_cache* cache, int64_t weights_len, int64_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return set_error(kErrInvalid, "kv4_evict_workspace_size: bytes is NULL");
+  Kv4View c;
+  const int rc = to_view(cache, "kv4_evict", &c);
+  if (rc != kOk) return rc;
+  if (weights_len < 0) return set_error(kErrInvalid, "kv4_evict: weights of %lld tokens", (long long)weights_len);
+  *bytes = kv4_evict_workspace(c, weights_len);
+  return kOk;
+}
+
 int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weights_len, int32_t budget, int32_t recent,
-                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, vqx_stream_t stream) {
+                  const vqx_kv4_cache* out, int32_t* index, float* out_weights, void* workspace,
+                  int64_t workspace_bytes, vqx_stream_t stream) {
   g_err[0] = 0;
   Kv4View c, o;
   int rc = to_view(cache, "kv4_evict", &c);
@@ -721,7 +733,11 @@ int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weig
   const uint64_t a = (uint64_t)(uintptr_t)c.codes, z = (uint64_t)(uintptr_t)o.codes;
   if (a < z + out_bytes && z < a + in_bytes)
     return set_error(kErrInvalid, "kv4_evict: the kept tokens go to another cache, not onto this one");
-  return kv4_evict(c, cache->dim, weights, weights_len, budget, recent, o, index, out->lengths, out_weights,
+  const int64_t need = kv4_evict_workspace(c, weights_len);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(kErrInvalid, "kv4_evict: needs a 16-byte aligned workspace of %lld bytes, not %lld",
+                     (long long)need, (long long)workspace_bytes);
+  return kv4_evict(c, cache->dim, weights, weights_len, budget, recent, o, index, out->lengths, out_weights, workspace,
                    (hipStream_t)stream);
 }
 

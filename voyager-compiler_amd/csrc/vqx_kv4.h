@@ -71,7 +71,8 @@ int kv4_append(const Kv4View& c, int dim, const Kv4Tokens& t, const void* key, c
                int64_t key_sn, int64_t key_sh, int64_t value_sn, int64_t value_sh, hipStream_t st);
 int kv4_read(const Kv4View& c, int dim, const Kv4Tokens& t, void* key, void* value, int dtype, hipStream_t st);
 int kv4_evict(const Kv4View& c, int dim, const float* weights, int64_t weights_len, int budget, int recent,
-              const Kv4View& out, int32_t* index, int32_t* kept, float* out_weights, hipStream_t st);
+              const Kv4View& out, int32_t* index, int32_t* kept, float* out_weights, void* ws, hipStream_t st);
+int64_t kv4_evict_workspace(const Kv4View& c, int64_t weights_len);  // bytes
 
 // Queries [n, heads, D] of the new tokens and what becomes of their scores.
 struct Kv4Query {

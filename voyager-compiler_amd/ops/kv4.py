@@ -296,7 +296,11 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
     if out_weights.shape[2] != budget:
         _refuse(what, f"out_weights are for {out_weights.shape[2]} tokens, the budget is {budget}")
     index = torch.empty((c.seqs, c.kv_heads, budget), dtype=torch.int32, device=device)
-    _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow,
+    need = ctypes.c_int64(0)
+    _lib.call("vqx_kv4_evict_workspace_size", c, weights.shape[2], need)
+    need = need.value
+    ws = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
+    _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow, ws, need,
               _lib.stream_of(codes))
     return index, kept
 
