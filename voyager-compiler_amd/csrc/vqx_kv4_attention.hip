@@ -1017,7 +1017,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 }
 
 // Splits of a row that one wave joins.
-constexpr int kFewSplits = 8;
+constexpr int kFewSplits = 16;
 
 // The splits of one row joined, in their order: kShare waves of a workgroup a
 // row, which take its splits in turn.  One where there are few splits, as for
@@ -1039,18 +1039,36 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   const int64_t size = (int64_t)plan.rows * (D + 2);
   const float* o_n = ws + (int64_t)slot * plan.splits * size + (int64_t)n * D;
   const float* m_n = ws + (int64_t)slot * plan.splits * size + (int64_t)plan.rows * D + n;
+  // the first sums are on their way while the references are compared
+  constexpr int kAhead = 4;
+  const int first = kShare == 1 ? 0 : wave;
+  float part[kAhead][kPer], part_m[kAhead], part_l[kAhead];
+  auto fetch = [&](int s0) {
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int s = s0 + a * kShare < splits ? s0 + a * kShare : splits - 1;
+      part_m[a] = m_n[s * size], part_l[a] = m_n[s * size + plan.rows];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) part[a][k] = o_n[s * size + lane * kPer + k];
+    }
+  };
+  fetch(first);
   float m = kLowest;
   for (int s = lane; s < splits; s += 64) m = __builtin_fmaxf(m, m_n[s * size]);
   for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
   float l = 0.0f, o[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
-#pragma unroll 4
-  for (int s = kShare == 1 ? 0 : wave; s < splits; s += kShare) {
-    const float f = __builtin_amdgcn_exp2f(m_n[s * size] - m);
-    l += m_n[s * size + plan.rows] * f;
+  for (int s = first; s < splits; s += kAhead * kShare) {
+    if (s > first) fetch(s);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] += o_n[s * size + lane * kPer + k] * f;
+    for (int a = 0; a < kAhead; ++a) {
+      if (s + a * kShare >= splits) break;
+      const float f = __builtin_amdgcn_exp2f(part_m[a] - m);
+      l += part_l[a] * f;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) o[k] += part[a][k] * f;
+    }
   }
   if constexpr (kShare > 1) {
 #pragma unroll
@@ -1250,11 +1268,11 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   p.rows = all > kRows && tiles >= kManyTiles ? 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3)) : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   const int64_t span = span_of(p.rows / q.group + 2);
-  // two workgroups for every compute unit, as many as are resident, and none
-  // with less than two steps a wave, eight of the kernel for many rows: one
+  // two workgroups for every compute unit, as many as are resident and no more,
+  // and none with less than two steps a wave, eight of the kernel for many rows: one
   // costs some 5 us beside its tokens (4 a unit instead of 2: 16 sequences of
   // 4000 tokens 27 and 23 us, one of 131073 47 and 38)
-  const int64_t heads = seqs * p.tiles, want = (2ll * num_cus() + heads - 1) / (heads > 0 ? heads : 1);
+  const int64_t heads = seqs * p.tiles, want = heads > 0 && 2ll * num_cus() > heads ? 2ll * num_cus() / heads : 1;
   const int64_t least = p.rows == kRows ? 2 * kWaves * kStep : 8 * kBlockStep;
   int64_t chunk = (span + want - 1) / want;
   if (chunk < least) chunk = least;
