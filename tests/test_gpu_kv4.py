@@ -532,3 +532,29 @@ def test_on_another_stream(ops):
         got = ops.kv4_attention(q, codes, scales, lens, None, None, table)
     side.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_the_serving_example(vqx):
+    """Its steps together: the attention is as near as 4 bits let it be, the
+    budget is kept, and the weights of a decode step are those of its heads."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_kv4.py")
+    spec = importlib.util.spec_from_file_location("serve_kv4", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    seqs, budget, steps, heads = 3, 96, 5, 16
+    r = example.serve(seqs=seqs, prompt=300, budget=budget, steps=steps, heads=heads, width=256, recent=16)
+    assert r["kept"] == [budget + steps] * seqs
+    # a value of 4 bits is off by at most a quarter of itself, or of 0.5 steps
+    # below its block's least level; the attention averages many
+    assert 0 < r["error"] < 0.25
+    assert r["outputs"].isfinite().all()
+    index = r["index"]
+    assert bool((index[..., 1:] > index[..., :-1]).all()) and bool((index >= 0).all())
+    # each step adds 1 for each query head: 16 admission queries and 5 steps, of
+    # which eviction kept a part
+    total = r["weights"].sum((1, 2)).cpu()
+    assert bool((total <= heads * (16 + steps) * (1 + 2.0 ** -10)).all())
+    assert bool((total >= heads * steps * (1 - 2.0 ** -10)).all())
