@@ -202,6 +202,25 @@ def test_attention_many_rows_nan_and_bad_pages(ops, dim, page):
     assert not out[:4].isnan()[..., 64:].any() and not out[new:].isnan().any()
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 0)])
+def test_attention_many_rows_of_values_of_many_sizes(ops, dim, page):
+    """Scales that grow along a sequence, zeros with the smallest scale, and a
+    page that is none over one that holds the largest of all."""
+    codes, scales, table = make_cache(2, 1, dim, 400, page)
+    for t, byte in ((5, 110), (6, 131), (70, 113), (71, 100), (130, 0), (201, 134), (399, 145)):
+        _, p, slot = ref.places(table, codes.shape[3], codes.shape[1], 0, [t])[0]
+        scales[1, p, 0, slot, 1] = byte
+        if byte == 0:
+            codes[1, p, 0, slot] = 0
+    if page:
+        codes, scales, table = (torch.cat([x[:, :1], x], 1) if i < 2 else x + 1 for i, x in enumerate((codes, scales, table)))
+        scales[1, 0] = 254  # what a token without a page reads
+        table[1, 1] = -1
+    codes, scales, table = widened(codes, scales, table, 2 * 8)
+    q = torch.randn(2 * 40, 3, dim, generator=torch.Generator().manual_seed(1)).bfloat16()
+    check_attention(ops, "bf16", q, codes, scales, torch.tensor([400, 100], dtype=torch.int32), table=table, weigh=False)
+
+
 def test_attention_many_rows_ragged(ops):
     new, most = [0, 1, 70, 9, 0, 130], 100
     lens = torch.tensor([40, 300, 170, 4, 0, 140], dtype=torch.int32)
