@@ -577,3 +577,40 @@ def test_the_serving_example(vqx):
     total = r["weights"].sum((1, 2)).cpu()
     assert bool((total <= heads * (16 + steps) * (1 + 2.0 ** -10)).all())
     assert bool((total >= heads * steps * (1 - 2.0 ** -10)).all())
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_a_cache_past_32_bits(ops, many):
+    """The same pages at the far end of a cache of 5 GiB a plane: every operator
+    finds them there and writes nothing else."""
+    dim, kv, page, seqs = 128, 2, 64, 2
+    pages = 5 * 2 ** 30 // (kv * page * dim // 2)
+    far = torch.tensor([[pages - 1, pages - 3], [pages - 2, pages - 5]], dtype=torch.int32, device=DEV)
+    near_table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    if many:  # the kernel for many rows, by room
+        far, near_table = (torch.nn.functional.pad(t, (0, 4000), value=-1) for t in (far, near_table))
+    big_c = torch.empty(2, pages, kv, page, dim // 2, dtype=torch.uint8, device=DEV)
+    big_s = torch.empty(2, pages, kv, page, dim // 32, dtype=torch.uint8, device=DEV)
+    c, s, _ = on(*make_cache(4, kv, dim, page, 0))
+    big_c[:, far[:, :2].flatten().long()], big_s[:, far[:, :2].flatten().long()] = c, s
+    lens = torch.tensor([128, 100], dtype=torch.int32, device=DEV)
+    new = 40 if many else 1
+    x = torch.randn(seqs * new, 8, dim, device=DEV).bfloat16()
+    got = []
+    for codes, scales, table in ((big_c, big_s, far), (c, s, near_table)):
+        ops.kv4_append(x[:, 4:6], x[:, 6:], codes, scales, lens, None, table)
+        k, v = ops.kv4_read(codes, scales, lens, seqs * new, None, table)
+        out, lse = ops.kv4_attention(x[:, :4], codes, scales, lens, None, None, table)
+        w = torch.zeros(seqs, kv, 128, device=DEV)
+        ops.kv4_accumulate(x[:, :4], lse, codes, scales, lens, w, None, None, table)
+        oc, os_, ow = torch.zeros(2, 2, kv, 50, 64, dtype=torch.uint8, device=DEV), torch.zeros(
+            2, 2, kv, 50, 4, dtype=torch.uint8, device=DEV), torch.zeros(seqs, kv, 50, device=DEV)
+        index, _ = ops.kv4_evict(codes, scales, w, lens, 50, 8, oc, os_, ow, table)
+        got.append((k, v, out, lse, w, index, oc, os_, ow))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    # and into it
+    ops.kv4_evict(c, s, w, lens, 50, 8, big_c, big_s, ow, near_table, far[:, :2].contiguous())
+    for b in range(seqs):
+        same(big_c[:, int(far[b, 0]), :, :50], oc[:, b], "codes")
+        same(big_s[:, int(far[b, 0]), :, :50], os_[:, b], "scales")

@@ -131,7 +131,8 @@ def workspace(L, cache, q):
     (dict(kv_heads=0), ValueError, "sizes"), (dict(page_size=0), ValueError, "sizes"), (dict(seqs=-1), ValueError, "sizes"),
     (dict(table=None, pages=1), ValueError, "without a table"),
     (dict(pages=1 << 31), RuntimeError, "2\\^32 rows"), (dict(pages=1 << 30, page_size=32), RuntimeError, "2\\^32 rows"),
-    (dict(pages_per_seq=1 << 26), RuntimeError, "2\\^30 tokens"), (dict(seqs=1 << 24), RuntimeError, "2\\^24 heads")])
+    (dict(pages_per_seq=1 << 26), RuntimeError, "2\\^30 tokens"), (dict(seqs=1 << 24), RuntimeError, "2\\^24 heads"),
+    (dict(kv_heads=1 << 17), RuntimeError, "131072 kv heads")])
 def test_library_cache_refusals(vqx, how, error, message):
     L = vqx._lib
     with pytest.raises(error, match=message):

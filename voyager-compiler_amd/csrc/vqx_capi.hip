@@ -114,6 +114,7 @@ static int to_view(const vqx_kv4_cache* c, const char* what, Kv4View* v) {
     return set_error(kErrInvalid, "%s: null cache tensor, or no pages", what);
   if (c->dim != 64 && c->dim != 128 && c->dim != 256)
     return set_error(kErrInvalid, "%s: heads of 64, 128 or 256 elements, not %d", what, c->dim);
+  if (c->kv_heads > 1 << 16) return set_error(kErrUnsupported, "%s: %d kv heads", what, c->kv_heads);
   if (c->seqs < 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->pages < 0 || c->pages_per_seq < 0)
     return set_error(kErrInvalid, "%s: negative or empty sizes", what);
   if (!aligned(c->codes, 16) || !aligned(c->scales, (unsigned)c->dim / 32))

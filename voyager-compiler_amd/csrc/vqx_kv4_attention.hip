@@ -1353,11 +1353,12 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   const int64_t span = span_of(p.rows / q.group + 2);
   // two workgroups for every compute unit, as many as are resident and no more,
-  // and none with less than two steps a wave, eight of the kernel for many rows: one
-  // costs some 5 us beside its tokens (4 a unit instead of 2: 16 sequences of
-  // 4000 tokens 27 and 23 us, one of 131073 47 and 38)
+  // and none with fewer than eight steps (of a wave, of the workgroup): one costs
+  // some 5 us beside its tokens, a join 4 and its launch (4 a unit instead of 2:
+  // 16 sequences of 4000 tokens 27 and 23 us, one of 131073 47 and 38; one of
+  // 1000 tokens whole 10, in four splits 12)
   const int64_t heads = seqs * p.tiles, want = heads > 0 && 2ll * num_cus() > heads ? 2ll * num_cus() / heads : 1;
-  const int64_t least = p.rows == kRows ? 2 * kWaves * kStep : 8 * kBlockStep;
+  const int64_t least = p.rows == kRows ? 8 * kWaves * kStep : 8 * kBlockStep;
   int64_t chunk = (span + want - 1) / want;
   if (chunk < least) chunk = least;
   chunk = (chunk + kWaves * kStep - 1) / (kWaves * kStep) * (kWaves * kStep);
