@@ -139,79 +139,117 @@ Kv4Share share_of(const Kv4View& c, int dim, int n) {
   return Kv4Share{(int32_t)tokens, (int32_t)((n + tokens - 1) / tokens)};
 }
 
-// work(plane, token, head, part, row) for every 8 values of this workgroup's
-// tokens; the rows are found once a token, for all of them at a time.
-template <int kDim, typename F>
-__device__ __forceinline__ void for_new_values(const Kv4View& c, const Kv4Tokens& q, const Kv4Share& share, F work) {
+// One thread's 8 values: the part-th of a row of head h of new token i.
+struct Item {
+  uint32_t plane, h, part, row;
+  int i;
+};
+
+// take(item, what) and then put(item, what) for every 8 values of this
+// workgroup's tokens, kAhead of them taken before the first is put; the rows are
+// found once a token, for all of them at a time.  A thread without an item of
+// its own takes the last one and does not put it, so that the four threads of a
+// block stay together.
+template <int kDim, typename What, typename Take, typename Put>
+__device__ __forceinline__ void for_new_values(const Kv4View& c, const Kv4Tokens& q, const Kv4Share& share, Take take,
+                                               Put put) {
   constexpr uint32_t kPerRow = kDim / 8;
+  constexpr int kAhead = 2;
   __shared__ uint32_t rows[kMostTokens];
   const uint32_t plane = blockIdx.x >= (uint32_t)share.groups;
   const int i0 = (int)(blockIdx.x - plane * (uint32_t)share.groups) * share.tokens;
   const int count = q.n - i0 < share.tokens ? q.n - i0 : share.tokens;
   if ((int)threadIdx.x < count) rows[threadIdx.x] = new_token_row(c, q, i0 + (int)threadIdx.x);
   __syncthreads();
-  // the four threads of a block stay together: items are a multiple of 8
   const uint32_t per = c.kv * kPerRow, items = (uint32_t)count * per;
   uint32_t token = threadIdx.x / per, rest = threadIdx.x % per;
   const uint32_t step_token = 256 / per, step_rest = 256 % per;
-  for (uint32_t w = threadIdx.x; w < items; w += 256) {
-    const uint32_t h = rest / kPerRow, part = rest % kPerRow, row = rows[token];
-    work(plane, i0 + (int)token, h, part, row == kNoRow ? kNoRow : row + h * c.size);
-    token += step_token, rest += step_rest;
-    if (rest >= per) rest -= per, ++token;
+  for (uint32_t w = threadIdx.x; w < items; w += kAhead * 256) {
+    Item item[kAhead];
+    What what[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const bool own = w + a * 256 < items;
+      const uint32_t t = own ? token : (uint32_t)count - 1, r = own ? rest : per - kPerRow + threadIdx.x % kPerRow;
+      const uint32_t h = r / kPerRow, row = rows[t];
+      item[a] = Item{plane, h, r % kPerRow, row == kNoRow ? kNoRow : row + h * c.size, i0 + (int)t};
+      take(item[a], what[a]);
+      token += step_token, rest += step_rest;
+      if (rest >= per) rest -= per, ++token;
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) put(item[a], what[a], w + a * 256 < items);
   }
 }
 
-// Bound by the values' bytes; a call of a decode step by its launch.
+// Bound by the values' bytes (10377 tokens of 32 heads of 128, bf16, keys and
+// values: 215 MB in 56 us, 3.9 TB/s; reading them back 38 us); a call of a decode
+// step by its launch (3.4 us).
 template <int kDim, typename T>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Tokens q, Kv4Share share, const void* key,
                                                          const void* value, int64_t key_sn, int64_t key_sh,
                                                          int64_t value_sn, int64_t value_sh) {
   constexpr uint32_t kPerRow = kDim / 8;
-  for_new_values<kDim>(c, q, share, [&](uint32_t plane, int i, uint32_t h, uint32_t part, uint32_t row) {
-    Raw8F raw;
-    load8(plane ? value : key, (int64_t)i * (plane ? value_sn : key_sn) + (int64_t)h * (plane ? value_sh : key_sh) + part * 8,
-          T(), raw);
-    float x[8];
-    values8(raw, T(), x);
-    // the largest magnitude as a bit pattern, so that a NaN is the largest
-    uint32_t amax = 0;
+  struct Raw {
+    Raw8F v;
+  };
+  for_new_values<kDim, Raw>(
+      c, q, share,
+      [&](const Item& t, Raw& raw) {
+        load8(t.plane ? value : key,
+              (int64_t)t.i * (t.plane ? value_sn : key_sn) + (int64_t)t.h * (t.plane ? value_sh : key_sh) + t.part * 8, T(),
+              raw.v);
+      },
+      [&](const Item& t, const Raw& raw, bool own) {
+        float x[8];
+        values8(raw.v, T(), x);
+        // the largest magnitude as a bit pattern, so that a NaN is the largest
+        uint32_t amax = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = umax32(amax, f2u(x[j]) & 0x7FFFFFFFu);
-    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 1));
-    amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 2));
-    int e = (amax == 0 ? -126 : log2_floor(u2f(amax), T())) - 2;
-    e = e < -127 ? -127 : (e > 127 ? 127 : e);
-    const bool finite = amax < 0x7F800000u;
-    const float r = exp2i(-e);
-    uint32_t v[4];
+        for (int j = 0; j < 8; ++j) amax = umax32(amax, f2u(x[j]) & 0x7FFFFFFFu);
+        amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 1));
+        amax = umax32(amax, (uint32_t)__shfl_xor((int)amax, 2));
+        int e = (amax == 0 ? -126 : log2_floor(u2f(amax), T())) - 2;
+        e = e < -127 ? -127 : (e > 127 ? 127 : e);
+        const bool finite = amax < 0x7F800000u;
+        const float r = exp2i(-e);
+        uint32_t v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)  // + 0: both zeros have code 0
-      v[j] = pack_bf16x2(__builtin_fmaf(x[2 * j], r, 0.0f), __builtin_fmaf(x[2 * j + 1], r, 0.0f));
-    const uint32_t code = fp4_codes(v);
-    if (row == kNoRow) return;
-    const uint64_t at = plane * c.plane_rows + row;
-    reinterpret_cast<uint32_t*>(c.codes)[at * kPerRow + part] = finite ? code : 0u;
-    // a block with an infinity or a NaN is NaN as a whole
-    if ((part & 3) == 0) c.scales[at * (kPerRow / 4) + part / 4] = (uint8_t)(finite ? e + 127 : 255);
-  });
+        for (int j = 0; j < 4; ++j)  // + 0: both zeros have code 0
+          v[j] = pack_bf16x2(__builtin_fmaf(x[2 * j], r, 0.0f), __builtin_fmaf(x[2 * j + 1], r, 0.0f));
+        const uint32_t code = fp4_codes(v);
+        if (t.row == kNoRow || !own) return;
+        const uint64_t at = t.plane * c.plane_rows + t.row;
+        reinterpret_cast<uint32_t*>(c.codes)[at * kPerRow + t.part] = finite ? code : 0u;
+        // a block with an infinity or a NaN is NaN as a whole
+        if ((t.part & 3) == 0) c.scales[at * (kPerRow / 4) + t.part / 4] = (uint8_t)(finite ? e + 127 : 255);
+      });
 }
 
 template <int kDim, typename T>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4View c, Kv4Tokens q, Kv4Share share, void* key, void* value) {
   constexpr uint32_t kPerRow = kDim / 8;
-  for_new_values<kDim>(c, q, share, [&](uint32_t plane, int i, uint32_t h, uint32_t part, uint32_t row) {
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row != kNoRow) {
-      const uint64_t at = plane * c.plane_rows + row;
-      const uint32_t code = reinterpret_cast<const uint32_t*>(c.codes)[at * kPerRow + part];
-      const float s = kv4_scale(c.scales[at * (kPerRow / 4) + part / 4]);
-      fp4_values(code, x);
+  struct Raw {
+    uint32_t code, scale;
+  };
+  for_new_values<kDim, Raw>(
+      c, q, share,
+      [&](const Item& t, Raw& raw) {
+        raw = Raw{0u, 127u};
+        if (t.row != kNoRow) {
+          const uint64_t at = t.plane * c.plane_rows + t.row;
+          raw.code = reinterpret_cast<const uint32_t*>(c.codes)[at * kPerRow + t.part];
+          raw.scale = c.scales[at * (kPerRow / 4) + t.part / 4];
+        }
+      },
+      [&](const Item& t, const Raw& raw, bool own) {
+        float x[8];
+        fp4_values(raw.code, x);
+        const float s = kv4_scale(raw.scale);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= s;
-    }
-    store8(plane ? value : key, (((int64_t)i * c.kv + h) * kPerRow + part) * 8, T(), x);
-  });
+        for (int j = 0; j < 8; ++j) x[j] *= s;
+        if (own) store8(t.plane ? value : key, (((int64_t)t.i * c.kv + t.h) * kPerRow + t.part) * 8, T(), x);
+      });
 }
 
 // ---------------------------------------------------------------------------
@@ -386,7 +424,7 @@ __device__ __forceinline__ void read_keys(const Selection& s, const WaveRun& r, 
 // weight of the room-th heaviest by histograms of 11, 11 and 10 bits of the
 // key, fewer where one settles it, then each wave counts and writes the tokens
 // of its own run, lowest first, so that equal weights go by their place.  The
-// weights are read once: bound by a few latencies and barriers (640 tokens: 10
+// weights are read once: bound by a few latencies and barriers (640 tokens: 11
 // us).
 __global__ __launch_bounds__(kSelectThreads) void kv4_select_kernel(Kv4View c, const float* weights,
                                                                     int64_t weights_len, int budget, int recent,
@@ -418,9 +456,9 @@ __global__ __launch_bounds__(kSelectThreads) void kv4_select_kernel(Kv4View c, c
 // More tokens: the same by slices, a workgroup each, in four launches.  Launch
 // kPass < 3 leaves the histogram of its slice's keys for the bits that the
 // launches before settled, counts[pass][head][slice][bin]; the last one has
-// from them how many tokens the slices before it keep, and writes.  One
-// workgroup for a head of 50001 tokens took 52 us: instructions of 16 waves on
-// one compute unit.
+// from them how many tokens the slices before it keep, and writes.  Bound by the
+// latency of four launches (50001 tokens of 32 heads: 8, 10, 10 and 11 us); one
+// workgroup for a head took 52 us, instructions of 16 waves on one compute unit.
 template <int kPass>
 __global__ __launch_bounds__(kSelectThreads) void kv4_slice_kernel(Kv4View c, const float* weights,
                                                                    int64_t weights_len, int budget, int recent,
@@ -489,30 +527,51 @@ __global__ __launch_bounds__(kSelectThreads) void kv4_slice_kernel(Kv4View c, co
   }
 }
 
-// The kept tokens' rows into the other cache: D / 32 lanes a row of 16 bytes
-// each, the first of them with the row's scales as well.
+// The kept tokens' rows into the other cache: D / 32 lanes a row of 16 bytes and
+// a scale each, in both planes, kAhead rows of a thread on their way at a time.
+// Bound by the memory's lines: kept rows are mostly single ones, 64 bytes of
+// codes and 4 of scales (8192 of 50001 tokens of 32 heads: 71 MB in 20 us, with
+// one row on its way as with four).
 template <int D>
-__global__ __launch_bounds__(256) void kv4_move_kernel(Kv4View c, Kv4View out, const int32_t* index, int budget,
-                                                       uint64_t items) {
-  constexpr int kLanes = D / 32;
-  for (uint64_t w = (uint64_t)blockIdx.x * 256 + threadIdx.x; w < items; w += (uint64_t)gridDim.x * 256) {
-    const uint64_t slot = w / kLanes;
-    const uint32_t part = (uint32_t)(w % kLanes);
-    const int t = index[slot];
-    if (t < 0) continue;
-    const uint64_t head = slot / (uint32_t)budget;
-    const uint32_t j = (uint32_t)(slot - head * (uint32_t)budget);
-    const uint32_t b = (uint32_t)(head / c.kv), h = (uint32_t)(head - (uint64_t)b * c.kv);
-    const uint32_t from = kv4_page(c, b, (uint32_t)t), to = kv4_page(out, b, j);
-    if (to >= out.pages) continue;
-    const uint64_t src = kv4_row(c, from, h, (uint32_t)t), dst = kv4_row(out, to, h, j);
+__global__ __launch_bounds__(256) void kv4_move_kernel(Kv4View c, Kv4View out, const int32_t* index, uint32_t budget,
+                                                       uint32_t groups) {
+  constexpr uint32_t kLanes = D / 32, kEach = 256 / kLanes;
+  constexpr int kAhead = 4;
+  const uint32_t head = blockIdx.x / groups, b = head / c.kv, h = head % c.kv, part = threadIdx.x % kLanes;
+  const uint32_t first = blockIdx.x % groups * (kEach * kAhead) + threadIdx.x / kLanes;
+  int t[kAhead];
+  uint32_t from[kAhead], to[kAhead];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const uint32_t j = first + a * kEach;
+    t[a] = j < budget ? index[(uint64_t)head * budget + j] : -1;
+    to[a] = j < budget ? kv4_page(out, b, j) : 0xFFFFFFFFu;
+  }
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) from[a] = t[a] >= 0 ? kv4_page(c, b, (uint32_t)t[a]) : 0xFFFFFFFFu;
+  u32x4 code[kAhead][2];
+  uint8_t scale[kAhead][2];
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    const uint64_t row = kv4_row(c, from[a], h, (uint32_t)t[a]);
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
-      const uint64_t s = plane * c.plane_rows + src, d = plane * out.plane_rows + dst;
-      u32x4 v = {0u, 0u, 0u, 0u};  // a token without a page is kept as zeros
-      if (from < c.pages) v = ld_nt(reinterpret_cast<const u32x4*>(c.codes) + s * kLanes + part);
-      reinterpret_cast<u32x4*>(out.codes)[d * kLanes + part] = v;
-      out.scales[d * kLanes + part] = from < c.pages ? c.scales[s * kLanes + part] : (uint8_t)0;
+      // a token without a page is kept as zeros
+      const uint64_t s = (plane * c.plane_rows + row) * kLanes + part;
+      code[a][plane] = ld_nt(reinterpret_cast<const u32x4*>(c.codes) + s);
+      scale[a][plane] = c.scales[s];
+      if (from[a] >= c.pages) code[a][plane] = u32x4{0u, 0u, 0u, 0u}, scale[a][plane] = 0;
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a) {
+    if (t[a] < 0 || to[a] >= out.pages) continue;
+    const uint64_t row = kv4_row(out, to[a], h, first + a * kEach);
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      const uint64_t d = (plane * out.plane_rows + row) * kLanes + part;
+      reinterpret_cast<u32x4*>(out.codes)[d] = code[a][plane];
+      out.scales[d] = scale[a][plane];
     }
   }
 }
@@ -592,10 +651,13 @@ int kv4_evict(const Kv4View& c, int dim, const float* weights, int64_t weights_l
   }
   int rc = check_launch("kv4_evict (selection)");
   if (rc != kOk) return rc;
-  const uint64_t items = (uint64_t)c.seqs * c.kv * (uint64_t)budget * (uint64_t)(dim / 32);
-  const unsigned grid = grid_for((int64_t)items, 256, 16);
-#define VQX_KV4_MOVE(D) \
-  hipLaunchKernelGGL((kv4_move_kernel<D>), dim3(grid), dim3(256), 0, st, c, out, index, budget, items)
+  const uint32_t each = 4u * 256u / (uint32_t)(dim / 32), groups = ((uint32_t)budget + each - 1) / each;
+  if ((uint64_t)c.seqs * c.kv * groups >= 1ull << 31)
+    return set_error(kErrUnsupported, "kv4_evict: a budget of %d tokens for %u heads does not fit a launch", budget,
+                     c.seqs * c.kv);
+#define VQX_KV4_MOVE(D)                                                                                        \
+  hipLaunchKernelGGL((kv4_move_kernel<D>), dim3(c.seqs * c.kv * groups), dim3(256), 0, st, c, out, index, \
+                     (uint32_t)budget, groups)
   if (dim == 64)
     VQX_KV4_MOVE(64);
   else if (dim == 128)
