@@ -183,15 +183,16 @@ def test_library_evict_refusals(vqx):
     L = vqx._lib
     far = BASE << 20
 
-    def evict(budget=8, recent=2, weights=BASE, length=32, index=BASE, ow=BASE, codes=far, **out):
-        L.call("vqx_kv4_evict", lib_cache(L), weights, length, budget, recent, lib_cache(L, codes=codes, **out), index, ow,
-               None, 0, None)
+    def evict(budget=8, recent=2, weights=BASE, length=32, index=BASE, ow=far, codes=far, scales=far, **out):
+        L.call("vqx_kv4_evict", lib_cache(L), weights, length, budget, recent,
+               lib_cache(L, codes=codes, scales=scales, **out), index, ow, None, 0, None)
 
     for how, message in ((dict(budget=0), "budget of 0"), (dict(budget=33), "room for 32"), (dict(recent=-1), "-1 latest"),
                          (dict(recent=9), "9 latest"), (dict(weights=None), "null"), (dict(index=None), "null"),
                          (dict(ow=None), "null"), (dict(length=-1), "weights of -1"), (dict(kv_heads=4), "differ"),
                          (dict(dim=64), "differ"), (dict(seqs=1), "differ"), (dict(codes=BASE), "another cache"),
-                         (dict(codes=BASE + 4096), "another cache")):
+                         (dict(codes=BASE + 4096), "another cache"), (dict(scales=BASE + 64), "another cache"),
+                         (dict(ow=BASE), "another tensor"), (dict(ow=BASE + 4 * 32 * 4 - 4), "another tensor")):
         with pytest.raises(ValueError, match=message):
             evict(**how)
     big, n = lib_cache(L, pages=1 << 20, pages_per_seq=1 << 16), L.ctypes.c_int64(-1)
@@ -199,7 +200,8 @@ def test_library_evict_refusals(vqx):
     assert n.value > 0
     for ws, size in ((None, 0), (BASE, n.value - 1), (BASE + 4, n.value)):
         with pytest.raises(ValueError, match="workspace"):
-            L.call("vqx_kv4_evict", big, BASE, 1 << 16, 8, 2, lib_cache(L, codes=1 << 40), BASE, BASE, ws, size, None)
+            L.call("vqx_kv4_evict", big, BASE, 1 << 16, 8, 2, lib_cache(L, codes=1 << 40, scales=1 << 41), BASE, 1 << 42,
+                   ws, size, None)
     L.call("vqx_kv4_evict_workspace_size", big, 8192, n)
     assert n.value == 0
     with pytest.raises(ValueError, match="weights of -1"):

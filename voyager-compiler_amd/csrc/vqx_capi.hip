@@ -729,11 +729,17 @@ int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weig
     return set_error(kErrInvalid, "kv4_evict: %d latest tokens of a budget of %d", recent, budget);
   if (weights_len < 0) return set_error(kErrInvalid, "kv4_evict: weights of %lld tokens", (long long)weights_len);
   if (c.seqs > 0 && (!weights || !index || !out_weights)) return set_error(kErrInvalid, "kv4_evict: null tensor");
-  const uint64_t in_bytes = 2 * c.plane_rows * (uint64_t)(cache->dim / 2),
-                 out_bytes = 2 * o.plane_rows * (uint64_t)(cache->dim / 2);
-  const uint64_t a = (uint64_t)(uintptr_t)c.codes, z = (uint64_t)(uintptr_t)o.codes;
-  if (a < z + out_bytes && z < a + in_bytes)
+  auto overlap = [](const void* p, uint64_t n, const void* q, uint64_t m) {
+    const uint64_t a = (uint64_t)(uintptr_t)p, b = (uint64_t)(uintptr_t)q;
+    return a < b + m && b < a + n;
+  };
+  const uint64_t in_rows = 2 * c.plane_rows, out_rows = 2 * o.plane_rows, row = (uint64_t)cache->dim / 2,
+                 scale_row = (uint64_t)cache->dim / 32, heads = (uint64_t)c.seqs * c.kv;
+  if (overlap(c.codes, in_rows * row, o.codes, out_rows * row) ||
+      overlap(c.scales, in_rows * scale_row, o.scales, out_rows * scale_row))
     return set_error(kErrInvalid, "kv4_evict: the kept tokens go to another cache, not onto this one");
+  if (overlap(weights, heads * (uint64_t)weights_len * 4, out_weights, heads * (uint64_t)budget * 4))
+    return set_error(kErrInvalid, "kv4_evict: the kept weights go to another tensor, not onto these");
   const int64_t need = kv4_evict_workspace(c, weights_len);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return set_error(kErrInvalid, "kv4_evict: needs a 16-byte aligned workspace of %lld bytes, not %lld",

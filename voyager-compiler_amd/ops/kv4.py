@@ -210,7 +210,7 @@ def kv4_read(codes, scales, lengths, n, cu=None, table=None, dtype=torch.bfloat1
     if n < 0:
         _refuse(what, f"{n} new tokens")
     offsets = _offsets(cu, n, c.seqs, what, codes.device)
-    k = torch.empty((n, c.kv_heads, c.dim), dtype=dtype, device=codes.device)
+    k = codes.new_empty((n, c.kv_heads, c.dim), dtype=dtype)
     v = torch.empty_like(k)
     _lib.call("vqx_kv4_read", c, k.data_ptr(), v.data_ptr(), _FLOATS[dtype], n, offsets, _lib.stream_of(codes))
     return k, v
@@ -248,10 +248,10 @@ def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None,
     c = _cache(codes, scales, lengths, table, what)
     device = codes.device
     qs, q, key = _query(query, c, device, cu, most, scale, softcap, window, slopes, what)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(key[:2], dtype=torch.float32)
     need = _workspace_bytes(c, qs, device, key)
-    ws = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
+    ws = codes.new_empty(need).data_ptr() if need else None
     _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), ws, need, _lib.stream_of(codes))
     return out, lse
 
@@ -295,11 +295,11 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
     ow = _weights(out_weights, c.seqs, c.kv_heads, "out_weights", what, device)
     if out_weights.shape[2] != budget:
         _refuse(what, f"out_weights are for {out_weights.shape[2]} tokens, the budget is {budget}")
-    index = torch.empty((c.seqs, c.kv_heads, budget), dtype=torch.int32, device=device)
+    index = lengths.new_empty((c.seqs, c.kv_heads, budget))
     need = ctypes.c_int64(0)
     _lib.call("vqx_kv4_evict_workspace_size", c, weights.shape[2], need)
     need = need.value
-    ws = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
+    ws = codes.new_empty(need).data_ptr() if need else None
     _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow, ws, need,
               _lib.stream_of(codes))
     return index, kept
