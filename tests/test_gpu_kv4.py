@@ -128,10 +128,10 @@ def test_attention(ops, i):
 
 def widened(codes, scales, table, tiles):
     """The same cache with room for so many tokens that a call of `tiles` tiles
-    of 16 rows, over all sequences and kv heads, is one for many rows (100000
-    tiles of 16 rows by 32 tokens): a table of pages that are none, or longer
+    of 16 rows, over all sequences and kv heads, is one for many rows (200000
+    tiles of 16 rows by 32 tokens at most): a table of pages that are none, or longer
     sequences."""
-    room = -(-100000 // tiles) * 32 + 64
+    room = -(-200000 // tiles) * 32 + 64
     if table is not None:
         more = room // codes.shape[3] + 1 - table.shape[1]
         return codes, scales, torch.nn.functional.pad(table, (0, max(0, more)), value=-1)
@@ -163,7 +163,7 @@ def test_attention_many_rows(ops, i):
         how["slopes"] = torch.exp2(-8.0 * torch.arange(1, heads + 1) / heads)
     if how.get("window"):
         # a window bounds what a tile can see: more sequences, that have nothing
-        more = -(-100000 * 32 // (kv * -(-new * group // 16) * (how["window"] + new)))
+        more = -(-200000 * 32 // (kv * -(-new * group // 16) * (how["window"] + new)))
         lens = lens + [0] * more
         q = torch.nn.functional.pad(q, (0, 0, 0, 0, 0, new * more))
         if table is not None:
@@ -246,6 +246,45 @@ def test_attention_ragged(ops, kind, dim, most):
     q = torch.randn(sum(new), 6, dim, generator=g).to(TYPES[kind])
     out, lse = check_attention(ops, kind, q, codes, scales, lens, cu, most, table)
     assert torch.equal(lse[71:76].cpu(), torch.full((5, 6), -math.inf)) and not out[71:76].any()
+
+
+@pytest.mark.parametrize("kind,dim,page", [("bf16", 128, 16), ("f16", 64, 0), ("f32", 256, 48)])
+@pytest.mark.parametrize("new,lens,kv,many", [
+    ([1] * 37 + [100] + [1] * 35 + [5], [20 + i for i in range(37)] + [130] + [3 * i for i in range(36)], 3, False),
+    ([0, 1, 120, 1, 0, 2, 1], [0, 1700, 2000, 5, 900, 2, 1000], 1, False),
+    ([3, 0, 300, 0], [40, 7, 310, 0], 2, True),
+    ([0, 130, 2], [800, 5000, 70], 1, True),
+])
+def test_attention_mixed(ops, kind, dim, page, new, lens, kv, many):
+    """Few sequences with many new tokens among others with one or none: the
+    tiles that there are come one after another, over more than a wave's
+    sequences, with splits and without."""
+    cu = torch.tensor([0] + new).cumsum(0).int()
+    lens = torch.tensor(lens, dtype=torch.int32)
+    codes, scales, table = make_cache(len(new), kv, dim, int(lens.max()), page)
+    if many:
+        codes, scales, table = widened(codes, scales, table, sum(new) * 4 * kv // 16)
+    q = torch.randn(sum(new), kv * 4, dim, generator=torch.Generator().manual_seed(len(new))).to(TYPES[kind])
+    check_attention(ops, kind, q, codes, scales, lens, cu, max(new), table)
+
+
+def test_attention_mixed_more_than_most(ops):
+    """Offsets with more new tokens than `most`, out of order and past the end:
+    rows of sound sequences are right, the others' are NaN or left alone."""
+    new = [1, 1, 40, 1, 1, 1, 1, 1]
+    cu = torch.tensor([0] + new).cumsum(0).int()
+    lens = torch.full((8,), 60, dtype=torch.int32)
+    codes, scales, table = make_cache(8, 2, 128, 64, 16)
+    q = torch.randn(sum(new), 8, 128, generator=torch.Generator().manual_seed(1)).bfloat16()
+    d = on(q, codes, scales, lens, cu, table)
+    want, want_lse = ops.kv4_attention(d[0], d[1], d[2], d[3], d[4], 40, d[5])
+    out, lse = ops.kv4_attention(d[0], d[1], d[2], d[3], d[4], 30, d[5])
+    assert out[32:42].isnan().all() and lse[32:42].isnan().all()
+    got, want = torch.cat([out[:32], out[42:]]), torch.cat([want[:32], want[42:]]).cpu().double()
+    near(got, want, 2.0 ** -7 * want.abs() + 2.0 ** -6, "out")
+    cu[4:] = torch.tensor([1 << 30, -5, 1 << 30, 47, 0], dtype=torch.int32)
+    ops.kv4_attention(d[0], d[1], d[2], d[3], cu.to(DEV), 40, d[5])
+    torch.cuda.synchronize()
 
 
 def test_attention_of_more_than_most(ops):

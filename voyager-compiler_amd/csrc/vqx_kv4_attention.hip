@@ -122,6 +122,7 @@ struct QueryTerms {
 // its sums in the workspace: rows * D outputs, rows references and rows sums.
 struct Kv4Plan {
   int32_t rows, tiles, chunk, splits;
+  int32_t listed;  // tiles of a kv head that the workgroups are handed one by one; 0: tiles of every sequence
 };
 
 // Where the rows of one tile stand.
@@ -152,6 +153,63 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
   if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(step - 1);
   if (r.lo > r.hi) r.lo = r.hi & ~(step - 1);
   return r;
+}
+
+// Sequences and tiles counted through: where tile t of all that there are lies.
+__device__ __forceinline__ bool listed_tile(const Kv4View& c, const Kv4Query& q, const Kv4Plan& plan, uint32_t t,
+                                            uint32_t& b, int& tile) {
+  const int lane = threadIdx.x & 63;
+  uint32_t before = 0;
+  for (uint32_t b0 = 0; b0 < c.seqs; b0 += 64) {
+    int first, count = 0;
+    if (b0 + lane < c.seqs) kv4_span(q.tokens, b0 + lane, first, count);
+    if (count > q.most) count = q.most;
+    // no more than there are at all, whatever the offsets say: below 2^25
+    uint32_t mine = ((uint32_t)count * q.group + plan.rows - 1) / (uint32_t)plan.rows;
+    if (mine > (uint32_t)plan.listed) mine = plan.listed;
+    uint32_t sum = mine;
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t x = (uint32_t)__shfl_up((int)sum, d);
+      if (lane >= d) sum += x;
+    }
+    const uint64_t past = __ballot(before + sum > t);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      tile = (int)(t - before - (uint32_t)__builtin_amdgcn_readlane((int)(sum - mine), l));
+      return true;
+    }
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  }
+  return false;
+}
+
+// What a workgroup has to do.
+struct Place {
+  uint32_t b, h, split;
+  int tile;
+  int64_t at;  // of its sums in the workspace
+};
+
+// Heads first, so that with 8 of them each XCD's L2 has the cache of one (of
+// other numbers each XCD gets all in turn, or a long sequence would be one
+// XCD's: 4 ragged prompts of 300, 4 heads: 35 and 32 us); then the splits, then
+// the tiles from the last, which sees the most.  (Splits and tiles first put
+// the first tile of every sequence, often the only one, on one XCD: 64 sequences
+// with 128 new tokens at most, all but one with one: 242 and 50 us.)
+__device__ __forceinline__ bool place_of(const Kv4View& c, const Kv4Query& q, const Kv4Plan& plan, Place& p) {
+  const uint32_t heads = plan.listed ? c.kv : c.seqs * c.kv, rest = blockIdx.x / heads;
+  const uint32_t slot = (blockIdx.x + (c.kv % 8 ? rest : 0u)) % heads;
+  p.split = rest % (uint32_t)plan.splits;
+  const int t = (plan.listed ? plan.listed : plan.tiles) - 1 - (int)(rest / (uint32_t)plan.splits);
+  if (plan.listed) {
+    p.h = slot;
+    p.at = ((int64_t)t * c.kv + slot) * plan.splits + p.split;
+    return listed_tile(c, q, plan, (uint32_t)t, p.b, p.tile);
+  }
+  p.b = slot / c.kv, p.h = slot % c.kv, p.tile = t;
+  p.at = ((int64_t)slot * plan.tiles + t) * plan.splits + p.split;
+  return true;
 }
 
 // What a score becomes, in powers of two: capped by a tanh, less its slope for
@@ -453,9 +511,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
   __shared__ uint32_t part_bad[2][kRows];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t split = blockIdx.x % (uint32_t)plan.splits, slot = blockIdx.x / (uint32_t)plan.splits;
-  const int tile = (int)(slot % (uint32_t)plan.tiles);
-  const uint32_t b = slot / (uint32_t)plan.tiles / c.kv, h = slot / (uint32_t)plan.tiles % c.kv;
+  Place place;
+  if (!place_of(c, q, plan, place)) return;
+  const uint32_t b = place.b, h = place.h, split = place.split;
+  const int tile = place.tile;
   const TileRows rows = tile_rows(c, q, b, tile, kRows, kStep);
   const int r = tile * kRows + n;
   const bool live = r < rows.rows;
@@ -654,7 +713,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
       acc[j][i] = bad >> block & 1u ? __builtin_nanf("") : acc[j][i] * inv;
     }
   if (plan.splits > 1) {
-    float* o = ws + (int64_t)blockIdx.x * (kRows * D + 2 * kRows);
+    float* o = ws + place.at * (kRows * D + 2 * kRows);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -714,12 +773,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   __shared__ uint32_t top_scale[2];  // the largest scale byte of steps so far, as of the last odd and even one
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // heads first, so that with 8 of them each XCD's L2 has the cache of one;
-  // then the tiles from the last, which sees the most
-  const uint32_t heads = c.seqs * c.kv, slot = blockIdx.x % heads, rest = blockIdx.x / heads;
-  const uint32_t b = slot / c.kv, h = slot % c.kv;
-  const uint32_t split = rest % (uint32_t)plan.splits;
-  const int tile = plan.tiles - 1 - (int)(rest / (uint32_t)plan.splits);
+  Place place;
+  if (!place_of(c, q, plan, place)) return;
+  const uint32_t b = place.b, h = place.h, split = place.split;
+  const int tile = place.tile;
   const TileRows rows = tile_rows(c, q, b, tile, kBlockRows, kBlockStep);
   if (rows.count > q.most && tile == 0 && split == 0) fill_beyond<D, T>(q, rows, h, out, lse);
   if (tile * kBlockRows >= rows.rows) return;
@@ -1091,7 +1148,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) acc[y][j] = bad[y] >> (j / 2) & 1u ? acc[y][j] * __builtin_nanf("") : acc[y][j] * inv;
     if (plan.splits > 1) {
-      float* o = ws + (((int64_t)slot * plan.tiles + tile) * plan.splits + split) * (kBlockRows * D + 2 * kBlockRows);
+      float* o = ws + place.at * (kBlockRows * D + 2 * kBlockRows);
       const int r = row[y] - tile * kBlockRows;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4*>(o + r * D + 16 * j + 4 * g) = acc[y][j];
@@ -1118,10 +1175,15 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   __shared__ float sum[kWaves][D], sum_l[kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t id = kShare == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
-  const uint32_t slot = id / (uint32_t)plan.rows, b = slot / (uint32_t)plan.tiles / c.kv,
-                 h = slot / (uint32_t)plan.tiles % c.kv;
-  const int tile = (int)(slot % (uint32_t)plan.tiles), n = (int)(id % (uint32_t)plan.rows), r = tile * plan.rows + n;
+  const uint32_t slot = id / (uint32_t)plan.rows;
+  uint32_t b = slot / (uint32_t)plan.tiles / c.kv, h = slot / (uint32_t)plan.tiles % c.kv;
+  int tile = (int)(slot % (uint32_t)plan.tiles);
+  if (plan.listed) {
+    h = slot % c.kv;
+    if (!listed_tile(c, q, plan, slot / c.kv, b, tile)) return;
+  }
   if (b >= c.seqs) return;
+  const int n = (int)(id % (uint32_t)plan.rows), r = tile * plan.rows + n;
   const TileRows rows = tile_rows(c, q, b, tile, plan.rows, plan.rows == kRows ? kStep : kBlockStep);
   if (r >= rows.rows) return;
   const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
@@ -1193,7 +1255,7 @@ constexpr int weigh_tile(int dim, int q_terms) { return kRows * (q_terms * (dim 
 // bound by the reading of the keys (8 sequences of 2000: 8 us, its own latency),
 // many by vector instructions (260 rows over 16385 tokens, 16 heads: 44 us).
 template <int D, typename T, bool kExtra>
-__global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int chunks, int most_tiles, const float* lse,
+__global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, int most_tiles, const float* lse,
                                                         float* weights, int64_t weights_len) {
   constexpr int kRow = D / 2, kScales = D / 32, kWords = D / 32;
   constexpr int kParts = weigh_tokens(D) / 16;
@@ -1207,10 +1269,12 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
   static_assert(sizeof(Tile) == weigh_tile(D, kQ), "");
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t slot = blockIdx.x / (uint32_t)chunks, b = slot / c.kv, h = slot % c.kv;
+  const uint32_t heads = c.seqs * c.kv, chunk = blockIdx.x / heads;
+  const uint32_t slot = (blockIdx.x + (c.kv % 8 ? chunk : 0u)) % heads;
+  const uint32_t b = slot / c.kv, h = slot % c.kv;
   const TileRows all = tile_rows(c, q, b, 0, 0x40000000, kStep);
   const int end = all.hi < weights_len ? all.hi : (int)weights_len;
-  const int w0 = all.lo + (int)(blockIdx.x % (uint32_t)chunks) * kWaves * weigh_tokens(D);
+  const int w0 = all.lo + (int)chunk * kWaves * weigh_tokens(D);
   if (w0 >= end) return;
   const int t0 = w0 + wave * weigh_tokens(D);
   u32x4 key[kParts][kWords];
@@ -1337,33 +1401,62 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
   if (n < 4 * kParts && (valid >> u & 1u)) w[u] += sum;
 }
 
-// Tiles of 16 rows by 32 tokens of a call from which on the kernel for many rows
-// is taken.  Its workgroups have 8 times the rows and a time of their own of
-// some 20 us with the join, so that below they do not fill the card: bf16, heads
-// of 128, with it and with the other, 512 new tokens of 4096 (131072 tiles) 75
-// and 91 us, 2048 of 2048 (262144) 77 and 123, 8 x 256 of 1000 (128000) 55 and
-// 108, 8 x 64 of 2000 (64000) 51 and 53, 1024 of 1024 (65536) 58 and 46, 256 of
-// 2000 (32000) 40 and 29.
+// When the kernel for many rows is taken.  Its workgroups have 4 or 8 times the
+// rows and a time of their own of some 20 us with the join, so that they have to
+// be full and to fill the card.  Full: in the mean a sequence has 128 rows, or
+// the most that any has (32 sequences of 4000 tokens, one with 512 new
+// tokens and the others with one, bf16, heads of 128: 130 us with it and 43 with
+// the other; 8 with 300 and 24 with one, of 1000: 77 and 106).  To fill the card,
+// either so many tiles of 16 rows by 32 tokens that its splits are long enough
+// (twice as many where a workgroup has 64 rows): 512 new tokens of 4096 (131072
+// tiles) 79 and 92 us, 2048 of 2048 (262144) 86 and 120, 256 of 2000 (32000) 45
+// and 30; f16, heads of 256, 64 rows: 2048 of 2048 295 and 480, 3000 of 5000 with
+// 4 heads over 1 (118500) 296 and 187.
 constexpr int64_t kManyTiles = 100000;
+// Or a workgroup for every compute unit over few tokens, without splits: there
+// the other kernel's time is that of its workgroups' beginnings.  bf16, heads of
+// 128: 6 x 139 new tokens of 180, 8 heads each (432 workgroups), 25 and 43 us,
+// 16 x 64 of 500 (256) 33 and 42, 1 x 512 of 512 (128) 30 and 20, 1 x 1000 of 1000
+// (256, two splits) 64 and 42; of 256: 6 x 139 of 180 54 and 120.
+constexpr int64_t kShortSpan = 2048;
+
+// Tiles of all kv heads, each of which has all its splits.
+int64_t slots_of(const Kv4View& c, const Kv4Plan& p) {
+  return (int64_t)c.kv * (p.listed ? (int64_t)p.listed : (int64_t)p.tiles * c.seqs);
+}
 
 Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   Kv4Plan p;
-  const int64_t all = (int64_t)q.most * q.group, seqs = (int64_t)c.seqs * c.kv;
+  const int64_t all = (int64_t)q.most * q.group;
   // the most tokens that rows of `tokens` new ones can see
   auto span_of = [&](int64_t tokens) {
     const int64_t seen = (int64_t)q.window + tokens + kBlockStep;
     return q.window && seen < (int64_t)c.cap ? seen : (int64_t)c.cap;
   };
-  const double tiles = (double)seqs * ((all + kRows - 1) / kRows) * (double)(span_of(q.most) / kStep);
-  p.rows = all > kRows && tiles >= kManyTiles ? 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3)) : kRows;
+  // no more tiles of a kv head than these, of sequences with less than the most
+  auto tiles_of = [&](int64_t rows) {
+    const int64_t every = c.seqs * ((all + rows - 1) / rows);
+    const int64_t there = (int64_t)q.tokens.n * q.group / rows + (q.tokens.n < (int64_t)c.seqs ? q.tokens.n : c.seqs);
+    return q.tokens.cu && there < every ? there : every;
+  };
+  const int many = 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3));
+  const double steps = (double)c.kv * tiles_of(kRows) * (double)(span_of(q.most) / kStep);
+  const int64_t blocks = c.kv * tiles_of(many), room = span_of(many / q.group + 2);
+  const bool full = (int64_t)q.tokens.n * q.group >= c.seqs * (all < 128 ? all : 128);
+  const bool whole = room <= 8 * kBlockStep ? blocks >= num_cus() : room <= kShortSpan && blocks > num_cus();
+  p.rows = all > kRows && full && (whole || steps >= (many == 64 ? 2 : 1) * kManyTiles) ? many : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
+  const int64_t there = tiles_of(p.rows);
+  // where most tiles would have no rows (32 sequences of 4000 tokens, one with
+  // 512 new tokens, heads of 128: 131 us with all tiles, 43 with those there are)
+  p.listed = 2 * there <= (int64_t)c.seqs * p.tiles && there < 1 << 25 ? (int32_t)there : 0;
   const int64_t span = span_of(p.rows / q.group + 2);
   // two workgroups for every compute unit, as many as are resident and no more,
   // and none with fewer than eight steps (of a wave, of the workgroup): one costs
   // some 5 us beside its tokens, a join 4 and its launch (4 a unit instead of 2:
   // 16 sequences of 4000 tokens 27 and 23 us, one of 131073 47 and 38; one of
   // 1000 tokens whole 10, in four splits 12)
-  const int64_t heads = seqs * p.tiles, want = heads > 0 && 2ll * num_cus() > heads ? 2ll * num_cus() / heads : 1;
+  const int64_t heads = slots_of(c, p), want = heads > 0 && 2ll * num_cus() > heads ? 2ll * num_cus() / heads : 1;
   const int64_t least = p.rows == kRows ? 8 * kWaves * kStep : 8 * kBlockStep;
   int64_t chunk = (span + want - 1) / want;
   if (chunk < least) chunk = least;
@@ -1379,7 +1472,7 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
 int64_t kv4_workspace(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return 0;
   const Kv4Plan p = kv4_plan(c, dim, q, dtype);
-  return p.splits > 1 ? (int64_t)c.seqs * c.kv * p.tiles * p.splits * p.rows * (dim + 2) * 4 : 0;
+  return p.splits > 1 ? slots_of(c, p) * p.splits * p.rows * (dim + 2) * 4 : 0;
 }
 
 #define VQX_KV4_DIMS(CALL, T)  \
@@ -1404,7 +1497,7 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
   const Kv4Plan p = kv4_plan(c, dim, q, dtype);
   const bool extra = q.softcap != 0.0f || q.slopes;
   const bool whole = !c.table || c.size % (p.rows == kRows ? kStep : kBlockStep) == 0;
-  const int64_t slots = (int64_t)p.tiles * c.seqs * c.kv;
+  const int64_t slots = slots_of(c, p);
   if (slots * (p.splits > p.rows ? p.splits : p.rows) >= 1ll << 31)
     return set_error(kErrUnsupported, "kv4_attention: %lld tiles of %d splits do not fit a launch", (long long)slots,
                      p.splits);
@@ -1457,10 +1550,10 @@ int kv4_accumulate(const Kv4View& c, int dim, const Kv4Query& q, int dtype, cons
 #define VQX_KV4_WEIGH(D, T)                                                                                          \
   do {                                                                                                               \
     if (extra)                                                                                                       \
-      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, true>), grid, dim3(256), most * tile, st, c, q, (int)chunks, most,  \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, true>), grid, dim3(256), most * tile, st, c, q, most,  \
                          lse, weights, weights_len);                                                                 \
     else                                                                                                             \
-      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, false>), grid, dim3(256), most * tile, st, c, q, (int)chunks, most, \
+      hipLaunchKernelGGL((kv4_weigh_kernel<D, T, false>), grid, dim3(256), most * tile, st, c, q, most, \
                          lse, weights, weights_len);                                                                 \
   } while (0)
   VQX_KV4_TYPES(VQX_KV4_WEIGH)
