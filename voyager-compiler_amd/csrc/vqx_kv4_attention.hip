@@ -1344,15 +1344,19 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
     for (int tile = 0; tile < batch; ++tile) {
       const float base = held[tile].lse[n];
       const int pos = token < tokens ? all.base + token : -1;
-      const int pos_first = __builtin_amdgcn_readfirstlane(pos), pos_last = __builtin_amdgcn_readlane(pos, 15);
+      // the last tile may be a part of one; rows before the sequence's beginning
+      // have negative places, so that a place does not tell
+      const bool part = (first + tile + 1) * kRows > all.rows;
+      const int pos_first = __builtin_amdgcn_readfirstlane(pos);
+      const int pos_last = part ? all.base + tokens - 1 : __builtin_amdgcn_readlane(pos, 15);
       const Curve curve = curve_of(q, (int)h * q.group + which);
       token += step_token, which += step_which;
       if (which >= q.group) which -= q.group, ++token;
       // a window that has passed these tokens, or rows that have not come to them
       if (q.window && pos_first - q.window >= t0 + weigh_tokens(D) - 1) continue;
-      if (pos_last >= pos_first && pos_last < t0) continue;
+      if (pos_last < t0) continue;
       const bool masked = valid != (kParts == 4 ? ~0ull : 0xFFFFFFFFull) || t0 + weigh_tokens(D) - 1 > pos_first ||
-                          (q.window && t0 <= pos_last - q.window) || pos_last < pos_first;
+                          (q.window && t0 <= pos_last - q.window) || part;
       float x[4 * kParts];
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
