@@ -23,9 +23,6 @@ namespace vqx {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 struct Bf16 {};
 struct F16 {};
@@ -744,33 +741,25 @@ constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 :
 // values of a step are turned into bf16 once, the values transposed, into LDS
 // (two buffers, one barrier a step), and read by all four waves.  Bound by the
 // vector instructions of the softmax (half of the time) beside the matrix ones
-// (28%): a prompt of 8192 tokens, 32 heads over 8 of 128: 660 us, 833 TFLOP/s.
+// (28%): a prompt of 8192 tokens, 32 heads over 8 of 128: 727 us, 756 TFLOP/s.
 //
-// For bf16 outputs the second product, half of the matrix work, has the weights
-// as one term: fp16, off by 2^-12 of itself (one bf16 term, 2^-8, left outputs
-// off by 0.0022 of their norm, where their own rounding leaves 0.0016).  The
-// values are fp16 then too, relative to the largest scale that the workgroup
-// has met, 2^12 of it: exact for blocks down to 2^-35 of that scale, off by
-// 2^-37 of it below.  A step with a larger one scales the sums down, once or
-// twice in a sequence.  (Steps of other values taken as bf16 instead, in the same
-// kernel: 73 registers spilled, 598 -> 1012 us for a prompt of 8192 tokens.)
+// Weights of bf16 outputs are two bf16 terms here as in the other kernel, a
+// third of the matrix work more than one.  As one fp16 term, with the values as
+// fp16 relative to the largest scale that the workgroup had met, the same prompt
+// took 660 us; but values 2^36 below that scale came back as zeros, also where
+// it was another block's, or that of a token that the row does not see.
 template <int D, typename T, bool kExtra, bool kWhole>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out,
                                                                          float* lse, float* ws) {
   constexpr int kTiles = D / 16;
   constexpr int kVWords = Loaded<D>::kWords, kKWords = D / 32, kRow = D / 2, kScales = D / 32;
   constexpr int kKScales = D == 256 ? 2 : 1;  // of a thread's keys
-  constexpr bool kHalf = std::is_same<T, Bf16>::value;
-  constexpr int kP = kHalf ? 1 : Terms<T>::kP;
-  // weights are carried 2^7 times as large where they become fp16: below 2^15,
-  // and those that vanish are below 2^-32 of the reference's
-  constexpr float kLift = kHalf ? 7.0f : 0.0f;
+  constexpr int kP = Terms<T>::kP;
   constexpr int kSub = block_sub(D, Terms<T>::kQ), kBlockRows = 64 * kSub;
   // rows a 16-byte bank group off each other's
   __shared__ __align__(16) uint16_t kt[2][kBlockStep][D + 8];
   __shared__ __align__(16) uint16_t vt[2][D][kBlockStep + 8];
   __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block of values
-  __shared__ uint32_t top_scale[2];  // the largest scale byte of steps so far, as of the last odd and even one
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Place place;
@@ -813,7 +802,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     for (int j = 0; j < kTiles; ++j) acc[y][j] = f32x4{0, 0, 0, 0};
   }
   if (tid < 2) nan_step[tid] = -1;
-  if (tid < 2) top_scale[tid] = 0;
 
   // Loads go round without a branch, so that each wait is for its own: a token
   // past the end is the last one, which no row counts.  Where pages hold whole
@@ -838,7 +826,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
       for (int i = 0; i < 4; ++i) p.v[i] = kv4_page(c, b, clamped(t0 + 4 * quad + i));
     }
   };
-  uint32_t k[kKWords], ks[kKScales], v[4][kVWords], vs[4], v_pages = 0xFu;
+  uint32_t k[kKWords], ks[kKScales], v[4][kVWords], vs[4], v_pages;
   auto take_keys = [&](const uint8_t* codes, const uint8_t* scales, uint32_t at, uint32_t scale_at) {
     if constexpr (D == 64) {
       const u32x2 a = *reinterpret_cast<const u32x2*>(codes + (at + 8 * k_part));
@@ -871,40 +859,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         load_values<D>(codes + (w * kRow + element / 2), v[i]);
         vs[i] = scales[w * kScales + element / 32];
       }
-      if (kHalf) v_pages = page < c.pages ? 0xFu : 0u;
+      v_pages = page < c.pages ? 0xFu : 0u;
       const int left = end - t0;
       const uint64_t there = left >= kBlockStep ? ~0ull : (left > 0 ? (1ull << left) - 1 : 0ull);
       return page < c.pages ? there : 0ull;
     } else {
       const uint64_t at = kv4_row(c, p.k, h, clamped(t0 + k_token));
       take_keys(c.codes + at * kRow, c.scales + at * kScales, 0u, 0u);
-      if (kHalf) v_pages = 0;
+      v_pages = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t v_at = c.plane_rows + kv4_row(c, p.v[i], h, clamped(t0 + 4 * quad + i));
         load_values<D>(c.codes + v_at * kRow + element / 2, v[i]);
         vs[i] = c.scales[v_at * kScales + element / 32];
-        if (kHalf) v_pages |= (uint32_t)(p.v[i] < c.pages) << i;
+        v_pages |= (uint32_t)(p.v[i] < c.pages) << i;
       }
       return __ballot(t0 + lane < end && p.all < c.pages);
     }
   };
-  // The scales of the step whose values were loaded last; a token without a page
-  // has none, it is somewhere else's.  known: the largest of the steps before.
-  auto meet_scales = [&](int step, uint32_t known) {
-    if constexpr (kHalf) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!(v_pages >> i & 1u)) vs[i] = 0;
-        top = umax32(top, vs[i] == 255 ? 0u : vs[i]);
-      }
-      if (top > known) atomicMax(&top_scale[step & 1], top);  // a maximum: no order in it
-    }
-  };
   // A step's place in LDS: a lane of the second product takes tokens
   // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
-  auto store = [&](int step, uint32_t top) {
+  auto store = [&](int step) {
     uint16_t* kto = &kt[step & 1][k_token][k_part * (D / 4)];
 #pragma unroll
     for (int i = 0; i < kKWords; ++i) {
@@ -915,23 +890,23 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     uint16_t* to = &vt[step & 1][element][32 * (quad >> 3) + 8 * (quad & 3) + 4 * (quad >> 2 & 1)];
     constexpr int kNext = kBlockStep + 8;
     float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // a token without a page has none, it is somewhere else's
+      if (!(v_pages >> i & 1u)) vs[i] = 0;
     if (umax32(umax32(vs[0], vs[1]), umax32(vs[2], vs[3])) == 255) {
       nan_step[step & 1] = step;
 #pragma unroll
       for (int i = 0; i < 4; ++i) vs[i] = vs[i] == 255 ? 0u : vs[i];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // 2^(scale - top + 12), 2^-100 where that is all there is
-      f[i] = kHalf ? u2f((vs[i] + 139u > top + 27u ? vs[i] + 139u - top : 27u) << 23) : u2f(vs[i] << 23);
+    for (int i = 0; i < 4; ++i) f[i] = u2f(vs[i] << 23);
 #pragma unroll
     for (int w = 0; w < kVWords; ++w) {
       auto pair = [&](auto which) {
         constexpr int kByte = decltype(which)::value;
         uint32_t x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = kHalf ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v[i][w], f[i], kByte))
-                      : fp4_pair<kByte>(v[i][w], f[i]);
+        for (int i = 0; i < 4; ++i) x[i] = fp4_pair<kByte>(v[i][w], f[i]);
         const u32x2 even = {__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
         const u32x2 odd = {__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
         *reinterpret_cast<u32x2*>(to + (8 * w + 2 * kByte) * kNext) = even;
@@ -1020,37 +995,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 #pragma unroll
     for (int y = 0; y < kSub; ++y) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[y][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[y][j], scale, kLift - m[y]));
+      for (int j = 0; j < 8; ++j) x[y][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[y][j], scale, -m[y]));
       l[y] += ((x[y][0] + x[y][1]) + (x[y][2] + x[y][3])) + ((x[y][4] + x[y][5]) + (x[y][6] + x[y][7]));
     }
   };
   auto gather = [&](int step, int half, float (&x)[kSub][8]) {
     u32x4 p[kSub][kP];
 #pragma unroll
-    for (int y = 0; y < kSub; ++y) {
-      if constexpr (kHalf) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x2 two = {x[y][2 * j], x[y][2 * j + 1]};
-          p[y][0][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, f16x2));
-        }
-      } else {
-        split_terms(x[y], p[y]);
-      }
-    }
+    for (int y = 0; y < kSub; ++y) split_terms(x[y], p[y]);
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(&vt[step & 1][16 * j + n][32 * half + 8 * g]);
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(&vt[step & 1][16 * j + n][32 * half + 8 * g]);
 #pragma unroll
       for (int t = 0; t < kP; ++t)
 #pragma unroll
         for (int y = 0; y < kSub; ++y)
-          if constexpr (kHalf)
-            acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                               __builtin_bit_cast(f16x8, p[y][t]), acc[y][j], 0, 0, 0);
-          else
-            acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                                __builtin_bit_cast(bf16x8, p[y][t]), acc[y][j], 0, 0, 0);
+          acc[y][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, p[y][t]), acc[y][j], 0, 0, 0);
     }
   };
   // the blocks of values that were taken as tiny, for the rows that see them
@@ -1086,29 +1046,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     weights(x1);
     gather(step, 1, x1);
   };
-  auto read_top = [&](int step, uint32_t known) {
-    return umax32(known, (uint32_t)__builtin_amdgcn_readfirstlane((int)top_scale[step & 1]));
-  };
   if (steps > 0) {
     Pages next, later;  // of the step whose loads come next and of the one after
     pages_of(0, next);
     pages_of(1, later);
     uint64_t valid = load(0, next), valid_next;
     __syncthreads();
-    meet_scales(0, 0);
-    __syncthreads();
-    uint32_t top = read_top(0, 0);
-    store(0, top);
+    store(0);
     next = later;
     valid_next = load(1, next);
     pages_of(2, next);
-    meet_scales(1, top);
     for (int step = 0; step < steps; ++step) {
       const int t0 = begin + step * kBlockStep;
       __syncthreads();
       const bool nan = nan_step[step & 1] == step;
-      const uint32_t top_next = read_top(step + 1, top);
-      store(step + 1, top_next);
+      store(step + 1);
       const uint64_t valid_later = load(step + 2, next);
       pages_of(step + 3, next);
       if (t0 < mine.hi && t0 + kBlockStep > mine.lo) {
@@ -1116,24 +1068,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         if (nan) note_nan(valid, t0);
       }
       valid = valid_next, valid_next = valid_later;
-      if (kHalf && top_next != top) {
-        // the next step's values are relative to a larger scale
-        const float f = top_next - top < 126u ? u2f((127u - (top_next - top)) << 23) : 0.0f;
-#pragma unroll
-        for (int y = 0; y < kSub; ++y)
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) acc[y][j] *= f;
-        top = top_next;
-      }
-      meet_scales(step + 2, top);
-    }
-    if (kHalf) {
-      // the sums are relative to 2^(top - 127 + 12) and lifted as the weights' sum
-      const float f = exp2i((int)top - 139 < -126 ? -126 : (int)top - 139);
-#pragma unroll
-      for (int y = 0; y < kSub; ++y)
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) acc[y][j] *= f;
     }
   }
 
@@ -1152,11 +1086,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
       const int r = row[y] - tile * kBlockRows;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) *reinterpret_cast<f32x4*>(o + r * D + 16 * j + 4 * g) = acc[y][j];
-      if (g == 0) o[kBlockRows * D + r] = m[y] - kLift, o[kBlockRows * D + kBlockRows + r] = l[y];
+      if (g == 0) o[kBlockRows * D + r] = m[y], o[kBlockRows * D + kBlockRows + r] = l[y];
       continue;
     }
     const int64_t at = (int64_t)(rows.first + row[y] / q.group) * q.heads + (int64_t)h * q.group + row[y] % q.group;
-    if (g == 0) lse[at] = l[y] == 0.0f ? -__builtin_huge_valf() : (m[y] - kLift + __builtin_amdgcn_logf(l[y])) * kLn2;
+    if (g == 0) lse[at] = l[y] == 0.0f ? -__builtin_huge_valf() : (m[y] + __builtin_amdgcn_logf(l[y])) * kLn2;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) put4(out, at * D + 16 * j + 4 * g, acc[y][j], T());
   }
