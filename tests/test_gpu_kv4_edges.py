@@ -68,3 +68,68 @@ def test_values_of_the_smallest_size(ops, many):
     # all of one sign: the output's half step, the weights' 2^-8 at most, and
     # the spacing of bf16 below its normal range
     near(out, want, 2.0 ** -7 * want + 2.0 ** -133, "out")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("many", [False, True])
+def test_tokens_without_a_page_over_any_bytes(ops, kind, dim, page, many):
+    """The first row of the cache, which stands in for a token without a page,
+    holds values past every type's range: nothing of it is seen."""
+    codes, scales, table = make_cache(2, 1, dim, 160, page)
+    codes, scales = (torch.cat([x[:, :1], x], 1) for x in (codes, scales))
+    table = table + 1
+    codes[:, 0], scales[:, 0] = 0xFF, 254
+    table[0, 1], table[1, 0], table[1, -1] = -1, codes.shape[1], 2 ** 31 - 1
+    new = 20 if many else 1
+    if many:
+        codes, scales, table = widened(codes, scales, table, 2 * -(-new * 3 // 16))
+    q = torch.randn(2 * new, 3, dim, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    check_attention(ops, kind, q, codes, scales, torch.tensor([160, 150], dtype=torch.int32), table=table)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("byte,code", [(253, 6), (254, 4), (254, 15)])
+def test_values_past_the_range_in_masked_places(ops, kind, dim, page, many, byte, code):
+    """Values of 2^128 and of -1.5 * 2^129: rows that do not see them are as they
+    were; rows that do have their share of them, where the type holds it."""
+    new, lens = 30, torch.tensor([130, 96], dtype=torch.int32)
+    codes, scales, table = make_cache(2, 1, dim, 160, page)
+    if many:
+        codes, scales, table = widened(codes, scales, table, 2 * -(-new * 3 // 16))
+    q = torch.randn(2 * new, 3, dim, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    d = on(q, codes, scales, lens, table)
+    before, _ = ops.kv4_attention(d[0], d[1], d[2], d[3], None, None, d[4])
+    value_byte(codes, scales, table, 0, 125, byte, code=code)
+    dc, ds = on(codes, scales)
+    out, lse = ops.kv4_attention(d[0], dc, ds, d[3], None, None, d[4])
+    sees = torch.zeros(2 * new, dtype=torch.bool)
+    sees[25:30] = True
+    assert torch.equal(out[~sees], before[~sees])
+    want = ref.attention(q, codes, scales, lens, None, table)[0][sees]
+    top = torch.finfo(TYPES[kind]).max
+    got, held = out[sees].cpu().double(), want.abs() < 0.99 * top
+    # one value outweighs all others: its own weight's error, the half step
+    off = (got - want).abs() / want.abs()
+    assert not got.isnan().any() and float(off[held].max() if held.any() else 0.0) <= 2.0 ** -7
+    past = want.abs() > 1.01 * top
+    assert bool(got[past].isinf().all()) and torch.equal(got[past].sign(), want[past].sign())
+    assert held.any() or kind == "f16"
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("new,length", [(1, 40), (1, 9000), (40, 200), (300, 900)])
+def test_a_mean_of_the_largest_values(ops, kind, new, length):
+    """Values of 2^127 each: their sum is past the range, their mean is not."""
+    codes, scales, table = make_cache(1, 2, 128, length, 64)
+    codes[1], scales[1] = 0x44, 253
+    q = torch.randn(new, 8, 128, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    d = on(q, codes, scales, torch.tensor([length], dtype=torch.int32), table)
+    out, _ = ops.kv4_attention(d[0], d[1], d[2], d[3], None, None, d[4])
+    want = torch.full(out.shape, 2.0 ** 127, dtype=torch.float64)
+    # weights and their sum, each off by its terms and by fp32's sums
+    near(out, want, (torch.finfo(TYPES[kind]).eps / 2 + (2.0 ** -16 if kind == "bf16" else 0) + 2.0 ** -19) * want, "out")

@@ -50,6 +50,17 @@ constexpr float kLowest = -3.0e38f;  // below every finite score, and finite: no
 // A row's reference stays until a score passes it by this (in powers of two):
 // the weights then stay below 2^8, and the sums are rescaled a few times only.
 constexpr float kSlack = 8.0f;
+// Values in blocks with a scale byte from here on, 2^88 and up, are taken, as all
+// that are summed with them, 2^-40 times as large: the largest codes times the
+// largest scales are then within bf16, no weight of 0 meets an infinity, and
+// 2^30 weights of 2^8 keep their sums within fp32 (so they do below 2^88).
+// Blocks below 2^-87 beside such ones count as 2^-87.
+constexpr uint32_t kLargeScale = 215, kDown = 40;
+constexpr float kDownFactor = 0x1p-40f, kUpFactor = 0x1p40f;
+// A scale byte's bits, `down` powers of two lower.
+__device__ __forceinline__ float scale_bits(uint32_t byte, uint32_t down) {
+  return u2f(__builtin_elementwise_sub_sat(byte, down) << 23);
+}
 
 // 8 values from element i of p as bf16 terms, their sum the value.
 __device__ __forceinline__ void load_terms(const void* p, int64_t i, Bf16, u32x4 (&t)[1]) {
@@ -116,7 +127,7 @@ struct QueryTerms {
 
 // How a call is cut up.  A tile is `rows` query rows of one kv head (row r is
 // new token r / group, head r % group); each split of a tile's tokens leaves
-// its sums in the workspace: rows * D outputs, rows references and rows sums.
+// its results in the workspace: rows * D outputs, rows references and rows sums.
 struct Kv4Plan {
   int32_t rows, tiles, chunk, splits;
   int32_t listed;  // tiles of a kv head that the workgroups are handed one by one; 0: tiles of every sequence
@@ -506,6 +517,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
   __shared__ __align__(16) float part[2][kRows][kPad];
   __shared__ float part_m[2][kRows], part_l[2][kRows];
   __shared__ uint32_t part_bad[2][kRows];
+  __shared__ int part_down[2];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Place place;
@@ -529,6 +541,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
 
   float m = kLowest, l = 0.0f;
   uint32_t bad = 0;  // blocks of values that are NaN in a token the row sees
+  bool down = false;  // the wave's outputs are 2^-kDown of themselves
   f32x4 acc[kTiles];
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) acc[j] = f32x4{0, 0, 0, 0};
@@ -565,7 +578,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
       u32x4 p[Terms<T>::kP];
       split_terms(x, p);
       // this lane's block of each token's scales
-      float vs[8];
+      uint32_t vs[8];
       const uint32_t block = (uint32_t)n * (D / 16) / 32;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -576,14 +589,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
           w = s.vs[j >> 2][j & 3];
         else
           w = block >= 4 ? s.vs[j >> 2][2 * (j & 3) + 1] : s.vs[j >> 2][2 * (j & 3)];
-        vs[j] = u2f((w >> (8 * (block & 3)) & 0xFFu) << 23);
+        vs[j] = w >> (8 * (block & 3)) & 0xFFu;
       }
-      float most = vs[0];
+      uint32_t most = vs[0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) most = __builtin_fmaxf(most, vs[j]);
-      if (__ballot(most == __builtin_huge_valf())) {
-        // byte 255: a weight of 0 must not meet a NaN.  The value is taken as
-        // tiny, and the rows that see the token note its blocks.
+      for (int j = 1; j < 8; ++j) most = umax32(most, vs[j]);
+      if (__ballot(most >= kLargeScale)) {
+        // 255: a weight of 0 must not meet a NaN.  The value is taken as tiny, and
+        // the rows that see the token note its blocks.  A token that is not there
+        // has the scales of another one, or of none.
+        most = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint32_t nan = 0;
@@ -593,9 +608,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
             nan |= (uint32_t)((s.vs[j >> 2][byte >> 2] >> (8 * (byte & 3)) & 0xFFu) == 255u) << k;
           }
           if (seen >> j & 1u) bad |= nan;
-          if (vs[j] == __builtin_huge_valf()) vs[j] = 0.0f;
+          if (vs[j] == 255u || !(s.valid >> ((j >> 2) * 16 + 4 * g + (j & 3)) & 1u)) vs[j] = 0;
+          most = umax32(most, vs[j]);
+        }
+        if (!down && __ballot(most >= kLargeScale)) {
+          down = true;
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) acc[j] *= kDownFactor;
         }
       }
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = scale_bits(vs[j], down ? kDown : 0u);
 #pragma unroll
       for (int w = 0; w < Loaded<D>::kWords; ++w) {
         // byte by byte: two elements of two tokens in one word each, then the
@@ -605,8 +629,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
           u32x4 even, odd;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t x0 = fp4_pair<kByte>(s.v[2 * j][w], vs[2 * j]),
-                           x1 = fp4_pair<kByte>(s.v[2 * j + 1][w], vs[2 * j + 1]);
+            const uint32_t x0 = fp4_pair<kByte>(s.v[2 * j][w], f[2 * j]),
+                           x1 = fp4_pair<kByte>(s.v[2 * j + 1][w], f[2 * j + 1]);
             even[j] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
             odd[j] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
           }
@@ -681,6 +705,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
           *reinterpret_cast<f32x4*>(&part[z][n][g * kPer + i * kTiles + j]) =
               f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
       if (g == 0) part_m[z][n] = m, part_l[z][n] = l, part_bad[z][n] = bad;
+      if (lane == 0) part_down[z] = down;
     }
     __syncthreads();
     if (wave < half) {
@@ -689,25 +714,28 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
       m = top;
       l = l * f0 + part_l[wave][n] * f1;
       bad |= part_bad[wave][n];
+      const bool down1 = part_down[wave] != 0;
+      const float a0 = down1 && !down ? f0 * kDownFactor : f0, a1 = down && !down1 ? f1 * kDownFactor : f1;
+      down = down || down1;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < kTiles; j += 4) {
           const f32x4 o = *reinterpret_cast<const f32x4*>(&part[wave][n][g * kPer + i * kTiles + j]);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) acc[j + x][i] = acc[j + x][i] * f0 + o[x] * f1;
+          for (int x = 0; x < 4; ++x) acc[j + x][i] = acc[j + x][i] * a0 + o[x] * a1;
         }
     }
     __syncthreads();
   }
   if (wave != 0) return;
-  const float inv = plan.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l, up = down ? kUpFactor : 1.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
       const uint32_t block = (uint32_t)(g * kPer + i * kTiles + j) / 32;
-      acc[j][i] = bad >> block & 1u ? __builtin_nanf("") : acc[j][i] * inv;
+      acc[j][i] = bad >> block & 1u ? __builtin_nanf("") : acc[j][i] * inv * up;
     }
   if (plan.splits > 1) {
     float* o = ws + place.at * (kRows * D + 2 * kRows);
@@ -741,7 +769,7 @@ constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 :
 // values of a step are turned into bf16 once, the values transposed, into LDS
 // (two buffers, one barrier a step), and read by all four waves.  Bound by the
 // vector instructions of the softmax (half of the time) beside the matrix ones
-// (28%): a prompt of 8192 tokens, 32 heads over 8 of 128: 727 us, 756 TFLOP/s.
+// (28%): a prompt of 8192 tokens, 32 heads over 8 of 128: 737 us, 746 TFLOP/s.
 //
 // Weights of bf16 outputs are two bf16 terms here as in the other kernel, a
 // third of the matrix work more than one.  As one fp16 term, with the values as
@@ -759,7 +787,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   // rows a 16-byte bank group off each other's
   __shared__ __align__(16) uint16_t kt[2][kBlockStep][D + 8];
   __shared__ __align__(16) uint16_t vt[2][D][kBlockStep + 8];
-  __shared__ int nan_step[2];  // of the buffer's step if it has a NaN block of values
+  // the last even and odd step with a NaN block of values, and with a large one
+  __shared__ int notes[2][2];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Place place;
@@ -801,7 +830,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) acc[y][j] = f32x4{0, 0, 0, 0};
   }
-  if (tid < 2) nan_step[tid] = -1;
+  uint32_t down = 0;  // kDown: values and outputs are 2^-kDown of themselves
+  if (tid < 4) notes[tid >> 1][tid & 1] = -1;
 
   // Loads go round without a branch, so that each wait is for its own: a token
   // past the end is the last one, which no row counts.  Where pages hold whole
@@ -877,6 +907,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
       return __ballot(t0 + lane < end && p.all < c.pages);
     }
   };
+  // The scales of the step whose values were loaded last.
+  auto note_scales = [&](int step) {
+    if (umax32(umax32(vs[0], vs[1]), umax32(vs[2], vs[3])) < kLargeScale) return;
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!(v_pages >> i & 1u)) vs[i] = 0;  // a token without a page has another's scales, or none's
+      if (vs[i] == 255) notes[step & 1][0] = step, vs[i] = 0;
+      most = umax32(most, vs[i]);
+    }
+    if (most >= kLargeScale) notes[step & 1][1] = step;
+  };
   // A step's place in LDS: a lane of the second product takes tokens
   // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
   auto store = [&](int step) {
@@ -891,15 +933,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     constexpr int kNext = kBlockStep + 8;
     float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // a token without a page has none, it is somewhere else's
-      if (!(v_pages >> i & 1u)) vs[i] = 0;
-    if (umax32(umax32(vs[0], vs[1]), umax32(vs[2], vs[3])) == 255) {
-      nan_step[step & 1] = step;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vs[i] = vs[i] == 255 ? 0u : vs[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = u2f(vs[i] << 23);
+    for (int i = 0; i < 4; ++i) f[i] = scale_bits(vs[i], down);
 #pragma unroll
     for (int w = 0; w < kVWords; ++w) {
       auto pair = [&](auto which) {
@@ -1046,20 +1080,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     weights(x1);
     gather(step, 1, x1);
   };
+  // Noted in the iteration before the step's store, read in the one of the store.
+  auto noted = [&](int step, int what) { return __builtin_amdgcn_readfirstlane(notes[step & 1][what]) == step; };
   if (steps > 0) {
     Pages next, later;  // of the step whose loads come next and of the one after
     pages_of(0, next);
     pages_of(1, later);
     uint64_t valid = load(0, next), valid_next;
     __syncthreads();
+    note_scales(0);
+    __syncthreads();
+    bool nan = noted(0, 0);
+    if (noted(0, 1)) down = kDown;
     store(0);
     next = later;
     valid_next = load(1, next);
     pages_of(2, next);
+    note_scales(1);
     for (int step = 0; step < steps; ++step) {
       const int t0 = begin + step * kBlockStep;
       __syncthreads();
-      const bool nan = nan_step[step & 1] == step;
+      const bool nan_next = noted(step + 1, 0), lower = down == 0 && noted(step + 1, 1);
+      if (lower) down = kDown;
       store(step + 1);
       const uint64_t valid_later = load(step + 2, next);
       pages_of(step + 3, next);
@@ -1067,7 +1109,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
         work(step, valid);
         if (nan) note_nan(valid, t0);
       }
-      valid = valid_next, valid_next = valid_later;
+      valid = valid_next, valid_next = valid_later, nan = nan_next;
+      if (lower) {
+#pragma unroll
+        for (int y = 0; y < kSub; ++y)
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) acc[y][j] *= kDownFactor;
+      }
+      note_scales(step + 2);
     }
   }
 
@@ -1078,9 +1127,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     bad[y] |= (uint32_t)__shfl_xor((int)bad[y], 16);
     bad[y] |= (uint32_t)__shfl_xor((int)bad[y], 32);
     if (row[y] >= rows.rows) continue;
-    const float inv = plan.splits > 1 ? 1.0f : (l[y] == 0.0f ? 0.0f : 1.0f / l[y]);
+    const float inv = l[y] == 0.0f ? 0.0f : 1.0f / l[y], up = down ? kUpFactor : 1.0f;
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) acc[y][j] = bad[y] >> (j / 2) & 1u ? acc[y][j] * __builtin_nanf("") : acc[y][j] * inv;
+    for (int j = 0; j < kTiles; ++j)
+      acc[y][j] = bad[y] >> (j / 2) & 1u ? acc[y][j] * __builtin_nanf("") : acc[y][j] * inv * up;
     if (plan.splits > 1) {
       float* o = ws + place.at * (kBlockRows * D + 2 * kBlockRows);
       const int r = row[y] - tile * kBlockRows;
@@ -1106,7 +1156,7 @@ template <int D, typename T, int kShare>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out, float* lse,
                                                        const float* ws) {
   constexpr int kPer = D / 64;
-  __shared__ float sum[kWaves][D], sum_l[kWaves];
+  __shared__ float sum[kWaves][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t id = kShare == 1 ? blockIdx.x * kWaves + wave : blockIdx.x;
   const uint32_t slot = id / (uint32_t)plan.rows;
@@ -1138,10 +1188,18 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
     }
   };
   fetch(first);
-  float m = kLowest;
-  for (int s = lane; s < splits; s += 64) m = __builtin_fmaxf(m, m_n[s * size]);
+  float m = kLowest, l = 0.0f;
+  for (int s = lane; s < splits; s += 64) {
+    const float m1 = m_n[s * size], top = __builtin_fmaxf(m, m1);
+    l = l * __builtin_amdgcn_exp2f(m - top) + m_n[s * size + plan.rows] * __builtin_amdgcn_exp2f(m1 - top);
+    m = top;
+  }
+  const float mine = m;
   for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
-  float l = 0.0f, o[kPer];
+  l *= __builtin_amdgcn_exp2f(mine - m);
+  for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  float o[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
   for (int s = first; s < splits; s += kAhead * kShare) {
@@ -1149,8 +1207,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       if (s + a * kShare >= splits) break;
-      const float f = __builtin_amdgcn_exp2f(part_m[a] - m);
-      l += part_l[a] * f;
+      const float f = part_l[a] * __builtin_amdgcn_exp2f(part_m[a] - m) * inv;  // a split's share
 #pragma unroll
       for (int k = 0; k < kPer; ++k) o[k] += part[a][k] * f;
     }
@@ -1158,10 +1215,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   if constexpr (kShare > 1) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) sum[wave][lane * kPer + k] = o[k];
-    if (lane == 0) sum_l[wave] = l;
     __syncthreads();
     if (wave != 0) return;
-    l = (sum_l[0] + sum_l[1]) + (sum_l[2] + sum_l[3]);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int d = lane * kPer + k;
@@ -1170,9 +1225,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   }
   const int64_t row = (int64_t)(rows.first + r / q.group) * q.heads + (int)h * q.group + r % q.group;
   if (lane == 0) lse[row] = l == 0.0f ? -__builtin_huge_valf() : (m + __builtin_amdgcn_logf(l)) * kLn2;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) put(out, row * D + lane * kPer + k, o[k] * inv, T());
+  for (int k = 0; k < kPer; ++k) put(out, row * D + lane * kPer + k, o[k], T());
 }
 
 // Tokens of a wave that weighs.
