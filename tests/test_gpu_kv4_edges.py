@@ -133,3 +133,20 @@ def test_a_mean_of_the_largest_values(ops, kind, new, length):
     want = torch.full(out.shape, 2.0 ** 127, dtype=torch.float64)
     # weights and their sum, each off by its terms and by fp32's sums
     near(out, want, (torch.finfo(TYPES[kind]).eps / 2 + (2.0 ** -16 if kind == "bf16" else 0) + 2.0 ** -19) * want, "out")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 2.0 ** -110, -2.0 ** -110])
+def test_scales_of_next_to_nothing(ops, kind, many, scale):
+    """Keys of 2^105: a scale of 0 makes every score 0, one of 2^-110 makes
+    ordinary scores of them."""
+    codes, scales, table = make_cache(2, 1, 128, 100, 16)
+    scales[0] += 105
+    if many:
+        codes, scales, table = widened(codes, scales, table, 2 * 8)
+    new = 40 if many else 1
+    q = torch.randn(2 * new, 3, 128, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    lens = torch.tensor([100, 77], dtype=torch.int32)
+    check_attention(ops, kind, q, codes, scales, lens, table=table, scale=scale)
+    check_attention(ops, kind, q, codes, scales, lens, table=table, scale=scale, softcap=3.0)

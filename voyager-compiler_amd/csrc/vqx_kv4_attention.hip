@@ -100,11 +100,11 @@ __device__ __forceinline__ int key_element(int i, int g) {
 }
 
 // 8 elements of a row's query from element i as the B operand's terms, a
-// negative scale's sign included.
+// negative scale's sign included; zeros where the scale is 0.
 template <typename T, int kTerms>
 __device__ __forceinline__ void load_query(const Kv4Query& q, int64_t i, bool live, T, u32x4 (&t)[kTerms]) {
   const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u;
-  if (live) {
+  if (live && q.scale != 0.0f) {
     load_terms(q.q, i, T(), t);
 #pragma unroll
     for (int k = 0; k < kTerms; ++k) t[k] ^= flip;
@@ -231,8 +231,8 @@ struct Curve {
 
 __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   Curve k;
-  // not 0: a masked score, -inf, stays one
-  k.scale = __builtin_fmaxf(__builtin_fabsf(q.scale) * kLog2e, 1e-30f);
+  // not 0: a masked score, -inf, stays one (the queries are 0 where the scale is)
+  k.scale = __builtin_fmaxf(__builtin_fabsf(q.scale) * kLog2e, 0x1p-126f);
   k.capped = q.softcap != 0.0f;
   k.inner = k.capped ? __builtin_fabsf(q.scale) / q.softcap : 0.0f;
   k.outer = q.softcap * kLog2e;
