@@ -1,0 +1,53 @@
+"""What the host side of the 4-bit cache's operators hands to the library, with
+the library replaced by a stand-in: no GPU needed."""
+
+import weakref
+
+import pytest
+import torch
+
+from tests.test_kv4_checks import cache_args, kv4  # noqa: F401
+
+
+class Codes(torch.Tensor):
+    """Notes the memory that is allocated like it."""
+    made = []
+
+    def new_empty(self, *args, **kwargs):
+        t = torch.empty(*args, dtype=torch.uint8)
+        Codes.made.append((t.data_ptr(), weakref.ref(t)))
+        return t
+
+
+@pytest.fixture
+def library(kv4, monkeypatch):  # noqa: F811
+    """Records of (entry point, whether its workspace is still held)."""
+    calls = []
+    Codes.made.clear()
+
+    def call(name, *args):
+        if name.endswith("workspace_size"):
+            args[-1].value = 4096
+        else:
+            held = {at: ref() is not None for at, ref in Codes.made}
+            calls.append((name, args[-2], held.get(args[-3])))
+
+    monkeypatch.setattr(kv4._lib, "call", call)
+    monkeypatch.setattr(kv4._lib, "require_device", lambda *a: None)
+    monkeypatch.setattr(kv4._lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(kv4, "_workspace_bytes", lambda *a: 4096)
+    return calls
+
+
+def test_attention_holds_its_workspace(kv4, library):  # noqa: F811
+    codes, scales, lengths, table = cache_args()
+    kv4.kv4_attention(torch.zeros(2, 4, 128), codes.as_subclass(Codes), scales, lengths, table=table)
+    assert library == [("vqx_kv4_attention", 4096, True)]
+
+
+def test_evict_holds_its_workspace(kv4, library):  # noqa: F811
+    codes, scales, lengths, table = cache_args()
+    out = cache_args()
+    kv4.kv4_evict(codes.as_subclass(Codes), scales, torch.zeros(2, 2, 32), lengths, 8, 2, out[0], out[1],
+                  torch.zeros(2, 2, 8), table, out[3])
+    assert library == [("vqx_kv4_evict", 4096, True)]

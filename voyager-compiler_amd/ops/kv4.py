@@ -251,8 +251,8 @@ def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None,
     out = q.new_empty(q.shape)
     lse = q.new_empty(key[:2], dtype=torch.float32)
     need = _workspace_bytes(c, qs, device, key)
-    ws = codes.new_empty(need).data_ptr() if need else None
-    _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), ws, need, _lib.stream_of(codes))
+    ws = codes.new_empty(need) if need else None  # held until the kernels that use it are enqueued
+    _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), need, _lib.stream_of(codes))
     return out, lse
 
 
@@ -299,8 +299,8 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
     need = ctypes.c_int64(0)
     _lib.call("vqx_kv4_evict_workspace_size", c, weights.shape[2], need)
     need = need.value
-    ws = codes.new_empty(need).data_ptr() if need else None
-    _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow, ws, need,
+    ws = codes.new_empty(need) if need else None  # held until the kernels that use it are enqueued
+    _lib.call("vqx_kv4_evict", c, w, weights.shape[2], budget, recent, o, index.data_ptr(), ow, _lib.ptr(ws), need,
               _lib.stream_of(codes))
     return index, kept
 
