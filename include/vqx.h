@@ -760,7 +760,8 @@ int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, c
  * [seqs, kv_heads, weights_len]; lengths past weights_len count as that; equal
  * weights by the lower place, NaN above all), in their order, moved to the
  * front of `out`, another cache with as many sequences and kv heads and room
- * for budget tokens each (neither it nor out_weights may overlap the inputs).  index: int32 [seqs, kv_heads, budget], where each
+ * for budget tokens each (neither it, its lengths among that, nor out_weights
+ * may overlap the inputs).  index: int32 [seqs, kv_heads, budget], where each
  * kept token was, -1 past the end; out->lengths: their number; out_weights:
  * fp32 [seqs, kv_heads, budget], their weights, 0 past the end.  workspace:
  * vqx_kv4_evict_workspace_size bytes for the same cache and weights_len, 16-byte

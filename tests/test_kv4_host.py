@@ -51,3 +51,18 @@ def test_evict_holds_its_workspace(kv4, library):  # noqa: F811
     kv4.kv4_evict(codes.as_subclass(Codes), scales, torch.zeros(2, 2, 32), lengths, 8, 2, out[0], out[1],
                   torch.zeros(2, 2, 8), table, out[3])
     assert library == [("vqx_kv4_evict", 4096, True)]
+
+
+def test_library_evict_refuses_lengths_over_its_input(vqx):
+    """The first head of a sequence writes its new length, the others read the
+    old one: the same place for both would give each head another selection."""
+    L = vqx._lib
+    base, seqs = 1 << 20, 2
+
+    def cache(at, lengths):
+        return L.VqxKv4Cache(codes=at, scales=at, table=base, lengths=lengths, pages=4, pages_per_seq=2, kv_heads=2,
+                             page_size=16, dim=128, seqs=seqs)
+
+    for new in (base, base + 4 * seqs - 4, base - 4 * seqs + 4):
+        with pytest.raises(ValueError, match="new lengths go to another tensor"):
+            L.call("vqx_kv4_evict", cache(base, base), base, 32, 8, 2, cache(base << 20, new), base, base << 21, None, 0, None)

@@ -744,6 +744,9 @@ int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weig
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return set_error(kErrInvalid, "kv4_evict: needs a 16-byte aligned workspace of %lld bytes, not %lld",
                      (long long)need, (long long)workspace_bytes);
+  // a sequence's heads read its length after the first of them has written the new one
+  if (overlap(c.lengths, (uint64_t)c.seqs * 4, o.lengths, (uint64_t)c.seqs * 4))
+    return set_error(kErrInvalid, "kv4_evict: the new lengths go to another tensor, not onto these");
   return kv4_evict(c, cache->dim, weights, weights_len, budget, recent, o, index, out->lengths, out_weights, workspace,
                    (hipStream_t)stream);
 }
