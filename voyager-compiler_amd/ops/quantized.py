@@ -1205,9 +1205,10 @@ def _dense_product(a, a_code, a_scale, b, b_code, b_scale, block_size, b_kdim, b
     out = torch.empty(nb, rows, N, dtype=torch.bfloat16, device=a.device)
     ws_bytes = _dense_workspace_bytes(nb, rows, N, Kp, a.device)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=a.device) if ws_bytes else None
+    bias = None if bias is None else bias.contiguous()
     _lib.call("vqx_dense_matmul", _lib.ptr(ad), Kp, 0 if a_shared or nb == 1 else rows * Kp, _lib.ptr(bd), Kp,
-              0 if b_shared else N * Kp, None if bias is None else _lib.ptr(bias.contiguous()), _lib.ptr(out), nb, rows,
-              N, Kp, _lib.ptr(ws), ws_bytes, _lib.stream_of(a))
+              0 if b_shared else N * Kp, _lib.ptr(bias), _lib.ptr(out), nb, rows, N, Kp, _lib.ptr(ws), ws_bytes,
+              _lib.stream_of(a))
     return out.reshape(*batch_shape, M, N)
 
 
@@ -1872,9 +1873,9 @@ def dequantize_mx_packed(codes, scale, dtype, block_size, shape, out_dtype=torch
         raise ValueError(f"scale dtype {scale.dtype} not in float32/bfloat16/uint8(E8M0)")
     dtab = fmt.tables(codes.device)["decode"]
     out = torch.empty(list(shape), dtype=out_dtype, device=codes.device)
-    _lib.call("vqx_mx_decode", _lib.ptr(codes.contiguous()), fmt.code_bits, _lib.ptr(dtab), dtab.numel(),
-              _lib.ptr(scale.contiguous()), kind, n, block_size, _lib.ptr(out), _lib.dtype_tag(out_dtype),
-              _lib.stream_of(codes))
+    codes, scale = codes.contiguous(), scale.contiguous()  # copies that live until the kernel is enqueued
+    _lib.call("vqx_mx_decode", _lib.ptr(codes), fmt.code_bits, _lib.ptr(dtab), dtab.numel(), _lib.ptr(scale), kind,
+              n, block_size, _lib.ptr(out), _lib.dtype_tag(out_dtype), _lib.stream_of(codes))
     return out
 
 
