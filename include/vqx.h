@@ -697,6 +697,7 @@ typedef struct vqx_kv4_cache {
  * with a window only those with t > p - window.  Its score of t is
  *   s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);
  *   slopes (fp32 [heads], or NULL): s -= slopes[x] (p - t).
+ * scale is finite, and scale / softcap too.
  */
 typedef struct vqx_kv4_query {
   const void* q;

@@ -66,3 +66,36 @@ def test_library_evict_refuses_lengths_over_its_input(vqx):
     for new in (base, base + 4 * seqs - 4, base - 4 * seqs + 4):
         with pytest.raises(ValueError, match="new lengths go to another tensor"):
             L.call("vqx_kv4_evict", cache(base, base), base, 32, 8, 2, cache(base << 20, new), base, base << 21, None, 0, None)
+
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.mark.parametrize("how,message", [
+    (dict(scale=NAN), "scale is finite"), (dict(scale=INF), "scale is finite"), (dict(scale=-INF), "scale is finite"),
+    (dict(scale=1e39), "scale is finite"), (dict(softcap=1e-46), "too small"), (dict(softcap=1e-39), "too small"),
+    (dict(scale=1e8, softcap=1e-35), "too small"), (dict(scale=-1e8, softcap=1e-35), "too small")])
+def test_scale_refusals(kv4, how, message):  # noqa: F811
+    args = cache_args()
+    d = dict(scale=None, softcap=0.0)
+    d.update(how)
+    with pytest.raises(ValueError, match=message):
+        kv4._query(torch.zeros(6, 4, 128), kv4._cache(*args, "x"), args[0].device, None, None, d["scale"], d["softcap"],
+                   0, None, "x")
+
+
+@pytest.mark.parametrize("scale,softcap,message", [
+    (NAN, 0.0, "not finite"), (INF, 0.0, "not finite"), (-INF, 30.0, "not finite"), (1.0, 1e-39, "too small"),
+    (-1e8, 1e-35, "too small")])
+def test_library_scale_refusals(vqx, scale, softcap, message):
+    L = vqx._lib
+    base, n = 1 << 20, L.ctypes.c_int64(-1)
+    cache = L.VqxKv4Cache(codes=base, scales=base, table=base, lengths=base, pages=4, pages_per_seq=2, kv_heads=2,
+                          page_size=16, dim=128, seqs=2)
+    q = L.VqxKv4Query(q=base, cu=None, slopes=None, n=2, stride_n=512, stride_h=128, dtype=1, heads=4, most=0, window=0,
+                      scale=scale, softcap=softcap)
+    with pytest.raises(ValueError, match=message):
+        L.call("vqx_kv4_attention_workspace_size", cache, q, n)
+    for scale, softcap in ((0.0, 30.0), (-3e38, 0.0), (-3e38, 3e38), (1e-30, 1e-37)):
+        q.scale, q.softcap = scale, softcap
+        L.call("vqx_kv4_attention_workspace_size", cache, q, n)

@@ -181,8 +181,14 @@ static int to_query(const Kv4View& c, int dim, const vqx_kv4_query* q, const cha
   if (q->n > 0 && !q->q) return set_error(kErrInvalid, "%s: null tensor", what);
   rc = kv4_strided(q->q, q->dtype, q->stride_n, q->stride_h, what);
   if (rc != kOk) return rc;
+  const float size = q->scale < 0.0f ? -q->scale : q->scale;
+  if (!(size <= 3.4028235e38f)) return set_error(kErrInvalid, "%s: the scale is not finite", what);
   if (!(q->softcap >= 0.0f) || q->softcap > 3.0e38f)
     return set_error(kErrInvalid, "%s: a softcap is positive, or 0 for none", what);
+  // scores are multiplied by their quotient
+  if (q->softcap != 0.0f && !(q->softcap >= 1.17549435e-38f && size / q->softcap <= 3.4028235e38f))
+    return set_error(kErrInvalid, "%s: a softcap of %g is too small for a scale of %g", what, (double)q->softcap,
+                     (double)q->scale);
   if (q->window < 0 || q->window >= 1 << 30)
     return set_error(kErrInvalid, "%s: a window is positive and below 2^30, or 0 for none", what);
   if (q->most < 0) return set_error(kErrInvalid, "%s: most is negative", what);

@@ -63,6 +63,9 @@ def _impl(name):
 _FLOATS = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
+_FP32_MAX, _FP32_TINY = torch.finfo(torch.float32).max, torch.finfo(torch.float32).tiny
+
+
 def _refuse(what, message):
     raise ValueError(f"vqx: {what}: {message}")
 
@@ -155,8 +158,13 @@ def _query(query, cache, device, cu, most, scale, softcap, window, slopes, what)
         most = n
     if not 0 <= window < 2 ** 30:
         _refuse(what, f"a window is positive and below 2^30, or 0 for none, not {window}")
+    scale = dim ** -0.5 if scale is None else scale
+    if not -_FP32_MAX <= scale <= _FP32_MAX:
+        _refuse(what, f"a scale is finite in float32, not {scale}")
     if not 0.0 <= softcap < math.inf:
         _refuse(what, f"a softcap is positive, or 0 for none, not {softcap}")
+    if softcap != 0.0 and not (_FP32_TINY <= softcap and abs(scale) <= _FP32_MAX * softcap):
+        _refuse(what, f"a softcap of {softcap} is too small for a scale of {scale} in float32")
     bias = None
     if slopes is not None:
         if slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous():
@@ -166,7 +174,7 @@ def _query(query, cache, device, cu, most, scale, softcap, window, slopes, what)
             _refuse(what, f"slopes are on {slopes.device}, the cache on {device}")
         bias = slopes.data_ptr()
     return (_lib.VqxKv4Query(q.data_ptr(), offsets, bias, n, sn, sh, tag, heads, most, window,
-                             dim ** -0.5 if scale is None else scale, softcap),
+                             scale, softcap),
             q, (n, heads, tag, most, window, cu is None))
 
 
