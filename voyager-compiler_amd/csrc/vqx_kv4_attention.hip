@@ -57,10 +57,6 @@ constexpr float kSlack = 8.0f;
 // Blocks below 2^-87 beside such ones count as 2^-87.
 constexpr uint32_t kLargeScale = 215, kDown = 40;
 constexpr float kDownFactor = 0x1p-40f, kUpFactor = 0x1p40f;
-// A scale byte's bits, `down` powers of two lower.
-__device__ __forceinline__ float scale_bits(uint32_t byte, uint32_t down) {
-  return u2f(__builtin_elementwise_sub_sat(byte, down) << 23);
-}
 
 // 8 values from element i of p as bf16 terms, their sum the value.
 __device__ __forceinline__ void load_terms(const void* p, int64_t i, Bf16, u32x4 (&t)[1]) {
@@ -103,11 +99,11 @@ __device__ __forceinline__ int key_element(int i, int g) {
 // negative scale's sign included; zeros where the scale is 0.
 template <typename T, int kTerms>
 __device__ __forceinline__ void load_query(const Kv4Query& q, int64_t i, bool live, T, u32x4 (&t)[kTerms]) {
-  const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u;
-  if (live && q.scale != 0.0f) {
+  const uint32_t flip = q.scale < 0.0f ? 0x80008000u : 0u, keep = q.scale == 0.0f ? 0u : ~0u;
+  if (live) {
     load_terms(q.q, i, T(), t);
 #pragma unroll
-    for (int k = 0; k < kTerms; ++k) t[k] ^= flip;
+    for (int k = 0; k < kTerms; ++k) t[k] = (t[k] & keep) ^ flip;
   } else {
 #pragma unroll
     for (int k = 0; k < kTerms; ++k) t[k] = u32x4{0, 0, 0, 0};
@@ -594,7 +590,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
       uint32_t most = vs[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) most = umax32(most, vs[j]);
-      if (__ballot(most >= kLargeScale)) {
+      if (__ballot(most >= kLargeScale) || down) {
         // 255: a weight of 0 must not meet a NaN.  The value is taken as tiny, and
         // the rows that see the token note its blocks.  A token that is not there
         // has the scales of another one, or of none.
@@ -616,10 +612,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) acc[j] *= kDownFactor;
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vs[j] = __builtin_elementwise_sub_sat(vs[j], down ? kDown : 0u);
       }
       float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = scale_bits(vs[j], down ? kDown : 0u);
+      for (int j = 0; j < 8; ++j) f[j] = u2f(vs[j] << 23);
 #pragma unroll
       for (int w = 0; w < Loaded<D>::kWords; ++w) {
         // byte by byte: two elements of two tokens in one word each, then the
@@ -921,7 +919,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   };
   // A step's place in LDS: a lane of the second product takes tokens
   // 4 g .. 4 g + 3 and 16 + 4 g .. of 32 as 16 bytes.
-  auto store = [&](int step) {
+  auto store_keys = [&](int step) {
     uint16_t* kto = &kt[step & 1][k_token][k_part * (D / 4)];
 #pragma unroll
     for (int i = 0; i < kKWords; ++i) {
@@ -929,11 +927,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
       *reinterpret_cast<u32x4*>(kto + 8 * i) =
           u32x4{fp4_pair<0>(k[i], f), fp4_pair<1>(k[i], f), fp4_pair<2>(k[i], f), fp4_pair<3>(k[i], f)};
     }
+  };
+  auto store_values = [&](int step) {
     uint16_t* to = &vt[step & 1][element][32 * (quad >> 3) + 8 * (quad & 3) + 4 * (quad >> 2 & 1)];
     constexpr int kNext = kBlockStep + 8;
     float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = scale_bits(vs[i], down);
+    for (int i = 0; i < 4; ++i) f[i] = u2f(__builtin_elementwise_sub_sat(vs[i], down) << 23);
 #pragma unroll
     for (int w = 0; w < kVWords; ++w) {
       auto pair = [&](auto which) {
@@ -1081,7 +1081,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     gather(step, 1, x1);
   };
   // Noted in the iteration before the step's store, read in the one of the store.
-  auto noted = [&](int step, int what) { return __builtin_amdgcn_readfirstlane(notes[step & 1][what]) == step; };
+  auto noted = [&](int step, int what) { return notes[step & 1][what] == step; };
   if (steps > 0) {
     Pages next, later;  // of the step whose loads come next and of the one after
     pages_of(0, next);
@@ -1091,8 +1091,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     note_scales(0);
     __syncthreads();
     bool nan = noted(0, 0);
-    if (noted(0, 1)) down = kDown;
-    store(0);
+    if (__ballot(noted(0, 1))) down = kDown;
+    store_keys(0);
+    store_values(0);
     next = later;
     valid_next = load(1, next);
     pages_of(2, next);
@@ -1100,9 +1101,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     for (int step = 0; step < steps; ++step) {
       const int t0 = begin + step * kBlockStep;
       __syncthreads();
-      const bool nan_next = noted(step + 1, 0), lower = down == 0 && noted(step + 1, 1);
+      const bool nan_next = noted(step + 1, 0), large = noted(step + 1, 1);
+      store_keys(step + 1);
+      const bool lower = down == 0 && __ballot(large);
       if (lower) down = kDown;
-      store(step + 1);
+      store_values(step + 1);
       const uint64_t valid_later = load(step + 2, next);
       pages_of(step + 3, next);
       if (t0 < mine.hi && t0 + kBlockStep > mine.lo) {
@@ -1188,16 +1191,18 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
     }
   };
   fetch(first);
+  // where there are few, lanes a row of them apart take the same split
+  constexpr int kLanes = kShare == 1 ? kFewSplits : 64;
   float m = kLowest, l = 0.0f;
-  for (int s = lane; s < splits; s += 64) {
+  for (int s = lane & (kLanes - 1); s < splits; s += kLanes) {
     const float m1 = m_n[s * size], top = __builtin_fmaxf(m, m1);
     l = l * __builtin_amdgcn_exp2f(m - top) + m_n[s * size + plan.rows] * __builtin_amdgcn_exp2f(m1 - top);
     m = top;
   }
   const float mine = m;
-  for (int d = 1; d < 64; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
+  for (int d = 1; d < kLanes; d *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, d));
   l *= __builtin_amdgcn_exp2f(mine - m);
-  for (int d = 1; d < 64; d *= 2) l += __shfl_xor(l, d);
+  for (int d = 1; d < kLanes; d *= 2) l += __shfl_xor(l, d);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   float o[kPer];
 #pragma unroll
