@@ -171,7 +171,7 @@ static int kv4_strided(const void* p, int32_t dtype, int64_t sn, int64_t sh, con
   return kOk;
 }
 
-static int to_query(const Kv4View& c, int dim, const vqx_kv4_query* q, const char* what, Kv4Query* v) {
+static int to_query(const Kv4View& c, const vqx_kv4_query* q, const char* what, Kv4Query* v) {
   if (!q) return set_error(kErrInvalid, "%s: query is NULL", what);
   int rc = kv4_float(q->dtype, what);
   if (rc == kOk) rc = to_tokens(c, q->cu, q->n, what, &v->tokens);
@@ -204,7 +204,6 @@ static int to_query(const Kv4View& c, int dim, const vqx_kv4_query* q, const cha
   v->scale = q->scale;
   v->softcap = q->softcap;
   v->slopes = q->slopes;
-  (void)dim;
   return kOk;
 }
 
@@ -672,7 +671,7 @@ int vqx_kv4_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_q
   Kv4View c;
   Kv4Query q;
   int rc = to_view(cache, "kv4_attention", &c);
-  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_attention", &q);
+  if (rc == kOk) rc = to_query(c, query, "kv4_attention", &q);
   if (rc != kOk) return rc;
   *bytes = kv4_workspace(c, cache->dim, q, query->dtype);
   return kOk;
@@ -684,7 +683,7 @@ int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, vo
   Kv4View c;
   Kv4Query q;
   int rc = to_view(cache, "kv4_attention", &c);
-  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_attention", &q);
+  if (rc == kOk) rc = to_query(c, query, "kv4_attention", &q);
   if (rc != kOk || query->n == 0) return rc;
   if (!out || !lse) return set_error(kErrInvalid, "kv4_attention: null tensor");
   if (!aligned(out, 16)) return set_error(kErrInvalid, "kv4_attention: out must be 16-byte aligned");
@@ -701,7 +700,7 @@ int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, c
   Kv4View c;
   Kv4Query q;
   int rc = to_view(cache, "kv4_accumulate", &c);
-  if (rc == kOk) rc = to_query(c, cache->dim, query, "kv4_accumulate", &q);
+  if (rc == kOk) rc = to_query(c, query, "kv4_accumulate", &q);
   if (rc != kOk || query->n == 0) return rc;
   if (!lse || !weights) return set_error(kErrInvalid, "kv4_accumulate: null tensor");
   if (weights_len < 0) return set_error(kErrInvalid, "kv4_accumulate: weights of %lld tokens", (long long)weights_len);
