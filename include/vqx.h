@@ -738,9 +738,10 @@ int vqx_kv4_read(const vqx_kv4_cache* cache, void* key, void* value, int32_t dty
  * out [n, heads, dim] (the query's dtype) = softmax(scores) . values and lse
  * [n, heads] = the log of the scores' exponentials' sum, fp32.  A row that sees
  * nothing has out 0 and lse -inf.  An output element is NaN where the row sees
- * a NaN key, or a NaN block of values with that element.  workspace:
- * vqx_kv4_attention_workspace_size bytes for the same cache and query (it does
- * not read the tensors), 16-byte aligned, or NULL where that is 0.
+ * a NaN key, or a NaN block of values with that element.  Blocks of values with a
+ * scale below 2^-87 count as if it were that where a block with one of 2^88 or
+ * more is read beside them.  workspace: vqx_kv4_attention_workspace_size bytes for the same cache and query (it
+ * does not read the tensors), 16-byte aligned, or NULL where that is 0.
  */
 int vqx_kv4_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes);
 int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, void* out, float* lse, void* workspace,
@@ -764,9 +765,11 @@ int vqx_kv4_accumulate(const vqx_kv4_cache* cache, const vqx_kv4_query* query, c
  * for budget tokens each (neither it, its lengths among that, nor out_weights
  * may overlap the inputs).  index: int32 [seqs, kv_heads, budget], where each
  * kept token was, -1 past the end; out->lengths: their number; out_weights:
- * fp32 [seqs, kv_heads, budget], their weights, 0 past the end.  workspace:
- * vqx_kv4_evict_workspace_size bytes for the same cache and weights_len, 16-byte
- * aligned, or NULL where that is 0.
+ * fp32 [seqs, kv_heads, budget], their weights (of the heaviest ones -0 as 0 and
+ * a NaN as the quiet one), 0 past the end.  Attention over `out` takes distances,
+ * for windows and slopes, between its slots: the tokens between do not count any
+ * more.  workspace: vqx_kv4_evict_workspace_size bytes for the same cache and
+ * weights_len, 16-byte aligned, or NULL where that is 0.
  */
 int vqx_kv4_evict_workspace_size(const vqx_kv4_cache* cache, int64_t weights_len, int64_t* bytes);
 int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weights_len, int32_t budget, int32_t recent,

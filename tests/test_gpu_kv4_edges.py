@@ -150,3 +150,20 @@ def test_scales_of_next_to_nothing(ops, kind, many, scale):
     lens = torch.tensor([100, 77], dtype=torch.int32)
     check_attention(ops, kind, q, codes, scales, lens, table=table, scale=scale)
     check_attention(ops, kind, q, codes, scales, lens, table=table, scale=scale, softcap=3.0)
+
+
+@pytest.mark.parametrize("how", [dict(window=20), dict(slopes=True), dict(window=33, slopes=True, softcap=5.0)])
+def test_distances_in_an_evicted_cache(ops, how):
+    """Windows and slopes count the slots of the cache that eviction has filled."""
+    seqs, kv, group, dim, budget = 2, 2, 3, 64, 48
+    codes, scales, table = make_cache(seqs, kv, dim, 200, 16)
+    oc, os_, ot = make_cache(seqs, kv, dim, budget, 8, 9)
+    w = torch.rand(seqs, kv, 200, generator=torch.Generator().manual_seed(1))
+    lens = torch.tensor([200, 30], dtype=torch.int32)
+    d = on(codes, scales, w, lens, oc, os_, torch.zeros(seqs, kv, budget), table, ot)
+    _, kept = ops.kv4_evict(d[0], d[1], d[2], d[3], budget, 8, d[4], d[5], d[6], d[7], d[8])
+    how = dict(how)
+    if how.get("slopes"):
+        how["slopes"] = torch.exp2(-8.0 * torch.arange(1, kv * group + 1) / (kv * group))
+    q = torch.randn(seqs, kv * group, dim, generator=torch.Generator().manual_seed(2)).bfloat16()
+    check_attention(ops, "bf16", q, d[4].cpu(), d[5].cpu(), kept.cpu(), table=ot, **how)

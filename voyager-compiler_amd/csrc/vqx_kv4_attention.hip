@@ -499,7 +499,7 @@ __device__ __forceinline__ void fill_beyond(const Kv4Query& q, const TileRows& r
 // that reading is the bound.  A workgroup has one tile, one kv head and one
 // run of tokens; its four waves take steps of 32 tokens in turn, each straight
 // from memory into the operands' registers, one step ahead, and are joined at
-// the end.  64 sequences of 4096 tokens, 32 kv heads of 128, bf16: 176 us, 5.6
+// the end.  64 sequences of 4096 tokens, 32 kv heads of 128, bf16: 178 us, 5.6
 // TB/s.  With fewer tokens a workgroup's own time shows: 4.5 us and 0.7 us for
 // each step of its waves (one sequence of 131073 tokens, 8 kv heads: 33 us, 4.3
 // TB/s; 16 of 4000 at most: 19 us).
@@ -766,8 +766,10 @@ constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 :
 // 16 where a wave has one tile), and walks over the tokens by 64.  Keys and
 // values of a step are turned into bf16 once, the values transposed, into LDS
 // (two buffers, one barrier a step), and read by all four waves.  Bound by the
-// vector instructions of the softmax (half of the time) beside the matrix ones
-// (28%): a prompt of 8192 tokens, 32 heads over 8 of 128: 737 us, 746 TFLOP/s.
+// matrix instructions (busy for 46% of the SIMDs' cycles) and the vector ones of
+// the softmax (issuing for 56%), which two waves a SIMD overlap a little: a prompt
+// of 8192 tokens, 32 heads over 8 of 128, 740 us; its 824 GFLOP with both terms
+// of the weights at 1.11 PFLOP/s, where a large library product reaches 1.21.
 //
 // Weights of bf16 outputs are two bf16 terms here as in the other kernel, a
 // third of the matrix work more than one.  As one fp16 term, with the values as
@@ -1401,20 +1403,21 @@ __global__ __launch_bounds__(256) void kv4_weigh_kernel(Kv4View c, Kv4Query q, i
 // When the kernel for many rows is taken.  Its workgroups have 4 or 8 times the
 // rows and a time of their own of some 20 us with the join, so that they have to
 // be full and to fill the card.  Full: in the mean a sequence has 128 rows, or
-// the most that any has (32 sequences of 4000 tokens, one with 512 new
-// tokens and the others with one, bf16, heads of 128: 130 us with it and 43 with
-// the other; 8 with 300 and 24 with one, of 1000: 77 and 106).  To fill the card,
-// either so many tiles of 16 rows by 32 tokens that its splits are long enough
-// (twice as many where a workgroup has 64 rows): 512 new tokens of 4096 (131072
-// tiles) 79 and 92 us, 2048 of 2048 (262144) 86 and 120, 256 of 2000 (32000) 45
-// and 30; f16, heads of 256, 64 rows: 2048 of 2048 295 and 480, 3000 of 5000 with
-// 4 heads over 1 (118500) 296 and 187.
+// the most that any has (bf16, heads of 128, with it and with the other: 32
+// sequences of up to 4000 tokens, one with 512 new tokens and the others with
+// one, 140 and 37 us; of up to 1000, 8 with 300 and 24 with one, 80 and 86).  To
+// fill the card, either so many tiles of 16 rows by 32 tokens that its splits are
+// long enough (twice as many where a workgroup has 64 rows): 256 new tokens of
+// 2000 (32000 tiles) 43 and 27 us, 2 x 350 of 2000 (90112) 85 and 63, 512 of 4096
+// (131072) 84 and 82, 2 x 700 of 1800 (162400) 88 and 89, 2 x 65 of 16385 (139264)
+// 103 and 153, 2048 of 2048 (262144) 93 and 96; f16, heads of 256, 64 rows: 3000
+// of 5000 with 4 heads over 1 (118500) 304 and 168, 2048 of 2048 288 and 463.
 constexpr int64_t kManyTiles = 100000;
 // Or a workgroup for every compute unit over few tokens, without splits: there
 // the other kernel's time is that of its workgroups' beginnings.  bf16, heads of
-// 128: 6 x 139 new tokens of 180, 8 heads each (432 workgroups), 25 and 43 us,
-// 16 x 64 of 500 (256) 33 and 42, 1 x 512 of 512 (128) 30 and 20, 1 x 1000 of 1000
-// (256, two splits) 64 and 42; of 256: 6 x 139 of 180 54 and 120.
+// 128: 6 x 139 new tokens of 180, 8 heads each (432 workgroups), 22 and 31 us,
+// 16 x 64 of 500 (256) 30 and 32, 1 x 512 of 512 (128) 28 and 16, 1 x 1000 of 1000
+// (256, two splits) 64 and 33; of 256: 6 x 139 of 180 50 and 119.
 constexpr int64_t kShortSpan = 2048;
 
 // Tiles of all kv heads, each of which has all its splits.
@@ -1444,11 +1447,14 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   p.rows = all > kRows && full && (whole || steps >= (many == 64 ? 2 : 1) * kManyTiles) ? many : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   const int64_t there = tiles_of(p.rows);
-  // where most tiles would have no rows (32 sequences of 4000 tokens, one with
-  // 512 new tokens, heads of 128: 131 us with all tiles, 43 with those there are)
+  // where most tiles would have no rows (32 sequences of up to 4000 tokens, one
+  // with 512 new tokens, heads of 128: 115 us with all tiles, 37 with those there are)
   p.listed = 2 * there <= (int64_t)c.seqs * p.tiles && there < 1 << 25 ? (int32_t)there : 0;
   const int64_t span = span_of(p.rows / q.group + 2);
-  // two workgroups for every compute unit, as many as are resident and no more,
+  // The tokens are cut as if every sequence filled its room, since the lengths are
+  // not known here: with room for 131072, 16 sequences of 16000 take 111 us (55 with
+  // room for 16000), 256 new tokens of 2000 104 (26).
+  // Two workgroups for every compute unit, as many as are resident and no more,
   // and none with fewer than eight steps (of a wave, of the workgroup): one costs
   // some 5 us beside its tokens, a join 4 and its launch (4 a unit instead of 2:
   // 16 sequences of 4000 tokens 27 and 23 us, one of 131073 47 and 38; one of

@@ -1,8 +1,10 @@
 """A serving cache of keys and values in 4 bits, and the attention that reads it.
 
-``torch.ops.quantized_ops.kv4_*``, this build's own: the reference has no cache.
-The cache holds keys and values in the packed form of ``quantize_mx_packed(x,
-"fp4_e2m1", -1, 32)``, page by page:
+``torch.ops.quantized_ops.kv4_*``, this package's own: the reference has no cache.
+They are for inference: no gradient passes through them.  The cache holds keys
+and values in the layout of ``quantize_mx_packed(x, "fp4_e2m1", -1, 32)``, page
+by page (but for quotients of 255 / 1024, which that rounds up as the reference
+does and ``kv4_append`` to the nearer 0, and for scales below E8M0's 2^-127):
 
 * ``codes``  uint8 [2, pages, kv heads, page size, D / 2], keys then values,
   element 2 i in the low nibble; D is 64, 128 or 256;
@@ -21,7 +23,15 @@ A step of a server: ``kv4_append`` the new keys and values, ``kv4_attention``
 (and, where tokens are to be weighed, ``kv4_accumulate``), and where a cache
 has grown over its budget ``kv4_evict`` into another one.  All of it is
 enqueued on the current stream without a look at the device's data, so a decode
-step can be captured into a graph and replayed as ``lengths`` grows.
+step can be captured into a graph and replayed as ``lengths`` grows.  Since the
+lengths are not looked at, work is shared out as if each sequence filled its
+room (the table's pages): a table many times as wide as the sequences costs up
+to four times the time.
+
+A place is a slot of the cache.  ``kv4_evict`` moves the kept tokens to the
+front, for each kv head others, so that in a cache that it has filled distances
+are of slots: ``window`` and ``slopes`` no longer count the tokens that were
+between.
 """
 
 import ctypes
@@ -286,9 +296,10 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
               out_table=None):
     """Keep min(budget, length) tokens of each sequence for each kv head, the
     latest `recent` and the heaviest before them, in their order at the front of
-    the other cache; equal weights go by the lower place.  Returns (index int32
-    [sequences, kv heads, budget]: where each kept token was, -1 past the end;
-    the new lengths); out_weights gets their weights, 0 past the end."""
+    the other cache; equal weights go by the lower place, NaN is above all.
+    Returns (index int32 [sequences, kv heads, budget]: where each kept token
+    was, -1 past the end; the new lengths); out_weights gets their weights (a
+    heavy -0 as 0, a heavy NaN as the quiet one), 0 past the end."""
     what = "kv4_evict"
     _lib.require_device(codes, what)
     c = _cache(codes, scales, lengths, table, what)
