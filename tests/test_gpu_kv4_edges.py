@@ -167,3 +167,14 @@ def test_distances_in_an_evicted_cache(ops, how):
         how["slopes"] = torch.exp2(-8.0 * torch.arange(1, kv * group + 1) / (kv * group))
     q = torch.randn(seqs, kv * group, dim, generator=torch.Generator().manual_seed(2)).bfloat16()
     check_attention(ops, "bf16", q, d[4].cpu(), d[5].cpu(), kept.cpu(), table=ot, **how)
+
+
+@pytest.mark.parametrize("kind,dim,length,new", [("bf16", 64, 100001, 1), ("f32", 128, 70000, 2), ("f16", 256, 18000, 1)])
+def test_more_splits_than_lanes(ops, kind, dim, length, new):
+    """One head of one long sequence, cut into up to a hundred splits; the last
+    part of it weighs most, as a slope has it, or all of it the same."""
+    codes, scales, table = make_cache(1, 1, dim, length, 64)
+    q = torch.randn(new, 2, dim, generator=torch.Generator().manual_seed(1)).to(TYPES[kind])
+    lens = torch.tensor([length], dtype=torch.int32)
+    check_attention(ops, kind, q, codes, scales, lens, table=table, scale=0.01)
+    check_attention(ops, kind, q, codes, scales, lens, table=table, slopes=torch.tensor([0.001, 0.5]))
