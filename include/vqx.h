@@ -776,6 +776,43 @@ int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weig
                   const vqx_kv4_cache* out, int32_t* index, float* out_weights, void* workspace,
                   int64_t workspace_bytes, vqx_stream_t stream);
 
+/*
+ * Rotary positions (this library's own).  The first 2 pairs elements of a head
+ * are turned in pairs, x = x_i with y = x_(i + pairs), or x_2i with x_(2i + 1)
+ * where interleaved is not 0:
+ *   x' = factor (x cos a - y sin a),  y' = factor (x sin a + y cos a),
+ *   a = positions[token] freqs[i]
+ * (back: by -a, which turns a gradient of the outputs into one of the inputs);
+ * the other elements stay.  Angles and products are in 64 bits, the result is
+ * rounded to fp32 and from there to the dtype.  freqs: fp32 [pairs], angles
+ * below 2^51; positions: int32 [tokens].
+ */
+typedef struct vqx_turn {
+  const float* freqs;
+  const int32_t* positions;
+  int32_t pairs;
+  int32_t interleaved;
+  int32_t back;
+  float factor;
+} vqx_turn;
+
+/* x [n, heads, dim] of dtype F32, BF16 or F16, strides in elements, rows
+ * contiguous and starting on 16 bytes; out: dense, 16-byte aligned, not x.  dim:
+ * a multiple of 8 up to 1024, at least 2 pairs; pairs at least 1. */
+int vqx_rotary(const void* x, int32_t dtype, int64_t n, int64_t heads, int64_t dim, int64_t stride_n, int64_t stride_h,
+               const vqx_turn* turn, void* out, vqx_stream_t stream);
+
+/*
+ * vqx_rotary of the new tokens' queries [n, heads, dim] (into out, dense) and of
+ * their keys, and vqx_kv4_append of those keys and the values, in one launch.
+ * A key is rounded to its dtype before it is quantized, as the two calls would
+ * have it.  positions NULL: the tokens' places in the cache.
+ */
+int vqx_kv4_append_rotary(const vqx_kv4_cache* cache, const vqx_turn* turn, const void* query, int32_t heads,
+                          int64_t query_stride_n, int64_t query_stride_h, const void* key, int64_t key_stride_n,
+                          int64_t key_stride_h, const void* value, int64_t value_stride_n, int64_t value_stride_h,
+                          int32_t dtype, int64_t n, const int32_t* cu, void* out, vqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,12 +99,24 @@ class VqxKv4Query(ctypes.Structure):
     ]
 
 
+class VqxTurn(ctypes.Structure):
+    _fields_ = [
+        ("freqs", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("pairs", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("back", ctypes.c_int32),
+        ("factor", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _KC = ctypes.POINTER(VqxKv4Cache)
 _KQ = ctypes.POINTER(VqxKv4Query)
+_KT = ctypes.POINTER(VqxTurn)
 
 _SIGNATURES = {
     "vqx_version": ([], ctypes.c_char_p),
@@ -173,6 +185,9 @@ _SIGNATURES = {
     "vqx_kv4_accumulate": ([_KC, _KQ, _P, _P, _I64, _P], ctypes.c_int),
     "vqx_kv4_evict_workspace_size": ([_KC, _I64, ctypes.POINTER(_I64)], ctypes.c_int),
     "vqx_kv4_evict": ([_KC, _P, _I64, _I32, _I32, _KC, _P, _P, _P, _I64, _P], ctypes.c_int),
+    "vqx_rotary": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _KT, _P, _P], ctypes.c_int),
+    "vqx_kv4_append_rotary": ([_KC, _KT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _P],
+                              ctypes.c_int),
 }
 
 _lib = None

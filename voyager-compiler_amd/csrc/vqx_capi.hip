@@ -6,6 +6,7 @@
 #include "../../include/vqx.h"
 #include "vqx_kernels.h"
 #include "vqx_kv4.h"
+#include "vqx_rotary.h"
 
 namespace vqx {
 
@@ -204,6 +205,17 @@ static int to_query(const Kv4View& c, const vqx_kv4_query* q, const char* what, 
   v->scale = q->scale;
   v->softcap = q->softcap;
   v->slopes = q->slopes;
+  return kOk;
+}
+
+static int to_turn(const vqx_turn* t, int64_t dim, bool places, const char* what, Turn* v) {
+  if (!t) return set_error(kErrInvalid, "%s: turn is NULL", what);
+  if (!t->freqs || (!t->positions && !places)) return set_error(kErrInvalid, "%s: null tensor", what);
+  if (t->pairs < 1 || 2ll * t->pairs > dim)
+    return set_error(kErrInvalid, "%s: %d pairs of a head of %lld elements", what, t->pairs, (long long)dim);
+  const float size = t->factor < 0.0f ? -t->factor : t->factor;
+  if (!(size <= 3.4028235e38f)) return set_error(kErrInvalid, "%s: the factor is not finite", what);
+  *v = Turn{t->freqs, t->positions, t->pairs, t->interleaved != 0, t->back != 0, t->factor};
   return kOk;
 }
 
@@ -754,6 +766,55 @@ int vqx_kv4_evict(const vqx_kv4_cache* cache, const float* weights, int64_t weig
     return set_error(kErrInvalid, "kv4_evict: the new lengths go to another tensor, not onto these");
   return kv4_evict(c, cache->dim, weights, weights_len, budget, recent, o, index, out->lengths, out_weights, workspace,
                    (hipStream_t)stream);
+}
+
+int vqx_rotary(const void* x, int32_t dtype, int64_t n, int64_t heads, int64_t dim, int64_t stride_n, int64_t stride_h,
+               const vqx_turn* turn, void* out, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Turn t;
+  int rc = kv4_float(dtype, "rotary");
+  if (rc != kOk) return rc;
+  if (dim < 8 || dim > 1024 || dim % 8 != 0)
+    return set_error(kErrInvalid, "rotary: heads of 8 to 1024 elements, a multiple of 8, not %lld", (long long)dim);
+  if (n < 0 || heads < 0 || n >= 1ll << 30 || heads * dim >= 1ll << 24)
+    return set_error(kErrInvalid, "rotary: %lld tokens of %lld heads", (long long)n, (long long)heads);
+  rc = to_turn(turn, dim, n == 0, "rotary", &t);
+  if (rc != kOk || n == 0 || heads == 0) return rc;
+  if (!x || !out) return set_error(kErrInvalid, "rotary: null tensor");
+  rc = kv4_strided(x, dtype, stride_n, stride_h, "rotary");
+  if (rc != kOk) return rc;
+  if (!aligned(out, 16) || out == x) return set_error(kErrInvalid, "rotary: out must be 16-byte aligned, and not x");
+  return rotary(t, Rows{x, stride_n, stride_h, (int32_t)heads, (int32_t)dim}, dtype, n, out, (hipStream_t)stream);
+}
+
+int vqx_kv4_append_rotary(const vqx_kv4_cache* cache, const vqx_turn* turn, const void* query, int32_t heads,
+                          int64_t query_stride_n, int64_t query_stride_h, const void* key, int64_t key_stride_n,
+                          int64_t key_stride_h, const void* value, int64_t value_stride_n, int64_t value_stride_h,
+                          int32_t dtype, int64_t n, const int32_t* cu, void* out, vqx_stream_t stream) {
+  g_err[0] = 0;
+  const char* what = "kv4_append_rotary";
+  Kv4View c;
+  Kv4Tokens q;
+  Turn t;
+  int rc = to_view(cache, what, &c);
+  if (rc == kOk) rc = kv4_float(dtype, what);
+  if (rc == kOk) rc = to_tokens(c, cu, n, what, &q);
+  if (rc == kOk) rc = to_turn(turn, cache->dim, true, what, &t);
+  if (rc != kOk) return rc;
+  if (heads <= 0 || (int64_t)heads * cache->dim >= 1ll << 24)
+    return set_error(kErrInvalid, "%s: %d query heads", what, heads);
+  if (n == 0) return kOk;
+  if (!query || !key || !value || !out) return set_error(kErrInvalid, "%s: null tensor", what);
+  rc = kv4_strided(query, dtype, query_stride_n, query_stride_h, what);
+  if (rc == kOk) rc = kv4_strided(key, dtype, key_stride_n, key_stride_h, what);
+  if (rc == kOk) rc = kv4_strided(value, dtype, value_stride_n, value_stride_h, what);
+  if (rc != kOk) return rc;
+  if (!aligned(out, 16) || out == query)
+    return set_error(kErrInvalid, "%s: out must be 16-byte aligned, and not the query", what);
+  const int32_t kv = cache->kv_heads, dim = cache->dim;
+  return kv4_append_rotary(c, dim, q, t, Rows{query, query_stride_n, query_stride_h, heads, dim},
+                           Rows{key, key_stride_n, key_stride_h, kv, dim},
+                           Rows{value, value_stride_n, value_stride_h, kv, dim}, dtype, out, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``, ``kv4.py``)."""
+"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``, ``kv4.py``, ``rotary.py``)."""
 
 from .quantized import (  # noqa: F401
     calculate_mx_qparam,
@@ -12,4 +12,12 @@ from .quantized import (  # noqa: F401
     register_table,
     vmap,
 )
-from .kv4 import kv4_accumulate, kv4_append, kv4_attention, kv4_evict, kv4_read  # noqa: F401
+from .kv4 import (  # noqa: F401
+    kv4_accumulate,
+    kv4_append,
+    kv4_append_rotary,
+    kv4_attention,
+    kv4_evict,
+    kv4_read,
+)
+from .rotary import rotary, rotary_frequencies  # noqa: F401

@@ -61,6 +61,10 @@ _SCHEMAS = {
         "kv4_evict(Tensor codes, Tensor scales, Tensor weights, Tensor lengths, int budget, int recent, "
         "Tensor(a!) out_codes, Tensor(b!) out_scales, Tensor(c!) out_weights, Tensor? table=None, "
         "Tensor? out_table=None) -> (Tensor, Tensor)"),
+    "kv4_append_rotary": (
+        "kv4_append_rotary(Tensor query, Tensor key, Tensor value, Tensor(a!) codes, Tensor(b!) scales, Tensor lengths, "
+        "Tensor freqs, Tensor? cu=None, Tensor? table=None, Tensor? positions=None, *, bool interleaved=False, "
+        "float factor=1.0) -> Tensor"),
 }
 for _s in _SCHEMAS.values():
     quantized_ops_lib.define(_s)
@@ -78,6 +82,17 @@ _FP32_MAX, _FP32_TINY = torch.finfo(torch.float32).max, torch.finfo(torch.float3
 
 def _refuse(what, message):
     raise ValueError(f"vqx: {what}: {message}")
+
+
+def _launch(name, device, *args):
+    """The library's entry point on the tensors' device and its current stream."""
+    at = device.index
+    stream = torch._C._cuda_getCurrentRawStream(at)
+    if at == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
 
 
 def _int32(t, n, name, what, device):
@@ -198,6 +213,22 @@ def _weights(weights, seqs, kv, name, what, device):
     return weights.data_ptr()
 
 
+def _turn(freqs, positions, n, dim, interleaved, factor, back, what, device):
+    """How pairs are turned, as the library takes it; positions: None for places
+    in a cache."""
+    if freqs.dtype != torch.float32 or freqs.dim() != 1 or not freqs.is_contiguous():
+        _refuse(what, f"freqs must be a contiguous float32 vector, not {freqs.dtype} {list(freqs.shape)}")
+    pairs = freqs.shape[0]
+    if not 1 <= pairs <= dim // 2:
+        _refuse(what, f"{pairs} frequencies for the pairs of a head of {dim}")
+    if freqs.device != device:
+        _refuse(what, f"freqs are on {freqs.device}, the heads on {device}")
+    if not -_FP32_MAX <= factor <= _FP32_MAX:
+        _refuse(what, f"a factor is finite in float32, not {factor}")
+    at = None if positions is None else _int32(positions, n, "positions", what, device)
+    return _lib.VqxTurn(freqs.data_ptr(), at, pairs, interleaved, back, factor)
+
+
 @_impl("kv4_append")
 def kv4_append(key, value, codes, scales, lengths, cu=None, table=None):
     """Quantize the new tokens' keys and values [n, kv heads, D] into their
@@ -214,6 +245,35 @@ def kv4_append(key, value, codes, scales, lengths, cu=None, table=None):
     offsets = _offsets(cu, n, c.seqs, what, device)
     _lib.call("vqx_kv4_append", c, k.data_ptr(), v.data_ptr(), tag, n, kn, kh, vn, vh, offsets,
               _lib.stream_of(codes))
+
+
+@_impl("kv4_append_rotary")
+def kv4_append_rotary(query, key, value, codes, scales, lengths, freqs, cu=None, table=None, positions=None, *,
+                      interleaved=False, factor=1.0):
+    """``rotary`` of the new tokens' queries [n, heads, D], which are returned,
+    and of their keys, which go into the cache with the values as by
+    ``kv4_append``, in one launch.  positions: int32 [n], or None for the tokens'
+    places in the cache; in one that ``kv4_evict`` has thinned out a place is no
+    position."""
+    what = "kv4_append_rotary"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    device, kv, dim = codes.device, c.kv_heads, c.dim
+    q, qn, qh, qtag = _rows(query, None, dim, "query", what, device)
+    k, kn, kh, tag = _rows(key, kv, dim, "key", what, device)
+    v, vn, vh, vtag = _rows(value, kv, dim, "value", what, device)
+    n, heads, _ = q.shape
+    if k.shape[0] != n or v.shape[0] != n or qtag != tag or vtag != tag:
+        _refuse(what, f"query, key and value differ: {query.dtype} {list(query.shape)}, {key.dtype} {list(key.shape)}, "
+                      f"{value.dtype} {list(value.shape)}")
+    if heads == 0:
+        _refuse(what, "0 query heads")
+    offsets = _offsets(cu, n, c.seqs, what, device)
+    t = _turn(freqs, positions, n, dim, interleaved, factor, False, what, device)
+    out = q.new_empty((n, heads, dim))
+    _launch("vqx_kv4_append_rotary", device, c, t, q.data_ptr(), heads, qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn,
+            vh, tag, n, offsets, out.data_ptr())
+    return out
 
 
 @_impl("kv4_read")
@@ -330,6 +390,11 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
 @torch.library.register_fake("quantized_ops::kv4_append")
 def _(key, value, codes, scales, lengths, cu=None, table=None):
     return None
+
+
+@torch.library.register_fake("quantized_ops::kv4_append_rotary")
+def _(query, key, value, codes, scales, lengths, freqs, cu=None, table=None, positions=None, **kwargs):
+    return query.new_empty(query.shape)
 
 
 @torch.library.register_fake("quantized_ops::kv4_read")
