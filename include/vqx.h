@@ -813,6 +813,46 @@ int vqx_kv4_append_rotary(const vqx_kv4_cache* cache, const vqx_turn* turn, cons
                           int64_t key_stride_h, const void* value, int64_t value_stride_n, int64_t value_stride_h,
                           int32_t dtype, int64_t n, const int32_t* cu, void* out, vqx_stream_t stream);
 
+/*
+ * Pages for the new tokens of a step, on the device.  grow (int32 [seqs]): how
+ * many tokens each sequence gets, below 0 where it ends.  free_pages (int32
+ * [pages]) holds page numbers of which the first count[0] are free; table is
+ * int32 [seqs, pages_per_seq], -1 (or anything outside [0, pages)) where a
+ * sequence has no page.
+ * First the sequences that end give the pages of their rows back, sequence by
+ * sequence and in the rows' order, behind the free ones; their rows become -1
+ * and their lengths 0.  Then each sequence is given the pages that its new tokens
+ * lack, taken from the end of the free ones, sequence by sequence, and its
+ * length grows.  One that has not the room in its row is passed over; one that
+ * the pages do not last for, or whose tokens do not fit into n, gets nothing, and
+ * neither do those behind it that need a page (or tokens): nobody overtakes.
+ * cu (int32 [seqs + 1]): the offsets of the new tokens of those that were served
+ * (a sequence that was not has none); positions (int32 [n]): their places in their
+ * sequences; slots (int64 [n]): page * page_size + place in the page; both -1
+ * past the last new token.  Pages that a row has behind its length (after
+ * vqx_kv4_accept) are used before others are taken.
+ */
+int vqx_kv4_reserve(const int32_t* grow, int32_t* lengths, int32_t* table, int32_t* free_pages, int32_t* count,
+                    int64_t seqs, int64_t pages_per_seq, int64_t pages, int64_t page_size, int64_t n, int32_t* cu,
+                    int32_t* positions, int64_t* slots, vqx_stream_t stream);
+
+/*
+ * Which of a tree of drafted tokens stay.  tree (int64 [n]): bit j of a new
+ * token's mask says that its sequence's new token j is among its ancestors or
+ * is itself.  drafts (int64 [n]): the tokens' numbers; sampled (int64 [n]): what
+ * the model says comes after each.  The first new token of a sequence is
+ * accepted; then, from the accepted token i on, the first j > i with tree[j] ==
+ * (tree[i] | 1 << j) and drafts[j] == sampled[i], until there is none.  Of more
+ * than 64 new tokens of a sequence the first 64 are looked at.
+ * path (int32 [n]): at the i-th new token of a sequence the i-th accepted one's
+ * place among them, -1 past the last; accepted (int32 [seqs]): their number;
+ * next (int64 [seqs]): sampled of the last one, -1 where there are no new tokens.
+ * The accepted tokens' keys and values are moved to the front of the sequence's
+ * new tokens and cache->lengths is cut by those that were not accepted.
+ */
+int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_t* drafts, const int64_t* sampled,
+                   int64_t n, const int32_t* cu, int32_t* path, int32_t* accepted, int64_t* next, vqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

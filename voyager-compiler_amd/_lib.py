@@ -188,6 +188,8 @@ _SIGNATURES = {
     "vqx_rotary": ([_P, _I32, _I64, _I64, _I64, _I64, _I64, _KT, _P, _P], ctypes.c_int),
     "vqx_kv4_append_rotary": ([_KC, _KT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _P],
                               ctypes.c_int),
+    "vqx_kv4_reserve": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P], ctypes.c_int),
+    "vqx_kv4_accept": ([_KC, _P, _P, _P, _I64, _P, _P, _P, _P, _P], ctypes.c_int),
 }
 
 _lib = None

@@ -817,4 +817,36 @@ int vqx_kv4_append_rotary(const vqx_kv4_cache* cache, const vqx_turn* turn, cons
                            Rows{value, value_stride_n, value_stride_h, kv, dim}, dtype, out, (hipStream_t)stream);
 }
 
+int vqx_kv4_reserve(const int32_t* grow, int32_t* lengths, int32_t* table, int32_t* free_pages, int32_t* count,
+                    int64_t seqs, int64_t pages_per_seq, int64_t pages, int64_t page_size, int64_t n, int32_t* cu,
+                    int32_t* positions, int64_t* slots, vqx_stream_t stream) {
+  g_err[0] = 0;
+  if (seqs < 0 || seqs >= 1ll << 24 || pages < 0 || pages >= 1ll << 31 || pages_per_seq < 1 || page_size < 1)
+    return set_error(kErrInvalid, "kv4_reserve: %lld sequences of %lld pages of %lld tokens, %lld pages in all",
+                     (long long)seqs, (long long)pages_per_seq, (long long)page_size, (long long)pages);
+  if (pages_per_seq >= 1ll << 30 || page_size >= 1ll << 30 || pages_per_seq * page_size >= 1ll << 30)
+    return set_error(kErrUnsupported, "kv4_reserve: room for 2^30 tokens or more in a sequence");
+  if (n < 0 || n >= 1ll << 30) return set_error(kErrInvalid, "kv4_reserve: %lld new tokens", (long long)n);
+  if (!count || !cu || (pages > 0 && !free_pages) || (seqs > 0 && (!grow || !lengths || !table)) ||
+      (n > 0 && (!positions || !slots)))
+    return set_error(kErrInvalid, "kv4_reserve: null tensor");
+  if (seqs > 0 && grow == lengths) return set_error(kErrInvalid, "kv4_reserve: grow and lengths are one tensor");
+  return kv4_reserve(Kv4Pages{grow, lengths, table, free_pages, count, (int32_t)seqs, (int32_t)pages_per_seq,
+                              (int32_t)pages, (int32_t)page_size, n, cu, positions, slots},
+                     (hipStream_t)stream);
+}
+
+int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_t* drafts, const int64_t* sampled,
+                   int64_t n, const int32_t* cu, int32_t* path, int32_t* accepted, int64_t* next, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Tokens q;
+  int rc = to_view(cache, "kv4_accept", &c);
+  if (rc == kOk) rc = to_tokens(c, cu, n, "kv4_accept", &q);
+  if (rc != kOk) return rc;
+  if ((n > 0 && (!tree || !drafts || !sampled || !path)) || (c.seqs > 0 && (!accepted || !next)))
+    return set_error(kErrInvalid, "kv4_accept: null tensor");
+  return kv4_accept(c, cache->dim, q, tree, drafts, sampled, path, accepted, next, (hipStream_t)stream);
+}
+
 }  // extern "C"

@@ -93,4 +93,23 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
 int kv4_accumulate(const Kv4View& c, int dim, const Kv4Query& q, int dtype, const float* lse, float* weights,
                    int64_t weights_len, hipStream_t st);
 
+// Pages for new tokens: `grow` of each sequence, below 0 where it ends.
+struct Kv4Pages {
+  const int32_t* grow;  // [seqs]
+  int32_t* lengths;     // [seqs]
+  int32_t* table;       // [seqs, per]
+  int32_t* free;        // [pages], the first count[0] are free
+  int32_t* count;       // [1]
+  int32_t seqs, per, pages, size;
+  int64_t n;           // room for positions and slots
+  int32_t* cu;         // [seqs + 1]
+  int32_t* positions;  // [n]
+  int64_t* slots;      // [n]
+};
+int kv4_reserve(const Kv4Pages& p, hipStream_t st);
+
+// Which drafted tokens are confirmed; their rows moved to the front, c.lengths cut.
+int kv4_accept(const Kv4View& c, int dim, const Kv4Tokens& q, const int64_t* tree, const int64_t* drafts,
+               const int64_t* tokens, int32_t* path, int32_t* count, int64_t* next, hipStream_t st);
+
 }  // namespace vqx

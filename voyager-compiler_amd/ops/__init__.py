@@ -13,11 +13,13 @@ from .quantized import (  # noqa: F401
     vmap,
 )
 from .kv4 import (  # noqa: F401
+    kv4_accept,
     kv4_accumulate,
     kv4_append,
     kv4_append_rotary,
     kv4_attention,
     kv4_evict,
     kv4_read,
+    kv4_reserve,
 )
 from .rotary import rotary, rotary_frequencies  # noqa: F401

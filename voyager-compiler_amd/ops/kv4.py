@@ -65,6 +65,12 @@ _SCHEMAS = {
         "kv4_append_rotary(Tensor query, Tensor key, Tensor value, Tensor(a!) codes, Tensor(b!) scales, Tensor lengths, "
         "Tensor freqs, Tensor? cu=None, Tensor? table=None, Tensor? positions=None, *, bool interleaved=False, "
         "float factor=1.0) -> Tensor"),
+    "kv4_reserve": (
+        "kv4_reserve(Tensor grow, Tensor(a!) lengths, Tensor(b!) table, Tensor(c!) free, Tensor(d!) count, "
+        "SymInt page_size, SymInt n) -> (Tensor, Tensor, Tensor)"),
+    "kv4_accept": (
+        "kv4_accept(Tensor tree, Tensor drafts, Tensor sampled, Tensor(a!) codes, Tensor(b!) scales, "
+        "Tensor(c!) lengths, Tensor? cu=None, Tensor? table=None) -> (Tensor, Tensor, Tensor)"),
 }
 for _s in _SCHEMAS.values():
     quantized_ops_lib.define(_s)
@@ -384,6 +390,80 @@ def kv4_evict(codes, scales, weights, lengths, budget, recent, out_codes, out_sc
     return index, kept
 
 
+@_impl("kv4_reserve")
+def kv4_reserve(grow, lengths, table, free, count, page_size, n):
+    """Pages for the new tokens of a step.  grow (int32 [sequences]): how many
+    tokens each sequence gets, below 0 where it ends; free (int32 [pages]): page
+    numbers, the first count (int32 [1]) of them free; table: -1 where a sequence
+    has no page.  Sequences that end give their pages back (behind the free ones,
+    in their order; row -1, length 0).  Then each is given, from the end of the
+    free ones, the pages that its new tokens lack, and its length grows.  One
+    without the room in its row is passed over; from the first on that the free
+    pages do not last for, or whose tokens do not fit into n, none gets a page (or
+    tokens past n).  Returns (cu int32 [sequences + 1]: offsets of the new tokens
+    of those that were served, positions int32 [n]: their places in their
+    sequences, slots int64 [n]: page * page_size + place in the page); positions
+    and slots are -1 past the last new token."""
+    what = "kv4_reserve"
+    _lib.require_device(lengths, what)
+    device = lengths.device
+    if lengths.dim() != 1:
+        _refuse(what, f"lengths must be [sequences], not {list(lengths.shape)}")
+    seqs = lengths.shape[0]
+    if table.dim() != 2 or table.shape[0] != seqs or table.dtype != torch.int32 or not table.is_contiguous():
+        _refuse(what, f"table must be a contiguous int32 tensor [{seqs}, pages of a sequence], not {table.dtype} "
+                      f"{list(table.shape)}")
+    if table.device != device:
+        _refuse(what, f"table is on {table.device}, the lengths on {device}")
+    if free.dim() != 1:
+        _refuse(what, f"free must be [pages], not {list(free.shape)}")
+    if n < 0:
+        _refuse(what, f"{n} new tokens")
+    given = (_int32(grow, seqs, "grow", what, device), _int32(lengths, seqs, "lengths", what, device), table.data_ptr(),
+             _int32(free, free.shape[0], "free", what, device), _int32(count, 1, "count", what, device))
+    cu, positions = lengths.new_empty(seqs + 1), lengths.new_empty(n)
+    slots = lengths.new_empty(n, dtype=torch.int64)
+    _launch("vqx_kv4_reserve", device, *given, seqs, table.shape[1], free.shape[0], page_size, n, cu.data_ptr(),
+            positions.data_ptr(), slots.data_ptr())
+    return cu, positions, slots
+
+
+def _int64(t, n, name, what, device):
+    """The address of t, a contiguous int64 vector of n on the cache's device."""
+    if t.dtype != torch.int64 or t.shape != (n,) or not t.is_contiguous():
+        _refuse(what, f"{name} must be a contiguous int64 tensor of shape [{n}], not {t.dtype} {list(t.shape)}")
+    if t.device != device:
+        _refuse(what, f"{name} is on {t.device}, the cache on {device}")
+    return t.data_ptr()
+
+
+@_impl("kv4_accept")
+def kv4_accept(tree, drafts, sampled, codes, scales, lengths, cu=None, table=None):
+    """Keep the drafted tokens that the model confirms.  tree (int64 [n]): as
+    kv4_tree_attention takes it; drafts (int64 [n]): the new tokens' numbers;
+    sampled (int64 [n]): what comes after each.  A sequence's first new token is
+    accepted; then, from the accepted token i on, the first j > i with tree[j] ==
+    tree[i] | 1 << j (a child of i) and drafts[j] == sampled[i], until there is
+    none.  Their keys and values are moved to the front of the sequence's new
+    tokens, and lengths is cut by the others.  Returns (path int32 [n]: at the i-th
+    new token of a sequence which of them was accepted as the i-th, -1 past the
+    last; how many were, int32 [sequences]; the token that comes next, int64
+    [sequences], -1 where there were no new ones)."""
+    what = "kv4_accept"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    device = codes.device
+    if tree.dim() != 1:
+        _refuse(what, f"tree must be [new tokens], not {list(tree.shape)}")
+    n = tree.shape[0]
+    offsets = _offsets(cu, n, c.seqs, what, device)
+    given = [_int64(t, n, name, what, device) for t, name in ((tree, "tree"), (drafts, "drafts"), (sampled, "sampled"))]
+    path, accepted = lengths.new_empty(n), lengths.new_empty(c.seqs)
+    follows = sampled.new_empty(c.seqs)
+    _launch("vqx_kv4_accept", device, c, *given, n, offsets, path.data_ptr(), accepted.data_ptr(), follows.data_ptr())
+    return path, accepted, follows
+
+
 # ---------------------------------------------------------------------------
 # fake (meta) implementations for tracing
 # ---------------------------------------------------------------------------
@@ -417,3 +497,13 @@ def _(query, lse, codes, scales, lengths, weights, cu=None, most=None, table=Non
 def _(codes, scales, weights, lengths, budget, recent, out_codes, out_scales, out_weights, table=None,
       out_table=None):
     return (lengths.new_empty((lengths.shape[0], codes.shape[2], budget)), torch.empty_like(lengths))
+
+
+@torch.library.register_fake("quantized_ops::kv4_reserve")
+def _(grow, lengths, table, free, count, page_size, n):
+    return lengths.new_empty(lengths.shape[0] + 1), lengths.new_empty(n), lengths.new_empty(n, dtype=torch.int64)
+
+
+@torch.library.register_fake("quantized_ops::kv4_accept")
+def _(tree, drafts, sampled, codes, scales, lengths, cu=None, table=None):
+    return lengths.new_empty(tree.shape[0]), torch.empty_like(lengths), sampled.new_empty(lengths.shape[0])
