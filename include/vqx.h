@@ -748,6 +748,21 @@ int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, vo
                       int64_t workspace_bytes, vqx_stream_t stream);
 
 /*
+ * vqx_kv4_attention of a tree of drafted tokens.  tree (int64 [n]): bit j of a
+ * new token's mask says that it sees its sequence's new token j: its ancestors
+ * and itself.  The new tokens lie in the cache one after another, behind the
+ * base = length - count tokens before them, which every row sees (as far as the
+ * window has it).  For windows and slopes a row's place is base + the number of
+ * its mask's bits - 1, and new token j is as many places before it as the mask
+ * has bits above j.  Bits of tokens that the sequence does not have do not
+ * count.  No sequence has more than 64 new tokens (most says so where n is more).
+ * Masks of 1 .. 1 up to the token's own bit are the rows of vqx_kv4_attention.
+ */
+int vqx_kv4_tree_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes);
+int vqx_kv4_tree_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, const int64_t* tree, void* out,
+                           float* lse, void* workspace, int64_t workspace_bytes, vqx_stream_t stream);
+
+/*
  * weights[b][x][t] += the sum over sequence b's new tokens and kv head x's
  * query heads of exp(score - lse), for the tokens t < weights_len that they
  * see; weights: fp32 [seqs, kv_heads, weights_len], lse as vqx_kv4_attention

@@ -189,6 +189,8 @@ _SIGNATURES = {
     "vqx_kv4_append_rotary": ([_KC, _KT, _P, _I32, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _P, _P],
                               ctypes.c_int),
     "vqx_kv4_reserve": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P], ctypes.c_int),
+    "vqx_kv4_tree_attention_workspace_size": ([_KC, _KQ, ctypes.POINTER(_I64)], ctypes.c_int),
+    "vqx_kv4_tree_attention": ([_KC, _KQ, _P, _P, _P, _P, _I64, _P], ctypes.c_int),
     "vqx_kv4_accept": ([_KC, _P, _P, _P, _I64, _P, _P, _P, _P, _P], ctypes.c_int),
 }
 

@@ -205,6 +205,7 @@ static int to_query(const Kv4View& c, const vqx_kv4_query* q, const char* what, 
   v->scale = q->scale;
   v->softcap = q->softcap;
   v->slopes = q->slopes;
+  v->tree = nullptr;
   return kOk;
 }
 
@@ -702,6 +703,45 @@ int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, vo
   const int64_t need = kv4_workspace(c, cache->dim, q, query->dtype);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return set_error(kErrInvalid, "kv4_attention: needs a 16-byte aligned workspace of %lld bytes, not %lld",
+                     (long long)need, (long long)workspace_bytes);
+  return kv4_attention(c, cache->dim, q, query->dtype, out, lse, (float*)workspace, (hipStream_t)stream);
+}
+
+// A query of drafted tokens, 64 of a sequence at most.
+static int to_tree(const Kv4View& c, const vqx_kv4_query* query, const int64_t* tree, const char* what, Kv4Query* q) {
+  const int rc = to_query(c, query, what, q);
+  if (rc != kOk) return rc;
+  if (q->most > 64) return set_error(kErrInvalid, "%s: %d new tokens of a sequence, 64 at most", what, q->most);
+  q->tree = tree;
+  return kOk;
+}
+
+int vqx_kv4_tree_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return set_error(kErrInvalid, "kv4_tree_attention_workspace_size: bytes is NULL");
+  Kv4View c;
+  Kv4Query q;
+  int rc = to_view(cache, "kv4_tree_attention", &c);
+  // what a tree holds is not read: any address stands for one
+  if (rc == kOk) rc = to_tree(c, query, reinterpret_cast<const int64_t*>(query), "kv4_tree_attention", &q);
+  if (rc != kOk) return rc;
+  *bytes = kv4_workspace(c, cache->dim, q, query->dtype);
+  return kOk;
+}
+
+int vqx_kv4_tree_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, const int64_t* tree, void* out,
+                           float* lse, void* workspace, int64_t workspace_bytes, vqx_stream_t stream) {
+  g_err[0] = 0;
+  Kv4View c;
+  Kv4Query q;
+  int rc = to_view(cache, "kv4_tree_attention", &c);
+  if (rc == kOk) rc = to_tree(c, query, tree, "kv4_tree_attention", &q);
+  if (rc != kOk || query->n == 0) return rc;
+  if (!tree || !out || !lse) return set_error(kErrInvalid, "kv4_tree_attention: null tensor");
+  if (!aligned(out, 16)) return set_error(kErrInvalid, "kv4_tree_attention: out must be 16-byte aligned");
+  const int64_t need = kv4_workspace(c, cache->dim, q, query->dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(kErrInvalid, "kv4_tree_attention: needs a 16-byte aligned workspace of %lld bytes, not %lld",
                      (long long)need, (long long)workspace_bytes);
   return kv4_attention(c, cache->dim, q, query->dtype, out, lse, (float*)workspace, (hipStream_t)stream);
 }

@@ -84,6 +84,7 @@ struct Kv4Query {
   int32_t window;        // 0: none
   float scale, softcap;  // softcap 0: none
   const float* slopes;   // [heads], or NULL
+  const int64_t* tree;   // [n], or NULL: the new tokens are one after another
 };
 
 // Bytes of workspace a call needs (0: none).

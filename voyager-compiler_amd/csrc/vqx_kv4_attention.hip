@@ -26,6 +26,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 struct Bf16 {};
 struct F16 {};
+// What becomes of scores: nothing but the mask of a prompt; a cap or slopes too;
+// all that of new tokens that are a tree.
+enum Mode { kPlain, kCurved, kTreed };
 template <typename T>
 struct Terms;
 template <>
@@ -138,6 +141,7 @@ struct TileRows {
   int pos_min, pos_max;
 };
 
+template <bool kTree = false>
 __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile, int tile_size,
                                               int step) {
   TileRows r;
@@ -152,6 +156,12 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
   const int r0 = tile * tile_size, r1 = r0 + tile_size < r.rows ? r0 + tile_size : r.rows;
   r.pos_min = r.base + r0 / q.group;
   r.pos_max = r1 > r0 ? r.base + (r1 - 1) / q.group : -1;
+  if constexpr (kTree) {
+    // a row is at a place from base - 1 (of no ancestors, itself not among them)
+    // to base + count - 1, and may see any of the new tokens
+    r.pos_min = r.base - 1;
+    if (r1 > r0) r.pos_max = r.base + r.count - 1;
+  }
   r.hi = r.pos_max + 1 < 0 ? 0 : ((uint32_t)(r.pos_max + 1) > c.cap ? (int)c.cap : r.pos_max + 1);
   r.lo = 0;
   if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(step - 1);
@@ -237,11 +247,10 @@ __device__ __forceinline__ Curve curve_of(const Kv4Query& q, int head) {
   return k;
 }
 
-// Capped and sloped scores of a lane's 8 tokens, of which token j is t0 + (j / 4)
-// 16 + j % 4.  tanh to fp32's own error: up to 0.75 an odd polynomial (fitted to
+// Capped scores of a lane's 8 tokens.  tanh to fp32's own error: up to 0.75 an odd polynomial (fitted to
 // 2^-25 of tanh), beyond by the exponential, which no wave computes whose
 // scores are all within the polynomial's range: a cap is mostly well above.
-__device__ __forceinline__ void curve_scores(const Curve& k, float (&x)[8], int pos, int t0) {
+__device__ __forceinline__ void cap_scores(const Curve& k, float (&x)[8]) {
   if (k.capped) {
     float most = 0.0f;
 #pragma unroll
@@ -272,10 +281,58 @@ __device__ __forceinline__ void curve_scores(const Curve& k, float (&x)[8], int 
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] *= k.scale;
   }
+}
+
+// Capped and sloped scores of a lane's 8 tokens, of which token j is t0 + (j / 4)
+// 16 + j % 4.
+__device__ __forceinline__ void curve_scores(const Curve& k, float (&x)[8], int pos, int t0) {
+  cap_scores(k, x);
   if (k.sloped) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] -= k.slope * (float)(pos - (t0 + (j >> 2) * 16 + (j & 3)));
   }
+}
+
+// A row among drafted tokens: what it sees of them and where that puts it.
+struct Line {
+  uint64_t mask;  // its ancestors and itself, as bits of the new tokens
+  int base;       // the first new token's place
+  int pos;        // the row's: as far behind the cached tokens as it has ancestors
+  bool live;
+};
+
+__device__ __forceinline__ Line line_of(const Kv4Query& q, const TileRows& rows, int token, bool live) {
+  Line l;
+  l.live = live;
+  l.base = rows.base;
+  const uint64_t all = rows.count < 64 ? (1ull << rows.count) - 1 : ~0ull;
+  l.mask = live ? (uint64_t)q.tree[rows.first + token] & all : 0;
+  l.pos = rows.base + __popcll(l.mask) - 1;
+  return l;
+}
+
+// How far before the row token t is: of the new tokens only the row's ancestors
+// count.  -1: it is not seen.
+__device__ __forceinline__ int distance(const Line& l, int t) {
+  const int d = t - l.base;
+  if (d < 0) return l.live ? l.pos - t : -1;
+  return d < 64 && (l.mask >> d & 1u) ? (int)__popcll(l.mask >> d >> 1) : -1;
+}
+
+// Slopes and mask of a row among drafted tokens on its capped scores; which of
+// the 8 it sees, as bits.  Token j is t0 + (j / 4) 16 + j % 4, bit u + 16 (j / 4) + j
+// % 4 of valid says that it is there.
+__device__ __forceinline__ uint32_t line_scores(const Curve& k, const Line& l, float (&x)[8], uint32_t valid, int u, int t0,
+                                                int window) {
+  uint32_t seen = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = (j >> 2) * 16 + (j & 3), away = distance(l, t0 + i);
+    const bool in = (valid >> (u + i) & 1u) && away >= 0 && (window == 0 || away < window);
+    x[j] = in ? x[j] - k.slope * (float)away : -__builtin_huge_valf();
+    seen |= (uint32_t)in << j;
+  }
+  return seen;
 }
 
 // The keys and values of one step of 32 tokens as a wave's loads leave them.
@@ -437,11 +494,20 @@ __device__ __forceinline__ void step_scores(const QueryTerms<D, T>& q, const Loa
 }
 
 // The row's curve and mask on those scores; seen: bit 4 i + r.
-template <bool kExtra>
-__device__ __forceinline__ void finish_scores(const Curve& k, float (&x)[8], uint32_t valid, int t0, int g, int pos,
-                                              int window, bool masked, uint32_t& seen) {
+template <Mode kMode>
+__device__ __forceinline__ void finish_scores(const Curve& k, const Line& line, float (&x)[8], uint32_t valid, int t0, int g,
+                                              int pos, int window, bool masked, uint32_t& seen) {
   seen = 0xFFu;
-  if (kExtra) {
+  if constexpr (kMode == kTreed) {
+    if (masked) {
+      cap_scores(k, x);
+      seen = line_scores(k, line, x, valid, 4 * g, t0 + 4 * g, window);
+    } else {
+      curve_scores(k, x, pos, t0 + 4 * g);
+    }
+    return;
+  }
+  if (kMode == kCurved) {
     curve_scores(k, x, pos, t0 + 4 * g);
   } else {
 #pragma unroll
@@ -503,7 +569,7 @@ __device__ __forceinline__ void fill_beyond(const Kv4Query& q, const TileRows& r
 // TB/s.  With fewer tokens a workgroup's own time shows: 4.5 us and 0.7 us for
 // each step of its waves (one sequence of 131073 tokens, 8 kv heads: 33 us, 4.3
 // TB/s; 16 of 4000 at most: 19 us).
-template <int D, typename T, bool kExtra, bool kWhole>
+template <int D, typename T, Mode kMode, bool kWhole>
 __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_rows_kernel(Kv4View c, Kv4Query q,
                                                                                         Kv4Plan plan, void* out,
                                                                                         float* lse, float* ws) {
@@ -520,7 +586,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
   if (!place_of(c, q, plan, place)) return;
   const uint32_t b = place.b, h = place.h, split = place.split;
   const int tile = place.tile;
-  const TileRows rows = tile_rows(c, q, b, tile, kRows, kStep);
+  const TileRows rows = tile_rows<kMode == kTreed>(c, q, b, tile, kRows, kStep);
   const int r = tile * kRows + n;
   const bool live = r < rows.rows;
   const int token = r / q.group, head = (int)h * q.group + r % q.group;
@@ -532,7 +598,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
   if (end > rows.hi) end = rows.hi;
   if (begin >= end && split > 0) return;
   const int steps = begin < end ? (end - begin + kStep - 1) / kStep : 0;
-  const int pos = live ? rows.base + token : -1;
+  Line line = {};
+  if constexpr (kMode == kTreed) line = line_of(q, rows, token, live);
+  const int pos = kMode == kTreed ? line.pos : (live ? rows.base + token : -1);
   const Curve curve = curve_of(q, live ? head : (int)h * q.group);
 
   float m = kLowest, l = 0.0f;
@@ -556,7 +624,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
       step_scores<D, T>(terms, s, x);
       const bool masked = needs_mask(rows, s.valid, s.t0, q.window);
       uint32_t seen;
-      finish_scores<kExtra>(curve, x, s.valid, s.t0, g, pos, q.window, masked, seen);
+      finish_scores<kMode>(curve, line, x, s.valid, s.t0, g, pos, q.window, masked, seen);
       float top = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = __builtin_fmaxf(top, x[j]);
@@ -776,7 +844,7 @@ constexpr int block_sub(int dim, int q_terms) { return dim * q_terms > 256 ? 1 :
 // fp16 relative to the largest scale that the workgroup had met, the same prompt
 // took 660 us; but values 2^36 below that scale came back as zeros, also where
 // it was another block's, or that of a token that the row does not see.
-template <int D, typename T, bool kExtra, bool kWhole>
+template <int D, typename T, Mode kMode, bool kWhole>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4View c, Kv4Query q, Kv4Plan plan, void* out,
                                                                          float* lse, float* ws) {
   constexpr int kTiles = D / 16;
@@ -795,7 +863,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   if (!place_of(c, q, plan, place)) return;
   const uint32_t b = place.b, h = place.h, split = place.split;
   const int tile = place.tile;
-  const TileRows rows = tile_rows(c, q, b, tile, kBlockRows, kBlockStep);
+  constexpr bool kTree = kMode == kTreed;
+  const TileRows rows = tile_rows<kTree>(c, q, b, tile, kBlockRows, kBlockStep);
   if (rows.count > q.most && tile == 0 && split == 0) fill_beyond<D, T>(q, rows, h, out, lse);
   if (tile * kBlockRows >= rows.rows) return;
   const int begin = rows.lo + (int)split * plan.chunk;
@@ -806,8 +875,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
 
   // the wave's own rows
   const int r0 = tile * kBlockRows + wave * kSub * 16;
-  const TileRows mine = tile_rows(c, q, b, tile * kWaves + wave, 16 * kSub, kStep);
+  const TileRows mine = tile_rows<kTree>(c, q, b, tile * kWaves + wave, 16 * kSub, kStep);
   int row[kSub], pos[kSub];
+  Line line[kSub];
   Curve curve[kSub];
   u32x4 terms[kSub][kKWords][Terms<T>::kQ];
 #pragma unroll
@@ -816,6 +886,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     const bool live = row[y] < rows.rows;
     const int token = row[y] / q.group, head = (int)h * q.group + row[y] % q.group;
     pos[y] = live ? rows.base + token : -1;
+    if constexpr (kTree) line[y] = line_of(q, rows, token, live), pos[y] = line[y].pos;
     curve[y] = curve_of(q, live ? head : (int)h * q.group);
     const int64_t at = (int64_t)(rows.first + token) * q.sn + (int64_t)head * q.sh;
 #pragma unroll
@@ -980,28 +1051,45 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     }
   };
   // which of a half step's scores the row sees, as bits
-  auto seen_of = [&](uint32_t valid, int t0, int at) {
+  auto seen_of = [&](uint32_t valid, int t0, int y) {
     uint32_t seen = 0;
+    const int at = pos[y];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int u = (j >> 2) * 16 + 4 * g + (j & 3), t = t0 + u;
-      seen |= (uint32_t)((valid >> u & 1u) && t <= at && (q.window == 0 || t > at - q.window)) << j;
+      if constexpr (kTree) {
+        const int away = distance(line[y], t);
+        seen |= (uint32_t)((valid >> u & 1u) && away >= 0 && (q.window == 0 || away < q.window)) << j;
+      } else {
+        seen |= (uint32_t)((valid >> u & 1u) && t <= at && (q.window == 0 || t > at - q.window)) << j;
+      }
     }
     return seen;
   };
-  const float scale = kExtra ? 1.0f : curve[0].scale;
+  const float scale = kMode != kPlain ? 1.0f : curve[0].scale;
   // curve and mask, and the references moved where a score passes them
   auto settle = [&](float (&x)[kSub][8], uint32_t valid, int t0) {
-    if (kExtra) {
-#pragma unroll
-      for (int y = 0; y < kSub; ++y) curve_scores(curve[y], x[y], pos[y], t0 + 4 * g);
-    }
-    if (needs_mask(mine, valid, t0, q.window)) {
+    const bool masked = needs_mask(mine, valid, t0, q.window);
+    if constexpr (kTree) {
 #pragma unroll
       for (int y = 0; y < kSub; ++y) {
-        const uint32_t seen = seen_of(valid, t0, pos[y]);
+        if (masked)
+          cap_scores(curve[y], x[y]), line_scores(curve[y], line[y], x[y], valid, 4 * g, t0 + 4 * g, q.window);
+        else
+          curve_scores(curve[y], x[y], pos[y], t0 + 4 * g);
+      }
+    } else {
+      if (kMode == kCurved) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : -__builtin_huge_valf();
+        for (int y = 0; y < kSub; ++y) curve_scores(curve[y], x[y], pos[y], t0 + 4 * g);
+      }
+      if (masked) {
+#pragma unroll
+        for (int y = 0; y < kSub; ++y) {
+          const uint32_t seen = seen_of(valid, t0, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[y][j] = seen >> j & 1u ? x[y][j] : -__builtin_huge_valf();
+        }
       }
     }
     float top[kSub];
@@ -1055,7 +1143,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int y = 0; y < kSub; ++y) {
-        const uint32_t seen = seen_of((uint32_t)(valid >> (32 * half)), t0 + 32 * half, pos[y]);
+        const uint32_t seen = seen_of((uint32_t)(valid >> (32 * half)), t0 + 32 * half, y);
 #pragma clang loop unroll(disable)
         for (int j = 0; j < 8; ++j) {
           const int t = t0 + 32 * half + (j >> 2) * 16 + 4 * g + (j & 3);
@@ -1173,7 +1261,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   }
   if (b >= c.seqs) return;
   const int n = (int)(id % (uint32_t)plan.rows), r = tile * plan.rows + n;
-  const TileRows rows = tile_rows(c, q, b, tile, plan.rows, plan.rows == kRows ? kStep : kBlockStep);
+  const int step = plan.rows == kRows ? kStep : kBlockStep;
+  const TileRows rows = q.tree ? tile_rows<true>(c, q, b, tile, plan.rows, step) : tile_rows(c, q, b, tile, plan.rows, step);
   if (r >= rows.rows) return;
   const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
   const int64_t size = (int64_t)plan.rows * (D + 2);
@@ -1441,7 +1530,9 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   };
   const int many = 64 * block_sub(dim, dtype == kBF16 ? 1 : (dtype == kF16 ? 2 : 3));
   const double steps = (double)c.kv * tiles_of(kRows) * (double)(span_of(q.most) / kStep);
-  const int64_t blocks = c.kv * tiles_of(many), room = span_of(many / q.group + 2);
+  // new tokens of a tile of `rows`, all of a sequence's where any may see any
+  auto tokens_of = [&](int64_t rows) { return q.tree ? (int64_t)q.most : rows / q.group + 2; };
+  const int64_t blocks = c.kv * tiles_of(many), room = span_of(tokens_of(many));
   const bool full = (int64_t)q.tokens.n * q.group >= c.seqs * (all < 128 ? all : 128);
   const bool whole = room <= 8 * kBlockStep ? blocks >= num_cus() : room <= kShortSpan && blocks > num_cus();
   p.rows = all > kRows && full && (whole || steps >= (many == 64 ? 2 : 1) * kManyTiles) ? many : kRows;
@@ -1450,7 +1541,7 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   // where most tiles would have no rows (32 sequences of up to 4000 tokens, one
   // with 512 new tokens, heads of 128: 115 us with all tiles, 37 with those there are)
   p.listed = 2 * there <= (int64_t)c.seqs * p.tiles && there < 1 << 25 ? (int32_t)there : 0;
-  const int64_t span = span_of(p.rows / q.group + 2);
+  const int64_t span = span_of(tokens_of(p.rows));
   // The tokens are cut as if every sequence filled its room, since the lengths are
   // not known here: with room for 131072, 16 sequences of 16000 take 111 us (55 with
   // room for 16000), 256 new tokens of 2000 104 (26).
@@ -1498,23 +1589,28 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
                   hipStream_t st) {
   if (q.tokens.n == 0 || c.seqs == 0 || q.most == 0) return kOk;
   const Kv4Plan p = kv4_plan(c, dim, q, dtype);
-  const bool extra = q.softcap != 0.0f || q.slopes;
+  const bool curved = q.softcap != 0.0f || q.slopes;
   const bool whole = !c.table || c.size % (p.rows == kRows ? kStep : kBlockStep) == 0;
   const int64_t slots = slots_of(c, p);
   if (slots * (p.splits > p.rows ? p.splits : p.rows) >= 1ll << 31)
     return set_error(kErrUnsupported, "kv4_attention: %lld tiles of %d splits do not fit a launch", (long long)slots,
                      p.splits);
   const dim3 grid((unsigned)(slots * p.splits));
+#define VQX_KV4_MODE(NAME, D, T, MODE)                                                                               \
+  do {                                                                                                             \
+    if (whole)                                                                                                     \
+      hipLaunchKernelGGL((NAME<D, T, MODE, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                 \
+    else                                                                                                           \
+      hipLaunchKernelGGL((NAME<D, T, MODE, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                \
+  } while (0)
 #define VQX_KV4_LAUNCH(NAME, D, T)                                                                                   \
   do {                                                                                                             \
-    if (extra && whole)                                                                                            \
-      hipLaunchKernelGGL((NAME<D, T, true, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                 \
-    else if (extra)                                                                                                \
-      hipLaunchKernelGGL((NAME<D, T, true, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                \
-    else if (whole)                                                                                                \
-      hipLaunchKernelGGL((NAME<D, T, false, true>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);                \
+    if (q.tree)                                                                                                    \
+      VQX_KV4_MODE(NAME, D, T, kTreed);                                                                            \
+    else if (curved)                                                                                               \
+      VQX_KV4_MODE(NAME, D, T, kCurved);                                                                           \
     else                                                                                                           \
-      hipLaunchKernelGGL((NAME<D, T, false, false>), grid, dim3(256), 0, st, c, q, p, out, lse, ws);               \
+      VQX_KV4_MODE(NAME, D, T, kPlain);                                                                            \
   } while (0)
 #define VQX_KV4_ROWS(D, T)                                                                                         \
   do {                                                                                                             \
@@ -1532,6 +1628,7 @@ int kv4_attention(const Kv4View& c, int dim, const Kv4Query& q, int dtype, void*
   VQX_KV4_TYPES(VQX_KV4_ROWS)
 #undef VQX_KV4_ROWS
 #undef VQX_KV4_LAUNCH
+#undef VQX_KV4_MODE
   return check_launch("kv4_attention");
 }
 

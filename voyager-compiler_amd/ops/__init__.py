@@ -21,5 +21,6 @@ from .kv4 import (  # noqa: F401
     kv4_evict,
     kv4_read,
     kv4_reserve,
+    kv4_tree_attention,
 )
 from .rotary import rotary, rotary_frequencies  # noqa: F401

@@ -68,6 +68,10 @@ _SCHEMAS = {
     "kv4_reserve": (
         "kv4_reserve(Tensor grow, Tensor(a!) lengths, Tensor(b!) table, Tensor(c!) free, Tensor(d!) count, "
         "SymInt page_size, SymInt n) -> (Tensor, Tensor, Tensor)"),
+    "kv4_tree_attention": (
+        "kv4_tree_attention(Tensor query, Tensor codes, Tensor scales, Tensor lengths, Tensor tree, Tensor? cu=None, "
+        "int? most=None, Tensor? table=None, *, float? scale=None, float softcap=0.0, int window=0, "
+        "Tensor? slopes=None) -> (Tensor, Tensor)"),
     "kv4_accept": (
         "kv4_accept(Tensor tree, Tensor drafts, Tensor sampled, Tensor(a!) codes, Tensor(b!) scales, "
         "Tensor(c!) lengths, Tensor? cu=None, Tensor? table=None) -> (Tensor, Tensor, Tensor)"),
@@ -90,14 +94,13 @@ def _refuse(what, message):
     raise ValueError(f"vqx: {what}: {message}")
 
 
-def _launch(name, device, *args):
-    """The library's entry point on the tensors' device and its current stream."""
-    at = device.index
-    stream = torch._C._cuda_getCurrentRawStream(at)
-    if at == torch.cuda.current_device():
+def _launch(name, t, *args):
+    """The library's entry point on t's device and that device's current stream."""
+    stream, at = _lib.stream_of(t), t.device.index
+    if at is None or at == torch.cuda.current_device():
         _lib.call(name, *args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(at):
             _lib.call(name, *args, stream)
 
 
@@ -277,7 +280,7 @@ def kv4_append_rotary(query, key, value, codes, scales, lengths, freqs, cu=None,
     offsets = _offsets(cu, n, c.seqs, what, device)
     t = _turn(freqs, positions, n, dim, interleaved, factor, False, what, device)
     out = q.new_empty((n, heads, dim))
-    _launch("vqx_kv4_append_rotary", device, c, t, q.data_ptr(), heads, qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn,
+    _launch("vqx_kv4_append_rotary", codes, c, t, q.data_ptr(), heads, qn, qh, k.data_ptr(), kn, kh, v.data_ptr(), vn,
             vh, tag, n, offsets, out.data_ptr())
     return out
 
@@ -303,17 +306,17 @@ def kv4_read(codes, scales, lengths, n, cu=None, table=None, dtype=torch.bfloat1
 _WS = {}
 
 
-def _workspace_bytes(c, qs, device, key):
-    """Workspace vqx_kv4_attention needs for these sizes on ``device`` (0: no
+def _workspace_bytes(c, qs, device, key, entry="vqx_kv4_attention"):
+    """Workspace that entry point needs for these sizes on ``device`` (0: no
     splits to join), cached per sizes."""
-    key = (c.pages_per_seq, c.page_size, c.kv_heads, c.dim, c.seqs, device.index, key)
+    key = (c.pages_per_seq, c.page_size, c.kv_heads, c.dim, c.seqs, device.index, entry, key)
     n = _WS.get(key)
     if n is None:
         if len(_WS) >= 4096:
             _WS.clear()
         got = ctypes.c_int64(0)
         with torch.cuda.device(device):
-            _lib.call("vqx_kv4_attention_workspace_size", c, qs, got)
+            _lib.call(entry + "_workspace_size", c, qs, got)
         n = _WS[key] = got.value
     return n
 
@@ -337,6 +340,34 @@ def kv4_attention(query, codes, scales, lengths, cu=None, most=None, table=None,
     need = _workspace_bytes(c, qs, device, key)
     ws = codes.new_empty(need) if need else None  # held until the kernels that use it are enqueued
     _lib.call("vqx_kv4_attention", c, qs, out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), need, _lib.stream_of(codes))
+    return out, lse
+
+
+@_impl("kv4_tree_attention")
+def kv4_tree_attention(query, codes, scales, lengths, tree, cu=None, most=None, table=None, *, scale=None, softcap=0.0,
+                       window=0, slopes=None):
+    """kv4_attention of new tokens that are a tree of drafts, 64 of a sequence at
+    most (``most``, where there are more in all).  tree (int64 [n]): bit j of a
+    token's mask says that it sees its sequence's new token j: its ancestors and
+    itself.  All see the cached tokens before the new ones.  For ``window`` and
+    ``slopes`` a token stands as far behind those as it has ancestors, and an
+    ancestor as far before it as there are others between.  Bits of tokens that
+    the sequence does not have do not count."""
+    what = "kv4_tree_attention"
+    _lib.require_device(codes, what)
+    c = _cache(codes, scales, lengths, table, what)
+    device = codes.device
+    qs, q, key = _query(query, c, device, cu, most, scale, softcap, window, slopes, what)
+    n = key[0]
+    masks = _int64(tree, n, "tree", what, device)
+    longest = n // c.seqs if cu is None and c.seqs else qs.most or n
+    if longest > 64:
+        _refuse(what, f"up to {longest} new tokens of a sequence, 64 at most (say most if none has more)")
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(key[:2], dtype=torch.float32)
+    need = _workspace_bytes(c, qs, device, key, "vqx_kv4_tree_attention")
+    ws = codes.new_empty(need) if need else None  # held until the kernels that use it are enqueued
+    _launch("vqx_kv4_tree_attention", codes, c, qs, masks, out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), need)
     return out, lse
 
 
@@ -423,7 +454,7 @@ def kv4_reserve(grow, lengths, table, free, count, page_size, n):
              _int32(free, free.shape[0], "free", what, device), _int32(count, 1, "count", what, device))
     cu, positions = lengths.new_empty(seqs + 1), lengths.new_empty(n)
     slots = lengths.new_empty(n, dtype=torch.int64)
-    _launch("vqx_kv4_reserve", device, *given, seqs, table.shape[1], free.shape[0], page_size, n, cu.data_ptr(),
+    _launch("vqx_kv4_reserve", lengths, *given, seqs, table.shape[1], free.shape[0], page_size, n, cu.data_ptr(),
             positions.data_ptr(), slots.data_ptr())
     return cu, positions, slots
 
@@ -460,7 +491,7 @@ def kv4_accept(tree, drafts, sampled, codes, scales, lengths, cu=None, table=Non
     given = [_int64(t, n, name, what, device) for t, name in ((tree, "tree"), (drafts, "drafts"), (sampled, "sampled"))]
     path, accepted = lengths.new_empty(n), lengths.new_empty(c.seqs)
     follows = sampled.new_empty(c.seqs)
-    _launch("vqx_kv4_accept", device, c, *given, n, offsets, path.data_ptr(), accepted.data_ptr(), follows.data_ptr())
+    _launch("vqx_kv4_accept", codes, c, *given, n, offsets, path.data_ptr(), accepted.data_ptr(), follows.data_ptr())
     return path, accepted, follows
 
 
@@ -507,3 +538,8 @@ def _(grow, lengths, table, free, count, page_size, n):
 @torch.library.register_fake("quantized_ops::kv4_accept")
 def _(tree, drafts, sampled, codes, scales, lengths, cu=None, table=None):
     return lengths.new_empty(tree.shape[0]), torch.empty_like(lengths), sampled.new_empty(lengths.shape[0])
+
+
+@torch.library.register_fake("quantized_ops::kv4_tree_attention")
+def _(query, codes, scales, lengths, tree, cu=None, most=None, table=None, **kwargs):
+    return query.new_empty(query.shape), query.new_empty(query.shape[:2], dtype=torch.float32)

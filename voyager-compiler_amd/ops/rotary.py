@@ -36,7 +36,7 @@ def rotary(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     t = kv4._turn(freqs, positions, n, dim, interleaved, factor, back, what, device)
     x, sn, sh, tag = kv4._rows(x, None, dim, "x", what, device)
     out = x.new_empty((n, heads, dim))
-    kv4._launch("vqx_rotary", device, x.data_ptr(), tag, n, heads, dim, sn, sh, t, out.data_ptr())
+    kv4._launch("vqx_rotary", x, x.data_ptr(), tag, n, heads, dim, sn, sh, t, out.data_ptr())
     return out
 
 
