@@ -868,6 +868,29 @@ int vqx_kv4_reserve(const int32_t* grow, int32_t* lengths, int32_t* table, int32
 int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_t* drafts, const int64_t* sampled,
                    int64_t n, const int32_t* cu, int32_t* path, int32_t* accepted, int64_t* next, vqx_stream_t stream);
 
+/*
+ * A token for each row of logits [rows, vocab] (F32, BF16 or F16; stride
+ * elements between rows) from a given number random[row] in [0, 1) (this
+ * library's own).  A token's weight is w = 2^40 exp((x - the row's largest) /
+ * temperature), rounded to a whole number, in 64 bits; all sums are exact.  Of
+ * a row's tokens, from the largest logit down and equal ones by index, are kept
+ *   the first top_k (0 or less, or vocab: all);
+ *   of those, each before which less than top_p of their sum lies (1 or more, or
+ *   NaN: all; 0 or less: the first);
+ *   of those, the ones with w >= min_p 2^40 (0 or less, or NaN: all; above 1 as 1).
+ * tokens[row] (int64): in the order of their indexes the first whose sum with
+ * those before it is above floor(random * total) (random below 0 or NaN as 0,
+ * from 1 on the last); chances[row] (fp32): log(w / total).  A temperature of
+ * 0 or less, or NaN: the first of the largest logits, chance 0.  A NaN is never
+ * drawn; a row without a logit above -inf has token -1 and chance -inf; infinite
+ * ones are as likely as each other, and no others are drawn.
+ * temperature, top_k, top_p, min_p: [rows], int32 for top_k and fp32 for the
+ * others, or NULL (1, and none).  vocab: 1 .. 2^22.
+ */
+int vqx_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride,
+                      const float* random, const float* temperature, const int32_t* top_k, const float* top_p,
+                      const float* min_p, int64_t* tokens, float* chances, vqx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

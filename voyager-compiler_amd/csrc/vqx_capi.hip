@@ -7,6 +7,7 @@
 #include "vqx_kernels.h"
 #include "vqx_kv4.h"
 #include "vqx_rotary.h"
+#include "vqx_sampling.h"
 
 namespace vqx {
 
@@ -887,6 +888,23 @@ int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_
   if ((n > 0 && (!tree || !drafts || !sampled || !path)) || (c.seqs > 0 && (!accepted || !next)))
     return set_error(kErrInvalid, "kv4_accept: null tensor");
   return kv4_accept(c, cache->dim, q, tree, drafts, sampled, path, accepted, next, (hipStream_t)stream);
+}
+
+int vqx_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride,
+                      const float* random, const float* temperature, const int32_t* top_k, const float* top_p,
+                      const float* min_p, int64_t* tokens, float* chances, vqx_stream_t stream) {
+  g_err[0] = 0;
+  const int rc = kv4_float(dtype, "sample_tokens");
+  if (rc != kOk) return rc;
+  if (rows < 0 || rows >= 1ll << 31) return set_error(kErrInvalid, "sample_tokens: %lld rows", (long long)rows);
+  // the weights' sum is to stay below 2^63
+  if (vocab < 1 || vocab > 1ll << 22)
+    return set_error(kErrInvalid, "sample_tokens: 1 to 2^22 logits in a row, not %lld", (long long)vocab);
+  if (rows == 0) return kOk;
+  if (!logits || !random || !tokens || !chances) return set_error(kErrInvalid, "sample_tokens: null tensor");
+  if (!aligned(logits, dtype == kF32 ? 4 : 2)) return set_error(kErrInvalid, "sample_tokens: logits are not aligned");
+  return sample(Sampling{logits, stride, rows, (int32_t)vocab, random, temperature, top_k, top_p, min_p, tokens, chances},
+                dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

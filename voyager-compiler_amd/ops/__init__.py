@@ -1,4 +1,5 @@
-"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``, ``kv4.py``, ``rotary.py``)."""
+"""``torch.ops.quantized_ops`` on MI355X kernels (see ``quantized.py``, ``kv4.py``,
+``rotary.py``, ``sampling.py``)."""
 
 from .quantized import (  # noqa: F401
     calculate_mx_qparam,
@@ -24,3 +25,4 @@ from .kv4 import (  # noqa: F401
     kv4_tree_attention,
 )
 from .rotary import rotary, rotary_frequencies  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401
