@@ -31,6 +31,9 @@ constexpr float kNone = -__builtin_huge_valf();
 
 typedef unsigned long long u64;
 
+// of a lambda: what it takes stays in registers
+#define VQX_INLINE __attribute__((always_inline))
+
 // ---------------------------------------------------------------------------
 // a row's logits, 8 at a time from aligned addresses
 // ---------------------------------------------------------------------------
@@ -157,13 +160,27 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
 // ---------------------------------------------------------------------------
 // a workgroup's sums
 // ---------------------------------------------------------------------------
+// What lane i has from another lane of its row or from the end of a row before it,
+// 0 where there is none.
+template <int kControl, int kRows>
+__device__ __forceinline__ u64 from_lane(u64 x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, kRows, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, kRows, 0xF, false);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32 | lo;
+}
+// The sum up to each lane: by shifts within rows of 16 lanes, then the ends of
+// the rows before (a scan by permutes through LDS takes five times as long).
 __device__ __forceinline__ u64 wave_scan(u64 x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const u64 y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  x += from_lane<0x111, 0xF>(x);
+  x += from_lane<0x112, 0xF>(x);
+  x += from_lane<0x114, 0xF>(x);
+  x += from_lane<0x118, 0xF>(x);
+  x += from_lane<0x142, 0xA>(x);
+  x += from_lane<0x143, 0xC>(x);
   return x;
 }
 
@@ -173,25 +190,30 @@ struct Shared {
   uint32_t count[kBins];
   double powers[64];
   float tops[kWaves];
-  u64 sums[kWaves];
+  u64 sums[4][kWaves];
   u64 found[4];
-  int at, listed;
+  int at, listed, spot[3], near[3];
 };
 
-// The sum of what the threads before this one have, and of all.
+// The sum of what the threads before this one have, and of all.  Callers that
+// follow each other without a barrier have slots of their own and no fence.
+template <int kSlot = 0, bool kFence = true>
 __device__ __forceinline__ u64 scan_before(Shared& s, u64 x, u64& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u64 upto = wave_scan(x);
+  if (kFence) __syncthreads();
+  if (lane == 63) s.sums[kSlot][wave] = upto;
   __syncthreads();
-  if (lane == 63) s.sums[wave] = upto;
-  __syncthreads();
-  u64 before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? s.sums[w] : 0;
-    all += s.sums[w];
-  }
+  // every row of 16 lanes has the waves' sums, summed up to each
+  static_assert(kWaves == 16, "");
+  u64 sum = s.sums[kSlot][lane & 15];
+  sum += from_lane<0x111, 0xF>(sum);
+  sum += from_lane<0x112, 0xF>(sum);
+  sum += from_lane<0x114, 0xF>(sum);
+  sum += from_lane<0x118, 0xF>(sum);
+  const int w = __builtin_amdgcn_readfirstlane(wave);
+  const u64 before = w > 0 ? lane_of(sum, w - 1) : 0;
+  all = lane_of(sum, 15);
   return before + upto - x;
 }
 __device__ __forceinline__ u64 sum_of(Shared& s, u64 x) {
@@ -237,29 +259,83 @@ __device__ __forceinline__ Cut find_bin(Shared& s, const Cut& base, u64 most, do
   return c;
 }
 
+// What a share is of all: the weight that kept tokens have before them is below
+// it (no share at all is the first token's).
+__device__ __forceinline__ double share_of(float share, u64 all) {
+  return share > 0.0f ? (double)share * (double)all : 0.5;
+}
+
 __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0, s.mass[i] = 0;
   __syncthreads();
 }
 
-// A row's logits, 8 to a call: what(logits, the first one's index).  Four loads
-// are on their way before the first is used.
+// A row's first vectors, held in registers: 64 of each thread, so that a row of
+// 131072 two-byte logits is read once (256 such rows read a second time, from
+// beyond the L2s, take 13 us).
+template <typename T>
+struct Held {
+  static constexpr int kVectors = std::is_same<T, float>::value ? 8 : 16;
+  Raw<T> r[kVectors];
+
+  __device__ __forceinline__ void load(const Row<T>& row) {
+    const int v0 = row.whole + (int)threadIdx.x;
+#pragma unroll
+    for (int a = 0; a < kVectors; ++a) {
+      if (row.whole + a * kThreads >= row.past) break;
+      r[a] = row.raw(v0 + a * kThreads < row.past ? v0 + a * kThreads : row.past - 1);
+    }
+  }
+};
+
+// A row's whole vectors from the begin-th of each thread on, what(raw, the first
+// element's index); four loads are on their way before the first is used.
 template <typename T, typename What>
-__device__ __forceinline__ void each_vector(const Row<T>& row, What what) {
+__device__ __forceinline__ void each_raw(const Row<T>& row, What what, int begin = 0) {
   constexpr int kAhead = 4;
-  for (int v = row.whole + (int)threadIdx.x; v < row.past; v += kAhead * kThreads) {
+  for (int v = row.whole + begin * kThreads + (int)threadIdx.x; v < row.past; v += kAhead * kThreads) {
     Raw<T> r[kAhead];
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) r[a] = row.raw(v + a * kThreads < row.past ? v + a * kThreads : v);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       if (v + a * kThreads >= row.past) break;
-      float x[8];
-      values(r[a], x);
-      what(x, row.first(v + a * kThreads));
+      what(r[a], row.first(v + a * kThreads));
     }
   }
+}
+struct NotHeld {};
+template <typename H>
+constexpr int held_vectors() {
+  if constexpr (std::is_same<H, NotHeld>::value)
+    return 0;
+  else
+    return H::kVectors;
+}
+template <typename T, typename What>
+__device__ __forceinline__ void each_raw(const Row<T>& row, NotHeld, What what) {
+  each_raw(row, what);
+}
+template <typename T, typename What>
+__device__ __forceinline__ void each_raw(const Row<T>& row, const Held<T>& held, What what) {
+  const int v0 = row.whole + (int)threadIdx.x;
+#pragma unroll
+  for (int a = 0; a < Held<T>::kVectors; ++a) {
+    if (row.whole + a * kThreads >= row.past) break;
+    if (v0 + a * kThreads < row.past) what(held.r[a], row.first(v0 + a * kThreads));
+  }
+  each_raw(row, what, Held<T>::kVectors);
+}
+// A row's logits, 8 to a call: what(logits, the first one's index).
+template <typename T, typename What, typename H = NotHeld>
+__device__ __forceinline__ void each_vector(const Row<T>& row, What what, const H& held = H()) {
+  auto one = [&](const Raw<T>& r, int e) VQX_INLINE {
+    float x[8];
+    values(r, x);
+    what(x, e);
+  };
+  each_raw(row, held, one);
   // the first and the last, where they are parts of one
   const int part = threadIdx.x == 0 && row.whole > 0 ? 0 : (threadIdx.x == 64 && row.past >= row.whole ? row.past : -1);
   if (part >= 0 && part < row.vectors) {
@@ -373,141 +449,256 @@ __device__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut
   return o;
 }
 
-// The tokens of a bin that the listed ones are in, of those up to `cut`, gathered
-// behind each other: order and weight.  Their number, or more than kMostNear.
-constexpr int kEach = kMostListed / kThreads;
-constexpr int kMostNear = 512;
+constexpr int kEach = kMostListed / kThreads;  // listed tokens of a thread
+constexpr int kMostNear = 512;                 // tokens of a bin that are compared with each other
 
-template <typename In>
-__device__ __forceinline__ int gather_near(Shared& s, const u64 (&o)[kEach], const u64 (&w)[kEach], In in) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.listed = 0;
-  __syncthreads();
+// The indexes of a row's tokens whose bins are up to `last`, and perhaps of some
+// in the next, into the list; s.listed: their number.
+template <typename T, typename H>
+__device__ __forceinline__ void list_tokens(Shared& s, const Row<T>& row, const H& held, const Scale& scale, int last) {
+  uint32_t* list = reinterpret_cast<uint32_t*>(s.list);
+  // Logits are compared as they are, bf16 in the upper half of a word with the
+  // lower half behind it: that moves them by less than their last place, 2^-7 of
+  // them (an infinity would become a NaN; where there is one it is compared by
+  // itself).  The border is lower by that and by the roundings here.
+  const float span = (float)(last + 1) / scale.coarse;
+  float least = scale.top - span;
+  least -= __builtin_fabsf(least) * 0x1p-6f + (__builtin_fabsf(scale.top) + span) * 0x1p-20f + 0x1p-100f;
+  if (!(least > -3.4028235e38f)) least = -3.4028235e38f;  // every finite one
+  const bool infinite = scale.top == -kNone;
+  if (infinite) least = scale.top;
+  // a bit for each element, from the highest down
+  auto marks = [&](const Raw<T>& r, bool there, uint32_t bits) VQX_INLINE -> uint32_t {
+    if constexpr (std::is_same<T, Bf16>::value) {
 #pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    if (in(j)) {
-      const int at = atomicAdd(&s.listed, 1);
-      if (at < kMostNear) s.list[2 * at] = o[j], s.list[2 * at + 1] = w[j];
+      for (int j = 0; j < 4; ++j) {
+        bits = 2 * bits + (u2f(r.a[j] << 16) >= least);
+        bits = 2 * bits + (u2f(infinite ? r.a[j] & 0xFFFF0000u : r.a[j]) >= least);
+      }
+    } else {
+      float x[8];
+      values(r, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits = 2 * bits + (x[j] >= least);
     }
-  __syncthreads();
-  return s.listed;
+    return there ? bits : bits & ~0xFFu;
+  };
+  // one addition to the list's length for a wave, then a marked element of each
+  // lane at a time
+  auto put = [&](auto& bits, int v0) VQX_INLINE {
+    constexpr int kWords = sizeof(bits) / 4;
+    int n = 0;
+#pragma unroll
+    for (int g = 0; g < kWords; ++g) n += __popc(bits[g]);
+    const u64 upto = wave_scan((u64)n);
+    const int all = (int)lane_of(upto, 63);
+    if (all == 0) return;
+    int at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(&s.listed, all);
+    at = __builtin_amdgcn_readfirstlane(at) + (int)upto - n;
+#pragma unroll
+    for (int g = 0; g < kWords; ++g) {
+      while (bits[g]) {
+        const int i = __builtin_clz(bits[g]);
+        bits[g] &= ~(0x80000000u >> i);
+        if (at < kMostListed) list[at] = (uint32_t)(row.first(v0 + (4 * g + i / 8) * kThreads) + i % 8);
+        ++at;
+      }
+    }
+  };
+  const int v0 = row.whole + (int)threadIdx.x;
+  constexpr int kHeld = held_vectors<H>();
+  if constexpr (kHeld > 0) {
+    uint32_t bits[kHeld / 4];
+#pragma unroll
+    for (int g = 0; g < kHeld / 4; ++g) {
+      bits[g] = 0;
+      if (row.whole + 4 * g * kThreads >= row.past) continue;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) bits[g] = marks(held.r[4 * g + a], v0 + (4 * g + a) * kThreads < row.past, bits[g]);
+    }
+    put(bits, v0);
+  }
+  for (int v = kHeld; row.whole + v * kThreads < row.past; v += 4) {
+    Raw<T> r[4];
+    const int first = v0 + v * kThreads;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) r[a] = row.raw(first + a * kThreads < row.past ? first + a * kThreads : row.past - 1);
+    uint32_t bits[1] = {0};
+#pragma unroll
+    for (int a = 0; a < 4; ++a) bits[0] = marks(r[a], first + a * kThreads < row.past, bits[0]);
+    put(bits, first);
+  }
+  // what is not in whole vectors, a thread each
+  const int head = row.whole ? (8 - row.before < row.size ? 8 - row.before : row.size) : 0, tail = row.first(row.past);
+  const int i = threadIdx.x < 8 ? (int)threadIdx.x : tail + (int)threadIdx.x - 8;
+  if (threadIdx.x < 8 ? i < head : (threadIdx.x < 16 && i >= head && i < row.size)) {
+    if (element(row.base, (int64_t)i + row.before, T()) >= least) {
+      const int at = atomicAdd(&s.listed, 1);
+      if (at < kMostListed) list[at] = (uint32_t)i;
+    }
+  }
 }
 
 // The token drawn where all that can be kept lies in bins up to `last` and those
 // have few tokens: they are listed, and what is left is about the list.  most:
-// tokens kept by count, which end in bin `at`, 0 for all; mass: what a share is of,
-// where it is not of the first `most`.
-enum Few { kDrawn, kTooMany, kTooNear };  // kTooNear: and the masses of the bins are gone
-template <typename T>
-__device__ Few few(Shared& s, const Row<T>& row, const Scale& scale, const Sampling& p, int64_t r, int last, u64 most,
-                   const Cut& at, bool by_share, float share, u64 mass, double bar) {
-  uint32_t n = 0;
-  for (int b = threadIdx.x; b <= last; b += kThreads) n += s.count[b];
-  const u64 all = sum_of(s, n);
-  if (all > (u64)kMostListed) return kTooMany;
-  __syncthreads();
+// tokens kept by count, 0 for all; mass: what a share is of, where it is not of
+// the first `most`.  A cut is found by finer bins and, in the one where it falls,
+// by comparing that one's tokens with each other.  The histogram is gone
+// afterwards.
+enum Few { kDrawn, kTooMany, kTooNear };
+__device__ __forceinline__ u64* index_bins(Shared& s) {
+  static_assert(kMostListed / 2 >= kBins && kMostListed / 2 >= 2 * 2 * kMostNear, "");
+  return s.list + kMostListed / 2;  // behind the list of tokens and those of near ones
+}
+// What few() finds: needs a barrier on either side.
+__device__ __forceinline__ void clear_few(Shared& s) {
+  const int b0 = 2 * (int)threadIdx.x;
+  u64* drawn = index_bins(s);
+  s.count[b0] = 0, s.count[b0 + 1] = 0, s.mass[b0] = 0, s.mass[b0 + 1] = 0, drawn[b0] = 0, drawn[b0 + 1] = 0;
+  if (threadIdx.x < 3) s.spot[threadIdx.x] = kBins, s.near[threadIdx.x] = 0;
   if (threadIdx.x == 0) s.listed = 0;
+}
+template <typename T, typename H>
+__device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, const Scale& scale, const Sampling& p, int64_t r,
+                   int last, u64 most, bool by_share, float share, u64 mass, double bar) {
+  const int b0 = 2 * (int)threadIdx.x;
+  u64* drawn = index_bins(s);
+  list_tokens(s, row, held, scale, last);
   __syncthreads();
-  each_vector(row, [&](const float(&x)[8], int e) {
-    bool any = false;
-    int b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = bin_of(scale, x[j]), any |= b[j] <= last;
-    if (!any) return;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (b[j] <= last) {
-        const int at = atomicAdd(&s.listed, 1);
-        if (at < kMostListed) s.list[at] = order(sound(x[j]), e + j);
-      }
-  });
-  __syncthreads();
-  const int listed = s.listed < kMostListed ? s.listed : kMostListed;
+  const int listed = s.listed;
+  if (listed > kMostListed) return kTooMany;
+  const uint32_t* list = reinterpret_cast<const uint32_t*>(s.list);
   u64 o[kEach], w[kEach];
   int bin[kEach];
   bool keeps[kEach];
+  float x[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int i = j * kThreads + (int)threadIdx.x;
     keeps[j] = i < listed;
-    o[j] = keeps[j] ? s.list[i] : ~0ull;
-    const float x = logit_of(o[j]);
-    w[j] = keeps[j] ? weight(scale, x) : 0;
-    bin[j] = keeps[j] ? bin_of(scale, x) : kBins;
+    const uint32_t at = list[keeps[j] ? i : 0];
+    x[j] = keeps[j] ? sound(element(row.base, (int64_t)at + row.before, T())) : kNone;
+    o[j] = order(x[j], (int)at);
   }
-  const Cut none = {kBins, 0, 0};
-  if (most > 0 && at.bin < kBins) {
-    const int near = gather_near(s, o, w, [&](int j) { return bin[j] == at.bin; });
-    if (near > kMostNear) return kTooNear;
+  const float fine = (float)kBins / (float)(last + 1);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      if (bin[j] != at.bin) {
-        keeps[j] = keeps[j] && bin[j] < at.bin;
-        continue;
+  for (int j = 0; j < kEach; ++j) {
+    w[j] = 0, bin[j] = kBins;
+    if (j * kThreads >= listed) continue;
+    const float y = x[j] == scale.top ? 0.0f : (scale.top - x[j]) * scale.coarse;
+    keeps[j] = keeps[j] && y < (float)(last + 1);
+    if (!keeps[j]) continue;
+    w[j] = weight(scale, x[j]);
+    bin[j] = (int)(y * fine);
+    if (bin[j] >= kBins) bin[j] = kBins - 1;
+  }
+  // the tokens of one bin, order and weight, each cut's in one half of the list
+  auto gather_near = [&](int which, int half, auto in) {
+    u64* near = s.list + half * 2 * kMostNear;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (keeps[j] && in(j)) {
+        const int at = atomicAdd(&s.near[which], 1);
+        if (at < kMostNear) near[2 * at] = o[j], near[2 * at + 1] = w[j];
       }
-      u64 rank = at.count;
-      for (int i = 0; i < near; ++i) rank += s.list[2 * i] < o[j];
-      keeps[j] = rank < most;
+    __syncthreads();
+    return near;
+  };
+  if (most > 0) {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (keeps[j]) atomicAdd(&s.count[bin[j]], 1u);
+    __syncthreads();
+    const u64 c0 = s.count[b0], c1 = s.count[b0 + 1];
+    u64 all;
+    const u64 before = scan_before<1, false>(s, c0 + c1, all);
+    if (before < most && before + c0 + c1 >= most) {
+      const bool second = before + c0 < most;
+      s.spot[0] = b0 + second, s.found[0] = second ? before + c0 : before;
+    }
+    __syncthreads();
+    const int spot = s.spot[0];
+    if (spot < kBins) {
+      const u64 first = s.found[0];
+      const u64* near = gather_near(0, 0, [&](int j) { return bin[j] == spot; });
+      const int n = s.near[0];
+      if (n > kMostNear) return kTooNear;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (bin[j] == spot) {
+          u64 rank = first;
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) rank += near[2 * i] < o[j];
+          keeps[j] = keeps[j] && rank < most;
+        } else {
+          keeps[j] = keeps[j] && bin[j] < spot;
+        }
+      }
     }
   }
   if (by_share) {
-    // the masses of the bins, and of all where it is of the first `most`
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
-    __syncthreads();
-    u64 mine = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
-      if (keeps[j]) atomicAdd(&s.mass[bin[j]], w[j]), mine += w[j];
-    if (most > 0) mass = sum_of(s, mine);
+      if (keeps[j]) atomicAdd(&s.mass[bin[j]], w[j]);
     __syncthreads();
-    const double wanted = share > 0.0f ? (double)share * (double)mass : 0.5;
-    const Cut c = find_bin<true>(s, none, 0, wanted);
-    if (c.bin < kBins) {
-      const int near = gather_near(s, o, w, [&](int j) { return keeps[j] && bin[j] == c.bin; });
-      if (near > kMostNear) return kTooNear;
+    const u64 m0 = s.mass[b0], m1 = s.mass[b0 + 1];
+    u64 all;
+    const u64 before = scan_before<2, false>(s, m0 + m1, all);
+    const double wanted = share_of(share, most > 0 ? all : mass);
+    if ((double)before < wanted && (double)(before + m0 + m1) >= wanted) {
+      const bool second = (double)(before + m0) < wanted;
+      s.spot[1] = b0 + second, s.found[1] = second ? before + m0 : before;
+    }
+    __syncthreads();
+    const int spot = s.spot[1];
+    if (spot < kBins) {
+      const u64 first = s.found[1];
+      const u64* near = gather_near(1, 1, [&](int j) { return bin[j] == spot; });
+      const int n = s.near[1];
+      if (n > kMostNear) return kTooNear;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
-        if (!keeps[j] || bin[j] != c.bin) {
-          keeps[j] = keeps[j] && bin[j] < c.bin;
-          continue;
+        if (!keeps[j]) continue;
+        if (bin[j] == spot) {
+          u64 sum = first;
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) sum += near[2 * i] < o[j] ? near[2 * i + 1] : 0;
+          keeps[j] = (double)sum < wanted;
+        } else {
+          keeps[j] = bin[j] < spot;
         }
-        u64 before = c.mass;
-        for (int i = 0; i < near; ++i) before += s.list[2 * i] < o[j] ? s.list[2 * i + 1] : 0;
-        keeps[j] = (double)before < wanted;
       }
     }
   }
   // the kept ones by their index: bins of as many indexes, and in the bin where
   // the random number falls one by one
   const int shift = 32 - __builtin_clz((unsigned)(p.vocab - 1) | (kBins - 1)) - 11;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
-  __syncthreads();
-  u64 mine = 0;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     keeps[j] = keeps[j] && w[j] > 0 && (double)w[j] >= bar;
-    if (keeps[j]) atomicAdd(&s.mass[(uint32_t)o[j] >> shift], w[j]), mine += w[j];
-  }
-  const u64 total = sum_of(s, mine), target = target_of(p.random[r], total);
-  const int b0 = 2 * (int)threadIdx.x;
-  u64 sum;
-  const u64 m0 = s.mass[b0], m1 = s.mass[b0 + 1], before = scan_before(s, m0 + m1, sum);
-  if (target >= before && target < before + m0 + m1) {
-    const bool second = target >= before + m0;
-    s.at = b0 + second, s.found[0] = second ? before + m0 : before;
+    if (keeps[j]) atomicAdd(&drawn[(uint32_t)o[j] >> shift], w[j]);
   }
   __syncthreads();
-  const int run = s.at;
-  const u64 rest = target - s.found[0];
-  const int near = gather_near(s, o, w, [&](int j) { return keeps[j] && (int)((uint32_t)o[j] >> shift) == run; });
-  if (near > kMostNear) return kTooNear;
+  u64 total;
+  const u64 m0 = drawn[b0], m1 = drawn[b0 + 1], before = scan_before<3, false>(s, m0 + m1, total);
+  const u64 target = target_of(p.random[r], total);
+  if (target >= before && target < before + m0 + m1) {
+    const bool second = target >= before + m0;
+    s.spot[2] = b0 + second, s.found[2] = second ? before + m0 : before;
+  }
+  __syncthreads();
+  const int spot = s.spot[2];
+  const u64 rest = target - s.found[2];
+  auto here = [&](int j) { return (int)((uint32_t)o[j] >> shift) == spot; };
+  const u64* near = gather_near(2, 0, here);
+  const int n = s.near[2];
+  if (n > kMostNear) return kTooNear;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    if (!keeps[j] || (int)((uint32_t)o[j] >> shift) != run) continue;
+    if (!keeps[j] || !here(j)) continue;
     u64 upto = 0;
-    for (int i = 0; i < near; ++i) upto += (uint32_t)s.list[2 * i] < (uint32_t)o[j] ? s.list[2 * i + 1] : 0;
+    for (int i = 0; i < n; ++i) upto += (uint32_t)near[2 * i] < (uint32_t)o[j] ? near[2 * i + 1] : 0;
     if (rest >= upto && rest < upto + w[j]) {
       p.tokens[r] = (int64_t)(uint32_t)o[j];
       p.chances[r] = (float)log((double)w[j] / (double)total);
@@ -525,13 +716,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
   const Row<T> row(p.logits, r * p.stride, p.vocab);
+  Held<T> held;
+  held.load(row);
+  const float t = p.temperature ? p.temperature[r] : 1.0f;
+  const int k = p.top_k ? p.top_k[r] : 0;
+  const float share = p.top_p ? p.top_p[r] : 1.0f, least = p.min_p ? p.min_p[r] : 0.0f;
   if (tid < 64) s.powers[tid] = exp2((double)tid / 64.0);
-
+  clear_few(s);
   float top = kNone;
-  each_vector(row, [&](const float(&x)[8], int) {
+  each_vector(row, [&](const float(&x)[8], int) VQX_INLINE {
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, x[j]);  // a NaN is no maximum
-  });
+  }, held);
+  const float mine = top;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
   if (lane == 0) s.tops[wave] = top;
@@ -539,7 +736,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) top = __builtin_fmaxf(top, s.tops[w]);
   top += 0.0f;
-  const float t = p.temperature ? p.temperature[r] : 1.0f;
   if (top == kNone || !(t > 0.0f)) {
     // the first that is the largest
     int at = p.vocab;
@@ -566,76 +762,91 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   scale.coarse = coarse < 1e30 ? (float)coarse : 1e30f;
   scale.powers = s.powers;
 
-  const int k = p.top_k ? p.top_k[r] : 0;
-  const float share = p.top_p ? p.top_p[r] : 1.0f, least = p.min_p ? p.min_p[r] : 0.0f;
   const bool by_count = k > 0 && k < p.vocab, by_share = share < 1.0f;
   const double bar = least > 0.0f ? (least < 1.0f ? (double)least * kUnit : kUnit) : 0.0;
   u64 cut = ~0ull;
-  if (by_count || by_share || bar > 0.0) {
-    const Cut none = {kBins, 0, 0};
-    Cut at = none;
-    u64 mass = 0;
-    // of the bins' masses none is needed where the first k tokens, or those above
-    // a share of the largest, are few
-    auto count_bins = [&](auto with_masses) {
-      clear_bins(s);
-      each_vector(row, [&](const float(&x)[8], int) {
+  const Cut none = {kBins, 0, 0};
+  // the last bin that a kept token can be in, as far as it is known without a
+  // histogram: by the share of the largest weight (one bin more for a bin's
+  // rounding), and by the k-th of the threads' largest logits
+  int last = kBins;
+  if (bar > 0.0 && !(by_share && by_count)) {
+    const float y = -__builtin_amdgcn_logf(least) * kFine + 1.0f;
+    if (y < (float)kBins) last = y > 0.0f ? (int)y : 0;
+  }
+  const int tight = last;
+  if (by_count && k <= kThreads) {
+    uint32_t* count = reinterpret_cast<uint32_t*>(index_bins(s));
+    const int b = bin_of(scale, mine), b0 = 2 * tid;
+    if (b < kBins) atomicAdd(&count[b], 1u);
+    __syncthreads();
+    const u64 c0 = count[b0], c1 = count[b0 + 1];
+    u64 all;
+    const u64 before = scan_before<0, false>(s, c0 + c1, all);
+    index_bins(s)[b0] = 0, index_bins(s)[b0 + 1] = 0;
+    if (before < (u64)k && before + c0 + c1 >= (u64)k) s.at = before + c0 < (u64)k ? b0 + 1 : b0;
+    __syncthreads();
+    if (all >= (u64)k && s.at < last) last = s.at;
+  }
+  // a histogram, with masses only where few tokens cannot do without
+  u64 mass = 0;
+  auto count_bins = [&](bool with_masses) {
+    clear_bins(s);
+    each_vector(row, [&](const float(&x)[8], int) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int b = bin_of(scale, x[j]);
-          if (b < kBins) {
-            atomicAdd(&s.count[b], 1u);
-            if (decltype(with_masses)::value) atomicAdd(&s.mass[b], weight(scale, sound(x[j])));
-          }
+      for (int j = 0; j < 8; ++j) {
+        const int b = bin_of(scale, x[j]);
+        if (b < kBins) {
+          atomicAdd(&s.count[b], 1u);
+          if (with_masses) atomicAdd(&s.mass[b], weight(scale, sound(x[j])));
         }
-      });
-      __syncthreads();
-    };
-    bool masses = by_share && !by_count;
-    if (masses) {
-      count_bins(std::true_type());
+      }
+    });
+    __syncthreads();
+    if (with_masses) {
+      mass = 0;
       for (int i = tid; i < kBins; i += kThreads) mass += s.mass[i];
       mass = sum_of(s, mass);
-    } else {
-      count_bins(std::false_type());
     }
-    if (by_count) at = find_bin<false>(s, none, (u64)k, 0.0);
-    // no share at all is the first token's
-    auto wanted = [&] { return share > 0.0f ? (double)share * (double)mass : 0.5; };
-    // the last bin that a kept token can be in
-    int last = kBins - 1;
-    if (by_count && at.bin < last) last = at.bin;
-    if (masses) {
-      const Cut by = find_bin<true>(s, none, 0, wanted());
-      if (by.bin < last) last = by.bin;
+  };
+  // few tokens, by what is known so far, or by a histogram of the row
+  const u64 most = by_count ? (u64)k : 0;
+  Few done = kTooMany;
+  if (last < kBins && !(by_share && !by_count)) done = few(s, row, held, scale, p, r, last, most, by_share, share, mass, bar);
+  if (done == kDrawn) return;
+  if (done == kTooMany && (by_count || by_share)) {
+    last = tight;
+    count_bins(!by_count);
+    const Cut c = by_count ? find_bin<false, true>(s, none, most, 0.0) : find_bin<true, true>(s, none, 0, share_of(share, mass));
+    const bool listable = c.bin < last ? c.count + s.count[c.bin] <= (u64)kMostListed : last < kBins;
+    if (c.bin < last) last = c.bin;
+    if (listable) {
+      __syncthreads();
+      clear_few(s);
+      __syncthreads();
+      if (few(s, row, NotHeld(), scale, p, r, last, most, by_share, share, mass, bar) == kDrawn) return;
     }
-    if (bar > 0.0 && (!by_share || masses)) {
-      const double y = (40.0 - log2(bar)) * kFine + 1.0;  // one more for the rounding of a bin
-      if (y < (double)last) last = (int)y;
-    }
-    const Few done = few(s, row, scale, p, r, last, by_count ? (u64)k : 0, at, by_share, share, mass, bar);
-    if (done == kDrawn) return;
+  }
+  if (by_count || by_share) {
+    // every token's weight, cut by cut
+    count_bins(true);
     if (by_count) {
-      if (by_share) {
-        count_bins(std::true_type());
-        for (int i = tid; i < kBins; i += kThreads) mass += s.mass[i];
-        mass = sum_of(s, mass);
-        at = find_bin<false, true>(s, none, (u64)k, 0.0);
-      }
-      if (at.bin < kBins) {
+      const Cut c = find_bin<false, true>(s, none, (u64)k, 0.0);
+      if (c.bin < kBins) {
         // the histogram is made again by a bin that is cut finer
-        const bool keeps = s.count[at.bin] <= (uint32_t)kMostListed;
-        cut = resolve<false>(s, row, scale, at, (u64)k, 0.0, mass);
-        if (by_share && !keeps) count_bins(std::true_type());
+        const bool keeps = s.count[c.bin] <= (uint32_t)kMostListed;
+        u64 upto;
+        cut = resolve<false>(s, row, scale, c, (u64)k, 0.0, upto);
+        if (by_share && !keeps) count_bins(true);
+        mass = upto;
       }
-    } else if (masses && done == kTooNear) {
-      count_bins(std::true_type());
     }
     if (by_share) {
-      const Cut by = find_bin<true>(s, none, 0, wanted());
-      if (by.bin < kBins) {
+      const double wanted = share_of(share, mass);
+      const Cut c = find_bin<true>(s, none, 0, wanted);
+      if (c.bin < kBins) {
         u64 upto;
-        const u64 o = resolve<true>(s, row, scale, by, 0, wanted(), upto);
+        const u64 o = resolve<true>(s, row, scale, c, 0, wanted, upto);
         cut = o < cut ? o : cut;
       }
     }
@@ -662,17 +873,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
     }
     upto = wave_scan(mine);
     __syncthreads();
-    if (lane == 63) s.sums[wave] = upto;
+    if (lane == 63) s.sums[0][wave] = upto;
     __syncthreads();
     u64 before = 0, all = 0;
     int run = 0;
     if (total == 0) {
-      for (int w = 0; w < kWaves; ++w) total += s.sums[w];
+      for (int w = 0; w < kWaves; ++w) total += s.sums[0][w];
       target = target_of(p.random[r], total);
     }
     for (int w = 0; w < kWaves; ++w) {
-      if (all + s.sums[w] > target) break;
-      all += s.sums[w];
+      if (all + s.sums[0][w] > target) break;
+      all += s.sums[0][w];
       run = w + 1;
     }
     target -= all;
