@@ -45,23 +45,32 @@ def _(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     return x.new_empty(x.shape)
 
 
-def _save(ctx, inputs, keyword_only_inputs, output):
-    _, positions, freqs = inputs
+class _Rotary(torch.autograd.Function):
+    """The turn with the turn back, its transpose, as gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, freqs, interleaved, factor, back):
+        ctx.save_for_backward(positions, freqs)
+        ctx.how = interleaved, factor, back
+        with torch._C._AutoDispatchBelowAutograd():
+            return torch.ops.quantized_ops.rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, freqs = ctx.saved_tensors
+        interleaved, factor, back = ctx.how
+        return torch.ops.quantized_ops.rotary(grad, positions, freqs, interleaved=interleaved, factor=factor,
+                                              back=not back), None, None, None, None, None
+
+
+@torch.library.impl(quantized_ops_lib, "rotary", "Autograd")
+def _rotary_autograd(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     if freqs.requires_grad:
-        raise ValueError("vqx: rotary: freqs have no gradient here")
-    ctx.save_for_backward(positions, freqs)
-    ctx.how = keyword_only_inputs
-
-
-def _back(ctx, grad):
-    positions, freqs = ctx.saved_tensors
-    how = ctx.how
-    # a turn's transpose is the turn back
-    return torch.ops.quantized_ops.rotary(grad, positions, freqs, interleaved=how["interleaved"], factor=how["factor"],
-                                          back=not how["back"]), None, None
-
-
-torch.library.register_autograd("quantized_ops::rotary", _back, setup_context=_save)
+        kv4._refuse("rotary", "freqs have no gradient here")
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, positions, freqs, interleaved, factor, back)
+    with torch._C._AutoDispatchBelowAutograd():
+        return torch.ops.quantized_ops.rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
 
 
 def rotary_frequencies(turned, base=10000.0, *, stretch=1.0, trained=None, slow=1.0, fast=4.0, device=None):
