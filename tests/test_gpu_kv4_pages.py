@@ -126,6 +126,23 @@ def test_reserve_all_end(ops):
     assert made[1].tolist() == [-1] * 5
 
 
+def test_reserve_many_entries(ops):
+    """More entries of rows than are looked at together, of rows that end and of
+    rows that grow; holes in them."""
+    grow, lengths, table, free, spare, size = scene(4, 1100, 45, 4, 12000, ending=0.0)
+    r = random.Random(2)
+    lengths = [min(n, 100) for n in lengths]
+    for row in table[::7]:
+        row[r.randrange(45)] = -1
+    check_reserve(ops, [r.choice([-1, 70, 61, 0]) for _ in range(1100)], lengths, table, free, spare, size, 80000)
+    check_reserve(ops, [r.choice([77, 3]) for _ in range(1100)], lengths, table, free, spare, size, 30000)
+
+
+def test_reserve_long_rows(ops):
+    check_reserve(ops, [9000, -1, 20000], [100, 9999, 0], [[*range(7)] + [-1] * 1400, [*range(7, 632)] + [-1] * 782,
+                                                         [-1] * 1407], list(range(632, 3000)) + [0] * 632, 2368, 16, 30000)
+
+
 def test_reserve_what_is_given_back_is_taken(ops):
     check_reserve(ops, [-3, 33], [32, 0], [[0, 1, -1], [-1, -1, -1]], [2, 5, 5], 1, 16, 40)
 

@@ -105,6 +105,21 @@ def test_rotary_strides(ops, vqx, view):
     same(got, ops.rotary(x.contiguous(), pos, freqs).cpu(), "a strided view")
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rotary_small_values(ops, vqx, kind):
+    """Subnormal values and results are neither lost nor flushed; what is not
+    turned comes back bit for bit."""
+    tiny = torch.finfo(TYPES[kind]).tiny
+    x = (torch.randn(20, 2, 64, dtype=torch.float64, generator=torch.Generator().manual_seed(1)) * tiny).to(TYPES[kind])
+    pos, freqs = torch.arange(20).int(), vqx.ops.rotary_frequencies(48)
+    for interleaved in (False, True):
+        want = turned(x, pos, freqs, interleaved)
+        got = ops.rotary(*on(x, pos, freqs), interleaved=interleaved)
+        # half a step of the subnormals, once to fp32 and once to the type
+        near(got, want, torch.finfo(x.dtype).eps * tiny / 2 + 2.0 ** -149 + torch.finfo(x.dtype).eps / 2 * want.abs(), "turned")
+        assert torch.equal(got[..., 48:].cpu().view(torch.uint8), x[..., 48:].contiguous().view(torch.uint8))
+
+
 def test_rotary_special_values(ops, vqx):
     """What is not finite reaches its own pair only."""
     x = torch.ones(2, 1, 64)

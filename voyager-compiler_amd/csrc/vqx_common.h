@@ -83,6 +83,30 @@ __device__ __forceinline__ void wave_lds_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
+// What lane i has from another lane of its row or from the end of a row before it,
+// 0 where there is none.
+template <int kControl, int kRows>
+__device__ __forceinline__ uint64_t from_lane(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, kRows, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, kRows, 0xF, false);
+  return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t x, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32 | lo;
+}
+// The sum up to each lane: by shifts within rows of 16 lanes, then the ends of
+// the rows before.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t x) {
+  x += from_lane<0x111, 0xF>(x);
+  x += from_lane<0x112, 0xF>(x);
+  x += from_lane<0x114, 0xF>(x);
+  x += from_lane<0x118, 0xF>(x);
+  x += from_lane<0x142, 0xA>(x);
+  x += from_lane<0x143, 0xC>(x);
+  return x;
+}
+
 // Exact fp16 <-> fp32 conversions in integer arithmetic (subnormals and signed
 // zeros kept, round to nearest even), independent of the device's fp16
 // denormal mode; torch's CPU conversions are the reference.

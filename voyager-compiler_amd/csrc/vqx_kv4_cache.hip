@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Tokens q,
     Raw8F v;
   };
   for_new_values<kDim, Raw>(
-      c, q, share, [](uint32_t, int, int) {},
+      c, q, share,
       [&](const Item& t, Raw& raw) {
         load8(t.plane ? value : key,
               (int64_t)t.i * (t.plane ? value_sn : key_sn) + (int64_t)t.h * (t.plane ? value_sh : key_sh) + t.part * 8, T(),
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4View c, Kv4Tokens q, K
     uint32_t code, scale;
   };
   for_new_values<kDim, Raw>(
-      c, q, share, [](uint32_t, int, int) {},
+      c, q, share,
       [&](const Item& t, Raw& raw) {
         raw = Raw{0u, 127u};
         if (t.row != kNoRow) {

@@ -9,92 +9,148 @@ namespace {
 // reserve: block table, offsets, positions and slots of the new tokens
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kSlotsEach = 2;  // of a thread of the second launch
 
 // The sum of the values of the threads before this one, and of all.
-__device__ __forceinline__ int64_t scan_before(int64_t x, int64_t* sums, int64_t& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t sum = x;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int64_t y = __shfl_up(sum, d);
-    if (lane >= d) sum += y;
-  }
+__device__ __forceinline__ int64_t scan_before(int64_t x, uint64_t* sums, int64_t& all) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t upto = wave_scan((uint64_t)x);
   __syncthreads();  // the sums of the scan before have been read
-  if (lane == 63) sums[wave] = sum;
+  if (lane == 63) sums[wave] = upto;
   __syncthreads();
-  int64_t before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    before += w < wave ? sums[w] : 0;
-    all += sums[w];
-  }
-  return before + sum - x;
+  static_assert(kWaves == 16, "");
+  uint64_t sum = sums[lane & 15];
+  sum += from_lane<0x111, 0xF>(sum);
+  sum += from_lane<0x112, 0xF>(sum);
+  sum += from_lane<0x114, 0xF>(sum);
+  sum += from_lane<0x118, 0xF>(sum);
+  all = (int64_t)lane_of(sum, 15);
+  return (int64_t)((wave > 0 ? lane_of(sum, wave - 1) : 0) + upto) - x;
 }
 
-__device__ __forceinline__ void fill_slots(const Kv4Pages& p, int64_t i) {
+// The last sequence that begins at or before new token i; cu: offsets, in LDS or
+// memory.
+__device__ __forceinline__ int sequence_at(const int32_t* cu, int seqs, int64_t i) {
+  int lo = 0, hi = seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (cu[mid] <= i)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void fill_slot(const Kv4Pages& p, const int32_t* cu, int64_t i) {
   int32_t position = -1;
   int64_t slot = -1;
-  if (i < p.cu[p.seqs]) {
-    int lo = 0, hi = p.seqs;  // the last sequence that begins at or before i
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (p.cu[mid] <= i)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    position = p.lengths[lo] - (p.cu[lo + 1] - (int32_t)i);
-    const int32_t page = p.table[(int64_t)lo * p.per + position / p.size];
+  if (i < cu[p.seqs]) {
+    const int b = sequence_at(cu, p.seqs, i);
+    position = p.lengths[b] - (cu[b + 1] - (int32_t)i);
+    const int32_t page = p.table[(int64_t)b * p.per + position / p.size];
     slot = (int64_t)page * p.size + position % p.size;
   }
   p.positions[i] = position;
   p.slots[i] = slot;
 }
 
+// Entries of rows one after another, kChunks of them a thread, 1024 apart: which
+// are marked and how many marked ones come before each.
+constexpr int kChunks = 8, kGroup = kChunks * kThreads;
+struct Entries {
+  int row[kChunks];      // which of the rows
+  int32_t* at[kChunks];  // NULL past the last
+  int32_t page[kChunks];
+  bool marked[kChunks];
+  int32_t before[kChunks];
+};
+
+// All loads on their way together, and one barrier for all: a wave's marks are
+// counted by a ballot, and each wave sums up the 128 counts itself.  Returns the
+// number of marks.
+// left: entries from the group's first on.
+template <typename Mark>
+__device__ __forceinline__ int mark_entries(Entries& e, int64_t left, int32_t (&counts)[kChunks * kWaves], Mark mark) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) e.page[k] = e.at[k] ? *e.at[k] : 0;
+  __syncthreads();  // counts before have been read
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    e.marked[k] = false;
+    if (k * kThreads >= left) {
+      if (lane == 0) counts[k * kWaves + wave] = 0;
+      continue;
+    }
+    e.marked[k] = e.at[k] && mark(e.page[k]);
+    const uint64_t bits = __ballot(e.marked[k]);
+    e.before[k] = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(bits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bits, 0));
+    if (lane == 0) counts[k * kWaves + wave] = __popcll(bits);
+  }
+  __syncthreads();
+  static_assert(kChunks * kWaves == 128, "");
+  const int one = counts[2 * lane], two = counts[2 * lane + 1];
+  const int upto = (int)wave_scan((uint64_t)(one + two));
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    if (k * kThreads >= left) break;
+    const int pair = (k * kWaves + wave) / 2;
+    const int sum = __builtin_amdgcn_readlane(upto - one - two, pair);
+    e.before[k] += wave & 1 ? sum + __builtin_amdgcn_readlane(one, pair) : sum;
+  }
+  return __builtin_amdgcn_readlane(upto, 63);
+}
+
 // One workgroup, a thread for each sequence: what they need depends on what
-// those before them were given.  Bound by the chains of loads.
+// those before them were given.  Entries of the table are read across the
+// threads, in their order (a thread's own row takes a line for each lane: 512
+// sequences, 51 of which end, 138 admitted with 1000 tokens in the mean, 30 us
+// with the rows of a thread each, 64 with an entry of them at a time).  Bound by
+// its chains of loads and barriers.
 __global__ __launch_bounds__(kThreads) void kv4_reserve_kernel(Kv4Pages p, bool slots) {
-  __shared__ int64_t sums[kWaves];
-  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ uint64_t sums[kWaves];
+  __shared__ int32_t counts[kChunks * kWaves];
+  __shared__ int64_t starts[kThreads + 1];             // of each sequence's entries
+  __shared__ int32_t firsts[kThreads];                 // the first of them in its row
+  __shared__ int64_t ranks[kThreads], ends[kThreads];  // lacking ones before the first and up to the last
+  __shared__ bool serves[kThreads];
+  const int tid = threadIdx.x;
   const int64_t cap = (int64_t)p.per * p.size;
   auto valid = [&](int32_t page) { return (uint32_t)page < (uint32_t)p.pages; };
+  Entries e;
   int64_t stock = p.count[0];
   stock = stock < 0 ? 0 : (stock > p.pages ? p.pages : stock);
-  // sequences that end give their pages back, in their order, a wave to a row
+  // sequences that end give their pages back, in their order
   for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
     const int b = b0 + tid;
-    const bool ends = b < p.seqs && p.grow[b] < 0;
-    const uint64_t ending = __ballot(ends);
-    int64_t given = 0;
-    for (uint64_t left = ending; left; left &= left - 1) {
-      const int l = __builtin_ctzll(left);
-      const int32_t* row = p.table + (int64_t)(b - lane + l) * p.per;
-      int n = 0;
-      for (int j = lane; j - lane < p.per; j += 64) n += __popcll(__ballot(j < p.per && valid(row[j < p.per ? j : 0])));
-      if (lane == l) given = n;
-    }
-    int64_t all;
-    const int64_t before = scan_before(given, sums, all);
-    for (uint64_t left = ending; left; left &= left - 1) {
-      const int l = __builtin_ctzll(left);
-      int32_t* row = p.table + (int64_t)(b - lane + l) * p.per;
-      int64_t to = stock + __shfl(before, l);
-      for (int j = lane; j - lane < p.per; j += 64) {
-        const int32_t page = j < p.per ? row[j] : -1;
-        const bool some = j < p.per && valid(page);
-        const uint64_t mask = __ballot(some);
-        const int64_t at = to + __popcll(mask & ((1ull << lane) - 1));
-        if (some && at < p.pages) p.free[at] = page;  // more pages than there are: one came back twice
-        if (j < p.per) row[j] = -1;
-        to += __popcll(mask);
+    const bool over = b < p.seqs && p.grow[b] < 0;
+    int64_t rows;
+    const int64_t at = scan_before(over, sums, rows);
+    if (over) firsts[at] = b, p.lengths[b] = 0;
+    __syncthreads();
+    for (int64_t i0 = 0; i0 < rows * p.per; i0 += kGroup) {
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int64_t n = i0 + k * kThreads + tid;
+        e.at[k] = nullptr;
+        if (i0 + k * kThreads >= rows * p.per) continue;
+        // 32 bits, but for rows of millions
+        e.row[k] = n >> 32 ? (int)(n / p.per) : (int)((uint32_t)n / (uint32_t)p.per);
+        e.at[k] = n < rows * p.per ? p.table + (int64_t)firsts[e.row[k]] * p.per + (n - (int64_t)e.row[k] * p.per) : nullptr;
       }
+      const int all = mark_entries(e, rows * p.per - i0, counts, valid);
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int64_t to = stock + e.before[k];
+        if (e.marked[k] && to < p.pages) p.free[to] = e.page[k];  // past it: one came back twice
+        if (e.at[k]) *e.at[k] = -1;
+      }
+      stock += all;
     }
-    if (ends) p.lengths[b] = 0;
-    stock += all;
+    __syncthreads();
   }
   if (stock > p.pages) stock = p.pages;
-  __syncthreads();
   // pages for those that grow
   int64_t needed = 0, tokens = 0, taken = 0, served_tokens = 0;
   for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
@@ -103,35 +159,92 @@ __global__ __launch_bounds__(kThreads) void kv4_reserve_kernel(Kv4Pages p, bool 
     const int32_t grow = there ? p.grow[b] : 0, length = there ? p.lengths[b] : 0;
     const int64_t wanted = grow > 0 ? grow : 0;
     const bool fits = there && length >= 0 && length + wanted <= cap;
-    int32_t* row = p.table + (int64_t)(there ? b : 0) * p.per;
     const int first = fits && wanted > 0 ? length / p.size : 0;
     const int last = fits && wanted > 0 ? (int)((length + wanted - 1) / p.size) + 1 : 0;
-    int64_t need = 0;
-    for (int j = first; j < last; ++j) need += !valid(row[j]);
-    int64_t all_need, all_tokens, all_served, all_taken;
-    const int64_t mine = needed + scan_before(need, sums, all_need);
+    // the entries of the new tokens of all of them, one after another
+    int64_t entries;
+    starts[tid] = scan_before(last - first, sums, entries);
+    firsts[tid] = first, ranks[tid] = 0, ends[tid] = 0;
+    if (tid == 0) starts[kThreads] = entries;
+    __syncthreads();
+    int most = kThreads;  // sequences of the tile, up to a power of two
+    while (most / 2 >= p.seqs - b0) most /= 2;
+    auto find = [&](int64_t i0) {
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) e.row[k] = 0;
+      // the last that starts at or before each, all chunks' searches side by side
+      for (int step = most / 2; step > 0; step /= 2)
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+          if (i0 + k * kThreads < entries && starts[e.row[k] + step] <= i0 + k * kThreads + tid) e.row[k] += step;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int64_t n = i0 + k * kThreads + tid;
+        e.at[k] = nullptr;
+        if (i0 + k * kThreads >= entries) continue;
+        e.at[k] = n < entries ? p.table + (int64_t)(b0 + e.row[k]) * p.per + firsts[e.row[k]] + (n - starts[e.row[k]]) : nullptr;
+      }
+    };
+    auto lacking = [&](int32_t page) { return !valid(page); };
+    int64_t found = 0;
+    for (int64_t i0 = 0; i0 < entries; i0 += kGroup) {
+      find(i0);
+      const int all = mark_entries(e, entries - i0, counts, lacking);
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const int64_t n = i0 + k * kThreads + tid;
+        if (!e.at[k]) continue;
+        const int row = e.row[k];
+        if (n == starts[row]) ranks[row] = found + e.before[k];
+        if (n + 1 == starts[row + 1]) ends[row] = found + e.before[k] + e.marked[k];
+      }
+      found += all;
+    }
+    __syncthreads();
+    const int64_t need = ends[tid] - ranks[tid], mine = needed + ranks[tid];
+    int64_t all_tokens, all_served, all_taken;
     const int64_t upto = tokens + scan_before(fits ? wanted : 0, sums, all_tokens) + wanted;
     const bool served = fits && (need == 0 || mine + need <= stock) && upto <= p.n;
     const int64_t cu = served_tokens + scan_before(served ? wanted : 0, sums, all_served);
     scan_before(served ? need : 0, sums, all_taken);
     if (there) p.cu[b] = (int32_t)cu;
-    if (served && wanted > 0) {
-      int64_t at = stock - 1 - mine;
-      for (int j = first; j < last; ++j)
-        if (!valid(row[j])) row[j] = p.free[at--];
-      p.lengths[b] = length + (int32_t)wanted;
+    if (served && wanted > 0) p.lengths[b] = length + (int32_t)wanted;
+    serves[tid] = served;
+    __syncthreads();
+    int64_t rank = needed;
+    for (int64_t i0 = 0; i0 < entries; i0 += kGroup) {
+      int all = 0;
+      if (entries > kGroup) find(i0), all = mark_entries(e, entries - i0, counts, lacking);  // one group's are still at hand
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+        if (e.marked[k] && serves[e.row[k]]) e.page[k] = p.free[stock - 1 - rank - e.before[k]];
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+        if (e.marked[k] && serves[e.row[k]]) *e.at[k] = e.page[k];
+      rank += all;
     }
-    needed += all_need, tokens += all_tokens, served_tokens += all_served, taken += all_taken;
+    __syncthreads();
+    needed += found, tokens += all_tokens, served_tokens += all_served, taken += all_taken;
   }
   if (tid == 0) p.cu[p.seqs] = (int32_t)served_tokens, p.count[0] = (int32_t)(stock - taken);
   if (!slots) return;
   __syncthreads();
-  for (int64_t i = tid; i < p.n; i += kThreads) fill_slots(p, i);
+  for (int64_t i = tid; i < p.n; i += kThreads) fill_slot(p, p.cu, i);
 }
 
+// Offsets that a workgroup searches in LDS.
+constexpr int kMostOffsets = 4096;
+
 __global__ __launch_bounds__(256) void kv4_slots_kernel(Kv4Pages p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < p.n) fill_slots(p, i);
+  __shared__ int32_t cu[kMostOffsets];
+  const bool local = p.seqs < kMostOffsets;
+  if (local)
+    for (int b = threadIdx.x; b <= p.seqs; b += 256) cu[b] = p.cu[b];
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * kSlotsEach * 256 + threadIdx.x;
+#pragma unroll
+  for (int a = 0; a < kSlotsEach; ++a)
+    if (i0 + a * 256 < p.n) fill_slot(p, local ? cu : p.cu, i0 + a * 256);
 }
 
 // Slots that the first launch's one workgroup fills by itself.
@@ -223,7 +336,8 @@ __global__ __launch_bounds__(256) void kv4_pack_kernel(Kv4View c, Kv4Tokens q, c
 int kv4_reserve(const Kv4Pages& p, hipStream_t st) {
   const bool few = p.n <= kFewSlots;
   hipLaunchKernelGGL(kv4_reserve_kernel, dim3(1), dim3(kThreads), 0, st, p, few);
-  if (!few) hipLaunchKernelGGL(kv4_slots_kernel, dim3((unsigned)((p.n + 255) / 256)), dim3(256), 0, st, p);
+  if (!few) hipLaunchKernelGGL(kv4_slots_kernel, dim3((unsigned)((p.n + 256 * kSlotsEach - 1) / (256 * kSlotsEach))),
+                               dim3(256), 0, st, p);
   return check_launch("kv4_reserve");
 }
 

@@ -146,11 +146,10 @@ struct Item {
 // workgroup's tokens, kAhead of them taken before the first is put; the rows are
 // found once a token, for all of them at a time.  A thread without an item of
 // its own takes the last one and does not put it, so that the four threads of a
-// block stay together.  setup(plane, first token, count) comes before the barrier
-// behind which the values are taken.
-template <int kDim, typename What, typename Setup, typename Take, typename Put>
-__device__ __forceinline__ void for_new_values(const Kv4View& c, const Kv4Tokens& q, const Kv4Share& share, Setup setup,
-                                               Take take, Put put) {
+// block stay together.
+template <int kDim, typename What, typename Take, typename Put>
+__device__ __forceinline__ void for_new_values(const Kv4View& c, const Kv4Tokens& q, const Kv4Share& share, Take take,
+                                               Put put) {
   constexpr uint32_t kPerRow = kDim / 8;
   constexpr int kAhead = 2;
   __shared__ uint32_t rows[kMostTokens];
@@ -158,7 +157,6 @@ __device__ __forceinline__ void for_new_values(const Kv4View& c, const Kv4Tokens
   const int i0 = (int)(blockIdx.x - plane * (uint32_t)share.groups) * share.tokens;
   const int count = q.n - i0 < share.tokens ? q.n - i0 : share.tokens;
   if ((int)threadIdx.x < count) rows[threadIdx.x] = new_token_row(c, q, i0 + (int)threadIdx.x);
-  setup(plane, i0, count);
   __syncthreads();
   const uint32_t per = c.kv * kPerRow, items = (uint32_t)count * per;
   uint32_t token = threadIdx.x / per, rest = threadIdx.x % per;

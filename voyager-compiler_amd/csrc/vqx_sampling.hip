@@ -160,30 +160,6 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
 // ---------------------------------------------------------------------------
 // a workgroup's sums
 // ---------------------------------------------------------------------------
-// What lane i has from another lane of its row or from the end of a row before it,
-// 0 where there is none.
-template <int kControl, int kRows>
-__device__ __forceinline__ u64 from_lane(u64 x) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, kControl, kRows, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), kControl, kRows, 0xF, false);
-  return (u64)hi << 32 | lo;
-}
-__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane);
-  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32 | lo;
-}
-// The sum up to each lane: by shifts within rows of 16 lanes, then the ends of
-// the rows before (a scan by permutes through LDS takes five times as long).
-__device__ __forceinline__ u64 wave_scan(u64 x) {
-  x += from_lane<0x111, 0xF>(x);
-  x += from_lane<0x112, 0xF>(x);
-  x += from_lane<0x114, 0xF>(x);
-  x += from_lane<0x118, 0xF>(x);
-  x += from_lane<0x142, 0xA>(x);
-  x += from_lane<0x143, 0xC>(x);
-  return x;
-}
-
 struct Shared {
   u64 list[kMostListed];
   u64 mass[kBins];
