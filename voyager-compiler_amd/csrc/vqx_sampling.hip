@@ -75,15 +75,17 @@ struct Row {
   int before;           // elements of vector 0 that are not the row's
   int size, vectors;
   int whole, past;  // vectors [whole, past) have 8 of the row's
+  bool infinite;    // where some are +inf those count as 0 and all others as -inf
 
   __device__ __forceinline__ Row(const void* p, int64_t offset, int n) {
-    const uintptr_t at = (uintptr_t)p + (uintptr_t)offset * kSize;
-    before = (int)(at & 15) / kSize;
-    base = reinterpret_cast<const uint8_t*>(at) - before * kSize;
+    const uint8_t* at = static_cast<const uint8_t*>(p) + offset * kSize;
+    before = (int)((uintptr_t)at & 15) / kSize;
+    base = at - before * kSize;
     size = n;
     vectors = (n + before + 7) / 8;
     whole = before > 0;
     past = (n + before) / 8;
+    infinite = false;
   }
   __device__ __forceinline__ int first(int v) const { return 8 * v - before; }
   __device__ __forceinline__ Raw<T> raw(int v) const {
@@ -93,14 +95,26 @@ struct Row {
     else
       return Raw<T>{reinterpret_cast<const u32x4*>(p)[0]};
   }
+  // NaN and both zeros as they are
+  __device__ __forceinline__ void logits(const Raw<T>& r, float (&x)[8]) const {
+    values(r, x);
+    if (infinite) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] == -kNone ? 0.0f : kNone;
+    }
+  }
+  __device__ __forceinline__ float logit(int i) const {
+    const float x = element(base, (int64_t)i + before, T());
+    return !infinite ? x : (x == -kNone ? 0.0f : kNone);
+  }
   // any vector: -inf where the row has no element
   __device__ __forceinline__ void load(int v, float (&x)[8]) const {
     const int e = first(v);
     if (e >= 0 && e + 8 <= size) {
-      values(raw(v), x);
+      logits(raw(v), x);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = e + j >= 0 && e + j < size ? element(base, 8 * (int64_t)v + j, T()) : kNone;
+      for (int j = 0; j < 8; ++j) x[j] = e + j >= 0 && e + j < size ? logit(e + j) : kNone;
     }
   }
 };
@@ -108,36 +122,58 @@ struct Row {
 // ---------------------------------------------------------------------------
 // weights and order
 // ---------------------------------------------------------------------------
-struct Scale {
-  float top;      // the row's largest logit
-  double inner;   // log2(e) / temperature
-  float coarse;   // that, in bins
-  const double* powers;  // 2^(j / 64) in LDS
+struct Shared {
+  u64 list[kMostListed];
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  double powers[64];
+  float tops[kWaves];
+  u64 sums[4][kWaves];
+  u64 found[4];
+  int at, listed, spot[3], near[3];
 };
 
-__device__ __forceinline__ u64 weight(const Scale& s, float x) {
-  if (x == s.top) return (u64)kUnit;
-  const double q = ((double)x - (double)s.top) * s.inner;
-  if (!(q > -41.5)) return 0;
-  const double n = __builtin_rint(64.0 * q);
-  const double r = __builtin_fma(n, -1.0 / 64.0, q);
-  // 2^r to 2^-54: Taylor's series in r ln 2, up to 0.0054
-  double p = 0x1.5d87fe78a6731p-10;                     // ln2^5 / 120
-  p = __builtin_fma(p, r, 0x1.3b2ab6fba4e77p-7);        // ln2^4 / 24
-  p = __builtin_fma(p, r, 0x1.c6b08d704a0c0p-5);        // ln2^3 / 6
-  p = __builtin_fma(p, r, 0x1.ebfbdff82c58fp-3);        // ln2^2 / 2
-  p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);        // ln2
-  p = __builtin_fma(p, r, 1.0);
-  const int i = (int)n;
-  const double unit = __builtin_bit_cast(double, (u64)(1023 + 40 + (i >> 6)) << 52);
-  // a number below 2^52 is rounded to a whole one by the addition
-  return __builtin_bit_cast(u64, __builtin_fma(s.powers[i & 63] * p, unit, 0x1p52)) - __builtin_bit_cast(u64, 0x1p52);
+struct Scale {
+  float top;     // the row's largest logit
+  double inner;  // 64 log2(e) / temperature
+  float coarse;  // log2(e) / temperature, in bins
+};
+
+// p r + c with c in scalar registers (the compiler copies a constant into vector
+// registers first, which is one instruction more for each).
+__device__ __forceinline__ double fma_constant(double p, double r, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(p), "v"(r), "s"(c));
+  return d;
+}
+
+// A whole number up to 2^40, as a double: sums of them are exact up to 2^53.
+__device__ __forceinline__ double weight(const Shared& s, const Scale& scale, float x) {
+  // 64ths of a halving; 42 of these are 0 already, a NaN or -inf is one of those
+  const double q = __builtin_fmax(((double)x - (double)scale.top) * scale.inner, -64.0 * kHalvings);
+  // a number below 2^51 is rounded to a whole one by the addition, which stands
+  // in the sum's low bits
+  const double n = q + 0x1.8p52;
+  const int i = (int)(uint32_t)__builtin_bit_cast(u64, n);
+  const double r = q - (n - 0x1.8p52);
+  // 2^(r / 64) to 2^-54: Taylor's series in r ln2 / 64, up to 0.0054
+  double p = fma_constant(0x1.5d87fe78a6731p-40, r, 0x1.3b2ab6fba4e77p-31);  // (ln2 / 64)^5 / 120, (ln2 / 64)^4 / 24
+  p = fma_constant(p, r, 0x1.c6b08d704a0c0p-23);                             // (ln2 / 64)^3 / 6
+  p = fma_constant(p, r, 0x1.ebfbdff82c58fp-15);                             // (ln2 / 64)^2 / 2
+  p = fma_constant(p, r, 0x1.62e42fefa39efp-7);                              // ln2 / 64
+  p = fma_constant(p, r, 1.0);
+  // times 2^((i % 64) / 64) 2^(i / 64) 2^40, rounded to a whole number
+  const u64 power = __builtin_bit_cast(u64, s.powers[i & 63]) + ((u64)(uint32_t)(((i >> 6) + 40) << 20) << 32);
+  return __builtin_fma(__builtin_bit_cast(double, power), p, 0x1p52) - 0x1p52;
+}
+__device__ __forceinline__ u64 whole_weight(const Shared& s, const Scale& scale, float x) {
+  return (u64)weight(s, scale, x);
 }
 
 // The bin of a logit, or kBins of one whose weight is 0; larger logits have no
 // larger bins.
 __device__ __forceinline__ int bin_of(const Scale& s, float x) {
-  const float y = x == s.top ? 0.0f : (s.top - x) * s.coarse;
+  const float y = (s.top - x) * s.coarse;
   return y < (float)(kHalvings * kFine) ? (int)y : kBins;
 }
 
@@ -160,17 +196,6 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
 // ---------------------------------------------------------------------------
 // a workgroup's sums
 // ---------------------------------------------------------------------------
-struct Shared {
-  u64 list[kMostListed];
-  u64 mass[kBins];
-  uint32_t count[kBins];
-  double powers[64];
-  float tops[kWaves];
-  u64 sums[4][kWaves];
-  u64 found[4];
-  int at, listed, spot[3], near[3];
-};
-
 // The sum of what the threads before this one have, and of all.  Callers that
 // follow each other without a barrier have slots of their own and no fence.
 template <int kSlot = 0, bool kFence = true>
@@ -241,6 +266,33 @@ __device__ __forceinline__ double share_of(float share, u64 all) {
   return share > 0.0f ? (double)share * (double)all : 0.5;
 }
 
+// A bin that is not before the one in which the masses come to `share`, from
+// counts: a token in bin b has at least the weight of the bin's end.
+__device__ __forceinline__ Cut find_least(Shared& s, double share) {
+  const int b = 2 * (int)threadIdx.x;
+  const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
+  // less what a bin's border, a weight's rounding and this power may be off by
+  auto at_least = [](int bin) {
+    const float w = 0x1p40f * __builtin_amdgcn_exp2f(-(float)(bin + 1) / kFine) * (1.0f - 0x1p-16f) - 1.0f;
+    return w > 0.0f ? (u64)w : 0;
+  };
+  const u64 m0 = c0 * at_least(b), m1 = c1 * at_least(b + 1);
+  if (threadIdx.x == 0) s.at = kBins;
+  u64 all;
+  u64 before = scan_before(s, c0 + c1, all);
+  u64 mass = scan_before(s, m0 + m1, all);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u64 m = i ? m1 : m0;
+    if ((double)mass < share && (double)(mass + m) >= share) s.at = b + i, s.found[0] = before;
+    before += i ? c1 : c0, mass += m;
+  }
+  __syncthreads();
+  const Cut c = {s.at, s.found[0], 0};
+  __syncthreads();
+  return c;
+}
+
 __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0, s.mass[i] = 0;
@@ -281,10 +333,23 @@ __device__ __forceinline__ void each_raw(const Row<T>& row, What what, int begin
     }
   }
 }
-struct NotHeld {};
+struct NotHeld {};  // four loads ahead
+struct OneAhead {};  // one: for much work on each, whose code is there once (unrolled it is fetched for one pass only)
+template <typename T, typename What>
+__device__ __forceinline__ void each_raw(const Row<T>& row, OneAhead, What what) {
+  int v = row.whole + (int)threadIdx.x;
+  if (v >= row.past) return;
+  Raw<T> next = row.raw(v);
+#pragma clang loop unroll(disable)
+  for (; v < row.past; v += kThreads) {
+    const Raw<T> r = next;
+    next = row.raw(v + kThreads < row.past ? v + kThreads : v);
+    what(r, row.first(v));
+  }
+}
 template <typename H>
 constexpr int held_vectors() {
-  if constexpr (std::is_same<H, NotHeld>::value)
+  if constexpr (std::is_same<H, NotHeld>::value || std::is_same<H, OneAhead>::value)
     return 0;
   else
     return H::kVectors;
@@ -308,7 +373,7 @@ template <typename T, typename What, typename H = NotHeld>
 __device__ __forceinline__ void each_vector(const Row<T>& row, What what, const H& held = H()) {
   auto one = [&](const Raw<T>& r, int e) VQX_INLINE {
     float x[8];
-    values(r, x);
+    row.logits(r, x);
     what(x, e);
   };
   each_raw(row, held, one);
@@ -322,10 +387,10 @@ __device__ __forceinline__ void each_vector(const Row<T>& row, What what, const 
 }
 template <typename T, typename What>
 __device__ __forceinline__ void each_token(const Row<T>& row, What what) {
-  each_vector(row, [&](const float(&x)[8], int e) {
+  each_vector(row, [&](const float(&x)[8], int e) VQX_INLINE {
 #pragma unroll
     for (int j = 0; j < 8; ++j) what(sound(x[j]), e + j);
-  });
+  }, OneAhead());
 }
 
 // The listed orders sorted, padded to a power of two with the largest.
@@ -351,13 +416,13 @@ __device__ __forceinline__ int sort_list(Shared& s, int n) {
 // too many tokens to sort it is cut into finer ones by their order, again and
 // again: an order's 64 bits end after six times.
 template <bool kShare, typename T>
-__device__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut, u64 most, double share, u64& upto) {
+__device__ __forceinline__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut, u64 most, double share, u64& upto) {
   u64 lo = 0, hi = ~0ull;
   uint32_t n = s.count[cut.bin];
   for (int level = 0; level < 6 && n > (uint32_t)kMostListed; ++level) {
     // the range that the tokens have
     u64 least = ~0ull, greatest = 0;
-    each_token(row, [&](float x, int i) {
+    each_token(row, [&](float x, int i) VQX_INLINE {
       const u64 o = order(x, i);
       if (bin_of(scale, x) == cut.bin && o >= lo && o <= hi) {
         least = o < least ? o : least;
@@ -373,12 +438,12 @@ __device__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut
     lo = s.found[2], hi = s.found[3];
     const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 11 ? bits - 11 : 0;
     clear_bins(s);
-    each_token(row, [&](float x, int i) {
+    each_token(row, [&](float x, int i) VQX_INLINE {
       const u64 o = order(x, i);
       if (bin_of(scale, x) == cut.bin && o >= lo && o <= hi) {
         const int b = (int)((o - lo) >> shift);
         atomicAdd(&s.count[b], 1u);
-        atomicAdd(&s.mass[b], weight(scale, x));
+        if (kShare) atomicAdd(&s.mass[b], whole_weight(s, scale, x));
       }
     });
     __syncthreads();
@@ -392,7 +457,7 @@ __device__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut
   __syncthreads();
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  each_token(row, [&](float x, int i) {
+  each_token(row, [&](float x, int i) VQX_INLINE {
     const u64 o = order(x, i);
     if (bin_of(scale, x) == cut.bin && o >= lo && o <= hi) {
       const int at = atomicAdd(&s.listed, 1);
@@ -407,7 +472,7 @@ __device__ u64 resolve(Shared& s, const Row<T>& row, const Scale& scale, Cut cut
   const int first = 4 * (int)threadIdx.x;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    w[j] = first + j < (int)n ? weight(scale, logit_of(s.list[first + j])) : 0;
+    w[j] = first + j < (int)n ? whole_weight(s, scale, logit_of(s.list[first + j])) : 0;
     mine += w[j];
   }
   u64 before = cut.mass + scan_before(s, mine, all);
@@ -435,25 +500,23 @@ __device__ __forceinline__ void list_tokens(Shared& s, const Row<T>& row, const 
   uint32_t* list = reinterpret_cast<uint32_t*>(s.list);
   // Logits are compared as they are, bf16 in the upper half of a word with the
   // lower half behind it: that moves them by less than their last place, 2^-7 of
-  // them (an infinity would become a NaN; where there is one it is compared by
-  // itself).  The border is lower by that and by the roundings here.
+  // them (an infinity would become a NaN; rows with one have their own way).  The
+  // border is lower by that and by the roundings here.
   const float span = (float)(last + 1) / scale.coarse;
   float least = scale.top - span;
   least -= __builtin_fabsf(least) * 0x1p-6f + (__builtin_fabsf(scale.top) + span) * 0x1p-20f + 0x1p-100f;
   if (!(least > -3.4028235e38f)) least = -3.4028235e38f;  // every finite one
-  const bool infinite = scale.top == -kNone;
-  if (infinite) least = scale.top;
   // a bit for each element, from the highest down
   auto marks = [&](const Raw<T>& r, bool there, uint32_t bits) VQX_INLINE -> uint32_t {
-    if constexpr (std::is_same<T, Bf16>::value) {
+    if (std::is_same<T, Bf16>::value && !row.infinite) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bits = 2 * bits + (u2f(r.a[j] << 16) >= least);
-        bits = 2 * bits + (u2f(infinite ? r.a[j] & 0xFFFF0000u : r.a[j]) >= least);
+        bits = 2 * bits + (u2f(r.a[j]) >= least);
       }
     } else {
       float x[8];
-      values(r, x);
+      row.logits(r, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) bits = 2 * bits + (x[j] >= least);
     }
@@ -509,7 +572,7 @@ __device__ __forceinline__ void list_tokens(Shared& s, const Row<T>& row, const 
   const int head = row.whole ? (8 - row.before < row.size ? 8 - row.before : row.size) : 0, tail = row.first(row.past);
   const int i = threadIdx.x < 8 ? (int)threadIdx.x : tail + (int)threadIdx.x - 8;
   if (threadIdx.x < 8 ? i < head : (threadIdx.x < 16 && i >= head && i < row.size)) {
-    if (element(row.base, (int64_t)i + row.before, T()) >= least) {
+    if (row.logit(i) >= least) {
       const int at = atomicAdd(&s.listed, 1);
       if (at < kMostListed) list[at] = (uint32_t)i;
     }
@@ -554,7 +617,7 @@ __device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, 
     const int i = j * kThreads + (int)threadIdx.x;
     keeps[j] = i < listed;
     const uint32_t at = list[keeps[j] ? i : 0];
-    x[j] = keeps[j] ? sound(element(row.base, (int64_t)at + row.before, T())) : kNone;
+    x[j] = keeps[j] ? sound(row.logit((int)at)) : kNone;
     o[j] = order(x[j], (int)at);
   }
   const float fine = (float)kBins / (float)(last + 1);
@@ -562,10 +625,10 @@ __device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, 
   for (int j = 0; j < kEach; ++j) {
     w[j] = 0, bin[j] = kBins;
     if (j * kThreads >= listed) continue;
-    const float y = x[j] == scale.top ? 0.0f : (scale.top - x[j]) * scale.coarse;
+    const float y = (scale.top - x[j]) * scale.coarse;
     keeps[j] = keeps[j] && y < (float)(last + 1);
     if (!keeps[j]) continue;
-    w[j] = weight(scale, x[j]);
+    w[j] = whole_weight(s, scale, x[j]);
     bin[j] = (int)(y * fine);
     if (bin[j] >= kBins) bin[j] = kBins - 1;
   }
@@ -683,6 +746,107 @@ __device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, 
   return kDrawn;
 }
 
+// The token drawn of those up to `cut` with weights from `bar` on, however many
+// they are: the masses of runs of 64 vectors, and in the run where the random
+// number falls a wave by itself.  Run 0 is the part of a vector that a row begins
+// with, the last one that it ends with.
+template <typename T>
+__device__ __forceinline__ void draw(Shared& s, const Row<T>& row, const Scale& scale, const Sampling& p, int64_t r,
+                                     u64 cut, double bar) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the last kept logit and the last index that is kept of it
+  const bool every = cut == ~0ull;
+  const float low = every ? kNone : logit_of(cut);
+  const int low_index = every ? 0x7FFFFFFF : (int)(uint32_t)cut;
+  auto kept = [&](float x, int i) VQX_INLINE -> double {
+    const double w = weight(s, scale, x);
+    // no branches: eight of these side by side
+    const bool in = ((x > low) | ((x == low) & (i <= low_index))) & (w >= bar);
+    return in ? w : 0.0;
+  };
+  auto sum_of_8 = [&](const Raw<T>& raw, int e) VQX_INLINE -> double {
+    float x[8];
+    row.logits(raw, x);
+    double a = 0.0, b = 0.0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a += kept(x[2 * j], e + 2 * j), b += kept(x[2 * j + 1], e + 2 * j + 1);
+    return a + b;
+  };
+  // of a part of a vector, -inf where it is not the row's
+  auto sum_of_part = [&](int v) -> double {
+    float x[8];
+    row.load(v, x);
+    double a = 0.0;
+    for (int j = 0; j < 8; ++j) a += kept(x[j], row.first(v) + j);
+    return a;
+  };
+  const int runs = (row.past - row.whole + 63) / 64;
+  int shift = 0;  // runs of a bin
+  while ((runs >> shift) > kBins - 3) ++shift;
+  const int tail = 2 + (runs >> shift);
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
+  __syncthreads();
+  auto put = [&](int run, double sum) VQX_INLINE {
+    const u64 upto = wave_scan((u64)sum);
+    if (lane == 63 && upto != 0) atomicAdd(&s.mass[1 + (run >> shift)], upto);
+  };
+  if (row.whole < row.past) {
+    int v = row.whole + (int)threadIdx.x, run = wave;
+    Raw<T> next = row.raw(v < row.past ? v : row.past - 1);
+#pragma clang loop unroll(disable)
+    for (; row.whole + run * 64 < row.past; run += kWaves, v += kThreads) {
+      const Raw<T> raw = next;
+      next = row.raw(v + kThreads < row.past ? v + kThreads : row.past - 1);
+      put(run, v < row.past ? sum_of_8(raw, row.first(v)) : 0.0);
+    }
+  }
+  if (threadIdx.x == 0 && row.whole > 0) s.mass[0] = (u64)sum_of_part(0);
+  if (threadIdx.x == 64 && row.past >= row.whole && row.past < row.vectors) s.mass[tail] = (u64)sum_of_part(row.past);
+  __syncthreads();
+  const int b0 = 2 * (int)threadIdx.x;
+  u64 total;
+  const u64 m0 = s.mass[b0], m1 = s.mass[b0 + 1], before = scan_before(s, m0 + m1, total);
+  const u64 target = target_of(p.random[r], total);
+  if (target >= before && target < before + m0 + m1) {
+    const bool second = target >= before + m0;
+    s.at = b0 + second, s.found[0] = second ? before + m0 : before;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const int bin = __builtin_amdgcn_readfirstlane(s.at);
+  u64 rest = target - s.found[0];
+  // the vectors of the bin, 64 at a time
+  const int first = bin == 0 ? 0 : (bin == tail ? row.past : row.whole + ((bin - 1) << shift) * 64);
+  const int end = bin == 0 ? 1 : (bin == tail ? row.past + 1 : first + (64 << shift) < row.past ? first + (64 << shift) : row.past);
+  for (int v = first + lane; v - lane < end; v += 64) {
+    float x[8];
+    double w[8], sum = 0.0;
+    row.load(v < end ? v : end - 1, x);
+    const int e = row.first(v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = v < end ? kept(x[j], e + j) : 0.0, sum += w[j];
+    const u64 upto = wave_scan((u64)sum), all = lane_of(upto, 63);
+    if (rest >= all) {
+      rest -= all;
+      continue;
+    }
+    u64 left = upto - (u64)sum;
+    if (rest >= left && rest < upto) {
+      int token = 0;
+      double weighs = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (weighs == 0.0 && rest < left + (u64)w[j]) weighs = w[j], token = e + j;
+        left += (u64)w[j];
+      }
+      p.tokens[r] = token;
+      p.chances[r] = (float)log(weighs / (double)total);
+    }
+    return;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // a row
 // ---------------------------------------------------------------------------
@@ -691,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
-  const Row<T> row(p.logits, r * p.stride, p.vocab);
+  Row<T> row(p.logits, r * p.stride, p.vocab);
   Held<T> held;
   held.load(row);
   const float t = p.temperature ? p.temperature[r] : 1.0f;
@@ -731,12 +895,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
     }
     return;
   }
+  if (top == -kNone) row.infinite = true, top = 0.0f;
   Scale scale;
   scale.top = top;
-  scale.inner = 1.44269504088896340736 / (double)t;
-  const double coarse = scale.inner * kFine;
+  scale.inner = 64.0 * 1.44269504088896340736 / (double)t;
+  const double coarse = scale.inner * (kFine / 64.0);
   scale.coarse = coarse < 1e30 ? (float)coarse : 1e30f;
-  scale.powers = s.powers;
 
   const bool by_count = k > 0 && k < p.vocab, by_share = share < 1.0f;
   const double bar = least > 0.0f ? (least < 1.0f ? (double)least * kUnit : kUnit) : 0.0;
@@ -753,7 +917,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   const int tight = last;
   if (by_count && k <= kThreads) {
     uint32_t* count = reinterpret_cast<uint32_t*>(index_bins(s));
-    const int b = bin_of(scale, mine), b0 = 2 * tid;
+    const int b = bin_of(scale, row.infinite && mine != -kNone ? kNone : __builtin_fminf(mine, top)), b0 = 2 * tid;
     if (b < kBins) atomicAdd(&count[b], 1u);
     __syncthreads();
     const u64 c0 = count[b0], c1 = count[b0 + 1];
@@ -764,27 +928,34 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
     __syncthreads();
     if (all >= (u64)k && s.at < last) last = s.at;
   }
-  // a histogram, with masses only where few tokens cannot do without
+  // a histogram: how many; and all weights' sum; and each bin's
   u64 mass = 0;
-  auto count_bins = [&](bool with_masses) {
+  enum Sums { kCounts, kTotal, kMasses };
+  auto count_bins = [&](auto what) VQX_INLINE {
+    constexpr Sums kWhat = decltype(what)::value;
     clear_bins(s);
-    each_vector(row, [&](const float(&x)[8], int) {
+    double sum = 0.0;
+    each_vector(row, [&](const float(&x)[8], int) VQX_INLINE {
+      double w[8];
+      if (kWhat != kCounts) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = weight(s, scale, x[j]), sum += w[j];
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int b = bin_of(scale, x[j]);
         if (b < kBins) {
           atomicAdd(&s.count[b], 1u);
-          if (with_masses) atomicAdd(&s.mass[b], weight(scale, sound(x[j])));
+          if (kWhat == kMasses) atomicAdd(&s.mass[b], (u64)w[j]);
         }
       }
-    });
+    }, std::conditional_t<kWhat == kCounts, NotHeld, OneAhead>());
     __syncthreads();
-    if (with_masses) {
-      mass = 0;
-      for (int i = tid; i < kBins; i += kThreads) mass += s.mass[i];
-      mass = sum_of(s, mass);
-    }
+    if (kWhat != kCounts) mass = sum_of(s, (u64)sum);
   };
+  auto counts = std::integral_constant<Sums, kCounts>();
+  auto with_total = std::integral_constant<Sums, kTotal>();
+  auto with_masses = std::integral_constant<Sums, kMasses>();
   // few tokens, by what is known so far, or by a histogram of the row
   const u64 most = by_count ? (u64)k : 0;
   Few done = kTooMany;
@@ -792,8 +963,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   if (done == kDrawn) return;
   if (done == kTooMany && (by_count || by_share)) {
     last = tight;
-    count_bins(!by_count);
-    const Cut c = by_count ? find_bin<false, true>(s, none, most, 0.0) : find_bin<true, true>(s, none, 0, share_of(share, mass));
+    Cut c;
+    if (by_count) {
+      count_bins(counts);
+      c = find_bin<false>(s, none, most, 0.0);
+    } else {
+      count_bins(with_total);
+      c = find_least(s, share_of(share, mass));
+    }
     const bool listable = c.bin < last ? c.count + s.count[c.bin] <= (u64)kMostListed : last < kBins;
     if (c.bin < last) last = c.bin;
     if (listable) {
@@ -804,16 +981,27 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
     }
   }
   if (by_count || by_share) {
-    // every token's weight, cut by cut
-    count_bins(true);
+    // cut by cut
+    if (by_share)
+      count_bins(with_masses);
+    else
+      count_bins(counts);
     if (by_count) {
-      const Cut c = find_bin<false, true>(s, none, (u64)k, 0.0);
+      const Cut c = by_share ? find_bin<false, true>(s, none, most, 0.0) : find_bin<false>(s, none, most, 0.0);
       if (c.bin < kBins) {
         // the histogram is made again by a bin that is cut finer
         const bool keeps = s.count[c.bin] <= (uint32_t)kMostListed;
         u64 upto;
-        cut = resolve<false>(s, row, scale, c, (u64)k, 0.0, upto);
-        if (by_share && !keeps) count_bins(true);
+        cut = resolve<false>(s, row, scale, c, most, 0.0, upto);
+        if (by_share && !keeps) {
+          // up to the cut, which is in the bin
+          double sum = 0.0;
+          each_token(row, [&](float x, int i) VQX_INLINE {
+            if (order(x, i) <= cut) sum += weight(s, scale, x);
+          });
+          upto = sum_of(s, (u64)sum);
+          count_bins(with_masses);
+        }
         mass = upto;
       }
     }
@@ -827,68 +1015,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
       }
     }
   }
-  auto kept = [&](float x, int i) -> u64 {
-    if (order(x, i) > cut) return 0;
-    const u64 w = weight(scale, x);
-    return (double)w >= bar ? w : 0;
-  };
-  // which run of vectors, then which of a wave's, then which token: the runs of
-  // the waves, then one of them shared out again
-  int from = 0, to = row.vectors;
-  u64 total = 0, target = 0;
-  while (true) {
-    const int each = (to - from + kWaves - 1) / kWaves, begin = from + wave * each;
-    const int end = begin + each < to ? begin + each : to;
-    u64 mine = 0, upto = 0;
-    for (int v = begin + lane; v < end; v += 64) {
-      float x[8];
-      row.load(v, x);
-      const int e = row.first(v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mine += kept(sound(x[j]), e + j);
-    }
-    upto = wave_scan(mine);
-    __syncthreads();
-    if (lane == 63) s.sums[0][wave] = upto;
-    __syncthreads();
-    u64 before = 0, all = 0;
-    int run = 0;
-    if (total == 0) {
-      for (int w = 0; w < kWaves; ++w) total += s.sums[0][w];
-      target = target_of(p.random[r], total);
-    }
-    for (int w = 0; w < kWaves; ++w) {
-      if (all + s.sums[0][w] > target) break;
-      all += s.sums[0][w];
-      run = w + 1;
-    }
-    target -= all;
-    from += run * each;
-    to = from + each < to ? from + each : to;
-    if (each > 64) continue;
-    // one vector a lane: the lane, then the token
-    if (wave != run) return;
-    before = upto - mine;
-    if (target >= before && target < upto) {
-      const int v = begin + lane;
-      float x[8];
-      row.load(v, x);
-      const int e = row.first(v);
-      u64 left = target - before, weighs = 0;
-      int token = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const u64 w = kept(sound(x[j]), e + j);
-        if (weighs == 0) {
-          if (left < w) weighs = w, token = e + j;
-          left -= w;
-        }
-      }
-      p.tokens[r] = token;
-      p.chances[r] = (float)log((double)weighs / (double)total);
-    }
-    return;
-  }
+  draw(s, row, scale, p, r, cut, bar);
 }
 
 }  // namespace
