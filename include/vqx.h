@@ -885,11 +885,16 @@ int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_
  * drawn; a row without a logit above -inf has token -1 and chance -inf; infinite
  * ones are as likely as each other, and no others are drawn.
  * temperature, top_k, top_p, min_p: [rows], int32 for top_k and fp32 for the
- * others, or NULL (1, and none).  vocab: 1 .. 2^22.
+ * others, or NULL (1, and none).  vocab: 1 .. 2^22.  workspace:
+ * vqx_sample_tokens_workspace_size bytes for the same sizes and by_count 1 where
+ * top_k is given, else 0; 16-byte aligned, or NULL where that is 0.  The same row,
+ * number and parameters give the same token with and without one.
  */
 int vqx_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride,
                       const float* random, const float* temperature, const int32_t* top_k, const float* top_p,
-                      const float* min_p, int64_t* tokens, float* chances, vqx_stream_t stream);
+                      const float* min_p, int64_t* tokens, float* chances, void* workspace, int64_t workspace_bytes,
+                      vqx_stream_t stream);
+int vqx_sample_tokens_workspace_size(int32_t dtype, int64_t rows, int64_t vocab, int32_t by_count, int64_t* bytes);
 
 #ifdef __cplusplus
 }

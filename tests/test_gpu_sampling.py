@@ -211,6 +211,51 @@ def test_many_rows_and_a_large_vocabulary(ops):
     check(ops, x, u, [0.1 * (i % 20) for i in range(700)], [i % 60 for i in range(700)])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab,start", [(8192, 0), (8193, 3), (32000, 1), (130001, 5), (260000, 0)])
+def test_rows_shared_out(ops, kind, vocab, start):
+    """Few long rows are shared out over workgroups where no number of tokens
+    bounds them; a top_k that keeps all takes the other way to the same tokens."""
+    x, u = rows(5, vocab, kind, vocab)
+    x[1, 7::3] = -math.inf
+    x[2, 100] = x[2, vocab - 1] = math.inf
+    x[3, ::2] = math.nan
+    x[4] = -math.inf
+    wide = torch.full((5, start + vocab + 1), 9.0, dtype=x.dtype)
+    wide[:, start:start + vocab] = x
+    view, u = wide.to(DEV)[:, start:start + vocab], torch.tensor(u, device=DEV)
+    every = torch.zeros(5, dtype=torch.int32, device=DEV)
+    f = lambda *v: torch.tensor(v, device=DEV)  # noqa: E731
+    for t, p, m in ((None, None, None), (f(1.0, 0.5, 2.0, 1.3, 1.0), None, None), (f(0.0, 0.3, 1.0, 0.0, 1.0), None, None),
+                    (None, f(0.9, 0.5, 0.3, 1.0, 0.9), None), (None, None, f(0.01, 0.0, 0.5, 0.3, 0.1)),
+                    (f(3.0, 0.2, 1.0, 1.0, 1.0), f(0.99, 0.01, 0.9, 0.0, 0.9), f(0.0, 0.1, 0.0, 1.0, 0.0)),
+                    (f(9.0, 9.0, 9.0, 9.0, 9.0), f(0.999, 0.7, 0.9, 0.9, 0.9), None)):
+        got, want = ops.sample_tokens(view, u, t, None, p, m), ops.sample_tokens(view, u, t, every, p, m)
+        assert torch.equal(got[0], want[0]), (t, p, m)
+        assert torch.equal(got[1], want[1])
+
+
+def test_shared_rows_graph(ops):
+    """Captured twice, replayed in turn: the launches of a row share what is theirs."""
+    x, u = torch.randn(2, 50000, device=DEV), torch.rand(2, device=DEV)
+    p = torch.full((2,), 0.8, device=DEV)
+    ops.sample_tokens(x, u, None, None, p)
+    graphs = []
+    for args in ((None, None, p), ()):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.sample_tokens(x, u, *args)
+        graphs.append((graph, out, args))
+    for i in range(4):
+        x.copy_(torch.randn(2, 50000)), u.copy_(torch.rand(2))
+        for graph, out, args in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, args in graphs:
+            want = ops.sample_tokens(x, u, *args)
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+
+
 def test_the_same_each_time(ops):
     x, u = rows(16, 60000, "bf16", 11)
     args = (x.to(DEV), torch.tensor(u, device=DEV), None, torch.full((16,), 20000, dtype=torch.int32, device=DEV),

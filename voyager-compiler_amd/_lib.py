@@ -191,7 +191,8 @@ _SIGNATURES = {
     "vqx_kv4_reserve": ([_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P], ctypes.c_int),
     "vqx_kv4_tree_attention_workspace_size": ([_KC, _KQ, ctypes.POINTER(_I64)], ctypes.c_int),
     "vqx_kv4_tree_attention": ([_KC, _KQ, _P, _P, _P, _P, _I64, _P], ctypes.c_int),
-    "vqx_sample_tokens": ([_P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P], ctypes.c_int),
+    "vqx_sample_tokens": ([_P, _I32, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], ctypes.c_int),
+    "vqx_sample_tokens_workspace_size": ([_I32, _I64, _I64, _I32, ctypes.POINTER(_I64)], ctypes.c_int),
     "vqx_kv4_accept": ([_KC, _P, _P, _P, _I64, _P, _P, _P, _P, _P], ctypes.c_int),
 }
 

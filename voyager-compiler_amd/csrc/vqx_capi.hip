@@ -221,6 +221,19 @@ static int to_turn(const vqx_turn* t, int64_t dim, bool places, const char* what
   return kOk;
 }
 
+static int to_sampling(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride, const float* random,
+                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                       int64_t* tokens, float* chances, Sampling* p) {
+  const int rc = kv4_float(dtype, "sample_tokens");
+  if (rc != kOk) return rc;
+  if (rows < 0 || rows >= 1ll << 31) return set_error(kErrInvalid, "sample_tokens: %lld rows", (long long)rows);
+  // the weights' sum is to stay below 2^63
+  if (vocab < 1 || vocab > 1ll << 22)
+    return set_error(kErrInvalid, "sample_tokens: 1 to 2^22 logits in a row, not %lld", (long long)vocab);
+  *p = Sampling{logits, stride, rows, (int32_t)vocab, random, temperature, top_k, top_p, min_p, tokens, chances};
+  return kOk;
+}
+
 extern "C" {
 
 const char* vqx_version(void) { return "vqx 0.1.0 gfx950"; }
@@ -890,21 +903,33 @@ int vqx_kv4_accept(const vqx_kv4_cache* cache, const int64_t* tree, const int64_
   return kv4_accept(c, cache->dim, q, tree, drafts, sampled, path, accepted, next, (hipStream_t)stream);
 }
 
+int vqx_sample_tokens_workspace_size(int32_t dtype, int64_t rows, int64_t vocab, int32_t by_count, int64_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return set_error(kErrInvalid, "sample_tokens_workspace_size: bytes is NULL");
+  Sampling p;
+  // top_k is not read: any address stands for one
+  const int rc = to_sampling(nullptr, dtype, rows, vocab, vocab, nullptr, nullptr,
+                             by_count ? reinterpret_cast<const int32_t*>(bytes) : nullptr, nullptr, nullptr, nullptr, nullptr, &p);
+  if (rc != kOk) return rc;
+  *bytes = sample_workspace(p);
+  return kOk;
+}
+
 int vqx_sample_tokens(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride,
                       const float* random, const float* temperature, const int32_t* top_k, const float* top_p,
-                      const float* min_p, int64_t* tokens, float* chances, vqx_stream_t stream) {
+                      const float* min_p, int64_t* tokens, float* chances, void* workspace, int64_t workspace_bytes,
+                      vqx_stream_t stream) {
   g_err[0] = 0;
-  const int rc = kv4_float(dtype, "sample_tokens");
-  if (rc != kOk) return rc;
-  if (rows < 0 || rows >= 1ll << 31) return set_error(kErrInvalid, "sample_tokens: %lld rows", (long long)rows);
-  // the weights' sum is to stay below 2^63
-  if (vocab < 1 || vocab > 1ll << 22)
-    return set_error(kErrInvalid, "sample_tokens: 1 to 2^22 logits in a row, not %lld", (long long)vocab);
-  if (rows == 0) return kOk;
+  Sampling p;
+  const int rc = to_sampling(logits, dtype, rows, vocab, stride, random, temperature, top_k, top_p, min_p, tokens, chances, &p);
+  if (rc != kOk || rows == 0) return rc;
   if (!logits || !random || !tokens || !chances) return set_error(kErrInvalid, "sample_tokens: null tensor");
   if (!aligned(logits, dtype == kF32 ? 4 : 2)) return set_error(kErrInvalid, "sample_tokens: logits are not aligned");
-  return sample(Sampling{logits, stride, rows, (int32_t)vocab, random, temperature, top_k, top_p, min_p, tokens, chances},
-                dtype, (hipStream_t)stream);
+  const int64_t need = sample_workspace(p);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return set_error(kErrInvalid, "sample_tokens: needs a 16-byte aligned workspace of %lld bytes, not %lld",
+                     (long long)need, (long long)workspace_bytes);
+  return sample(p, dtype, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -20,6 +20,7 @@ struct Sampling {
   float* chances;            // [rows]
 };
 
-int sample(const Sampling& p, int dtype, hipStream_t st);
+int64_t sample_workspace(const Sampling& p);  // bytes, 0: none
+int sample(const Sampling& p, int dtype, void* ws, hipStream_t st);
 
 }  // namespace vqx

@@ -75,6 +75,8 @@ struct Row {
   int before;           // elements of vector 0 that are not the row's
   int size, vectors;
   int whole, past;  // vectors [whole, past) have 8 of the row's
+  bool head;        // vector 0 has fewer, and so has
+  int tail;         // this one, -1: none
   bool infinite;    // where some are +inf those count as 0 and all others as -inf
 
   __device__ __forceinline__ Row(const void* p, int64_t offset, int n) {
@@ -85,8 +87,23 @@ struct Row {
     vectors = (n + before + 7) / 8;
     whole = before > 0;
     past = (n + before) / 8;
+    head = before > 0;
+    tail = past >= whole && past < vectors ? past : -1;
     infinite = false;
   }
+  __device__ __forceinline__ int runs() const { return past > whole ? (past - whole + 63) / 64 : 0; }
+  // The g-th of `parts` of the row: as many runs of 64 vectors each.
+  __device__ __forceinline__ Row part(int g, int parts) const {
+    Row r = *this;
+    const int each = (runs() + parts - 1) / parts * 64, begin = whole + g * each;
+    r.whole = begin < past ? begin : past;
+    r.past = begin + each < past ? begin + each : past;
+    if (r.past < r.whole) r.past = r.whole;
+    if (g > 0) r.head = false;
+    if (g + 1 < parts) r.tail = -1;
+    return r;
+  }
+
   __device__ __forceinline__ int first(int v) const { return 8 * v - before; }
   __device__ __forceinline__ Raw<T> raw(int v) const {
     const uint8_t* p = base + (int64_t)v * 8 * kSize;
@@ -139,14 +156,6 @@ struct Scale {
   float coarse;  // log2(e) / temperature, in bins
 };
 
-// p r + c with c in scalar registers (the compiler copies a constant into vector
-// registers first, which is one instruction more for each).
-__device__ __forceinline__ double fma_constant(double p, double r, double c) {
-  double d;
-  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(p), "v"(r), "s"(c));
-  return d;
-}
-
 // A whole number up to 2^40, as a double: sums of them are exact up to 2^53.
 __device__ __forceinline__ double weight(const Shared& s, const Scale& scale, float x) {
   // 64ths of a halving; 42 of these are 0 already, a NaN or -inf is one of those
@@ -157,11 +166,11 @@ __device__ __forceinline__ double weight(const Shared& s, const Scale& scale, fl
   const int i = (int)(uint32_t)__builtin_bit_cast(u64, n);
   const double r = q - (n - 0x1.8p52);
   // 2^(r / 64) to 2^-54: Taylor's series in r ln2 / 64, up to 0.0054
-  double p = fma_constant(0x1.5d87fe78a6731p-40, r, 0x1.3b2ab6fba4e77p-31);  // (ln2 / 64)^5 / 120, (ln2 / 64)^4 / 24
-  p = fma_constant(p, r, 0x1.c6b08d704a0c0p-23);                             // (ln2 / 64)^3 / 6
-  p = fma_constant(p, r, 0x1.ebfbdff82c58fp-15);                             // (ln2 / 64)^2 / 2
-  p = fma_constant(p, r, 0x1.62e42fefa39efp-7);                              // ln2 / 64
-  p = fma_constant(p, r, 1.0);
+  double p = __builtin_fma(0x1.5d87fe78a6731p-40, r, 0x1.3b2ab6fba4e77p-31);  // (ln2 / 64)^5 / 120, (ln2 / 64)^4 / 24
+  p = __builtin_fma(p, r, 0x1.c6b08d704a0c0p-23);                             // (ln2 / 64)^3 / 6
+  p = __builtin_fma(p, r, 0x1.ebfbdff82c58fp-15);                             // (ln2 / 64)^2 / 2
+  p = __builtin_fma(p, r, 0x1.62e42fefa39efp-7);                              // ln2 / 64
+  p = __builtin_fma(p, r, 1.0);
   // times 2^((i % 64) / 64) 2^(i / 64) 2^40, rounded to a whole number
   const u64 power = __builtin_bit_cast(u64, s.powers[i & 63]) + ((u64)(uint32_t)(((i >> 6) + 40) << 20) << 32);
   return __builtin_fma(__builtin_bit_cast(double, power), p, 0x1p52) - 0x1p52;
@@ -378,8 +387,8 @@ __device__ __forceinline__ void each_vector(const Row<T>& row, What what, const 
   };
   each_raw(row, held, one);
   // the first and the last, where they are parts of one
-  const int part = threadIdx.x == 0 && row.whole > 0 ? 0 : (threadIdx.x == 64 && row.past >= row.whole ? row.past : -1);
-  if (part >= 0 && part < row.vectors) {
+  const int part = threadIdx.x == 0 && row.head ? 0 : (threadIdx.x == 64 ? row.tail : -1);
+  if (part >= 0) {
     float x[8];
     row.load(part, x);
     what(x, row.first(part));
@@ -746,63 +755,65 @@ __device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, 
   return kDrawn;
 }
 
-// The token drawn of those up to `cut` with weights from `bar` on, however many
-// they are: the masses of runs of 64 vectors, and in the run where the random
-// number falls a wave by itself.  Run 0 is the part of a vector that a row begins
-// with, the last one that it ends with.
-template <typename T>
-__device__ __forceinline__ void draw(Shared& s, const Row<T>& row, const Scale& scale, const Sampling& p, int64_t r,
-                                     u64 cut, double bar) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the last kept logit and the last index that is kept of it
-  const bool every = cut == ~0ull;
-  const float low = every ? kNone : logit_of(cut);
-  const int low_index = every ? 0x7FFFFFFF : (int)(uint32_t)cut;
-  auto kept = [&](float x, int i) VQX_INLINE -> double {
+// The weight of a token that is kept, 0 of another: those up to `cut` with
+// weights from `bar` on.
+struct Kept {
+  float low;      // the last kept logit,
+  int low_index;  // and the last index that is kept of it
+  double bar;
+
+  __device__ __forceinline__ Kept(u64 cut, double least) {
+    const bool every = cut == ~0ull;
+    low = every ? kNone : logit_of(cut);
+    low_index = every ? 0x7FFFFFFF : (int)(uint32_t)cut;
+    bar = least;
+  }
+  __device__ __forceinline__ double operator()(const Shared& s, const Scale& scale, float x, int i) const {
     const double w = weight(s, scale, x);
     // no branches: eight of these side by side
     const bool in = ((x > low) | ((x == low) & (i <= low_index))) & (w >= bar);
     return in ? w : 0.0;
-  };
-  auto sum_of_8 = [&](const Raw<T>& raw, int e) VQX_INLINE -> double {
+  }
+};
+
+// The masses of a row's runs of 64 vectors: put(run, mass) by one lane each.
+template <typename T, typename Put>
+__device__ __forceinline__ void sum_runs(const Shared& s, const Row<T>& row, const Scale& scale, const Kept& kept, Put put) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row.whole >= row.past) return;
+  int v = row.whole + (int)threadIdx.x, run = wave;
+  Raw<T> next = row.raw(v < row.past ? v : row.past - 1);
+#pragma clang loop unroll(disable)
+  for (; row.whole + run * 64 < row.past; run += kWaves, v += kThreads) {
+    const Raw<T> raw = next;
+    next = row.raw(v + kThreads < row.past ? v + kThreads : row.past - 1);
     float x[8];
     row.logits(raw, x);
+    const int e = row.first(v);
     double a = 0.0, b = 0.0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a += kept(x[2 * j], e + 2 * j), b += kept(x[2 * j + 1], e + 2 * j + 1);
-    return a + b;
-  };
-  // of a part of a vector, -inf where it is not the row's
-  auto sum_of_part = [&](int v) -> double {
-    float x[8];
-    row.load(v, x);
-    double a = 0.0;
-    for (int j = 0; j < 8; ++j) a += kept(x[j], row.first(v) + j);
-    return a;
-  };
-  const int runs = (row.past - row.whole + 63) / 64;
-  int shift = 0;  // runs of a bin
-  while ((runs >> shift) > kBins - 3) ++shift;
-  const int tail = 2 + (runs >> shift);
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
-  __syncthreads();
-  auto put = [&](int run, double sum) VQX_INLINE {
-    const u64 upto = wave_scan((u64)sum);
-    if (lane == 63 && upto != 0) atomicAdd(&s.mass[1 + (run >> shift)], upto);
-  };
-  if (row.whole < row.past) {
-    int v = row.whole + (int)threadIdx.x, run = wave;
-    Raw<T> next = row.raw(v < row.past ? v : row.past - 1);
-#pragma clang loop unroll(disable)
-    for (; row.whole + run * 64 < row.past; run += kWaves, v += kThreads) {
-      const Raw<T> raw = next;
-      next = row.raw(v + kThreads < row.past ? v + kThreads : row.past - 1);
-      put(run, v < row.past ? sum_of_8(raw, row.first(v)) : 0.0);
-    }
+    for (int j = 0; j < 4; ++j) a += kept(s, scale, x[2 * j], e + 2 * j), b += kept(s, scale, x[2 * j + 1], e + 2 * j + 1);
+    const u64 upto = wave_scan(v < row.past ? (u64)(a + b) : 0);
+    if (lane == 63) put(run, upto);
   }
-  if (threadIdx.x == 0 && row.whole > 0) s.mass[0] = (u64)sum_of_part(0);
-  if (threadIdx.x == 64 && row.past >= row.whole && row.past < row.vectors) s.mass[tail] = (u64)sum_of_part(row.past);
+}
+// Of a vector that the row has a part of.
+template <typename T>
+__device__ __forceinline__ u64 sum_part(const Shared& s, const Row<T>& row, const Scale& scale, const Kept& kept, int v) {
+  float x[8];
+  row.load(v, x);
+  double a = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a += kept(s, scale, x[j], row.first(v) + j);
+  return (u64)a;
+}
+
+// The token drawn, given the masses in s.mass: bin 0 is the part of a vector that
+// a row begins with, then come 2^shift runs each, then the part that it ends with.
+template <typename T>
+__device__ __forceinline__ void pick(Shared& s, const Row<T>& row, const Scale& scale, const Sampling& p, int64_t r,
+                                     const Kept& kept, int shift) {
+  const int lane = threadIdx.x & 63, tail = 2 + (row.runs() >> shift);
   __syncthreads();
   const int b0 = 2 * (int)threadIdx.x;
   u64 total;
@@ -813,19 +824,19 @@ __device__ __forceinline__ void draw(Shared& s, const Row<T>& row, const Scale& 
     s.at = b0 + second, s.found[0] = second ? before + m0 : before;
   }
   __syncthreads();
-  if (wave != 0) return;
+  if (threadIdx.x >= 64) return;
   const int bin = __builtin_amdgcn_readfirstlane(s.at);
   u64 rest = target - s.found[0];
   // the vectors of the bin, 64 at a time
-  const int first = bin == 0 ? 0 : (bin == tail ? row.past : row.whole + ((bin - 1) << shift) * 64);
-  const int end = bin == 0 ? 1 : (bin == tail ? row.past + 1 : first + (64 << shift) < row.past ? first + (64 << shift) : row.past);
+  const int first = bin == 0 ? 0 : (bin == tail ? row.tail : row.whole + ((bin - 1) << shift) * 64);
+  const int end = bin == 0 ? 1 : (bin == tail ? row.tail + 1 : first + (64 << shift) < row.past ? first + (64 << shift) : row.past);
   for (int v = first + lane; v - lane < end; v += 64) {
     float x[8];
     double w[8], sum = 0.0;
     row.load(v < end ? v : end - 1, x);
     const int e = row.first(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = v < end ? kept(x[j], e + j) : 0.0, sum += w[j];
+    for (int j = 0; j < 8; ++j) w[j] = v < end ? kept(s, scale, x[j], e + j) : 0.0, sum += w[j];
     const u64 upto = wave_scan((u64)sum), all = lane_of(upto, 63);
     if (rest >= all) {
       rest -= all;
@@ -847,35 +858,144 @@ __device__ __forceinline__ void draw(Shared& s, const Row<T>& row, const Scale& 
   }
 }
 
+// Runs of 64 vectors that have a bin of their own, with two for the row's ends.
+constexpr int kMostRuns = kBins - 3;
+
+// The token drawn of those that are kept, however many they are: the masses of
+// runs, and in the one where the random number falls a wave by itself.
+template <typename T>
+__device__ __forceinline__ void draw(Shared& s, const Row<T>& row, const Scale& scale, const Sampling& p, int64_t r,
+                                     const Kept& kept) {
+  int shift = 0;
+  while ((row.runs() >> shift) > kMostRuns) ++shift;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0;
+  __syncthreads();
+  sum_runs(s, row, scale, kept, [&](int run, u64 mass) { if (mass) atomicAdd(&s.mass[1 + (run >> shift)], mass); });
+  if (threadIdx.x == 0 && row.head) s.mass[0] = sum_part(s, row, scale, kept, 0);
+  if (threadIdx.x == 64 && row.tail >= 0) s.mass[2 + (row.runs() >> shift)] = sum_part(s, row, scale, kept, row.tail);
+  pick(s, row, scale, p, r, kept, shift);
+}
+
 // ---------------------------------------------------------------------------
 // a row
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
-  __shared__ Shared s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
-  Row<T> row(p.logits, r * p.stride, p.vocab);
-  Held<T> held;
-  held.load(row);
-  const float t = p.temperature ? p.temperature[r] : 1.0f;
-  const int k = p.top_k ? p.top_k[r] : 0;
-  const float share = p.top_p ? p.top_p[r] : 1.0f, least = p.min_p ? p.min_p[r] : 0.0f;
-  if (tid < 64) s.powers[tid] = exp2((double)tid / 64.0);
-  clear_few(s);
+// What the workgroups of a row leave each other.
+constexpr int kMostParts = 256;
+struct Parts {
+  u64 runs[kBins];  // the masses of runs, as pick() takes them,
+  u64 mass[kBins];  // or the histogram
+  uint32_t count[kBins];
+  float tops[kMostParts];
+};
+
+__device__ __forceinline__ Scale scale_of(float top, float t) {
+  Scale scale;
+  scale.top = top;
+  scale.inner = 64.0 * 1.44269504088896340736 / (double)t;
+  const double coarse = scale.inner * (kFine / 64.0);
+  scale.coarse = coarse < 1e30 ? (float)coarse : 1e30f;
+  return scale;
+}
+// The least weight that is kept.
+__device__ __forceinline__ double bar_of(float least) {
+  return least > 0.0f ? (least < 1.0f ? (double)least * kUnit : kUnit) : 0.0;
+}
+// The largest of the lanes' and the waves'.
+__device__ __forceinline__ float top_of(Shared& s, float top) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) s.tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = __builtin_fmaxf(top, s.tops[w]);
+  return top + 0.0f;
+}
+template <typename T, typename H>
+__device__ __forceinline__ float largest(const Row<T>& row, const H& held) {
   float top = kNone;
   each_vector(row, [&](const float(&x)[8], int) VQX_INLINE {
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, x[j]);  // a NaN is no maximum
   }, held);
-  const float mine = top;
+  return top;
+}
+
+// Few rows: a row's largest logit by many workgroups; what the next launch adds
+// to is cleared.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_top_kernel(Sampling p, Parts* parts, int each) {
+  __shared__ Shared s;
+  const int64_t r = blockIdx.x / (unsigned)each;
+  const int g = (int)(blockIdx.x % (unsigned)each);
+  const Row<T> row = Row<T>(p.logits, r * p.stride, p.vocab).part(g, each);
+  const float top = top_of(s, largest(row, NotHeld()));
+  Parts& to = parts[r];
+  if (threadIdx.x == 0) to.tops[g] = top;
+  for (int i = g * kThreads + (int)threadIdx.x; i < kBins; i += each * kThreads) to.runs[i] = 0, to.mass[i] = 0, to.count[i] = 0;
+}
+
+// Few rows: the masses of its runs, or (top-p) its histogram.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_sums_kernel(Sampling p, Parts* parts, int each) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / (unsigned)each;
+  const int g = (int)(blockIdx.x % (unsigned)each);
+  Parts& to = parts[r];
+  const Row<T> whole(p.logits, r * p.stride, p.vocab);
+  Row<T> row = whole.part(g, each);
+  const float t = p.temperature ? p.temperature[r] : 1.0f, share = p.top_p ? p.top_p[r] : 1.0f;
+  const double bar = bar_of(p.min_p ? p.min_p[r] : 0.0f);
+  if (tid < 64) s.powers[tid] = exp2((double)tid / 64.0);
+  float top = top_of(s, tid < each ? to.tops[tid] : kNone);
+  if (top == kNone || !(t > 0.0f)) return;
+  if (top == -kNone) row.infinite = true, top = 0.0f;
+  const Scale scale = scale_of(top, t);
+  if (!(share < 1.0f)) {
+    const Kept kept(~0ull, bar);
+    const int before = 1 + (row.whole - whole.whole) / 64;
+    sum_runs(s, row, scale, kept, [&](int run, u64 mass) { to.runs[before + run] = mass; });
+    if (tid == 0 && row.head) to.runs[0] = sum_part(s, row, scale, kept, 0);
+    if (tid == 64 && row.tail >= 0) to.runs[2 + whole.runs()] = sum_part(s, row, scale, kept, row.tail);
+    return;
+  }
+  clear_bins(s);
+  each_vector(row, [&](const float(&x)[8], int) VQX_INLINE {
+    double w[8];
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
-  if (lane == 0) s.tops[wave] = top;
+    for (int j = 0; j < 8; ++j) w[j] = weight(s, scale, x[j]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int b = bin_of(scale, x[j]);
+      if (b < kBins) atomicAdd(&s.count[b], 1u), atomicAdd(&s.mass[b], (u64)w[j]);
+    }
+  }, OneAhead());
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = __builtin_fmaxf(top, s.tops[w]);
-  top += 0.0f;
+  for (int i = tid; i < kBins; i += kThreads)
+    if (s.count[i]) atomicAdd(&to.count[i], s.count[i]), atomicAdd(&to.mass[i], s.mass[i]);
+}
+
+// kParts: the launches above have been there.
+template <typename T, bool kParts>
+__global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p, const Parts* parts, int each) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  Row<T> row(p.logits, r * p.stride, p.vocab);
+  std::conditional_t<kParts, NotHeld, Held<T>> held;
+  if constexpr (!kParts) held.load(row);
+  const float t = p.temperature ? p.temperature[r] : 1.0f;
+  const int k = !kParts && p.top_k ? p.top_k[r] : 0;
+  const float share = p.top_p ? p.top_p[r] : 1.0f, least = p.min_p ? p.min_p[r] : 0.0f;
+  if (tid < 64) s.powers[tid] = exp2((double)tid / 64.0);
+  clear_few(s);
+  float mine = kNone;
+  if constexpr (!kParts)
+    mine = largest(row, held);
+  else if (tid < each)
+    mine = parts[r].tops[tid];
+  float top = top_of(s, mine);
   if (top == kNone || !(t > 0.0f)) {
     // the first that is the largest
     int at = p.vocab;
@@ -896,16 +1016,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
     return;
   }
   if (top == -kNone) row.infinite = true, top = 0.0f;
-  Scale scale;
-  scale.top = top;
-  scale.inner = 64.0 * 1.44269504088896340736 / (double)t;
-  const double coarse = scale.inner * (kFine / 64.0);
-  scale.coarse = coarse < 1e30 ? (float)coarse : 1e30f;
-
+  const Scale scale = scale_of(top, t);
   const bool by_count = k > 0 && k < p.vocab, by_share = share < 1.0f;
-  const double bar = least > 0.0f ? (least < 1.0f ? (double)least * kUnit : kUnit) : 0.0;
+  const double bar = bar_of(least);
   u64 cut = ~0ull;
   const Cut none = {kBins, 0, 0};
+  if constexpr (kParts) {
+    if (!by_share) {
+      for (int i = tid; i < kBins; i += kThreads) s.mass[i] = parts[r].runs[i];
+      pick(s, row, scale, p, r, Kept(cut, bar), 0);
+      return;
+    }
+  }
   // the last bin that a kept token can be in, as far as it is known without a
   // histogram: by the share of the largest weight (one bin more for a bin's
   // rounding), and by the k-th of the threads' largest logits
@@ -933,6 +1055,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
   enum Sums { kCounts, kTotal, kMasses };
   auto count_bins = [&](auto what) VQX_INLINE {
     constexpr Sums kWhat = decltype(what)::value;
+    if constexpr (kParts) {
+      u64 sum = 0;
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kThreads) {
+        s.count[i] = parts[r].count[i];
+        s.mass[i] = parts[r].mass[i], sum += s.mass[i];
+      }
+      mass = sum_of(s, sum);
+      __syncthreads();
+      return;
+    }
     clear_bins(s);
     double sum = 0.0;
     each_vector(row, [&](const float(&x)[8], int) VQX_INLINE {
@@ -969,7 +1102,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
       c = find_bin<false>(s, none, most, 0.0);
     } else {
       count_bins(with_total);
-      c = find_least(s, share_of(share, mass));
+      c = kParts ? find_bin<true, true>(s, none, 0, share_of(share, mass)) : find_least(s, share_of(share, mass));
     }
     const bool listable = c.bin < last ? c.count + s.count[c.bin] <= (u64)kMostListed : last < kBins;
     if (c.bin < last) last = c.bin;
@@ -1015,20 +1148,46 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p) {
       }
     }
   }
-  draw(s, row, scale, p, r, cut, bar);
+  draw(s, row, scale, p, r, Kept(cut, bar));
 }
 
 }  // namespace
 
-int sample(const Sampling& p, int dtype, hipStream_t st) {
+// Workgroups of a row of their own launches before the row's, 0 for none: where
+// rows are fewer than half the compute units, no number of tokens bounds what
+// is looked at and a part has 4096 logits or more.
+static int parts_of(const Sampling& p) {
+  if (p.top_k || p.rows == 0 || p.vocab > kMostRuns * 64 * 8) return 0;
+  int64_t each = num_cus() / p.rows;
+  if (each > p.vocab / 4096) each = p.vocab / 4096;
+  if (each > kMostParts) each = kMostParts;
+  return each < 2 ? 0 : (int)each;
+}
+
+int64_t sample_workspace(const Sampling& p) { return parts_of(p) ? p.rows * (int64_t)sizeof(Parts) : 0; }
+
+int sample(const Sampling& p, int dtype, void* ws, hipStream_t st) {
   if (p.rows == 0) return kOk;
-  const dim3 grid((unsigned)p.rows);
+  const int each = parts_of(p);
+  Parts* parts = static_cast<Parts*>(ws);
+  const dim3 grid((unsigned)p.rows), all((unsigned)(p.rows * each)), block(kThreads);
+#define VQX_SAMPLE(T)                                                                                \
+  do {                                                                                               \
+    if (each) {                                                                                      \
+      hipLaunchKernelGGL((sample_top_kernel<T>), all, block, 0, st, p, parts, each);                 \
+      hipLaunchKernelGGL((sample_sums_kernel<T>), all, block, 0, st, p, parts, each);                \
+      hipLaunchKernelGGL((sample_kernel<T, true>), grid, block, 0, st, p, parts, each);              \
+    } else {                                                                                         \
+      hipLaunchKernelGGL((sample_kernel<T, false>), grid, block, 0, st, p, parts, each);             \
+    }                                                                                                \
+  } while (0)
   if (dtype == kF32)
-    hipLaunchKernelGGL((sample_kernel<float>), grid, dim3(kThreads), 0, st, p);
+    VQX_SAMPLE(float);
   else if (dtype == kBF16)
-    hipLaunchKernelGGL((sample_kernel<Bf16>), grid, dim3(kThreads), 0, st, p);
+    VQX_SAMPLE(Bf16);
   else
-    hipLaunchKernelGGL((sample_kernel<F16>), grid, dim3(kThreads), 0, st, p);
+    VQX_SAMPLE(F16);
+#undef VQX_SAMPLE
   return check_launch("sample_tokens");
 }
 

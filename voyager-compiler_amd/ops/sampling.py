@@ -4,6 +4,8 @@
 step, and what ``kv4_accept`` compares drafted tokens with.
 """
 
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -24,6 +26,23 @@ def _of_rows(t, rows, dtype, name, what, device):
     if t.device != device:
         kv4._refuse(what, f"{name} is on {t.device}, the logits on {device}")
     return t.data_ptr()
+
+
+_WS = {}
+
+
+def _workspace_bytes(tag, rows, vocab, by_count, device):
+    """Workspace for these sizes on ``device``, cached per sizes."""
+    key = (tag, rows, vocab, by_count, device.index)
+    n = _WS.get(key)
+    if n is None:
+        if len(_WS) >= 4096:
+            _WS.clear()
+        got = ctypes.c_int64(0)
+        with torch.cuda.device(device):
+            _lib.call("vqx_sample_tokens_workspace_size", tag, rows, vocab, by_count, got)
+        n = _WS[key] = got.value
+    return n
 
 
 @torch.library.impl(quantized_ops_lib, "sample_tokens", "CUDA")
@@ -58,8 +77,10 @@ def sample_tokens(logits, random, temperature=None, top_k=None, top_p=None, min_
              _of_rows(min_p, rows, torch.float32, "min_p", what, device))
     tokens = random.new_empty(rows, dtype=torch.int64)
     chances = random.new_empty(rows)
+    need = _workspace_bytes(tag, rows, vocab, top_k is not None, device)
+    ws = random.new_empty(need, dtype=torch.uint8) if need else None  # held until the kernels that use it are enqueued
     kv4._launch("vqx_sample_tokens", logits, logits.data_ptr(), tag, rows, vocab, logits.stride(0), *given,
-                tokens.data_ptr(), chances.data_ptr())
+                tokens.data_ptr(), chances.data_ptr(), _lib.ptr(ws), need)
     return tokens, chances
 
 
