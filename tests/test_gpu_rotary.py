@@ -186,6 +186,28 @@ def test_rotary_graph(ops, vqx):
         same(out, ops.rotary(x, pos, freqs).cpu(), f"replay {i}")
 
 
+def test_rotary_backward_graph(ops, vqx):
+    """Forward and backward captured together follow x, positions and gradient."""
+    x = torch.randn(16, 4, 128, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.randn(16, 4, 128, device=DEV, dtype=torch.bfloat16)
+    pos, freqs = torch.arange(16, device=DEV, dtype=torch.int32), vqx.ops.rotary_frequencies(128, device=DEV)
+    call = lambda: torch.autograd.grad(ops.rotary(x, pos, freqs), x, y)[0]  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(4):
+        pos.fill_(i * 999)
+        y.copy_(torch.randn(16, 4, 128, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        same(got, call().cpu(), f"replay {i}")
+
+
 # ---------------------------------------------------------------------------
 # into the cache
 # ---------------------------------------------------------------------------

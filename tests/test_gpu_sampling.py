@@ -165,6 +165,34 @@ def test_parameters_out_of_range(ops):
           [-1.0, 0.0, 2.0, 0.0, -inf, 5.0])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_least_weights(ops, kind):
+    """Weights of a few units, rounded up to what min_p asks for, and half units."""
+    x = torch.full((8, 900), -math.inf).to(TYPES[kind])
+    x[:, 5] = 0.0
+    for i, z in enumerate((40.9, 40.6, 40.3, 39.7, 39.4, 39.2, 38.9, 41.2)):
+        x[i, 700] = -z * math.log(2.0)
+    for least in (0.6, 0.9, 1.0, 1.5, 2.0, 2.6, 0.3):
+        check(ops, x, [1.0] * 8, m=[least * 2.0 ** -40] * 8)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_logits_further_apart_than_their_type(ops, kind):
+    """The largest numbers of both signs, at temperatures that bring them together."""
+    x = torch.linspace(-3.3e38, 3.3e38, 700, dtype=torch.float64).repeat(6, 1).to(TYPES[kind])
+    u = [0.1, 0.5, 0.9, 0.02, 0.2, 0.999]
+    for k, p in ((None, None), ([690] * 6, None), ([1024] * 6, [0.999] * 6), (None, [0.9999] * 6), ([640, 3] * 3, [0.95] * 6)):
+        check(ops, x, u, t=[1e38, 2e38, 3e38, 5e37, 3e38, 1e37], k=k, p=p)
+
+
+def test_small_temperatures(ops):
+    """Down to the least number that fp32 has, and logits as near to each other."""
+    x = torch.arange(500.0).repeat(6, 1) * torch.tensor([1e-30, 1e-29, 3e-37, 1e-36, 1e-40, 3e-45])[:, None]
+    t = [2e-29, 1e-28, 2.0 ** -119, 2.0 ** -120, 2.0 ** -130, 1e-45]
+    for k, p in ((None, None), ([40] * 6, None), (None, [0.7] * 6), ([30] * 6, [0.8] * 6)):
+        check(ops, x, [0.3] * 6, t=t, k=k, p=p)
+
+
 def test_distribution(ops):
     """Even numbers give each token its share: of 4096 between its bounds, off by
     at most one on each side."""

@@ -26,7 +26,6 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048, kFine = 48, kHalvings = 42;
 constexpr int kMostListed = 4096;  // tokens that are sorted in LDS
 constexpr double kUnit = 0x1p40;
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNone = -__builtin_huge_valf();
 
 typedef unsigned long long u64;
@@ -153,7 +152,12 @@ struct Shared {
 struct Scale {
   float top;     // the row's largest logit
   double inner;  // 64 log2(e) / temperature
-  float coarse;  // log2(e) / temperature, in bins
+  // log2(e) / temperature, in bins, as three factors: halves of logits where the
+  // temperature is 1 and more, whose difference is no infinity, and two of the
+  // rest, which is past 32 bits for the smallest temperatures
+  float half, half_top, bins[2];
+  __device__ __forceinline__ float bin(float x) const { return __builtin_fmaf(-half, x, half_top) * bins[0] * bins[1]; }
+  __device__ __forceinline__ float span(int count) const { return (float)count / bins[0] / bins[1] / half; }  // of so many bins
 };
 
 // A whole number up to 2^40, as a double: sums of them are exact up to 2^53.
@@ -182,7 +186,7 @@ __device__ __forceinline__ u64 whole_weight(const Shared& s, const Scale& scale,
 // The bin of a logit, or kBins of one whose weight is 0; larger logits have no
 // larger bins.
 __device__ __forceinline__ int bin_of(const Scale& s, float x) {
-  const float y = (s.top - x) * s.coarse;
+  const float y = s.bin(x);
   return y < (float)(kHalvings * kFine) ? (int)y : kBins;
 }
 
@@ -308,7 +312,7 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
 }
 
-// A row's first vectors, held in registers: 64 of each thread, so that a row of
+// A row's first vectors, held in 64 registers of each thread, so that a row of
 // 131072 two-byte logits is read once (256 such rows read a second time, from
 // beyond the L2s, take 13 us).
 template <typename T>
@@ -511,7 +515,7 @@ __device__ __forceinline__ void list_tokens(Shared& s, const Row<T>& row, const 
   // lower half behind it: that moves them by less than their last place, 2^-7 of
   // them (an infinity would become a NaN; rows with one have their own way).  The
   // border is lower by that and by the roundings here.
-  const float span = (float)(last + 1) / scale.coarse;
+  const float span = scale.span(last + 1);
   float least = scale.top - span;
   least -= __builtin_fabsf(least) * 0x1p-6f + (__builtin_fabsf(scale.top) + span) * 0x1p-20f + 0x1p-100f;
   if (!(least > -3.4028235e38f)) least = -3.4028235e38f;  // every finite one
@@ -634,7 +638,7 @@ __device__ __forceinline__ Few few(Shared& s, const Row<T>& row, const H& held, 
   for (int j = 0; j < kEach; ++j) {
     w[j] = 0, bin[j] = kBins;
     if (j * kThreads >= listed) continue;
-    const float y = (scale.top - x[j]) * scale.coarse;
+    const float y = scale.bin(x[j]);
     keeps[j] = keeps[j] && y < (float)(last + 1);
     if (!keeps[j]) continue;
     w[j] = whole_weight(s, scale, x[j]);
@@ -893,8 +897,11 @@ __device__ __forceinline__ Scale scale_of(float top, float t) {
   Scale scale;
   scale.top = top;
   scale.inner = 64.0 * 1.44269504088896340736 / (double)t;
-  const double coarse = scale.inner * (kFine / 64.0);
-  scale.coarse = coarse < 1e30 ? (float)coarse : 1e30f;
+  scale.half = t < 1.0f ? 1.0f : 0.5f;
+  scale.half_top = scale.half * top;
+  const double bins = scale.inner * (kFine / 64.0) / (double)scale.half;
+  scale.bins[0] = (float)(bins > 0x1p100 ? 0x1p100 : bins);
+  scale.bins[1] = bins > 0x1p100 ? (float)(bins * 0x1p-100) : 1.0f;
   return scale;
 }
 // The least weight that is kept.
@@ -1029,11 +1036,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Sampling p, const Part
     }
   }
   // the last bin that a kept token can be in, as far as it is known without a
-  // histogram: by the share of the largest weight (one bin more for a bin's
-  // rounding), and by the k-th of the threads' largest logits
+  // histogram: by the share of the largest weight (half a unit less, which is
+  // rounded up to it, and one bin more for a bin's rounding), and by the k-th of
+  // the threads' largest logits
   int last = kBins;
   if (bar > 0.0 && !(by_share && by_count)) {
-    const float y = -__builtin_amdgcn_logf(least) * kFine + 1.0f;
+    const float y = -__builtin_amdgcn_logf(least - 0x1p-41f) * kFine + 1.0f;  // NaN: none
     if (y < (float)kBins) last = y > 0.0f ? (int)y : 0;
   }
   const int tight = last;
