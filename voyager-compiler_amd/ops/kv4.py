@@ -28,6 +28,12 @@ lengths are not looked at, work is shared out as if each sequence filled its
 room (the table's pages): a table many times as wide as the sequences costs up
 to four times the time.
 
+Around that step: ``kv4_reserve`` makes ``table``, ``cu``, positions and slots from
+how many tokens each sequence gets; ``kv4_append_rotary`` turns queries and keys
+on the way in.  With drafted tokens, ``kv4_tree_attention`` in the place of
+``kv4_attention``, ``sample_tokens`` (``sampling.py``) after it, and ``kv4_accept``,
+which keeps the drafted tokens that were drawn and cuts the lengths by the others.
+
 A place is a slot of the cache.  ``kv4_evict`` moves the kept tokens to the
 front, for each kv head others, so that in a cache that it has filled distances
 are of slots: ``window`` and ``slopes`` no longer count the tokens that were
