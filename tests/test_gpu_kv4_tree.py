@@ -142,6 +142,39 @@ def test_tree_many_rows(ops, kind, dim, how, page):
     check(ops, kind, *s[:4], forest(news, 2)[0], s[4], 64, s[5], **how)
 
 
+@pytest.mark.parametrize("kind,dim", [("bf16", 128), ("f16", 64), ("f32", 128), ("bf16", 256), ("f32", 64), ("f16", 256)])
+@pytest.mark.parametrize("how", [{}, dict(softcap=15.0, window=33, slopes=True)])
+@pytest.mark.parametrize("page", [0, 24])
+def test_tree_full_tiles(ops, kind, dim, how, page):
+    """Almost all of the workgroups' rows are there: those of many rows."""
+    lengths, news = [100, 64, 200, 90, 65, 150, 71, 480], [64, 64, 60, 64, 57, 64, 64, 64]
+    s = scene(kind, dim, 16, 8, lengths, news, page)
+    if how.get("slopes"):
+        how = dict(how, slopes=torch.linspace(0.01, 0.5, 128))
+    check(ops, kind, *s[:4], forest(news, 2)[0], s[4], 64, s[5], **how)
+
+
+@pytest.mark.parametrize("how", [{}, dict(slopes=True)])
+def test_tree_full_tiles_in_parts(ops, how):
+    """The same over a long sequence, in parts that are joined."""
+    s = scene("bf16", 64, 4, 8, [25100], [64], 128)
+    if how.get("slopes"):
+        how = dict(slopes=torch.linspace(0.0001, 0.005, 32))
+    check(ops, "bf16", *s[:4], forest([64], 5)[0], s[4], 64, s[5], **how)
+
+
+@pytest.mark.parametrize("seqs", [63, 64, 65])
+def test_tree_of_sequences_by_length(ops, seqs):
+    """Workgroups in the order of lengths, some of them equal or 0, up to 64
+    sequences."""
+    news = [1 + (5 * b) % 7 for b in range(seqs)]
+    lengths = [max((37 * b) % 90 // 4 * 4, news[b]) for b in range(seqs)]
+    s = scene("bf16", 64, 4, 4, lengths, news, 16)
+    given = s[3].clone()
+    given[::9] = 0  # nothing of these is there
+    check(ops, "bf16", *s[:3], given, forest(news, 1)[0], s[4], max(news), s[5])
+
+
 @pytest.mark.parametrize("kv,group,news", [(2, 4, [12, 1, 40]), (16, 8, [64, 64, 60])])
 @pytest.mark.parametrize("how", [dict(softcap=20.0), dict(slopes=True)])
 def test_a_chain_is_a_prompt(ops, kv, group, news, how):

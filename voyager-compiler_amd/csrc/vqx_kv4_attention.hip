@@ -133,6 +133,7 @@ struct QueryTerms {
 struct Kv4Plan {
   int32_t rows, tiles, chunk, splits;
   int32_t listed;  // tiles of a kv head that the workgroups are handed one by one; 0: tiles of every sequence
+  bool ranked;     // sequences in the order of their lengths
 };
 
 // Where the rows of one tile stand.
@@ -208,13 +209,32 @@ struct Place {
   int64_t at;  // of its sums in the workspace
 };
 
+// The i-th longest of up to 64 sequences, for all lanes.
+__device__ __forceinline__ uint32_t longest(const Kv4View& c, uint32_t i) {
+  const int lane = threadIdx.x & 63, there = lane < (int)c.seqs, length = there ? kv4_length(c, lane) : 0;
+  // no two the same: the lane below the length
+  const uint32_t mine = there ? (uint32_t)(length < 1 << 25 ? length : (1 << 25) - 1) << 6 | (uint32_t)(63 - lane) : 0;
+  uint32_t rank = 0;
+  for (int b = 0; b < (int)c.seqs; ++b) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, b) > mine;
+  return (uint32_t)__builtin_ctzll(__ballot(there && rank == i));
+}
+
 // Heads first, so that with 8 of them each XCD's L2 has the cache of one (of
 // other numbers each XCD gets all in turn, or a long sequence would be one
 // XCD's: 4 ragged prompts of 300, 4 heads: 35 and 32 us); then the splits, then
 // the tiles from the last, which sees the most.  (Splits and tiles first put
 // the first tile of every sequence, often the only one, on one XCD: 64 sequences
 // with 128 new tokens at most, all but one with one: 242 and 50 us.)
+template <bool kTree = false>
 __device__ __forceinline__ bool place_of(const Kv4View& c, const Kv4Query& q, const Kv4Plan& plan, Place& p) {
+  if (kTree && plan.ranked) {
+    const uint32_t each = c.kv * (uint32_t)(plan.tiles * plan.splits), in = blockIdx.x % each, rest = in / c.kv;
+    p.b = longest(c, blockIdx.x / each);
+    p.h = (in + (c.kv % 8 ? rest : 0u)) % c.kv, p.split = rest % (uint32_t)plan.splits;
+    p.tile = plan.tiles - 1 - (int)(rest / (uint32_t)plan.splits);
+    p.at = (((int64_t)p.b * c.kv + p.h) * plan.tiles + p.tile) * plan.splits + p.split;
+    return true;
+  }
   const uint32_t heads = plan.listed ? c.kv : c.seqs * c.kv, rest = blockIdx.x / heads;
   const uint32_t slot = (blockIdx.x + (c.kv % 8 ? rest : 0u)) % heads;
   p.split = rest % (uint32_t)plan.splits;
@@ -225,7 +245,7 @@ __device__ __forceinline__ bool place_of(const Kv4View& c, const Kv4Query& q, co
     return listed_tile(c, q, plan, (uint32_t)t, p.b, p.tile);
   }
   p.b = slot / c.kv, p.h = slot % c.kv, p.tile = t;
-  p.at = ((int64_t)slot * plan.tiles + t) * plan.splits + p.split;
+  p.at = (((int64_t)p.b * c.kv + p.h) * plan.tiles + t) * plan.splits + p.split;
   return true;
 }
 
@@ -587,7 +607,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : (D == 128 ? 2 : 1)) void kv4_row
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Place place;
-  if (!place_of(c, q, plan, place)) return;
+  if (!place_of<kMode == kTreed>(c, q, plan, place)) return;
   const uint32_t b = place.b, h = place.h, split = place.split;
   const int tile = place.tile;
   const TileRows rows = tile_rows<kMode == kTreed>(c, q, b, tile, kRows, kStep);
@@ -864,7 +884,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv4_block_kernel(Kv4Vie
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Place place;
-  if (!place_of(c, q, plan, place)) return;
+  if (!place_of<kMode == kTreed>(c, q, plan, place)) return;
   const uint32_t b = place.b, h = place.h, split = place.split;
   const int tile = place.tile;
   constexpr bool kTree = kMode == kTreed;
@@ -1539,7 +1559,22 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   const int64_t blocks = c.kv * tiles_of(many), room = span_of(tokens_of(many));
   const bool full = (int64_t)q.tokens.n * q.group >= c.seqs * (all < 128 ? all : 128);
   const bool whole = room <= 8 * kBlockStep ? blocks >= num_cus() : room <= kShortSpan && blocks > num_cus();
-  p.rows = all > kRows && full && (whole || steps >= (many == 64 ? 2 : 1) * kManyTiles) ? many : kRows;
+  bool block = all > kRows && full && (whole || steps >= (many == 64 ? 2 : 1) * kManyTiles);
+  // Drafted tokens are at most 64 of a sequence, whose last tile is often its only
+  // one, and a tile of 128 rows costs what 7 or 8 of 16 do however few it has (heads
+  // of 128, bf16, 8 kv heads, second kernel and first: 16 sequences of 8000 with 32
+  // rows 105 and 56 us, of 4000 with 96 rows 81 and 66, 8 of 6000 with 192 110 and 95;
+  // 20 of 5000, 16 kv heads with 40 rows 262 and 105): the second for those that fill
+  // seven eighths of its tiles (12 of 5000 with 128 rows 85 and 81; 3 of 30000, 5 kv
+  // heads with 120 rows 71 and 86, 32 of 3000 with 256 190 and 251, fp16 234 and 322).
+  // Short ones aside not where it has 64 rows (fp32: 12 of 5000 with 128 rows 141 and
+  // 113, 16 of 20000 with 256 963 and 989) nor with heads of 256 (16 of 9000 with 256
+  // rows 869 and 799, fp16 1085 and 947).
+  if (q.tree) {
+    const bool filled = 8ll * q.tokens.n * q.group >= 7 * tiles_of(many) * many;
+    block = filled && (whole || (many == 128 && dim <= 128 && steps >= kManyTiles));
+  }
+  p.rows = block ? many : kRows;
   p.tiles = (int32_t)((all + p.rows - 1) / p.rows);
   const int64_t there = tiles_of(p.rows);
   // where most tiles would have no rows (32 sequences of up to 4000 tokens, one
@@ -1562,6 +1597,11 @@ Kv4Plan kv4_plan(const Kv4View& c, int dim, const Kv4Query& q, int dtype) {
   p.chunk = (int32_t)chunk;
   p.splits = (int32_t)((span + chunk - 1) / chunk);
   if (p.splits < 1) p.splits = 1;
+  // Where not every compute unit has just one workgroup, those of the longest
+  // sequences begin first, all tiles of one together: trees of 16 sequences of up to
+  // 4000, 24 new tokens, 60 us as sequences come and 49, 32 with 8 new tokens of up to
+  // 2000 27 and 23; where all are as long it costs up to 3% (heads of 256 152 and 157).
+  p.ranked = q.tree && !p.listed && c.seqs > 1 && c.seqs <= 64 && heads * p.splits > num_cus();
   return p;
 }
 
