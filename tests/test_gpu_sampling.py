@@ -133,6 +133,27 @@ def test_long_cuts(ops, kind, k):
     check(ops, x, u, [0.5, 1.0, 2.0], None, [0.9, 0.5, 0.999])
 
 
+@pytest.mark.parametrize("vocab", [4000, 4096, 4097, 8001])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_long_cuts_of_short_rows(ops, vocab, kind):
+    """The same where workgroups are smaller: close, equal and ordinary logits."""
+    close, u = rows(3, vocab, kind, 9, spread=0.001)
+    flat = torch.zeros(3, vocab)
+    flat[1, ::2], flat[2, vocab // 4:] = -0.0, 1.0
+    k = [vocab // 3, vocab // 2, vocab - 5]
+    for x in (close, flat.to(TYPES[kind]), rows(3, vocab, kind, 2)[0]):
+        check(ops, x, u, None, k)
+        check(ops, x, u, None, k, [0.9, 0.5, 0.999])
+        check(ops, x, u, [0.5, 1.0, 2.0], None, [0.9, 0.5, 0.999], [0.0, 0.01, 0.2])
+
+
+def test_more_rows_than_compute_units(ops):
+    """Two workgroups of a compute unit; rows that differ in all they ask for."""
+    x, u = rows(520, 8300, "bf16", 5)
+    pick = lambda *a: [a[i % len(a)] for i in range(520)]  # noqa: E731
+    check(ops, x, u, pick(1.0, 0.7, 0.0, 1.3, 0.9), pick(0, 40, 700, 3000, 1, 8000), pick(1.0, 0.9, 0.99, 0.5), pick(0.0, 0.02, 0.0))
+
+
 def test_random_numbers_at_the_ends(ops):
     x, _ = rows(7, 999, "f32", 4)
     check(ops, x, [0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, math.nan, 1e-30])
