@@ -186,6 +186,15 @@ def test_rotary_graph(ops, vqx):
         same(out, ops.rotary(x, pos, freqs).cpu(), f"replay {i}")
 
 
+def test_rotary_gradient_of_the_gradient(ops, vqx):
+    """The turn is linear: the gradient's own gradient is the turn again."""
+    x, g, v = (torch.randn(9, 3, 64, device=DEV, requires_grad=True) for _ in range(3))
+    pos, freqs = torch.arange(9, device=DEV, dtype=torch.int32) * 77, vqx.ops.rotary_frequencies(48, device=DEV)
+    back, = torch.autograd.grad(ops.rotary(x, pos, freqs, factor=1.5), x, g, create_graph=True)
+    again, = torch.autograd.grad(back, g, v)
+    same(again, ops.rotary(v, pos, freqs, factor=1.5).detach().cpu(), "gradient of the gradient")
+
+
 def test_rotary_backward_graph(ops, vqx):
     """Forward and backward captured together follow x, positions and gradient."""
     x = torch.randn(16, 4, 128, device=DEV, dtype=torch.bfloat16, requires_grad=True)

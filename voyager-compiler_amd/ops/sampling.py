@@ -1,7 +1,8 @@
 """Tokens drawn from logits.
 
 ``torch.ops.quantized_ops.sample_tokens``, this package's own: the end of a decode
-step, and what ``kv4_accept`` compares drafted tokens with.
+step, and what ``kv4_accept`` compares drafted tokens with.  No gradient passes
+through it.
 """
 
 import ctypes
