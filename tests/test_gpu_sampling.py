@@ -154,6 +154,23 @@ def test_more_rows_than_compute_units(ops):
     check(ops, x, u, pick(1.0, 0.7, 0.0, 1.3, 0.9), pick(0, 40, 700, 3000, 1, 8000), pick(1.0, 0.9, 0.99, 0.5), pick(0.0, 0.02, 0.0))
 
 
+@pytest.mark.parametrize("vocab", [3000, 20000, 600000])
+def test_rows_by_themselves(ops, vocab):
+    """A row's token does not depend on how many rows are with it, nor then on
+    how its work is shared out."""
+    g = torch.Generator(DEV).manual_seed(vocab)
+    n = 300
+    x = (3 * torch.randn(n, vocab, device=DEV, generator=g)).bfloat16()
+    f = lambda lo, hi: lo + (hi - lo) * torch.rand(n, device=DEV, generator=g)  # noqa: E731
+    u, t, p, m = f(0, 1), f(0.5, 1.5), f(0.5, 1.05), f(-0.01, 0.03)
+    k = torch.randint(-2000, 9000, (n,), device=DEV, generator=g).int().clamp(min=0)
+    for args in ((t,), (t, k), (t, None, p), (t, k, p, m), (t, None, None, m)):
+        want = ops.sample_tokens(x, u, *args)
+        for first, end in ((0, 1), (5, 45), (100, 230)):
+            got = ops.sample_tokens(x[first:end], u[first:end], *(None if a is None else a[first:end] for a in args))
+            assert torch.equal(got[0], want[0][first:end]) and torch.equal(got[1], want[1][first:end]), (len(args), first)
+
+
 def test_random_numbers_at_the_ends(ops):
     x, _ = rows(7, 999, "f32", 4)
     check(ops, x, [0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, math.nan, 1e-30])
