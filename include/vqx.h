@@ -754,9 +754,10 @@ int vqx_kv4_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, vo
  * base = length - count tokens before them, which every row sees (as far as the
  * window has it).  For windows and slopes a row's place is base + the number of
  * its mask's bits - 1, and new token j is as many places before it as the mask
- * has bits above j.  Bits of tokens that the sequence does not have do not
- * count.  No sequence has more than 64 new tokens (most says so where n is more).
- * Masks of 1 .. 1 up to the token's own bit are the rows of vqx_kv4_attention.
+ * has bits above j.  Bits of tokens that the sequence does not have, or that are
+ * beyond the query's most, do not count.  No sequence has more than 64 new tokens
+ * (most says so where n is more).  Masks of 1 .. 1 up to the token's own bit are
+ * the rows of vqx_kv4_attention.
  */
 int vqx_kv4_tree_attention_workspace_size(const vqx_kv4_cache* cache, const vqx_kv4_query* query, int64_t* bytes);
 int vqx_kv4_tree_attention(const vqx_kv4_cache* cache, const vqx_kv4_query* query, const int64_t* tree, void* out,

@@ -30,7 +30,7 @@ struct Kv4Tokens {
   int32_t n, each;
 };
 
-__device__ __forceinline__ void kv4_span(const Kv4Tokens& q, uint32_t b, int& first, int& count) {
+__host__ __device__ __forceinline__ void kv4_span(const Kv4Tokens& q, uint32_t b, int& first, int& count) {
   if (q.cu) {
     // a table of offsets is the caller's data: no access follows it out of [0, n]
     const int lo = q.cu[b], hi = q.cu[b + 1];

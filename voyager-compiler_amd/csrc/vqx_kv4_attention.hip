@@ -146,8 +146,8 @@ struct TileRows {
 };
 
 template <bool kTree = false>
-__device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile, int tile_size,
-                                              int step) {
+__host__ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& q, uint32_t b, int tile,
+                                                       int tile_size, int step) {
   TileRows r;
   kv4_span(q.tokens, b, r.first, r.count);
   // room, new tokens and windows are below 2^30 (checked by the host), a length
@@ -162,15 +162,22 @@ __device__ __forceinline__ TileRows tile_rows(const Kv4View& c, const Kv4Query& 
   r.pos_max = r1 > r0 ? r.base + (r1 - 1) / q.group : -1;
   if constexpr (kTree) {
     // a row is at a place from base - 1 (of no ancestors, itself not among them)
-    // to base + count - 1, and may see any of the new tokens
+    // to base + n - 1, and may see any of the n new tokens that the call was told of
     r.pos_min = r.base - 1;
-    if (r1 > r0) r.pos_max = r.base + r.count - 1;
+    if (r1 > r0) r.pos_max = r.base + n - 1;
   }
   r.hi = r.pos_max + 1 < 0 ? 0 : ((uint32_t)(r.pos_max + 1) > c.cap ? (int)c.cap : r.pos_max + 1);
   r.lo = 0;
   if (q.window && r.pos_min >= q.window) r.lo = (r.pos_min - q.window + 1) & ~(step - 1);
   if (r.lo > r.hi) r.lo = r.hi & ~(step - 1);
   return r;
+}
+
+// The splits of a tile that have sums: as many as the workspace has room for, or
+// fewer.
+__host__ __device__ __forceinline__ int joined_splits(const TileRows& rows, const Kv4Plan& plan) {
+  const int n = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
+  return n < plan.splits ? n : plan.splits;
 }
 
 // Sequences and tiles counted through: where tile t of all that there are lies.
@@ -329,7 +336,9 @@ __device__ __forceinline__ Line line_of(const Kv4Query& q, const TileRows& rows,
   Line l;
   l.live = live;
   l.base = rows.base;
-  const uint64_t all = rows.count < 64 ? (1ull << rows.count) - 1 : ~0ull;
+  // bits of tokens beyond `most` lie outside the range that the plan is made for
+  const int n = rows.count < q.most ? rows.count : q.most;
+  const uint64_t all = n < 64 ? (1ull << n) - 1 : ~0ull;
   l.mask = live ? (uint64_t)q.tree[rows.first + token] & all : 0;
   l.pos = rows.base + __popcll(l.mask) - 1;
   return l;
@@ -1288,7 +1297,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4View c, Kv4Query q, Kv
   const int step = plan.rows == kRows ? kStep : kBlockStep;
   const TileRows rows = q.tree ? tile_rows<true>(c, q, b, tile, plan.rows, step) : tile_rows(c, q, b, tile, plan.rows, step);
   if (r >= rows.rows) return;
-  const int splits = rows.hi > rows.lo ? (rows.hi - rows.lo + plan.chunk - 1) / plan.chunk : 1;
+  const int splits = joined_splits(rows, plan);
   const int64_t size = (int64_t)plan.rows * (D + 2);
   const float* o_n = ws + (int64_t)slot * plan.splits * size + (int64_t)n * D;
   const float* m_n = ws + (int64_t)slot * plan.splits * size + (int64_t)plan.rows * D + n;

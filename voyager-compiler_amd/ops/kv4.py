@@ -358,7 +358,7 @@ def kv4_tree_attention(query, codes, scales, lengths, tree, cu=None, most=None, 
     itself.  All see the cached tokens before the new ones.  For ``window`` and
     ``slopes`` a token stands as far behind those as it has ancestors, and an
     ancestor as far before it as there are others between.  Bits of tokens that
-    the sequence does not have do not count."""
+    the sequence does not have, or beyond ``most``, do not count."""
     what = "kv4_tree_attention"
     _lib.require_device(codes, what)
     c = _cache(codes, scales, lengths, table, what)
