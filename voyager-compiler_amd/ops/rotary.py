@@ -45,11 +45,25 @@ def _(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     return x.new_empty(x.shape)
 
 
+_keys = torch._C._dispatch_keys
+_PLAIN = torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
+for _k in ("ADInplaceOrView", "AutogradCUDA", "AutocastCUDA"):
+    _PLAIN = _PLAIN | torch._C.DispatchKeySet(getattr(torch._C.DispatchKey, _k))
+
+
+def _plain(x, positions, freqs):
+    """Whether all that the dispatcher would do below autograd is to call the kernel:
+    there is no mode, and no tensor is of a kind that has a say before its data is
+    read, as a transform's, a tracer's or a negative view (a second way through the
+    dispatcher is 3 us of a call's 11, and 10 in a backward pass, whose thread has
+    just been woken)."""
+    return (_keys(x) == _PLAIN and _keys(freqs) == _PLAIN and _keys(positions) == _PLAIN
+            and not torch._C._len_torch_dispatch_stack())
+
+
 def _below(x, positions, freqs, interleaved, factor, back):
-    """The turn below autograd: at once where no mode or kind of tensor is to see
-    it (a second way through the dispatcher is 3 us of a call's 11, and 10 in a
-    backward pass, whose thread has just been woken)."""
-    if (type(x) is torch.Tensor or type(x) is torch.nn.Parameter) and x.is_cuda and not torch._C._len_torch_dispatch_stack():
+    """The turn below autograd."""
+    if _plain(x, positions, freqs):
         return rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
     with torch._C._AutoDispatchBelowAutograd():
         return torch.ops.quantized_ops.rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
@@ -68,8 +82,9 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, grad):
         positions, freqs = ctx.saved_tensors
         interleaved, factor, back = ctx.how
-        return _rotary_autograd(grad, positions, freqs, interleaved=interleaved, factor=factor,
-                                back=not back), None, None, None, None, None
+        at_once = not torch.is_grad_enabled() and _plain(grad, positions, freqs)
+        turn = rotary if at_once else torch.ops.quantized_ops.rotary
+        return turn(grad, positions, freqs, interleaved=interleaved, factor=factor, back=not back), None, None, None, None, None
 
 
 @torch.library.impl(quantized_ops_lib, "rotary", "Autograd")
