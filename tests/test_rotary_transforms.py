@@ -1,9 +1,11 @@
-"""``rotary`` under torch's transforms: batched gradients, vmap, tracing, views that
-are negative.  The turn is linear, so that each of these is the turn, or the turn
-back, of something.  On the CPU a plain turn stands in for the kernel."""
+"""``rotary`` under torch's transforms: batched gradients, vmap, grad and jvp of
+torch.func, forward mode, tracing, views that are negative.  The turn is linear, so
+that each of these is the turn, or the turn back, of something.  On the CPU a plain
+turn stands in for the kernel."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 
 def plain_turn(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
@@ -59,9 +61,10 @@ def test_batched_gradients_of_the_gradient(device, turn):
     assert torch.equal(got, each(turn[0], vs))
 
 
-def test_jacobian(device, turn):
+@pytest.mark.parametrize("strategy", ["reverse-mode", "forward-mode"])
+def test_jacobian(device, turn, strategy):
     x = heads(device)
-    got = torch.autograd.functional.jacobian(turn[0], x, vectorize=True)
+    got = torch.autograd.functional.jacobian(turn[0], x, vectorize=True, strategy=strategy)
     units = torch.eye(x.numel(), device=device).reshape(-1, *x.shape)
     assert torch.equal(got.flatten(3).movedim(-1, 0), each(turn[0], units))
 
@@ -78,6 +81,90 @@ def test_vmap_of_positions(device, turn):
     leaf = x.clone().requires_grad_()
     got = torch.func.vmap(lambda p: op(leaf, p, turn[3]))(many)
     assert torch.equal(got, each(lambda p: op(x, p, turn[3]), many))
+
+
+def test_func_grad(device, turn):
+    x, y = heads(device), heads(device, seed=1)
+    assert torch.equal(torch.func.grad(lambda v: (turn[0](v) * y).sum())(x), turn[1](y))
+    out, pull = torch.func.vjp(turn[0], x)
+    assert torch.equal(out, turn[0](x)) and torch.equal(pull(y)[0], turn[1](y))
+
+
+def test_func_grad_of_a_batch(device, turn):
+    xs, ys = heads(device, 3), heads(device, 3, seed=1)
+    got = torch.func.vmap(torch.func.grad(lambda v, y: (turn[0](v) * y).sum()))(xs, ys)
+    assert torch.equal(got, each(turn[1], ys))
+
+
+def test_func_grad_of_the_gradient(device, turn):
+    """Of a square's sum: twice the turn of a turn back, which is factor^2."""
+    x, v = heads(device), heads(device, seed=1)
+    first = torch.func.grad(lambda u: (turn[0](u) ** 2).sum())
+    got = torch.func.grad(lambda u: (first(u) * v).sum())(x)
+    assert torch.equal(got, turn[1](2 * turn[0](v)))
+
+
+def test_jvp(device, turn):
+    x, t = heads(device), heads(device, seed=1)
+    out, tangent = torch.func.jvp(turn[0], (x,), (t,))
+    assert torch.equal(out, turn[0](x)) and torch.equal(tangent, turn[0](t))
+    got = torch.func.jacfwd(turn[0])(x)
+    assert torch.equal(got, torch.func.jacrev(turn[0])(x).to(got.dtype))
+
+
+def test_jvp_of_the_gradient(device, turn):
+    """Forward over reverse: of half a square's sum, along t."""
+    x, t = heads(device), heads(device, seed=1)
+    _, got = torch.func.jvp(torch.func.grad(lambda u: 0.5 * (turn[0](u) ** 2).sum()), (x,), (t,))
+    assert torch.equal(got, turn[1](turn[0](t)))
+
+
+def test_forward_mode(device, turn):
+    x, t = heads(device), heads(device, seed=1)
+    for leaf in (x, x.clone().requires_grad_()):
+        with fwd.dual_level():
+            out, tangent = fwd.unpack_dual(turn[0](fwd.make_dual(leaf, t)))
+            assert torch.equal(out, turn[0](x)) and torch.equal(tangent, turn[0](t))
+            assert fwd.unpack_dual(turn[0](leaf)).tangent is None
+        assert out.requires_grad == leaf.requires_grad
+
+
+def test_a_leaf_beside_the_transform(device, turn):
+    """What a transform does not see keeps its own gradient."""
+    leaf, v, y = heads(device).requires_grad_(), heads(device, seed=1), heads(device, seed=2)
+    got = torch.func.grad(lambda u: (turn[0](leaf) * u).sum())(v)
+    assert torch.equal(got, turn[0](leaf.detach()))
+    assert torch.equal(torch.autograd.grad(got, leaf, y)[0], turn[1](y))
+
+
+def test_hessian(device, turn):
+    """Of half a square's sum: the turn's product with its transpose."""
+    x = heads(device)[:1]
+    op, pos, freqs = torch.ops.quantized_ops.rotary, turn[2][2:3], turn[3]
+    f = lambda u: 0.5 * (op(u, pos, freqs, factor=2.0) ** 2).sum()  # noqa: E731
+    want = torch.ones(2, 16, device=device)
+    want[:, :12] = 4.0  # factor^2 where heads are turned
+    # two turns, each rounded once, and the pair's sum: of terms up to 4
+    for got in (torch.func.hessian(f)(x), torch.func.jacrev(torch.func.jacrev(f))(x)):
+        assert float((got.reshape(32, 32) - torch.diag(want.flatten())).abs().max()) <= 4 * 2.0 ** -23
+
+
+def test_tangents_and_gradients_together(device, turn):
+    """Forward over reverse and reverse over forward, without torch.func."""
+    x, t, y = heads(device).requires_grad_(), heads(device, seed=1), heads(device, seed=2)
+    with fwd.dual_level():
+        out, tangent = fwd.unpack_dual(turn[0](fwd.make_dual(x, t) ** 2))
+        got, = torch.autograd.grad(tangent, x, y)  # of the turn of 2 x t
+        assert torch.equal(got, turn[1](y) * 2 * t) or torch.equal(got, turn[1](y) * (2 * t))
+        dual = fwd.make_dual(x, t)
+        first, = torch.autograd.grad(turn[0](dual).square().sum(), dual, create_graph=True)
+        assert torch.equal(fwd.unpack_dual(first).tangent, turn[1](2 * turn[0](t)))
+
+
+def test_tangents_of_frequencies_are_refused(device, turn):
+    x = heads(device)
+    with fwd.dual_level(), pytest.raises(ValueError, match="freqs have no gradient"):
+        torch.ops.quantized_ops.rotary(x, turn[2], fwd.make_dual(turn[3], turn[3]))
 
 
 @pytest.mark.parametrize("grad", [False, True])

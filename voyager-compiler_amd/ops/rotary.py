@@ -9,6 +9,9 @@ the cache; this one stands alone, and gradients pass through it.
 import math
 
 import torch
+from torch._functorch.autograd_function import enable_single_level_autograd_function
+from torch.autograd import forward_ad
+from torch.autograd.function import _SingleLevelFunction
 
 from .. import _lib
 from . import kv4
@@ -26,7 +29,8 @@ def rotary(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     (interleaved) (x[2 i], x[2 i + 1]), by the angle positions[token] * freqs[i]
     and times factor; back: by the negative angle.  positions: int32 [n]; freqs:
     fp32.  Angles and products are in 64 bits, rounded once to x's dtype.  The
-    gradient of x is the turn back; positions and freqs have none."""
+    gradient of x is the turn back, a tangent's the turn; positions and freqs have
+    none.  torch.func's transforms take it too (vmap one element at a time)."""
     what = "rotary"
     _lib.require_device(x, what)
     device = x.device
@@ -62,21 +66,27 @@ def _plain(x, positions, freqs):
 
 
 def _below(x, positions, freqs, interleaved, factor, back):
-    """The turn below autograd."""
-    if _plain(x, positions, freqs):
-        return rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
+    """The turn below autograd, by the dispatcher."""
     with torch._C._AutoDispatchBelowAutograd():
         return torch.ops.quantized_ops.rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
 
 
-class _Rotary(torch.autograd.Function):
-    """The turn with the turn back, its transpose, as gradient."""
+class _Rotary(_SingleLevelFunction):
+    """The turn with the turn back, its transpose, as gradient, and a tangent's turn
+    as tangent.  Like any of autograd's kernels it is for one level of it: torch.func's
+    transforms come here level by level.  modes: None where the kernel may be called
+    at once, or whether gradients and tangents are wanted, which those below are to
+    know."""
 
     @staticmethod
-    def forward(ctx, x, positions, freqs, interleaved, factor, back):
+    def forward(ctx, x, positions, freqs, interleaved, factor, back, modes):
         ctx.save_for_backward(positions, freqs)
         ctx.how = interleaved, factor, back
-        return _below(x, positions, freqs, interleaved, factor, back)
+        if modes is None:
+            return rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
+        ctx.save_for_forward(positions, freqs)
+        with torch.set_grad_enabled(modes[0]), forward_ad._set_fwd_grad_enabled(modes[1]):
+            return _below(x, positions, freqs, interleaved, factor, back)
 
     @staticmethod
     def backward(ctx, grad):
@@ -84,15 +94,30 @@ class _Rotary(torch.autograd.Function):
         interleaved, factor, back = ctx.how
         at_once = not torch.is_grad_enabled() and _plain(grad, positions, freqs)
         turn = rotary if at_once else torch.ops.quantized_ops.rotary
-        return turn(grad, positions, freqs, interleaved=interleaved, factor=factor, back=not back), None, None, None, None, None
+        return turn(grad, positions, freqs, interleaved=interleaved, factor=factor, back=not back), *[None] * 6
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        positions, freqs = ctx.saved_tensors
+        interleaved, factor, back = ctx.how
+        return torch.ops.quantized_ops.rotary(tangent, positions, freqs, interleaved=interleaved, factor=factor, back=back)
 
 
 @torch.library.impl(quantized_ops_lib, "rotary", "Autograd")
 def _rotary_autograd(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
     if freqs.requires_grad:
         kv4._refuse("rotary", "freqs have no gradient here")
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, positions, freqs, interleaved, factor, back)
+    tangents = forward_ad._current_level >= 0
+    if tangents and forward_ad.unpack_dual(freqs).tangent is not None:
+        kv4._refuse("rotary", "freqs have no gradient here")
+    grads = torch.is_grad_enabled()
+    if not tangents and _plain(x, positions, freqs):
+        if grads and x.requires_grad:
+            return _Rotary.apply(x, positions, freqs, interleaved, factor, back, None)
+        return rotary(x, positions, freqs, interleaved=interleaved, factor=factor, back=back)
+    if tangents or (grads and x.requires_grad):
+        with enable_single_level_autograd_function():
+            return _Rotary.apply(x, positions, freqs, interleaved, factor, back, (grads, torch._C._is_fwd_grad_enabled()))
     return _below(x, positions, freqs, interleaved, factor, back)
 
 
