@@ -200,3 +200,17 @@ def test_compiled_graphs(device, turn, grad):
     assert sum("rotary" in str(n.target) for n in made.graph.nodes) == 1 + grad
     for a, b in zip(made(x, *turn[2:]), both(x, *turn[2:])):
         assert torch.equal(a, b)
+
+
+def test_frequencies_that_are_a_parameter(device, turn):
+    """Are refused where a gradient of them could be asked for, and only there."""
+    op, x, freqs = torch.ops.quantized_ops.rotary, heads(device), torch.nn.Parameter(turn[3])
+    with torch.no_grad():
+        for leaf in (x, x.clone().requires_grad_()):
+            assert torch.equal(op(leaf, turn[2], freqs), op(x, turn[2], turn[3]))
+    for leaf in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="freqs have no gradient"):
+            op(leaf, turn[2], freqs)
+    leaf = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(op(leaf, turn[2], freqs.detach()).sum(), leaf)[0],
+                       op(torch.ones_like(x), turn[2], turn[3], back=True))

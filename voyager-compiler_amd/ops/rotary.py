@@ -105,12 +105,9 @@ class _Rotary(_SingleLevelFunction):
 
 @torch.library.impl(quantized_ops_lib, "rotary", "Autograd")
 def _rotary_autograd(x, positions, freqs, *, interleaved=False, factor=1.0, back=False):
-    if freqs.requires_grad:
+    grads, tangents = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if (grads and freqs.requires_grad) or (tangents and forward_ad.unpack_dual(freqs).tangent is not None):
         kv4._refuse("rotary", "freqs have no gradient here")
-    tangents = forward_ad._current_level >= 0
-    if tangents and forward_ad.unpack_dual(freqs).tangent is not None:
-        kv4._refuse("rotary", "freqs have no gradient here")
-    grads = torch.is_grad_enabled()
     if not tangents and _plain(x, positions, freqs):
         if grads and x.requires_grad:
             return _Rotary.apply(x, positions, freqs, interleaved, factor, back, None)
