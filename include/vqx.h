@@ -844,7 +844,8 @@ int vqx_kv4_append_rotary(const vqx_kv4_cache* cache, const vqx_turn* turn, cons
  * neither do those behind it that need a page (or tokens): nobody overtakes.
  * cu (int32 [seqs + 1]): the offsets of the new tokens of those that were served
  * (a sequence that was not has none); positions (int32 [n]): their places in their
- * sequences; slots (int64 [n]): page * page_size + place in the page; both -1
+ * sequences; slots (int64 [n]): page * page_size + place in the page, for what a
+ * caller keeps of each token beside the cache (nothing here reads them); both -1
  * past the last new token.  Pages that a row has behind its length (after
  * vqx_kv4_accept) are used before others are taken.
  */

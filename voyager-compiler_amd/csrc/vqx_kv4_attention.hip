@@ -27,10 +27,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct Bf16 {};
 struct F16 {};
 // What becomes of scores: nothing but the mask of a prompt; a cap or slopes too;
-// all that of new tokens that are a tree.  A tree's rows cost what a prompt's do:
-// its masks matter to the last steps only (drafted and plain on the same rows,
-// bf16 heads of 128: 16 sequences of 4000 with 24 new tokens 67 and 66 us, 8 of
-// 2000 with 16 20 and 19).
+// all that of new tokens that are a tree.  A tree's rows cost little more than a
+// prompt's: its masks matter to the last steps only (drafted and plain on the same
+// rows, bf16 heads of 128, from a graph: 16 sequences of 4000 with 24 new tokens 59
+// and 57 us, 8 of 2000 with 16 23 and 22, 32 of 2000 with 8 28 and 26, 4 of 8000
+// with 64 75 and 70; of 400 to 4000 with 24, where trees begin with the longest, 50
+// and 55).
 enum Mode { kPlain, kCurved, kTreed };
 template <typename T>
 struct Terms;

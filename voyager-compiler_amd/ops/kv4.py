@@ -440,7 +440,9 @@ def kv4_reserve(grow, lengths, table, free, count, page_size, n):
     tokens past n).  Returns (cu int32 [sequences + 1]: offsets of the new tokens
     of those that were served, positions int32 [n]: their places in their
     sequences, slots int64 [n]: page * page_size + place in the page); positions
-    and slots are -1 past the last new token."""
+    and slots are -1 past the last new token.  Slots are for what a program keeps of
+    each token beside the cache, under the same table; the operators here take the
+    table itself."""
     what = "kv4_reserve"
     _lib.require_device(lengths, what)
     device = lengths.device

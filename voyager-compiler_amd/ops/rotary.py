@@ -60,7 +60,7 @@ def _plain(x, positions, freqs):
     there is no mode, and no tensor is of a kind that has a say before its data is
     read, as a transform's, a tracer's or a negative view (a second way through the
     dispatcher is 3 us of a call's 11, and 10 in a backward pass, whose thread has
-    just been woken)."""
+    just been woken; looking at the keys is 1)."""
     return (_keys(x) == _PLAIN and _keys(freqs) == _PLAIN and _keys(positions) == _PLAIN
             and not torch._C._len_torch_dispatch_stack())
 
